@@ -57,7 +57,10 @@ typedef enum hq_status {
     HQ_ERR_CUDA = 4,              /* a CUDA runtime call failed; see hq_last_error_string */
     HQ_ERR_TIMEOUT = 5,           /* a bounded device-side wait gave up */
     HQ_ERR_MISALIGNED = 6,        /* a pointer breaks the 16-byte alignment rule */
-    HQ_ERR_UNSUPPORTED_DEVICE = 7 /* not an sm_100 device */
+    HQ_ERR_UNSUPPORTED_DEVICE = 7, /* not an sm_100 device */
+    HQ_ERR_OUT_OF_PAGES = 8,       /* a page pool has too few free pages for the call */
+    HQ_ERR_OUT_OF_MEMORY = 9,      /* host memory ran out */
+    HQ_ERR_BAD_INDEX = 10          /* a kernel met a length, row or page number out of range */
 } hq_status;
 
 typedef enum hq_dtype { HQ_F32 = 0, HQ_F16 = 1, HQ_BF16 = 2 } hq_dtype;
@@ -319,6 +322,143 @@ HQ_API hq_status hq_allreduce_sum(void* const* peer_bufs, unsigned* const* peer_
                                   int world, int rank, hq_dtype dtype, size_t count, unsigned epoch, int ctas,
                                   hq_stream_t stream);
 
+/* ------------------------------------------------- attention and its cache
+ * The decoder's attention between its QKV and O layers
+ * (hydrogen/src/model/native_decoder.cu:263 attends one row over a paged cache;
+ * hydrogen/src/attention/cascade_attention.cu attends over a shared prefix and
+ * the sequences' own keys and merges the two) for the rows of a split-fuse
+ * step, with grouped heads: query head h reads key/value head
+ * h / (n_heads / n_kv_heads).
+ *
+ *   out[t][h] = sum_j p_j v[j],  p = softmax over the keys j that row t sees of
+ *               scale * (q[t][h] . k[j]);  lse[t][h] = ln sum_j exp(scale * q . k[j])
+ *
+ * A row that sees no key gets zeros and an lse of -inf.  Scores, softmax
+ * statistics and output sums are fp32; the softmax weights are rounded to
+ * `dtype` for their product with v, and the output once.  Keys and values that
+ * a row does not see do not reach it, whatever they hold (Inf and NaN included).
+ *
+ * Strides count elements; the innermost dimension (head_dim) is contiguous;
+ * strides are multiples of 8 and pointers 16-byte aligned.  head_dim is a
+ * multiple of 8 up to 128, dtype HQ_F16 or HQ_BF16 for q, k, v and out alike.
+ * Lengths, row offsets and page tables are int32 arrays on the device, read
+ * when the kernels run, so that a captured call follows them on every replay.
+ * Rows of q and out outside every sequence are neither read nor written.
+ */
+
+/* [tokens][heads][head_dim] rows, e.g. a third of the QKV layer's output. */
+typedef struct hq_rows {
+    void* p;
+    int64_t stride_token, stride_head;
+} hq_rows;
+
+/* Pages [num_pages][page_size][n_kv_heads][head_dim], in any order of strides. */
+typedef struct hq_pages {
+    void* p;
+    int64_t stride_page, stride_token, stride_head;
+} hq_pages;
+
+typedef struct hq_attn_shape {
+    int n_tokens;   /* rows of q and out */
+    int n_seqs;
+    int max_q_len;  /* no sequence has more rows than this */
+    int n_heads, n_kv_heads, head_dim;
+    hq_dtype dtype;
+    float scale;    /* > 0; 1 / sqrt(head_dim) as a rule */
+} hq_attn_shape;
+
+/* A paged cache of one layer and the sequences' places in it.  Key j of
+ * sequence s is slot j % page_size of page page_table[s * table_stride +
+ * j / page_size]; kv_lens[s] counts the sequence's keys, those of this call's
+ * rows included.  page_size: a power of two from 16 to 256. */
+typedef struct hq_kv_view {
+    hq_pages k, v;
+    int num_pages, page_size;
+    const int32_t* page_table; /* [n_seqs][max_pages], rows table_stride apart */
+    int64_t table_stride;
+    int max_pages;
+    const int32_t* kv_lens;    /* [n_seqs] */
+} hq_kv_view;
+
+/*
+ * Attention within packed sequences (whole prompts): sequence s is the rows
+ * cu_seqlens[s] .. cu_seqlens[s+1]-1 of q, k, v and out (cu_seqlens: n_seqs + 1
+ * values).  causal != 0: row i of a sequence sees its rows 0..i, else all of
+ * the sequence.  lse (nullable): fp32 [n_tokens][n_heads].
+ */
+HQ_API size_t hq_attn_prompt_workspace_size(const hq_attn_shape* shape);
+HQ_API hq_status hq_attn_prompt(const hq_attn_shape* shape, const hq_rows* q, const hq_rows* k, const hq_rows* v,
+                                const int32_t* cu_seqlens, int causal, const hq_rows* out, float* lse,
+                                void* workspace, size_t ws_bytes, hq_stream_t stream);
+
+/*
+ * Attention of a step's rows over the paged cache, decode rows and prompt
+ * chunks alike: sequence s has the rows cu_q[s] .. cu_q[s+1]-1 (cu_q NULL: row
+ * s alone), and its row i of n sees its keys 0 .. kv_lens[s] - n + i, its own
+ * included (hq_kv_append writes them first).
+ * prefix_len > 0: every row also sees prefix_len keys that all sequences share,
+ * in the pages prefix_table[0 .. ceil(prefix_len / page_size) - 1] of the same
+ * cache; they stand before the sequences' own keys and are read once for all
+ * rows.  kv_lens and page_table count and hold the own keys only.
+ * max_kv_len: a bound of kv_lens that sizes the launch (results do not depend
+ * on it).  Workspace: hq_attn_paged_workspace_size bytes, 16-byte aligned, no
+ * initial value needed; calls that may run at the same time need different ones.
+ */
+HQ_API size_t hq_attn_paged_workspace_size(const hq_attn_shape* shape, int max_kv_len, int prefix_len);
+HQ_API hq_status hq_attn_paged(const hq_attn_shape* shape, const hq_rows* q, const hq_kv_view* cache,
+                               const int32_t* cu_q, int max_kv_len, const int32_t* prefix_table, int prefix_len,
+                               const hq_rows* out, float* lse, void* workspace, size_t ws_bytes, hq_stream_t stream);
+
+/*
+ * Writes a step's new keys and values into the pages: row i of the n rows of
+ * sequence s goes to slot kv_lens[s] - n + i (cu_q as in hq_attn_paged).  Rows
+ * that two sequences would write to one slot give it the bytes of either.
+ * Uses shape's n_tokens, n_seqs, n_kv_heads, head_dim and dtype.
+ */
+HQ_API hq_status hq_kv_append(const hq_attn_shape* shape, const hq_rows* k, const hq_rows* v, const hq_kv_view* cache,
+                              const int32_t* cu_q, hq_stream_t stream);
+
+typedef struct hq_page_move {
+    int32_t src, dst;
+} hq_page_move;
+
+/*
+ * Copies page moves[i].src over page moves[i].dst in each of n_bases page
+ * arrays (the keys and the values of every layer): page p of array b is the
+ * page_bytes bytes at bases[b] + p * page_stride_bytes.  Host arrays, read
+ * before the call returns.  A page may be copied to several places; a page that
+ * is written twice, or read and written, is refused (the order would matter).
+ * page_bytes and page_stride_bytes are multiples of 16.
+ */
+HQ_API hq_status hq_kv_copy_pages(void* const* bases, int n_bases, size_t page_stride_bytes, size_t page_bytes,
+                                  int num_pages, const hq_page_move* moves, int n_moves, hq_stream_t stream);
+
+/*
+ * Which pages of a cache belong to which sequence: reference counts and page
+ * lists, on the host (the reference's page pool, hydrogen/src/memory).  Not
+ * thread-safe.  Pages are taken lowest number first.  Sequences are named by
+ * small integers, which are used again after hq_kv_pool_free.  A call that
+ * fails changes nothing.
+ */
+typedef struct hq_kv_pool hq_kv_pool;
+HQ_API hq_kv_pool* hq_kv_pool_create(int num_pages, int page_size);
+HQ_API void hq_kv_pool_destroy(hq_kv_pool* p);
+HQ_API int hq_kv_pool_free_pages(const hq_kv_pool* p);
+/* A new, empty sequence, or one that shares all pages of `seq`; -1 on failure. */
+HQ_API int hq_kv_pool_new_seq(hq_kv_pool* p);
+HQ_API int hq_kv_pool_fork(hq_kv_pool* p, int seq);
+/* Room for n_tokens more keys.  Where the sequence's last page is partly filled
+ * and shared, it gets one of its own: *n_moves is then 1 and *move the copy that
+ * the caller makes (hq_kv_copy_pages) before it appends; else *n_moves is 0. */
+HQ_API hq_status hq_kv_pool_extend(hq_kv_pool* p, int seq, int n_tokens, hq_page_move* move, int* n_moves);
+HQ_API hq_status hq_kv_pool_free(hq_kv_pool* p, int seq);
+/* Length in keys, and pages (copies up to max_pages of them); -1: no such sequence. */
+HQ_API int hq_kv_pool_seq_len(const hq_kv_pool* p, int seq);
+HQ_API int hq_kv_pool_seq_pages(const hq_kv_pool* p, int seq, int32_t* pages, int max_pages);
+/* Renumbers the pages in use to 0 .. n-1 and writes the copies that this takes
+ * (at most as many as there are pages in use; no page is both read and written). */
+HQ_API hq_status hq_kv_pool_compact(hq_kv_pool* p, hq_page_move* moves, int max_moves, int* n_moves);
+
 /* Turn the launch overlap described at hq_gemm on (1, default) or off (0)
  * for the whole process. */
 HQ_API void hq_set_launch_overlap(int enable);
@@ -327,7 +467,10 @@ HQ_API void hq_set_launch_overlap(int enable);
  * Device-side error word: kernels that wait on barriers give up after a
  * bounded time and record a code here instead of hanging.  Synchronises the
  * current device, returns HQ_ERR_TIMEOUT (and clears the word) if any kernel
- * recorded a timeout since the last call, else HQ_OK.
+ * recorded a timeout since the last call, HQ_ERR_BAD_INDEX if an attention or
+ * cache kernel met a length, row or page number out of range (it skips what
+ * that number names, and never reads or writes outside the caller's buffers),
+ * else HQ_OK.
  */
 HQ_API hq_status hq_check_device_error(void);
 

@@ -13,7 +13,8 @@ LIB_PATH = os.path.join(_PKG, "libhq.so")
 
 # enums (include/hq.h)
 HQ_OK, HQ_ERR_INVALID_ARG, HQ_ERR_UNSUPPORTED_SHAPE, HQ_ERR_WORKSPACE_TOO_SMALL, HQ_ERR_CUDA, \
-    HQ_ERR_TIMEOUT, HQ_ERR_MISALIGNED, HQ_ERR_UNSUPPORTED_DEVICE = range(8)
+    HQ_ERR_TIMEOUT, HQ_ERR_MISALIGNED, HQ_ERR_UNSUPPORTED_DEVICE, HQ_ERR_OUT_OF_PAGES, HQ_ERR_OUT_OF_MEMORY, \
+    HQ_ERR_BAD_INDEX = range(11)
 HQ_F32, HQ_F16, HQ_BF16 = 0, 1, 2
 (HQ_WFMT_LINEAR_U4, HQ_WFMT_MARLIN_QUAD, HQ_WFMT_TILE_U4, HQ_WFMT_LINEAR_T2, HQ_WFMT_TILE_T2, HQ_WFMT_TQ1_0,
  HQ_WFMT_TILE_U4_K32) = range(7)
@@ -21,7 +22,8 @@ HQ_NOALLOC_SCRATCH_BYTES = 64 << 20  # scratch array of hq_gemm_noalloc
 HQ_GGML_F32, HQ_GGML_Q8_0, HQ_GGML_BF16, HQ_GGML_TQ1_0, HQ_GGML_TQ1_0_ALT = 0, 8, 30, 34, 143
 
 STATUS_NAMES = {0: "HQ_OK", 1: "HQ_ERR_INVALID_ARG", 2: "HQ_ERR_UNSUPPORTED_SHAPE", 3: "HQ_ERR_WORKSPACE_TOO_SMALL",
-                4: "HQ_ERR_CUDA", 5: "HQ_ERR_TIMEOUT", 6: "HQ_ERR_MISALIGNED", 7: "HQ_ERR_UNSUPPORTED_DEVICE"}
+                4: "HQ_ERR_CUDA", 5: "HQ_ERR_TIMEOUT", 6: "HQ_ERR_MISALIGNED", 7: "HQ_ERR_UNSUPPORTED_DEVICE",
+                8: "HQ_ERR_OUT_OF_PAGES", 9: "HQ_ERR_OUT_OF_MEMORY", 10: "HQ_ERR_BAD_INDEX"}
 
 # Every symbol include/hq.h declares, with (restype, argtypes).
 _vp, _i, _u32, _sz, _d = ctypes.c_void_p, ctypes.c_int, ctypes.c_uint32, ctypes.c_size_t, ctypes.c_double
@@ -45,6 +47,22 @@ SIGNATURES = {
     "hq_check_device_error": (_i, []),
     "hq_set_launch_overlap": (None, [_i]),
     "hq_allreduce_sum": (_i, [_vp, _vp, _vp, _i, _i, _i, _sz, _u32, _i, _vp]),
+    "hq_attn_prompt_workspace_size": (_sz, [_vp]),
+    "hq_attn_prompt": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, _vp, _sz, _vp]),
+    "hq_attn_paged_workspace_size": (_sz, [_vp, _i, _i]),
+    "hq_attn_paged": (_i, [_vp, _vp, _vp, _vp, _i, _vp, _i, _vp, _vp, _vp, _sz, _vp]),
+    "hq_kv_append": (_i, [_vp, _vp, _vp, _vp, _vp, _vp]),
+    "hq_kv_copy_pages": (_i, [_vp, _i, _sz, _sz, _i, _vp, _i, _vp]),
+    "hq_kv_pool_create": (_vp, [_i, _i]),
+    "hq_kv_pool_destroy": (None, [_vp]),
+    "hq_kv_pool_free_pages": (_i, [_vp]),
+    "hq_kv_pool_new_seq": (_i, [_vp]),
+    "hq_kv_pool_fork": (_i, [_vp, _i]),
+    "hq_kv_pool_extend": (_i, [_vp, _i, _i, _vp, _vp]),
+    "hq_kv_pool_free": (_i, [_vp, _i]),
+    "hq_kv_pool_seq_len": (_i, [_vp, _i]),
+    "hq_kv_pool_seq_pages": (_i, [_vp, _i, _vp, _i]),
+    "hq_kv_pool_compact": (_i, [_vp, _vp, _i, _vp]),
     "hq_batcher_create": (_vp, [_vp]),
     "hq_batcher_destroy": (None, [_vp]),
     "hq_batcher_reset": (None, [_vp]),

@@ -498,6 +498,8 @@ HQ_API hq_status hq_check_device_error(void) {
     cudaError_t e = read_and_clear_device_error(&code);
     if (e != cudaSuccess) return cuda_fail(e, "reading the device error word");
     if (code == kDevTimeout) return fail(HQ_ERR_TIMEOUT, "a kernel gave up waiting on a barrier (device timeout)");
+    if (code == kDevBadIndex)
+        return fail(HQ_ERR_BAD_INDEX, "an attention or cache kernel met a length, row or page number out of range");
     return HQ_OK;
 }
 

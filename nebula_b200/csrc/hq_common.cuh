@@ -15,7 +15,7 @@ namespace hq {
 // in the device error word (a __device__ variable of hq_api.cu whose address
 // every launch passes in) and the kernel winds down.  Read and cleared by
 // hq_check_device_error().
-enum DevError : unsigned { kDevOk = 0, kDevTimeout = 1 };
+enum DevError : unsigned { kDevOk = 0, kDevTimeout = 1, kDevBadIndex = 2 };
 
 constexpr unsigned long long kWaitBudgetNs = 2000000000ull;  // 2 s
 
