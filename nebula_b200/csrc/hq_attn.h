@@ -33,7 +33,14 @@ struct AttnArgs {
     cudaStream_t stream;
 };
 
-cudaError_t launch_attn_simple(const AttnArgs& a);
+// How a call's keys are split, and the workspace that the partial results take.
+struct AttnPlan {
+    int own, prefix;   // splits of the sequences' own keys, of the shared prefix
+    size_t part_rows;  // (row, head) partials of all splits; 0: out is written directly
+    size_t bytes;
+};
+AttnPlan attn_plan(int T, int Hq, int Hk, int D, int max_kv, int prefix_len, int sms);
+cudaError_t launch_attn(const AttnArgs& a);
 
 struct KvAppendArgs {
     int T, B, Hk, D;

@@ -109,13 +109,39 @@ void fill_shape(AttnArgs& a, const hq_attn_shape* s, const hq_rows* q, const hq_
     a.lse = lse;
 }
 
+// 0 for what the call refuses anyway.
+size_t workspace_bytes(const hq_attn_shape* s, int max_kv, int prefix_len) {
+    if (check_shape(s, true) != HQ_OK || s->n_tokens == 0 || max_kv < 0 || prefix_len < 0) return 0;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) dev = 0;
+    return attn_plan(s->n_tokens, s->n_heads, s->n_kv_heads, s->head_dim, max_kv, prefix_len, device_info(dev).sm_count).bytes;
+}
+
+hq_status check_workspace(const void* ws, size_t bytes, size_t need) {
+    if (need && !ws) return fail(HQ_ERR_INVALID_ARG, "null workspace (%zu bytes required)", need);
+    if (!aligned16(ws)) return fail(HQ_ERR_MISALIGNED, "workspace must be 16-byte aligned");
+    if (bytes < need) return fail(HQ_ERR_WORKSPACE_TOO_SMALL, "workspace %zu bytes < required %zu", bytes, need);
+    return HQ_OK;
+}
+
+// Keys and values are read through tensor maps: positive strides below 2^40 bytes.
+hq_status check_map(long long stride, long long count, const char* what) {
+    if (count > 1 && (stride <= 0 || stride >= (1LL << 39)))
+        return fail(HQ_ERR_UNSUPPORTED_SHAPE, "%s stride %lld", what, stride);
+    return HQ_OK;
+}
+
 }  // namespace
 
 extern "C" {
 
-HQ_API size_t hq_attn_prompt_workspace_size(const hq_attn_shape*) { return 0; }
+HQ_API size_t hq_attn_prompt_workspace_size(const hq_attn_shape* shape) {
+    return shape ? workspace_bytes(shape, shape->max_q_len, 0) : 0;
+}
 
-HQ_API size_t hq_attn_paged_workspace_size(const hq_attn_shape*, int, int) { return 0; }
+HQ_API size_t hq_attn_paged_workspace_size(const hq_attn_shape* shape, int max_kv_len, int prefix_len) {
+    return shape ? workspace_bytes(shape, max_kv_len, prefix_len) : 0;
+}
 
 HQ_API hq_status hq_attn_prompt(const hq_attn_shape* shape, const hq_rows* q, const hq_rows* k, const hq_rows* v,
                                 const int32_t* cu_seqlens, int causal, const hq_rows* out, float* lse, void* workspace,
@@ -127,6 +153,11 @@ HQ_API hq_status hq_attn_prompt(const hq_attn_shape* shape, const hq_rows* q, co
         (st = check_rows(out, "out")) != HQ_OK)
         return st;
     if (!cu_seqlens) return fail(HQ_ERR_INVALID_ARG, "null cu_seqlens");
+    for (const hq_rows* r : {k, v})
+        if ((st = check_map(r->stride_token, shape->n_tokens, "token")) != HQ_OK ||
+            (st = check_map(r->stride_head, shape->n_kv_heads, "head")) != HQ_OK)
+            return st;
+    if ((st = check_workspace(workspace, ws_bytes, hq_attn_prompt_workspace_size(shape))) != HQ_OK) return st;
     int dev = 0;
     if ((st = check_device(&dev)) != HQ_OK) return st;
     AttnArgs a{};
@@ -145,7 +176,7 @@ HQ_API hq_status hq_attn_prompt(const hq_attn_shape* shape, const hq_rows* q, co
     a.dev = dev;
     a.sm_count = device_info(dev).sm_count;
     a.stream = reinterpret_cast<cudaStream_t>(stream);
-    cudaError_t e = launch_attn_simple(a);
+    cudaError_t e = launch_attn(a);
     return e == cudaSuccess ? HQ_OK : cuda_fail(e, "attention launch");
 }
 
@@ -162,6 +193,13 @@ HQ_API hq_status hq_attn_paged(const hq_attn_shape* shape, const hq_rows* q, con
     if (prefix_len > 0 && !prefix_table) return fail(HQ_ERR_INVALID_ARG, "null prefix_table");
     if (!cu_q && shape->n_tokens < shape->n_seqs)
         return fail(HQ_ERR_INVALID_ARG, "%d sequences of one row in %d rows", shape->n_seqs, shape->n_tokens);
+    for (const hq_pages* r : {&cache->k, &cache->v})
+        if ((st = check_map(r->stride_token, cache->page_size, "token")) != HQ_OK ||
+            (st = check_map(r->stride_head, shape->n_kv_heads, "head")) != HQ_OK ||
+            (st = check_map(r->stride_page, cache->num_pages, "page")) != HQ_OK)
+            return st;
+    if ((st = check_workspace(workspace, ws_bytes, hq_attn_paged_workspace_size(shape, max_kv_len, prefix_len))) != HQ_OK)
+        return st;
     int dev = 0;
     if ((st = check_device(&dev)) != HQ_OK) return st;
     AttnArgs a{};
@@ -190,7 +228,7 @@ HQ_API hq_status hq_attn_paged(const hq_attn_shape* shape, const hq_rows* q, con
     a.dev = dev;
     a.sm_count = device_info(dev).sm_count;
     a.stream = reinterpret_cast<cudaStream_t>(stream);
-    cudaError_t e = launch_attn_simple(a);
+    cudaError_t e = launch_attn(a);
     return e == cudaSuccess ? HQ_OK : cuda_fail(e, "attention launch");
 }
 
