@@ -1,0 +1,28 @@
+// hq_attn.cuh -- device helpers that the attention and cache kernels share.
+#pragma once
+
+#include "hq_attn.h"
+#include "hq_attn_index.h"
+#include "hq_common.cuh"
+
+namespace hq {
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+template <bool kBF16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    uint32_t w;
+    if (kBF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi), "f"(lo));
+    else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi), "f"(lo));
+    return w;
+}
+
+__device__ __forceinline__ void bad_index(unsigned* err) {
+    if (err) atomicCAS(err, 0u, (unsigned)kDevBadIndex);
+}
+
+}  // namespace hq

@@ -33,14 +33,33 @@ struct AttnArgs {
     cudaStream_t stream;
 };
 
-// How a call's keys are split, and the workspace that the partial results take.
+// Sequences of at most kDecodeRows rows (tokens x G) over pages are the decode
+// kernel's, where it is launched; all others the tile kernel's.
+constexpr int kDecodeRows = 16;
+
+// What a call launches, and the workspace that its partial results take.
 struct AttnPlan {
-    int own, prefix;   // splits of the sequences' own keys, of the shared prefix
-    size_t part_rows;  // (row, head) partials of all splits; 0: out is written directly
+    bool decode, tile;
+    int prefix;         // key splits of the shared prefix (0: none)
+    int own;            // key splits of the tile kernel
+    int ctas, whole;    // decode kernel: CTAs; no (sequence, head) is split
+    size_t planes;      // partials of every (row, head): prefix, tile, decode
     size_t bytes;
 };
-AttnPlan attn_plan(int T, int Hq, int Hk, int D, int max_kv, int prefix_len, int sms);
+AttnPlan attn_plan(int T, int B, int max_q, int Hq, int Hk, int D, bool paged, int max_kv, int prefix_len, int sms);
 cudaError_t launch_attn(const AttnArgs& a);
+
+// The decode kernel's partial results and those of the prefix that they join.
+struct DecodeParts {
+    int ctas, whole, only;
+    float *slot_o, *slot_l;  // [ctas][2][16][D], [ctas][2][16]
+    float *own_o, *own_l;    // [T * Hq][D], [T * Hq]; null without a prefix
+    const float *pre_o, *pre_l;
+    int prefix_splits;
+};
+int decode_ctas(int B, int Hk, int max_kv, int sms);
+cudaError_t launch_attn_decode(const AttnArgs& a, const DecodeParts& parts);
+cudaError_t launch_attn_join(const AttnArgs& a, const DecodeParts& parts);
 
 struct KvAppendArgs {
     int T, B, Hk, D;

@@ -110,11 +110,13 @@ void fill_shape(AttnArgs& a, const hq_attn_shape* s, const hq_rows* q, const hq_
 }
 
 // 0 for what the call refuses anyway.
-size_t workspace_bytes(const hq_attn_shape* s, int max_kv, int prefix_len) {
-    if (check_shape(s, true) != HQ_OK || s->n_tokens == 0 || max_kv < 0 || prefix_len < 0) return 0;
+size_t workspace_bytes(const hq_attn_shape* s, bool paged, int max_kv, int prefix_len) {
+    if (check_shape(s, true) != HQ_OK || s->n_tokens == 0 || s->n_seqs == 0 || max_kv < 0 || prefix_len < 0) return 0;
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) dev = 0;
-    return attn_plan(s->n_tokens, s->n_heads, s->n_kv_heads, s->head_dim, max_kv, prefix_len, device_info(dev).sm_count).bytes;
+    return attn_plan(s->n_tokens, s->n_seqs, s->max_q_len, s->n_heads, s->n_kv_heads, s->head_dim, paged, max_kv, prefix_len,
+                     device_info(dev).sm_count)
+        .bytes;
 }
 
 hq_status check_workspace(const void* ws, size_t bytes, size_t need) {
@@ -136,11 +138,11 @@ hq_status check_map(long long stride, long long count, const char* what) {
 extern "C" {
 
 HQ_API size_t hq_attn_prompt_workspace_size(const hq_attn_shape* shape) {
-    return shape ? workspace_bytes(shape, shape->max_q_len, 0) : 0;
+    return shape ? workspace_bytes(shape, false, shape->max_q_len, 0) : 0;
 }
 
 HQ_API size_t hq_attn_paged_workspace_size(const hq_attn_shape* shape, int max_kv_len, int prefix_len) {
-    return shape ? workspace_bytes(shape, max_kv_len, prefix_len) : 0;
+    return shape ? workspace_bytes(shape, true, max_kv_len, prefix_len) : 0;
 }
 
 HQ_API hq_status hq_attn_prompt(const hq_attn_shape* shape, const hq_rows* q, const hq_rows* k, const hq_rows* v,

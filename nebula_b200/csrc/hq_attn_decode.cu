@@ -1,0 +1,701 @@
+// hq_attn_decode.cu -- attention of few rows over the paged cache: a decode step's
+// single tokens (the rows of a sequence and key/value head, tokens x G, are at
+// most 16), bound by reading the cache once.
+//
+// Work is cut into units of 128 keys of one (sequence, key/value head).  The
+// units of all sequences stand in one line (sequence, head, keys) of which every
+// CTA takes an equal share, whatever the lengths: each CTA sums up the lengths
+// itself, so no plan is made beforehand and a captured call follows them.  A warp
+// takes 16 keys of each unit, which lie in one page, through a ring of its own in
+// shared memory (cp.async, three units of 8 KB ahead; nothing but its own copies
+// to wait for): 128 KB in flight per SM, several times bandwidth x latency.
+//   S = Q K^T  mma.sync m16n8k16, the 16 rows (padded) x 16 keys
+//   P = 2^(c S - m), a running maximum m (moved, with O and the sum, only when
+//              it has grown by more than 2^8) and sum per warp and row
+//   O += P V   mma.sync, P straight from S's registers
+// The tensor rate is no bound here: 16 rows x 128 dims x 2 products a key need a
+// tenth of the rate that mma.sync has while 512 bytes of it arrive.
+// Where the CTA's share leaves a (sequence, head), its warps' sums are joined in
+// shared memory; one that no other CTA shares is written out, the others leave
+// normalised fp32 partials (at most two a CTA), joined by attn_join_kernel.
+#include "hq_attn.cuh"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace hq {
+
+namespace {
+
+constexpr int kWarps = 8;
+constexpr int kThreads = 32 * kWarps;
+constexpr int kSlice = 16;                 // keys of a warp in a unit
+constexpr int kUnit = kSlice * kWarps;
+constexpr int kMaxRows = kDecodeRows;      // 16: the MMA's M
+
+template <int DP>
+struct DecodeLayout {
+    static constexpr int kStages = 384 / DP;            // 3 (DP 128) or 6: 24 KB a warp
+    static constexpr int kStage = 2 * kSlice * DP * 2;  // K, then V
+    static constexpr int kRing = kWarps * kStages * kStage;
+    static constexpr int kPitch = DP + 2;               // floats of a row in the join buffer
+    static constexpr int kJoin = kWarps * 8 * kPitch * 4;
+    static constexpr int kSmem = kRing + kJoin;
+};
+
+struct DecodeParams {
+    const void* q;
+    long long q_st, q_sh;
+    void* o;
+    long long o_st, o_sh;
+    float* lse;
+    const void *k, *v;
+    long long k_sp, k_st, k_sh, v_sp, v_st, v_sh;
+    const int* cu_q;
+    const int* table;
+    long long table_stride;
+    const int* kv_lens;
+    int T, B, Hq, Hk, G, D;
+    int page_size, page_shift, num_pages, max_pages;
+    float scale_log2;
+    int only;   // no other kernel takes the sequences of more rows
+    int whole;  // no (sequence, head) is shared between CTAs
+    // partials: two slots of 16 rows a CTA; with a shared prefix the (sequence,
+    // head)s of one CTA leave theirs by row in own_o, own_l [T * Hq]
+    float *slot_o, *slot_l, *own_o, *own_l;
+    unsigned* err;
+};
+
+struct Seq {
+    int first, n, len, tiles;  // rows, keys, units per head
+};
+
+// Sequence s, tiles 0 if it is not this kernel's.
+__device__ __forceinline__ Seq seq_of(const int* cu_q, const int* kv_lens, int T, int G, int max_pages, int page_size, int s,
+                                      unsigned* err) {
+    Seq q{};
+    if (!seq_rows(cu_q, s, T, q.first, q.n)) {
+        bad_index(err);
+        return q;
+    }
+    if (q.n <= 0 || (long long)q.n * G > kMaxRows) return q;
+    q.len = kv_lens[s];
+    if (!len_ok(q.len, max_pages, page_size)) {
+        bad_index(err);
+        return q;
+    }
+    q.tiles = max(1, (q.len + kUnit - 1) / kUnit);
+    return q;
+}
+__device__ __forceinline__ Seq seq_of(const DecodeParams& p, int s) {
+    const Seq q = seq_of(p.cu_q, p.kv_lens, p.T, p.G, p.max_pages, p.page_size, s, p.err);
+    if (p.only && q.n > 0 && q.tiles == 0) bad_index(p.err);  // more rows than the caller's bound, or a bad length
+    return q;
+}
+
+// A place in the line of units.
+struct Place {
+    int s, h, tile;
+    Seq seq;
+};
+
+__device__ __forceinline__ void next_unit(const DecodeParams& p, Place& at) {
+    if (++at.tile < at.seq.tiles) return;
+    at.tile = 0;
+    if (++at.h < p.Hk) return;
+    at.h = 0;
+    do at.seq = ++at.s < p.B ? seq_of(p, at.s) : Seq{0, 0, 0, 1};
+    while (at.seq.tiles == 0);
+}
+
+__device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, bool have) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(have ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+
+// Sum of x over the block; `scratch`: kWarps values.  Two barriers.
+__device__ __forceinline__ long long block_sum(long long x, long long* scratch) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int d = 16; d; d >>= 1) x += __shfl_xor_sync(~0u, x, d);
+    __syncthreads();
+    if (lane == 0) scratch[threadIdx.x >> 5] = x;
+    __syncthreads();
+    x = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) x += scratch[w];
+    return x;
+}
+
+template <bool kBF16, int DP>
+__global__ void __launch_bounds__(kThreads, 1) attn_decode_kernel(const __grid_constant__ DecodeParams p) {
+    using L = DecodeLayout<DP>;
+    using T16 = typename std::conditional<kBF16, __nv_bfloat16, __half>::type;
+    constexpr float kShift = kBF16 ? 0.f : 6.f;  // fp16: P scaled by 2^6, as is the sum
+    constexpr int NS = L::kStages, RB = 2 * DP;  // RB: bytes of a key's row
+    constexpr int kChunks = DP / 8;
+
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ long long s_scan[kWarps];
+    __shared__ Place s_place[2];
+    __shared__ float s_m[kWarps][kMaxRows], s_l[kWarps][kMaxRows];
+    __shared__ unsigned s_bad[2][DP];  // keys (bit j: key len - 16 + j) whose value in that dim is NaN | +Inf << 16, -Inf
+    __shared__ int s_any_bad;
+    float* join = reinterpret_cast<float*>(smem + L::kRing);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int g = lane >> 2, t4 = lane & 3;
+    pdl_launch_dependents();
+
+    // ------------------------------------------- this CTA's share of the line
+    Seq mine{};
+    long long count = 0;
+    for (int s = tid; s < p.B; s += kThreads) {
+        mine = seq_of(p, s);
+        count += (long long)mine.tiles * p.Hk;
+    }
+    const long long total = block_sum(count, s_scan);
+    const long long ctas = min((long long)gridDim.x, total);  // that have work, one unit at least
+    if (blockIdx.x >= ctas) return;
+    long long u0 = total * blockIdx.x / ctas, u1 = total * (blockIdx.x + 1) / ctas;
+    if (tid < 2 * DP) (&s_bad[0][0])[tid] = 0;
+    if (tid == 0) s_any_bad = 0;
+    long long before = 0;
+    for (int s0 = 0; s0 < p.B; s0 += kThreads) {
+        const int s = s0 + tid;
+        if (p.B > kThreads) mine = s < p.B ? seq_of(p, s) : Seq{};
+        const long long n = (long long)mine.tiles * p.Hk;
+        long long incl = n;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const long long x = __shfl_up_sync(~0u, incl, d);
+            if (lane >= d) incl += x;
+        }
+        __syncthreads();
+        if (lane == 31) s_scan[warp] = incl;
+        __syncthreads();
+        long long lo = before + incl - n, all = before;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            if (w < warp) lo += s_scan[w];
+            all += s_scan[w];
+        }
+        for (int e = 0; e < 2; ++e) {
+            const long long u = e ? u1 : u0;
+            if (n > 0 && u >= lo && u < lo + n)
+                s_place[e] = Place{s, (int)((u - lo) / mine.tiles), (int)((u - lo) % mine.tiles), mine};
+        }
+        before = all;
+        if (before > u1) break;
+    }
+    __syncthreads();
+
+    Place at = s_place[0];
+    if (p.whole) {  // the (sequence, head)s that begin in this CTA's share
+        if (at.tile > 0) {
+            u0 += at.seq.tiles - at.tile;
+            if (u0 < total) {
+                at.tile = at.seq.tiles - 1;
+                next_unit(p, at);
+            }
+        }
+        const Place end = s_place[1];
+        if (u1 < total && end.tile > 0) u1 += end.seq.tiles - end.tile;
+        if (u0 >= u1) return;
+    }
+    Place ahead = at;  // `at`: the unit in work; `ahead`: the next one to load
+    const uint32_t ring = smem_u32(smem) + warp * NS * L::kStage;
+    auto page_of = [&](const Place& x) {
+        const int key = x.tile * kUnit + warp * kSlice;
+        return key < x.seq.len ? __ldg(p.table + x.s * p.table_stride + (key >> p.page_shift)) : 0;
+    };
+    int page = page_of(ahead);
+    // Requests this warp's keys of unit `ahead` into stage `st`; rows behind the last
+    // key and dims behind D are filled with zeros.
+    auto load = [&](int st) {
+        const int key = ahead.tile * kUnit + warp * kSlice;
+        if (key < ahead.seq.len) {
+            bool ok = page_ok(page, p.num_pages);
+            if (!ok) bad_index(p.err);
+            const long long pg = ok ? page : 0;
+            const int slot = key & (p.page_size - 1);
+            const T16* k = static_cast<const T16*>(p.k) + pg * p.k_sp + slot * p.k_st + ahead.h * p.k_sh;
+            const T16* v = static_cast<const T16*>(p.v) + pg * p.v_sp + slot * p.v_st + ahead.h * p.v_sh;
+            const int live = ok ? ahead.seq.len - key : 0;
+            const uint32_t dst = ring + st * L::kStage;
+#pragma unroll
+            for (int i = 0; i < kSlice * kChunks / 32; ++i) {
+                const int x = i * 32 + lane, r = x / kChunks, c = x % kChunks;
+                const bool have = r < live && c * 8 < p.D;
+                const uint32_t off = r * RB + ((c ^ (r & 7)) << 4);
+                cp_async16_zfill(dst + off, have ? k + r * p.k_st + c * 8 : k, have);
+                cp_async16_zfill(dst + kSlice * RB + off, have ? v + r * p.v_st + c * 8 : v, have);
+            }
+        }
+        cp_async_commit();
+    };
+
+    const int units = (int)(u1 - u0);
+    int loaded = 0;
+    auto load_next = [&]() {
+        if (loaded < units) {
+            load(loaded % NS);
+            if (++loaded < units) {
+                next_unit(p, ahead);
+                page = page_of(ahead);
+            }
+        } else {
+            cp_async_commit();
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < NS - 1; ++i) load_next();
+
+    uint32_t qf[DP / 16][4];
+    float o[DP / 8][4];
+    float m[2], l[2];
+    int lim[2], lim_min = 0, R = 0, tile0 = 0;
+    bool first_seg = true, fresh = true;
+    for (int u = 0; u < units; ++u) {
+        if (fresh) {  // a new (sequence, head): its rows of Q, rows g and g + 8 in this lane
+            fresh = false;
+            R = at.seq.n * p.G;
+            tile0 = at.tile;
+            lim_min = keys_seen(at.seq.len, at.seq.n, 0, 1);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int r = g + 8 * e;
+                const bool live = r < R;
+                const int tok = live ? r / p.G : 0, hd = at.h * p.G + (live ? r % p.G : 0);
+                lim[e] = live ? keys_seen(at.seq.len, at.seq.n, tok, 1) : at.seq.len;
+                m[e] = -INFINITY;
+                l[e] = 0.f;
+                const T16* q = static_cast<const T16*>(p.q) + (size_t)(at.seq.first + tok) * p.q_st + (size_t)hd * p.q_sh;
+#pragma unroll
+                for (int k = 0; k < DP / 16; ++k)
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const int d = 16 * k + 8 * x + 2 * t4;
+                        qf[k][e + 2 * x] = live && d < p.D ? __ldg(reinterpret_cast<const uint32_t*>(q + d)) : 0u;
+                    }
+            }
+#pragma unroll
+            for (int i = 0; i < DP / 8; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
+        }
+        load_next();
+        cp_async_wait<NS - 1>();
+        __syncwarp();
+        const int key0 = at.tile * kUnit + warp * kSlice;
+        if (key0 < at.seq.len) {
+            const uint32_t kst = ring + (u % NS) * L::kStage, vst = kst + kSlice * RB;
+            const bool masked = key0 + kSlice > lim_min;
+            if (masked && at.seq.n > 1) {
+                // Values that only some rows see and that are not finite would reach the
+                // others as 0 x NaN: taken out here, put back into the rows that see them
+                // at the end.  Only the last n <= 16 keys can be such.
+                const int lo = max(0, lim_min - key0), hi = min(kSlice, at.seq.len - key0);
+                for (int x = lane; x < (hi - lo) * kChunks; x += 32) {
+                    const int r = lo + x / kChunks, c = x % kChunks;
+                    const uint32_t a = vst + r * RB + ((c ^ (r & 7)) << 4);
+                    const uint4 v4 = lds128(a);
+                    uint32_t w[4] = {v4.x, v4.y, v4.z, v4.w};
+                    constexpr uint32_t kExp = kBF16 ? 0x7F80u : 0x7C00u;
+                    bool hit = false;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const uint32_t h = (w[e >> 1] >> (16 * (e & 1))) & 0xFFFFu;
+                        if ((h & kExp) == kExp) {
+                            const unsigned bit = 1u << (key0 + r - (at.seq.len - 16));
+                            if ((h & 0x7FFFu) != kExp) atomicOr(&s_bad[0][c * 8 + e], bit);
+                            else if (h & 0x8000u) atomicOr(&s_bad[1][c * 8 + e], bit);
+                            else atomicOr(&s_bad[0][c * 8 + e], bit << 16);
+                            w[e >> 1] &= ~(0xFFFFu << (16 * (e & 1)));
+                            hit = true;
+                        }
+                    }
+                    if (hit) {
+                        sts128(a, make_uint4(w[0], w[1], w[2], w[3]));
+                        s_any_bad = 1;
+                    }
+                }
+                __syncwarp();
+            }
+            float s[2][4] = {};
+            const int kr = ((lane >> 4) << 3) + (lane & 7), kc = (lane >> 3) & 1;
+#pragma unroll
+            for (int k = 0; k < DP / 16; ++k) {
+                uint32_t b[4];
+                ldsm4(kst + kr * RB + (((2 * k + kc) ^ (kr & 7)) << 4), b);
+                mma_16816<kBF16>(s[0], qf[k], b[0], b[1]);
+                mma_16816<kBF16>(s[1], qf[k], b[2], b[3]);
+            }
+            if (masked) {
+#pragma unroll
+                for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (key0 + 8 * nt + 2 * t4 + (e & 1) >= lim[e >> 1]) s[nt][e] = -INFINITY;
+            }
+            float mx[2], f[2];
+            bool move = false;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float x = fmaxf(fmaxf(s[0][2 * e], s[0][2 * e + 1]), fmaxf(s[1][2 * e], s[1][2 * e + 1]));
+                x = fmaxf(x, __shfl_xor_sync(~0u, x, 1));
+                x = fmaxf(x, __shfl_xor_sync(~0u, x, 2)) * p.scale_log2;
+                mx[e] = x;
+                f[e] = 1.f;
+                if (x > m[e] + 8.f) {
+                    f[e] = ex2(m[e] - x);
+                    m[e] = x;
+                    move = true;
+                }
+            }
+            if (__any_sync(~0u, move)) {
+                l[0] *= f[0];
+                l[1] *= f[1];
+#pragma unroll
+                for (int i = 0; i < DP / 8; ++i) {
+                    o[i][0] *= f[0];
+                    o[i][1] *= f[0];
+                    o[i][2] *= f[1];
+                    o[i][3] *= f[1];
+                }
+            }
+            uint32_t pf[4];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float sub = m[e] == -INFINITY ? 0.f : m[e] - kShift;
+#pragma unroll
+                for (int nt = 0; nt < 2; ++nt) {
+                    const float a = ex2(fmaf(s[nt][2 * e], p.scale_log2, -sub));
+                    const float b = ex2(fmaf(s[nt][2 * e + 1], p.scale_log2, -sub));
+                    l[e] += a + b;
+                    pf[e + 2 * nt] = pack2<kBF16>(a, b);
+                }
+            }
+            const int vr = (((lane >> 3) & 1) << 3) + (lane & 7), vc = lane >> 4;
+#pragma unroll
+            for (int i = 0; i < DP / 16; ++i) {
+                uint32_t b[4];
+                ldsm4_t(vst + vr * RB + (((2 * i + vc) ^ (vr & 7)) << 4), b);
+                mma_16816<kBF16>(o[2 * i], pf, b[0], b[1]);
+                mma_16816<kBF16>(o[2 * i + 1], pf, b[2], b[3]);
+            }
+        }
+        __syncwarp();  // the stage is read; the next load_next() may fill it
+
+        if (at.tile + 1 == at.seq.tiles || u + 1 == units) {
+            // ------------------------------------------ leave this (sequence, head)
+            const bool whole = tile0 == 0 && at.tile + 1 == at.seq.tiles;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                l[e] += __shfl_xor_sync(~0u, l[e], 1);
+                l[e] += __shfl_xor_sync(~0u, l[e], 2);
+                if (t4 == 0) {
+                    s_m[warp][g + 8 * e] = m[e];
+                    s_l[warp][g + 8 * e] = l[e];
+                }
+            }
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                if (8 * half >= R) break;
+                if (g + 8 * half < R) {
+#pragma unroll
+                    for (int i = 0; i < DP / 8; ++i)
+                        *reinterpret_cast<float2*>(join + (warp * 8 + g) * L::kPitch + 8 * i + 2 * t4) =
+                            make_float2(o[i][2 * half], o[i][2 * half + 1]);
+                }
+                __syncthreads();
+                // one warp a row, four dims a lane
+                const int r = 8 * half + warp, d = 4 * lane;
+                if (r < R) {
+                    float top = -INFINITY;
+#pragma unroll
+                    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_m[w][r]);
+                    const float base = top == -INFINITY ? 0.f : top;
+                    float sum = 0.f, acc[4] = {};
+#pragma unroll
+                    for (int w = 0; w < kWarps; ++w) {
+                        const float x = ex2(s_m[w][r] - base);
+                        sum += x * s_l[w][r];
+                        if (d < DP) {
+                            const float2* src = reinterpret_cast<const float2*>(join + (w * 8 + warp) * L::kPitch + d);
+                            const float2 a = src[0], b = src[1];
+                            acc[0] += x * a.x;
+                            acc[1] += x * a.y;
+                            acc[2] += x * b.x;
+                            acc[3] += x * b.y;
+                        }
+                    }
+                    const int tok = r / p.G, hd = at.h * p.G + r % p.G;
+                    const int see = keys_seen(at.seq.len, at.seq.n, tok, 1);
+                    const size_t row = (size_t)(at.seq.first + tok) * p.Hq + hd;
+                    const bool out = whole && !p.own_o;
+                    // no key: zeros; scores that are all -inf: NaN, or left to the join
+                    const float inv = sum != 0.f ? 1.f / sum : (out && see > 0 ? NAN : 0.f);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[e] = sum != 0.f ? acc[e] * inv : inv;
+                    if (s_any_bad && d < DP) {
+                        const int vis = see - (at.seq.len - 16);  // of the last 16 keys, the first `vis` are seen
+                        const unsigned mask = vis >= 16 ? 0xFFFFu : vis > 0 ? (1u << vis) - 1u : 0u;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const unsigned b0 = s_bad[0][d + e], b1 = s_bad[1][d + e];
+                            if ((b0 >> 16) & mask) acc[e] += INFINITY;
+                            if (b1 & mask) acc[e] -= INFINITY;
+                            if (b0 & mask) acc[e] = NAN;
+                        }
+                    }
+                    const float l2 = sum == 0.f ? -INFINITY : top - kShift + log2f(sum);
+                    if (out) {
+                        if (d < p.D)
+                            *reinterpret_cast<uint2*>(static_cast<T16*>(p.o) + (size_t)(at.seq.first + tok) * p.o_st +
+                                                      (size_t)hd * p.o_sh + d) =
+                                make_uint2(pack2<kBF16>(acc[0], acc[1]), pack2<kBF16>(acc[2], acc[3]));
+                        if (lane == 0 && p.lse) p.lse[row] = l2 * 0.693147180559945309417f;
+                    } else {
+                        const size_t slot = (size_t)(2 * blockIdx.x + (first_seg ? 0 : 1)) * kMaxRows + r;
+                        float* dst = whole ? p.own_o + row * p.D : p.slot_o + slot * p.D;
+                        if (d < p.D) *reinterpret_cast<float4*>(dst + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+                        if (lane == 0) (whole ? p.own_l[row] : p.slot_l[slot]) = l2;
+                    }
+                }
+                __syncthreads();
+            }
+            if (s_any_bad) {  // uniform: written before the barriers above
+                __syncthreads();
+                if (tid < 2 * DP) (&s_bad[0][0])[tid] = 0;
+                if (tid == 0) s_any_bad = 0;
+                __syncthreads();
+            }
+            first_seg = false;
+            fresh = true;
+        }
+        if (u + 1 < units) next_unit(p, at);
+    }
+    cp_async_wait<0>();
+}
+
+// Joins the partials of every (sequence, head) that more than one CTA worked on,
+// and with a shared prefix of every one, with the prefix's.  One block each; the
+// partials' weights first, then warp w adds up every eighth partial.
+struct JoinParams {
+    const float *slot_o, *slot_l, *own_o, *own_l;
+    const float *pre_o, *pre_l;  // [prefix_splits][T * Hq]
+    void* o;
+    long long o_st, o_sh;
+    float* lse;
+    const int* cu_q;
+    const int* kv_lens;
+    int T, B, Hq, Hk, G, D;
+    int page_size, max_pages;
+    int ctas, whole, prefix_splits, prefix_len;
+};
+
+template <bool kBF16>
+__global__ void __launch_bounds__(kThreads) attn_join_kernel(const JoinParams p) {
+    extern __shared__ __align__(16) float weights[];  // [partials][16]
+    __shared__ float buf[kWarps][8][128];
+    __shared__ long long scan[kWarps];
+    __shared__ float s_sum[kMaxRows], s_top[kMaxRows];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int s = blockIdx.x, hk = blockIdx.y;
+    pdl_wait();
+    const Seq me = seq_of(p.cu_q, p.kv_lens, p.T, p.G, p.max_pages, p.page_size, s, nullptr);
+    if (me.tiles == 0) return;
+    long long before = 0, total = 0;
+    for (int x = tid; x < p.B; x += kThreads) {
+        const long long n = (long long)seq_of(p.cu_q, p.kv_lens, p.T, p.G, p.max_pages, p.page_size, x, nullptr).tiles * p.Hk;
+        total += n;
+        if (x < s) before += n;
+    }
+    total = block_sum(total, scan);
+    before = block_sum(before, scan);
+    // CTA c has the units [total c / ctas, total (c + 1) / ctas)
+    const long long ctas = min((long long)p.ctas, total);
+    const long long ub = before + (long long)hk * me.tiles, ue = ub + me.tiles;
+    const int c0 = (int)(((ub + 1) * ctas - 1) / total), c1 = (int)((ue * ctas - 1) / total);
+    const bool whole = p.whole || c0 == c1;
+    if (whole && !p.prefix_splits) return;
+    const int own = whole ? 1 : c1 - c0 + 1, parts = own + p.prefix_splits;
+    const int R = me.n * p.G;
+    const size_t rows = (size_t)p.T * p.Hq;
+    const bool mid = ub != total * c0 / ctas;  // CTA c0 begins with another (sequence, head)
+    auto row_of = [&](int r) { return (size_t)(me.first + r / p.G) * p.Hq + hk * p.G + r % p.G; };
+    auto slot_of = [&](int i) { return (size_t)(2 * (c0 + i) + (i == 0 && mid ? 1 : 0)) * kMaxRows; };
+    for (int x = tid; x < parts * kMaxRows; x += kThreads) {
+        const int i = x / kMaxRows, r = x % kMaxRows;
+        if (r < R)
+            weights[x] = i >= own ? p.pre_l[(i - own) * rows + row_of(r)] : whole ? p.own_l[row_of(r)] : p.slot_l[slot_of(i) + r];
+    }
+    __syncthreads();
+    for (int r = warp; r < R; r += kWarps) {
+        float top = -INFINITY, sum = 0.f;
+        for (int i = lane; i < parts; i += 32) top = fmaxf(top, weights[i * kMaxRows + r]);
+        for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+        const float base = top == -INFINITY ? 0.f : top;
+        for (int i = lane; i < parts; i += 32) {
+            const float w = ex2(weights[i * kMaxRows + r] - base);
+            weights[i * kMaxRows + r] = w;
+            sum += w;
+        }
+        for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
+        if (lane == 0) {
+            s_sum[r] = sum;
+            s_top[r] = top;
+        }
+    }
+    __syncthreads();
+    const int d = 4 * lane;
+    for (int r0 = 0; r0 < R; r0 += 8) {
+        const int nr = min(8, R - r0);
+        float acc[8][4] = {};
+        if (d < p.D) {
+            for (int i = warp; i < parts; i += kWarps) {
+                const float* src = i >= own ? p.pre_o + (i - own) * rows * p.D
+                                            : whole ? p.own_o : p.slot_o + slot_of(i) * p.D;
+#pragma unroll
+                for (int r = 0; r < 8; ++r) {
+                    if (r >= nr) continue;
+                    const size_t at = i >= own || whole ? row_of(r0 + r) : (size_t)(r0 + r);
+                    const float4 x = *reinterpret_cast<const float4*>(src + at * p.D + d);
+                    const float w = weights[i * kMaxRows + r0 + r];
+                    acc[r][0] += w * x.x;
+                    acc[r][1] += w * x.y;
+                    acc[r][2] += w * x.z;
+                    acc[r][3] += w * x.w;
+                }
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+            *reinterpret_cast<float4*>(&buf[warp][r][d]) = make_float4(acc[r][0], acc[r][1], acc[r][2], acc[r][3]);
+        __syncthreads();
+        if (warp < nr) {
+            const int r = r0 + warp;
+            float x[4] = {};
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                const float4 y = *reinterpret_cast<const float4*>(&buf[w][warp][d]);
+                x[0] += y.x;
+                x[1] += y.y;
+                x[2] += y.z;
+                x[3] += y.w;
+            }
+            const int tok = r / p.G;
+            const float sum = s_sum[r];
+            const float inv =
+                sum != 0.f ? 1.f / sum : (p.prefix_len + keys_seen(me.len, me.n, tok, 1) > 0 ? NAN : 0.f);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = sum != 0.f ? x[e] * inv : inv;
+            if (d < p.D)
+                *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.o) + (size_t)(me.first + tok) * p.o_st +
+                                          (size_t)(hk * p.G + r % p.G) * p.o_sh + d) =
+                    make_uint2(pack2<kBF16>(x[0], x[1]), pack2<kBF16>(x[2], x[3]));
+            if (p.lse && lane == 0)
+                p.lse[row_of(r)] = sum == 0.f ? -INFINITY : (s_top[r] + log2f(sum)) * 0.693147180559945309417f;
+        }
+        __syncthreads();
+    }
+}
+
+template <bool kBF16, int DP>
+cudaError_t launch_one(const DecodeParams& p, int ctas, int dev, cudaStream_t s) {
+    auto fn = attn_decode_kernel<kBF16, DP>;
+    cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(fn), dev, DecodeLayout<DP>::kSmem);
+    if (e != cudaSuccess) return e;
+    fn<<<ctas, kThreads, DecodeLayout<DP>::kSmem, s>>>(p);
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+int decode_ctas(int B, int Hk, int max_kv, int sms) {
+    const long long units = (long long)B * Hk * std::max(1, (max_kv + kUnit - 1) / kUnit);
+    return (int)std::min<long long>(sms, units);
+}
+
+cudaError_t launch_attn_decode(const AttnArgs& a, const DecodeParts& parts) {
+    DecodeParams p{};
+    p.q = a.q;
+    p.q_st = a.q_st;
+    p.q_sh = a.q_sh;
+    p.o = a.o;
+    p.o_st = a.o_st;
+    p.o_sh = a.o_sh;
+    p.lse = a.lse;
+    p.k = a.k;
+    p.v = a.v;
+    p.k_sp = a.k_sp;
+    p.k_st = a.k_st;
+    p.k_sh = a.k_sh;
+    p.v_sp = a.v_sp;
+    p.v_st = a.v_st;
+    p.v_sh = a.v_sh;
+    p.cu_q = a.cu_q;
+    p.table = a.table;
+    p.table_stride = a.table_stride;
+    p.kv_lens = a.kv_lens;
+    p.T = a.T;
+    p.B = a.B;
+    p.Hq = a.Hq;
+    p.Hk = a.Hk;
+    p.G = a.G;
+    p.D = a.D;
+    p.page_size = a.page_size;
+    while ((1 << p.page_shift) < a.page_size) ++p.page_shift;
+    p.num_pages = a.num_pages;
+    p.max_pages = a.max_pages;
+    p.scale_log2 = a.scale * 1.44269504088896340736f;
+    p.only = parts.only;
+    p.whole = parts.whole;
+    p.slot_o = parts.slot_o;
+    p.slot_l = parts.slot_l;
+    p.own_o = parts.own_o;
+    p.own_l = parts.own_l;
+    p.err = a.err;
+    if (a.D <= 64)
+        return a.dtype == DType::BF16 ? launch_one<true, 64>(p, parts.ctas, a.dev, a.stream)
+                                      : launch_one<false, 64>(p, parts.ctas, a.dev, a.stream);
+    return a.dtype == DType::BF16 ? launch_one<true, 128>(p, parts.ctas, a.dev, a.stream)
+                                  : launch_one<false, 128>(p, parts.ctas, a.dev, a.stream);
+}
+
+cudaError_t launch_attn_join(const AttnArgs& a, const DecodeParts& parts) {
+    JoinParams j{parts.slot_o, parts.slot_l, parts.own_o, parts.own_l, parts.pre_o, parts.pre_l, a.o, a.o_st, a.o_sh, a.lse,
+                 a.cu_q, a.kv_lens, a.T, a.B, a.Hq, a.Hk, a.G, a.D, a.page_size, a.max_pages, parts.ctas, parts.whole,
+                 parts.prefix_splits, a.prefix_len};
+    auto fn = a.dtype == DType::BF16 ? attn_join_kernel<true> : attn_join_kernel<false>;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)a.B, (unsigned)a.Hk);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = (size_t)(parts.ctas + parts.prefix_splits) * kMaxRows * 4;
+    cfg.stream = a.stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, fn, j);
+}
+
+}  // namespace hq

@@ -32,9 +32,7 @@
 // normalised fp32 output and log2 of its sum, merged by attn_merge_kernel.
 // Every wait is bounded (hq_common.cuh): after one that gave up the roles run on
 // without waiting, so that all of them end.
-#include "hq_attn.h"
-#include "hq_attn_index.h"
-#include "hq_common.cuh"
+#include "hq_attn.cuh"
 #include "hq_tmap.h"
 
 #include <algorithm>
@@ -138,24 +136,6 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
         "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
         "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
-}
-
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-template <bool kBF16>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-    uint32_t w;
-    if (kBF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi), "f"(lo));
-    else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi), "f"(lo));
-    return w;
-}
-
-__device__ __forceinline__ void bad_index(unsigned* err) {
-    if (err) atomicCAS(err, 0u, (unsigned)kDevBadIndex);
 }
 
 // The sequence and 256-row block of this CTA: blocks are numbered through the
@@ -559,6 +539,7 @@ struct MergeParams {
     const int* kv_lens;  // null: packed rows
     int T, B, Hq, D, causal, prefix_len, splits;
     int page_size, max_pages;
+    int G, skip_rows;
 };
 
 template <bool kBF16>
@@ -569,12 +550,13 @@ __global__ void __launch_bounds__(256) attn_merge_kernel(const MergeParams p) {
     pdl_wait();
     if (row >= (long long)rows) return;
     const int t = (int)(row / p.Hq), h = (int)(row % p.Hq);
-    // the row's sequence: none of the kernels wrote anything for rows of none
+    // the row's sequence; rows of none, and those of the decode kernel, have no partials here
     int seen = -1;
     for (int s0 = 0; s0 < p.B && seen < 0; s0 += 32) {
         const int s = s0 + lane;
         int first = 0, n = 0, k = -1;
-        if (s < p.B && seq_rows(p.cu_q, s, p.T, first, n) && t >= first && t < first + n) {
+        if (s < p.B && seq_rows(p.cu_q, s, p.T, first, n) && t >= first && t < first + n &&
+            (long long)n * p.G > p.skip_rows) {
             const int len = p.kv_lens ? p.kv_lens[s] : n;
             if (!p.kv_lens || len_ok(len, p.max_pages, p.page_size)) k = keys_seen(len, n, t - first, p.causal);
         }
@@ -653,72 +635,112 @@ cudaError_t kv_maps(const AttnArgs& a, TileParams& p) {
 
 }  // namespace
 
-AttnPlan attn_plan(int T, int Hq, int Hk, int D, int max_kv, int prefix_len, int sms) {
+AttnPlan attn_plan(int T, int B, int max_q, int Hq, int Hk, int D, bool paged, int max_kv, int prefix_len, int sms) {
     AttnPlan pl{};
-    const long long rows = (long long)T * (Hq / Hk);
-    pl.own = key_splits(rows, Hk, max_kv, sms);
+    const int G = Hq / Hk;
+    const long long rows = (long long)T * G;
+    pl.tile = !paged || (long long)max_q * G > kDecodeRows;
+    pl.decode = paged && G <= kDecodeRows && (!pl.tile || B > 1);
     pl.prefix = prefix_len > 0 ? key_splits(rows, Hk, prefix_len, sms) : 0;
-    const int n = pl.own + pl.prefix;
-    pl.part_rows = n > 1 ? (size_t)n * T * Hq : 0;
-    pl.bytes = (pl.part_rows * (D + 1) * 4 + 255) & ~(size_t)255;
+    pl.own = pl.tile ? key_splits(rows, Hk, max_kv, sms) : 0;
+    pl.planes = pl.prefix;
+    if (pl.tile && pl.own + pl.prefix > 1) pl.planes += pl.own;
+    size_t slots = 0;
+    if (pl.decode) {
+        pl.ctas = decode_ctas(B, Hk, max_kv, sms);
+        // A join costs a launch: lengths that a CTA reads in less time are not split.
+        pl.whole = max_kv <= 256;
+        if (pl.prefix) ++pl.planes;
+        if (!pl.whole) slots = (size_t)pl.ctas * 2 * kDecodeRows;
+    }
+    pl.bytes = ((pl.planes * T * Hq + slots) * (D + 1) * 4 + 255) & ~(size_t)255;
     return pl;
 }
 
 cudaError_t launch_attn(const AttnArgs& a) {
-    const AttnPlan pl = attn_plan(a.T, a.Hq, a.Hk, a.D, a.max_kv, a.prefix_len, a.sm_count);
+    const AttnPlan pl = attn_plan(a.T, a.B, a.max_q, a.Hq, a.Hk, a.D, a.page_size > 0, a.max_kv, a.prefix_len, a.sm_count);
+    // workspace: outputs of the planes, of the decode slots, then the sums of both
+    const size_t rows = (size_t)a.T * a.Hq, slots = pl.decode && !pl.whole ? (size_t)pl.ctas * 2 * kDecodeRows : 0;
+    float* plane_o = reinterpret_cast<float*>(a.ws);
+    float* slot_o = plane_o + pl.planes * rows * a.D;
+    float* plane_l = slot_o + slots * a.D;
+    float* slot_l = plane_l + pl.planes * rows;
+
+    cudaError_t e = cudaSuccess;
     TileParams p;
     memset(&p, 0, sizeof p);
-    p.q = a.q;
-    p.q_st = a.q_st;
-    p.q_sh = a.q_sh;
-    p.o = a.o;
-    p.o_st = a.o_st;
-    p.o_sh = a.o_sh;
-    p.lse = a.lse;
-    p.cu_q = a.cu_q;
-    p.kv_lens = a.kv_lens;
-    p.T = a.T;
-    p.B = a.B;
-    p.Hq = a.Hq;
-    p.G = a.G;
-    p.D = a.D;
-    p.causal = a.causal;
-    p.scale_log2 = a.scale * 1.44269504088896340736f;
-    p.page_size = a.page_size;
-    p.box_rows = a.page_size ? std::min(a.page_size, kKeys) : kKeys;
-    p.num_pages = a.num_pages;
-    p.max_pages = a.max_pages;
-    p.err = a.err;
-    cudaError_t e = kv_maps(a, p);
-    if (e != cudaSuccess) return e;
-    const size_t rows = (size_t)a.T * a.Hq;
-    float* part_o = pl.part_rows ? reinterpret_cast<float*>(a.ws) : nullptr;
-    float* part_l = pl.part_rows ? part_o + pl.part_rows * a.D : nullptr;
+    if (pl.tile || pl.prefix) {
+        p.q = a.q;
+        p.q_st = a.q_st;
+        p.q_sh = a.q_sh;
+        p.o = a.o;
+        p.o_st = a.o_st;
+        p.o_sh = a.o_sh;
+        p.lse = a.lse;
+        p.cu_q = a.cu_q;
+        p.kv_lens = a.kv_lens;
+        p.T = a.T;
+        p.B = a.B;
+        p.Hq = a.Hq;
+        p.G = a.G;
+        p.D = a.D;
+        p.causal = a.causal;
+        p.scale_log2 = a.scale * 1.44269504088896340736f;
+        p.page_size = a.page_size;
+        p.box_rows = a.page_size ? std::min(a.page_size, kKeys) : kKeys;
+        p.num_pages = a.num_pages;
+        p.max_pages = a.max_pages;
+        p.err = a.err;
+        if ((e = kv_maps(a, p)) != cudaSuccess) return e;
+    }
     const int row_blocks = ceil_div((long long)a.T * a.G, 2 * kRows);
-    if (a.prefix_len) {
+    if (pl.prefix) {
         TileParams x = p;
         x.prefix_len = a.prefix_len;
         x.table = a.prefix_table;
         x.splits = pl.prefix;
-        x.part_o = part_o;
-        x.part_l = part_l;
+        x.part_o = plane_o;
+        x.part_l = plane_l;
         if ((e = launch_tile_any(a, x, row_blocks)) != cudaSuccess) return e;
     }
-    p.table = a.table;
-    p.table_stride = a.table_stride;
-    p.splits = pl.own;
-    p.part_o = part_o ? part_o + pl.prefix * rows * a.D : nullptr;
-    p.part_l = part_l ? part_l + pl.prefix * rows : nullptr;
-    // every sequence may end inside a block
-    const int blocks = (int)std::min((long long)row_blocks + a.B, (long long)0x7fffffff);
-    if ((e = launch_tile_any(a, p, blocks)) != cudaSuccess) return e;
-    if (!part_o) return cudaSuccess;
-    MergeParams m{part_o, part_l, a.o, a.o_st, a.o_sh, a.lse, a.cu_q, a.kv_lens, a.T, a.B, a.Hq, a.D, a.causal, a.prefix_len,
-                  pl.own + pl.prefix, a.page_size, a.max_pages};
-    const unsigned grid = (unsigned)((rows + 7) / 8);
-    if (a.dtype == DType::BF16) attn_merge_kernel<true><<<grid, 256, 0, a.stream>>>(m);
-    else attn_merge_kernel<false><<<grid, 256, 0, a.stream>>>(m);
-    return cudaGetLastError();
+    if (pl.tile) {
+        const bool part = pl.own + pl.prefix > 1;
+        p.table = a.table;
+        p.table_stride = a.table_stride;
+        p.splits = pl.own;
+        p.skip_rows = pl.decode ? kDecodeRows : 0;
+        p.part_o = part ? plane_o + pl.prefix * rows * a.D : nullptr;
+        p.part_l = part ? plane_l + pl.prefix * rows : nullptr;
+        // every sequence may end inside a block
+        const int blocks = (int)std::min((long long)row_blocks + a.B, (long long)0x7fffffff);
+        if ((e = launch_tile_any(a, p, blocks)) != cudaSuccess) return e;
+        if (part) {
+            MergeParams m{plane_o, plane_l, a.o, a.o_st, a.o_sh, a.lse, a.cu_q, a.kv_lens, a.T, a.B, a.Hq, a.D, a.causal,
+                          a.prefix_len, pl.own + pl.prefix, a.page_size, a.max_pages, a.G, p.skip_rows};
+            const unsigned grid = (unsigned)((rows + 7) / 8);
+            if (a.dtype == DType::BF16) attn_merge_kernel<true><<<grid, 256, 0, a.stream>>>(m);
+            else attn_merge_kernel<false><<<grid, 256, 0, a.stream>>>(m);
+            if ((e = cudaGetLastError()) != cudaSuccess) return e;
+        }
+    }
+    if (pl.decode) {
+        DecodeParts d{};
+        d.ctas = pl.ctas;
+        d.whole = pl.whole;
+        d.only = !pl.tile;
+        d.slot_o = slot_o;
+        d.slot_l = slot_l;
+        if (pl.prefix) {
+            d.own_o = plane_o + (pl.planes - 1) * rows * a.D;
+            d.own_l = plane_l + (pl.planes - 1) * rows;
+            d.pre_o = plane_o;
+            d.pre_l = plane_l;
+            d.prefix_splits = pl.prefix;
+        }
+        if ((e = launch_attn_decode(a, d)) != cudaSuccess) return e;
+        if (!pl.whole || pl.prefix) e = launch_attn_join(a, d);
+    }
+    return e;
 }
 
 }  // namespace hq

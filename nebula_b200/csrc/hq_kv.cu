@@ -1,19 +1,13 @@
 // hq_kv.cu -- device calls of the paged key/value cache: a step's rows into
 // their pages, and pages over other pages.  Both move bytes once: bound by HBM,
 // or by the launch where there is little to move.
-#include "hq_attn.h"
-#include "hq_attn_index.h"
-#include "hq_common.cuh"
+#include "hq_attn.cuh"
 
 #include <algorithm>
 
 namespace hq {
 
 namespace {
-
-__device__ __forceinline__ void bad_index(unsigned* err) {
-    if (err) atomicCAS(err, 0u, (unsigned)kDevBadIndex);
-}
 
 // One block per row: its place first, then 16 bytes a thread.
 __global__ void __launch_bounds__(256) kv_append_kernel(const KvAppendArgs a) {
