@@ -17,7 +17,7 @@ Row offsets, lengths and page tables are int32 device tensors, read when the ker
 from __future__ import annotations
 
 import ctypes
-import math
+import struct
 
 import numpy as np
 import torch
@@ -27,139 +27,106 @@ from ._lib import HQ_BF16, HQ_F16, HQError, check, lib
 
 __all__ = ["attn_prompt", "attn_paged", "kv_append", "kv_copy_pages", "PagePool", "KVCache"]
 
-_ref = ctypes.byref
 _DT = {torch.float16: HQ_F16, torch.bfloat16: HQ_BF16}
 
-
-class _Rows(ctypes.Structure):
-    _fields_ = [("p", ctypes.c_void_p), ("stride_token", ctypes.c_int64), ("stride_head", ctypes.c_int64)]
-
-
-class _Pages(ctypes.Structure):
-    _fields_ = [("p", ctypes.c_void_p), ("stride_page", ctypes.c_int64), ("stride_token", ctypes.c_int64),
-                ("stride_head", ctypes.c_int64)]
-
-
-class _Shape(ctypes.Structure):
-    _fields_ = [("n_tokens", ctypes.c_int), ("n_seqs", ctypes.c_int), ("max_q_len", ctypes.c_int),
-                ("n_heads", ctypes.c_int), ("n_kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int),
-                ("dtype", ctypes.c_int), ("scale", ctypes.c_float)]
-
-
-class _View(ctypes.Structure):
-    _fields_ = [("k", _Pages), ("v", _Pages), ("num_pages", ctypes.c_int), ("page_size", ctypes.c_int),
-                ("page_table", ctypes.c_void_p), ("table_stride", ctypes.c_int64), ("max_pages", ctypes.c_int),
-                ("kv_lens", ctypes.c_void_p)]
-
-
-class _Move(ctypes.Structure):
-    _fields_ = [("src", ctypes.c_int32), ("dst", ctypes.c_int32)]
+# The structures of include/hq.h as packed bytes: a call is shorter than building ctypes objects.
+_ROWS = struct.Struct("@Pqq").pack                # hq_rows
+_SHAPE = struct.Struct("@7if").pack               # hq_attn_shape
+_VIEW = struct.Struct("@PqqqPqqqiiPqi4xP").pack   # hq_kv_view
 
 
 def _bad(msg: str):
     raise HQError(_lib.HQ_ERR_INVALID_ARG, msg)
 
 
-def _rows(t: torch.Tensor, name: str, like: torch.Tensor, heads: int) -> _Rows:
-    if t.dim() != 3 or t.shape[0] != like.shape[0] or t.shape[1] != heads or t.shape[2] != like.shape[2]:
-        _bad(f"{name} must be [{like.shape[0]}, {heads}, {like.shape[2]}], got {tuple(t.shape)}")
-    if t.dtype != like.dtype or t.device != like.device:
+def _rows(t: torch.Tensor, name: str, like: torch.Tensor, shape: tuple) -> bytes:
+    """hq_rows of a [tokens, heads, head_dim] tensor beside `like`."""
+    if t.shape != shape:
+        _bad(f"{name} must be {list(shape)}, got {list(t.shape)}")
+    if t.dtype is not like.dtype or t.get_device() != like.get_device():
         _bad(f"{name}: {t.dtype} on {t.device} beside {like.dtype} on {like.device}")
     st, sh, sd = t.stride()
-    if sd != 1:
+    if sd != 1 and shape[2] > 1:
         _bad(f"{name}: head_dim must be contiguous")
-    return _Rows(t.data_ptr(), st, sh)
+    return _ROWS(t.data_ptr(), st, sh)
 
 
-def _pages(t: torch.Tensor, name: str, like: torch.Tensor) -> _Pages:
-    if t.dim() != 4 or t.shape[3] != like.shape[2]:
-        _bad(f"{name} must be [num_pages, page_size, kv_heads, {like.shape[2]}], got {tuple(t.shape)}")
-    if t.dtype != like.dtype or t.device != like.device:
-        _bad(f"{name}: {t.dtype} on {t.device} beside {like.dtype} on {like.device}")
-    sp, st, sh, sd = t.stride()
-    if sd != 1:
-        _bad(f"{name}: head_dim must be contiguous")
-    return _Pages(t.data_ptr(), sp, st, sh)
-
-
-def _index(t: torch.Tensor | None, name: str, shape: tuple, like: torch.Tensor):
-    """Device address of an int32 index tensor (None: null)."""
+def _index(t: torch.Tensor | None, name: str, n: int, like: torch.Tensor):
+    """Device address of n contiguous int32 (None: null)."""
     if t is None:
         return None
-    if t.dtype != torch.int32 or t.device != like.device or tuple(t.shape) != shape:
-        _bad(f"{name} must be int32 {list(shape)} on {like.device}, got {t.dtype} {list(t.shape)} on {t.device}")
-    if t.stride(-1) != 1 and t.shape[-1] > 1:
-        _bad(f"{name} must be contiguous")
+    if t.dtype is not torch.int32 or t.get_device() != like.get_device() or t.dim() != 1 or t.shape[0] != n or \
+            (n > 1 and t.stride(0) != 1):
+        _bad(f"{name} must be {n} contiguous int32 on {like.device}, got {t.dtype} {list(t.shape)} on {t.device}")
     return t.data_ptr()
 
 
-def _view(k_pages, v_pages, page_table, kv_lens, like) -> tuple[_View, int]:
-    if k_pages.shape != v_pages.shape:
-        _bad(f"key pages {tuple(k_pages.shape)} and value pages {tuple(v_pages.shape)} differ")
-    k, v = _pages(k_pages, "k_pages", like), _pages(v_pages, "v_pages", like)
-    if page_table.dim() != 2:
-        _bad("page_table must be [sequences, pages]")
-    n = page_table.shape[0]
-    table = _index(page_table, "page_table", (n, page_table.shape[1]), like)
-    return _View(k, v, k_pages.shape[0], k_pages.shape[1], table, page_table.stride(0), page_table.shape[1],
-                 _index(kv_lens, "kv_lens", (n,), like)), n
+def _view(k_pages, v_pages, page_table, kv_lens, like, D: int) -> tuple:
+    """(hq_kv_view, sequences, pages of a row of the table, page_size, kv_heads)."""
+    shape = k_pages.shape
+    if len(shape) != 4 or shape[3] != D:
+        _bad(f"k_pages must be [num_pages, page_size, kv_heads, {D}], got {list(shape)}")
+    if v_pages.shape != shape:
+        _bad(f"key pages {list(shape)} and value pages {list(v_pages.shape)} differ")
+    dev, dt = like.get_device(), like.dtype
+    if k_pages.dtype is not dt or v_pages.dtype is not dt or k_pages.get_device() != dev or v_pages.get_device() != dev:
+        _bad(f"pages of {k_pages.dtype}, {v_pages.dtype} on {k_pages.device}, {v_pages.device} beside {dt} on {like.device}")
+    kp, kt, kh, kd = k_pages.stride()
+    vp, vt, vh, vd = v_pages.stride()
+    if (kd != 1 or vd != 1) and D > 1:
+        _bad("pages: head_dim must be contiguous")
+    if page_table.dim() != 2 or page_table.dtype is not torch.int32 or page_table.get_device() != dev:
+        _bad(f"page_table must be [sequences, pages] int32 on {like.device}")
+    B, pages = page_table.shape
+    stride, inner = page_table.stride()
+    if inner != 1 and pages > 1:
+        _bad("page_table rows must be contiguous")
+    return _VIEW(k_pages.data_ptr(), kp, kt, kh, v_pages.data_ptr(), vp, vt, vh, shape[0], shape[1], page_table.data_ptr(),
+                 stride, pages, _index(kv_lens, "kv_lens", B, like) or 0), B, pages, shape[1], shape[2]
 
 
 def _dtype(q: torch.Tensor) -> int:
     dt = _DT.get(q.dtype)
     if dt is None:
         _bad(f"unsupported dtype {q.dtype}")
-    if q.device.type != "cuda":
+    if not q.is_cuda:
         _bad(f"tensors must be on a CUDA device, got {q.device}")
     return dt
 
 
-class _On:
-    """The device and stream of a call: makes `device` current where it is not, allocates on the launch stream."""
-    __slots__ = ("ptr", "ctx")
-
-    def __init__(self, device: torch.device, stream):
-        self.ctx = None
-        if stream is not None:
-            if stream.device != device:
-                _bad(f"a stream of {stream.device} for tensors on {device}")
-            self.ctx = torch.cuda.stream(stream)
-        elif device.index is not None and device.index != torch.cuda.current_device():
-            self.ctx = torch.cuda.device(device)
-
-    def __enter__(self):
-        if self.ctx is not None:
-            self.ctx.__enter__()
-        self.ptr = torch.cuda.current_stream().cuda_stream
-        return self.ptr
-
-    def __exit__(self, *e):
-        if self.ctx is not None:
-            self.ctx.__exit__(*e)
+def _on(q: torch.Tensor, stream):
+    """None where the tensors' device is current and the call goes on its current stream; else what makes it so (the
+    call's allocations are then that stream's, too)."""
+    if stream is not None:
+        if stream.device != q.device:
+            _bad(f"a stream of {stream.device} for tensors on {q.device}")
+        return torch.cuda.stream(stream)
+    return None if q.get_device() == torch._C._cuda_getDevice() else torch.cuda.device(q.device)
 
 
-def _outputs(q, out, lse, heads):
-    if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse_p = None
-    if lse is not None:
-        if lse.dtype != torch.float32 or tuple(lse.shape) != (q.shape[0], heads) or not lse.is_contiguous() or \
-                lse.device != q.device:
-            _bad(f"lse must be contiguous float32 [{q.shape[0]}, {heads}] on {q.device}")
-        lse_p = lse.data_ptr()
-    return out, _rows(out, "out", q, heads), lse_p
+def _raw_stream(q: torch.Tensor) -> int:
+    """Handle of the device's current stream (torch.cuda.current_stream builds an object for it, ten times slower)."""
+    return torch._C._cuda_getCurrentRawStream(q.get_device())
 
 
-def _workspace(need: int, workspace, device):
+def _lse(lse, q, heads):
+    if lse is None:
+        return None
+    if lse.dtype is not torch.float32 or lse.shape != (q.shape[0], heads) or not lse.is_contiguous() or \
+            lse.get_device() != q.get_device():
+        _bad(f"lse must be contiguous float32 [{q.shape[0]}, {heads}] on {q.device}")
+    return lse.data_ptr()
+
+
+def _workspace(need: int, workspace, q) -> tuple:
+    """(tensor kept until the call is enqueued, address, bytes)."""
     if workspace is None:
-        return torch.empty(need, dtype=torch.uint8, device=device) if need else None
-    if workspace.device != device or not workspace.is_contiguous():
-        _bad(f"workspace must be contiguous on {device}")
-    return workspace
-
-
-def _ws_args(ws):
-    return (None, 0) if ws is None else (ws.data_ptr(), ws.numel() * ws.element_size())
+        if not need:
+            return None, None, 0
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    elif workspace.get_device() != q.get_device() or not workspace.is_contiguous():
+        _bad(f"workspace must be contiguous on {q.device}")
+    return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
 
 
 def attn_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, max_seqlen: int, *,
@@ -169,18 +136,25 @@ def attn_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: t
     cu_seqlens[s] .. cu_seqlens[s+1]-1, at most max_seqlen of them.  Rows behind the last sequence keep what `out`
     holds.  lse: optional [T, Hq] float32 output (ln of the softmax denominator)."""
     dt = _dtype(q)
-    if q.dim() != 3 or k.dim() != 3 or cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
+    if q.dim() != 3 or k.dim() != 3 or cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1:
         _bad("q, k, v must be [tokens, heads, head_dim], cu_seqlens [sequences + 1]")
-    T, Hq, D = q.shape
-    Hk, B = k.shape[1], cu_seqlens.numel() - 1
-    rk, rv, rq = _rows(k, "k", q, Hk), _rows(v, "v", q, Hk), _rows(q, "q", q, Hq)
-    cu = _index(cu_seqlens, "cu_seqlens", (B + 1,), q)
-    sh = _Shape(T, B, max_seqlen, Hq, Hk, D, dt, 1.0 / math.sqrt(D) if scale is None else scale)
+    ctx = _on(q, stream)
+    if ctx is not None:
+        with ctx:
+            return attn_prompt(q, k, v, cu_seqlens, max_seqlen, causal=causal, scale=scale, out=out, lse=lse,
+                               workspace=workspace)
+    T, Hq, D = full = q.shape
+    Hk, B = k.shape[1], cu_seqlens.shape[0] - 1
+    kv = (T, Hk, D)
+    rk, rv, rq = _rows(k, "k", q, kv), _rows(v, "v", q, kv), _rows(q, "q", q, full)
+    cu = _index(cu_seqlens, "cu_seqlens", B + 1, q)
+    sh = _SHAPE(T, B, max_seqlen, Hq, Hk, D, dt, D ** -0.5 if scale is None else scale)
+    if out is None:
+        out = torch.empty(full, dtype=q.dtype, device=q.device)
     L = lib()
-    with _On(q.device, stream) as s:
-        out, ro, lse_p = _outputs(q, out, lse, Hq)
-        ws = _workspace(L.hq_attn_prompt_workspace_size(_ref(sh)), workspace, q.device)
-        check(L.hq_attn_prompt(_ref(sh), _ref(rq), _ref(rk), _ref(rv), cu, int(causal), _ref(ro), lse_p, *_ws_args(ws), s))
+    ws, ws_p, ws_n = _workspace(L.hq_attn_prompt_workspace_size(sh), workspace, q)
+    check(L.hq_attn_prompt(sh, rq, rk, rv, cu, int(causal), _rows(out, "out", q, full), _lse(lse, q, Hq), ws_p, ws_n,
+                           _raw_stream(q)))
     return out
 
 
@@ -196,27 +170,30 @@ def attn_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pa
     dt = _dtype(q)
     if q.dim() != 3:
         _bad("q must be [tokens, heads, head_dim]")
-    T, Hq, D = q.shape
-    view, B = _view(k_pages, v_pages, page_table, kv_lens, q)
-    Hk = k_pages.shape[2]
-    rq = _rows(q, "q", q, Hq)
-    cu = _index(cu_q, "cu_q", (B + 1,), q)
+    ctx = _on(q, stream)
+    if ctx is not None:
+        with ctx:
+            return attn_paged(q, k_pages, v_pages, page_table, kv_lens, cu_q, max_q_len, max_kv_len=max_kv_len,
+                              prefix_table=prefix_table, prefix_len=prefix_len, scale=scale, out=out, lse=lse,
+                              workspace=workspace)
+    T, Hq, D = full = q.shape
+    view, B, pages, page_size, Hk = _view(k_pages, v_pages, page_table, kv_lens, q, D)
+    rq = _rows(q, "q", q, full)
+    cu = _index(cu_q, "cu_q", B + 1, q)
     if max_kv_len is None:
-        max_kv_len = view.max_pages * view.page_size
+        max_kv_len = pages * page_size
     pt = None
     if prefix_len:
-        if prefix_table is None:
-            _bad("prefix_len without prefix_table")
-        pt = _index(prefix_table, "prefix_table", tuple(prefix_table.shape), q)
-        if prefix_table.dim() != 1 or prefix_table.shape[0] * view.page_size < prefix_len:
-            _bad(f"prefix_table {list(prefix_table.shape)} does not hold {prefix_len} keys")
-    sh = _Shape(T, B, max_q_len, Hq, Hk, D, dt, 1.0 / math.sqrt(D) if scale is None else scale)
+        if prefix_table is None or prefix_table.dim() != 1 or prefix_table.shape[0] * page_size < prefix_len:
+            _bad(f"prefix_table does not hold {prefix_len} keys")
+        pt = _index(prefix_table, "prefix_table", prefix_table.shape[0], q)
+    sh = _SHAPE(T, B, max_q_len, Hq, Hk, D, dt, D ** -0.5 if scale is None else scale)
+    if out is None:
+        out = torch.empty(full, dtype=q.dtype, device=q.device)
     L = lib()
-    with _On(q.device, stream) as s:
-        out, ro, lse_p = _outputs(q, out, lse, Hq)
-        ws = _workspace(L.hq_attn_paged_workspace_size(_ref(sh), max_kv_len, prefix_len), workspace, q.device)
-        check(L.hq_attn_paged(_ref(sh), _ref(rq), _ref(view), cu, max_kv_len, pt, prefix_len, _ref(ro), lse_p,
-                              *_ws_args(ws), s))
+    ws, ws_p, ws_n = _workspace(L.hq_attn_paged_workspace_size(sh, max_kv_len, prefix_len), workspace, q)
+    check(L.hq_attn_paged(sh, rq, view, cu, max_kv_len, pt, prefix_len, _rows(out, "out", q, full), _lse(lse, q, Hq), ws_p,
+                          ws_n, _raw_stream(q)))
     return out
 
 
@@ -228,60 +205,73 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: 
     dt = _dtype(k)
     if k.dim() != 3:
         _bad("k and v must be [tokens, kv_heads, head_dim]")
-    T, Hk, D = k.shape
-    view, B = _view(k_pages, v_pages, page_table, kv_lens, k)
-    if k_pages.shape[2] != Hk:
-        _bad(f"{Hk} heads into pages of {k_pages.shape[2]}")
-    rk, rv = _rows(k, "k", k, Hk), _rows(v, "v", k, Hk)
-    cu = _index(cu_q, "cu_q", (B + 1,), k)
-    with _On(k.device, stream) as s:
-        sh = _Shape(T, B, T, Hk, Hk, D, dt, 1.0)
-        check(lib().hq_kv_append(_ref(sh), _ref(rk), _ref(rv), _ref(view), cu, s))
+    ctx = _on(k, stream)
+    if ctx is not None:
+        with ctx:
+            return kv_append(k, v, k_pages, v_pages, page_table, kv_lens, cu_q)
+    T, Hk, D = full = k.shape
+    view, B, _, _, heads = _view(k_pages, v_pages, page_table, kv_lens, k, D)
+    if heads != Hk:
+        _bad(f"{Hk} heads into pages of {heads}")
+    cu = _index(cu_q, "cu_q", B + 1, k)
+    check(lib().hq_kv_append(_SHAPE(T, B, T, Hk, Hk, D, dt, 1.0), _rows(k, "k", k, full), _rows(v, "v", k, full), view, cu,
+                             _raw_stream(k)))
 
 
-def _moves(src, dst):
+def _moves(src, dst) -> np.ndarray:
     n = len(src)
     if len(dst) != n:
         _bad(f"{n} source pages and {len(dst)} destinations")
     both = np.empty((n, 2), np.int32)
-    both[:, 0], both[:, 1] = src, dst
-    return both, n
+    both[:, 0] = src
+    both[:, 1] = dst
+    return both
+
+
+def _page_bytes(shape, stride, size: int) -> int:
+    """Bytes of a page whose dimensions lie, in some order, in one block."""
+    run = 1
+    for st, n in sorted(zip(stride, shape)):
+        if n > 1:
+            if st != run:
+                _bad(f"a page must be one block of memory, got strides {tuple(stride)}")
+            run *= n
+    return run * size
 
 
 def kv_copy_pages(pools, src, dst, *, stream=None) -> None:
     """Copies page src[i] over page dst[i] (host integers) in every pool: tensors [num_pages, ...] of four
     dimensions, or [layers, num_pages, ...] of five, all of one geometry, a page being one block of memory.  A page
     may be copied to several places; one that is written twice, or read and written, is refused."""
-    both, n = _moves(src, dst)
-    bases, geometry = [], None
-    for t in pools:
-        if t.device.type != "cuda" or t.device != pools[0].device:
-            _bad("pools must be on one CUDA device")
-        if t.dim() not in (4, 5):
-            _bad(f"a pool has 4 or 5 dimensions, got {tuple(t.shape)}")
-        pages = t.dim() - 4
-        size = t.element_size()
-        inner = t[0, 0] if pages else t[0]
-        # one block: the strides of the inner dimensions, ascending, are the running product of their sizes
-        run = 1
-        for st, n_ in sorted((st, n_) for st, n_ in zip(inner.stride(), inner.shape) if n_ > 1):
-            if st != run:
-                _bad(f"a page must be one block of memory, got strides {inner.stride()}")
-            run *= n_
-        g = (t.shape[pages], t.stride(pages) * size, run * size)
-        if geometry not in (None, g):
-            _bad("pools of different geometry")
-        geometry = g
-        if pages:
-            step = t.stride(0) * size
-            bases += [t.data_ptr() + i * step for i in range(t.shape[0])]
-        else:
-            bases.append(t.data_ptr())
-    if not bases:
+    both = _moves(src, dst)
+    if not pools:
         return
-    with _On(pools[0].device, stream) as s:
-        check(lib().hq_kv_copy_pages((ctypes.c_void_p * len(bases))(*bases), len(bases), geometry[1], geometry[2],
-                                     geometry[0], both.ctypes.data, n, s))
+    first = pools[0]
+    if not first.is_cuda:
+        _bad(f"pools must be on a CUDA device, got {first.device}")
+    ctx = _on(first, stream)
+    if ctx is not None:
+        with ctx:
+            return kv_copy_pages(pools, src, dst)
+    dev, bases, geometry = first.get_device(), [], None
+    for t in pools:
+        shape, stride, size = t.shape, t.stride(), t.element_size()
+        if t.get_device() != dev or len(shape) not in (4, 5):
+            _bad(f"pools must be on {first.device}, of 4 or 5 dimensions: got {list(shape)} on {t.device}")
+        at = len(shape) - 4
+        g = (shape[at], stride[at] * size, _page_bytes(shape[at + 1:], stride[at + 1:], size))
+        if geometry is None:
+            geometry = g
+        elif geometry != g:
+            _bad("pools of different geometry")
+        p = t.data_ptr()
+        if at:
+            step = stride[0] * size
+            bases.extend(range(p, p + shape[0] * step, step) if step else [p] * shape[0])
+        else:
+            bases.append(p)
+    check(lib().hq_kv_copy_pages(struct.pack(f"@{len(bases)}P", *bases), len(bases), geometry[1], geometry[2], geometry[0],
+                                 both.ctypes.data, len(both), _raw_stream(first)))
 
 
 class PagePool:
@@ -323,11 +313,11 @@ class PagePool:
 
     def extend(self, seq: int, n_tokens: int) -> list[tuple[int, int]]:
         """Room for n_tokens more keys; returns the page copies, (source, destination), to make first."""
-        mv, n = _Move(), ctypes.c_int(0)
-        status = lib().hq_kv_pool_extend(self._h, seq, n_tokens, ctypes.byref(mv), ctypes.byref(n))
+        move, n = (ctypes.c_int32 * 2)(), ctypes.c_int(0)
+        status = lib().hq_kv_pool_extend(self._h, seq, n_tokens, move, ctypes.byref(n))
         if status != _lib.HQ_OK:
             raise HQError(status, f"sequence {seq} by {n_tokens} keys, {self.free_pages} pages free")
-        return [(mv.src, mv.dst)] if n.value else []
+        return [(move[0], move[1])] if n.value else []
 
     def free(self, seq: int) -> None:
         status = lib().hq_kv_pool_free(self._h, seq)

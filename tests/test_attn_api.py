@@ -15,19 +15,48 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 P = 0x10000  # an aligned address that no refused call follows
 
 
+class Rows(ctypes.Structure):
+    _fields_ = [("p", ctypes.c_void_p), ("stride_token", ctypes.c_int64), ("stride_head", ctypes.c_int64)]
+
+
+class Pages(ctypes.Structure):
+    _fields_ = [("p", ctypes.c_void_p), ("stride_page", ctypes.c_int64), ("stride_token", ctypes.c_int64),
+                ("stride_head", ctypes.c_int64)]
+
+
+class Shape(ctypes.Structure):
+    _fields_ = [("n_tokens", ctypes.c_int), ("n_seqs", ctypes.c_int), ("max_q_len", ctypes.c_int),
+                ("n_heads", ctypes.c_int), ("n_kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int),
+                ("dtype", ctypes.c_int), ("scale", ctypes.c_float)]
+
+
+class View(ctypes.Structure):
+    _fields_ = [("k", Pages), ("v", Pages), ("num_pages", ctypes.c_int), ("page_size", ctypes.c_int),
+                ("page_table", ctypes.c_void_p), ("table_stride", ctypes.c_int64), ("max_pages", ctypes.c_int),
+                ("kv_lens", ctypes.c_void_p)]
+
+
+def test_packed_structures():
+    """The wrappers' packed bytes are the structures of include/hq.h."""
+    assert at._ROWS(P, 5, -6) == bytes(Rows(P, 5, -6))
+    assert at._SHAPE(1, 2, 3, 4, 5, 6, 1, 0.5) == bytes(Shape(1, 2, 3, 4, 5, 6, 1, 0.5))
+    assert at._VIEW(P, 1, 2, 3, P + 16, 4, 5, 6, 7, 16, P + 32, 8, 9, P + 48) == \
+        bytes(View(Pages(P, 1, 2, 3), Pages(P + 16, 4, 5, 6), 7, 16, P + 32, 8, 9, P + 48))
+
+
 def shape(**kw):
     d = dict(n_tokens=4, n_seqs=2, max_q_len=4, n_heads=4, n_kv_heads=2, head_dim=64, dtype=_lib.HQ_F16, scale=0.125)
     d.update(kw)
-    return at._Shape(*d.values())
+    return Shape(*d.values())
 
 
 def rows(p=P, st=256, sh=64):
-    return at._Rows(p, st, sh)
+    return Rows(p, st, sh)
 
 
 def view(k=P, sp=4096, st=128, sh=64, num=8, page=16, table=P, stride=4, pages=4, lens=P):
-    pg = at._Pages(k, sp, st, sh)
-    return at._View(pg, pg, num, page, table, stride, pages, lens)
+    pg = Pages(k, sp, st, sh)
+    return View(pg, pg, num, page, table, stride, pages, lens)
 
 
 def prompt(sh=None, q=None, k=None, v=None, out=None, cu=P):
@@ -110,19 +139,26 @@ def test_python_refusals():
         at.attn_prompt(q.float(), k, k, cu, 3)
     with pytest.raises(E, match="destinations"):
         at.kv_copy_pages([], [1], [])
-    like = q
     for bad in (k[:2], k[:, :1], k[..., :32], k.float()):
         with pytest.raises(E):
-            at._rows(bad, "k", like, 2)
+            at._rows(bad, "k", q, (3, 2, 64))
     with pytest.raises(E, match="contiguous"):
-        at._rows(torch.zeros((3, 2, 128), dtype=torch.float16)[..., ::2], "k", like, 2)
-    with pytest.raises(E, match="int32"):
-        at._index(cu.long(), "cu", (2,), like)
-    with pytest.raises(E, match="contiguous"):
-        at._index(torch.zeros(4, dtype=torch.int32)[::2], "cu", (2,), like)
-    pages = torch.zeros((5, 16, 2, 64), dtype=torch.float16)
-    with pytest.raises(E, match="differ"):
-        at._view(pages, pages[:4], torch.zeros((1, 1), dtype=torch.int32), torch.zeros(1, dtype=torch.int32), like)
+        at._rows(torch.zeros((3, 2, 128), dtype=torch.float16)[..., ::2], "k", q, (3, 2, 64))
+    for bad in (cu.long(), cu[:1], torch.zeros(4, dtype=torch.int32)[::2], cu[None]):
+        with pytest.raises(E, match="contiguous int32"):
+            at._index(bad, "cu", 2, q)
+    pages, table, lens = torch.zeros((5, 16, 2, 64), dtype=torch.float16), torch.zeros((1, 1), dtype=torch.int32), cu[:1]
+    at._view(pages, pages, table, lens, q, 64)
+    for bad in ((pages, pages[:4], table, lens), (pages[0], pages[0], table, lens), (pages.float(), pages, table, lens),
+                (pages, pages, table[0], lens), (pages, pages, table.long(), lens), (pages, pages, table, cu),
+                (pages[..., ::2], pages[..., ::2], table, lens)):
+        with pytest.raises(E):
+            at._view(*bad, q, 64)
+    with pytest.raises(E, match="one block"):
+        at._page_bytes((16, 2, 64), (256, 64, 1), 2)
+    assert at._page_bytes((16, 2, 64), (64, 1024, 1), 2) == 4096
+    with pytest.raises(E, match="CUDA device"):
+        at.kv_copy_pages([pages], [0], [1])
     with pytest.raises(E, match="no pool"):
         at.PagePool(4, 20)
 
