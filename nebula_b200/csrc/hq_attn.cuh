@@ -25,4 +25,21 @@ __device__ __forceinline__ void bad_index(unsigned* err) {
     if (err) atomicCAS(err, 0u, (unsigned)kDevBadIndex);
 }
 
+// mbar_wait (hq_common.cuh) in few instructions: kernels that wait in many places
+// and run for microseconds are bound by fetching their code.
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, unsigned* err) {
+    unsigned long long t0 = 0;
+#pragma unroll 1
+    for (unsigned n = 0; !mbar_try_wait(bar, parity); ++n) {
+        if (n & 63u) continue;
+        const unsigned long long t = globaltimer_ns();
+        if (n == 0) t0 = t;
+        else if (t - t0 > kWaitBudgetNs) {
+            record_error(err, kDevTimeout);
+            return false;
+        }
+    }
+    return true;
+}
+
 }  // namespace hq

@@ -17,21 +17,26 @@
 // since it was last moved: until then the sums stay exact in fp32 and P, at most
 // 2^8 (2^14 in fp16, see kShift), in range.
 //
+// CTAs stay on their SM: warp 3 asks the launch hardware for the next block of
+// the grid (cluster launch control) and works out its rows and keys while the
+// others are on the current one; the next block's Q and first keys are loaded, and
+// its first S computed, while this one's output is written.
 //   warp 0        loads: one TMA box per 64 dims and up to 128 keys of a page
 //                 (page numbers from the table), K and V tiles alternate in a ring
 //   warp 1        issues the MMAs (one thread); owns the tensor memory
-//   warps 2, 3    V tiles that some row does not see in full: rows behind the
-//                 last key are zeroed (0 x NaN would reach the sum), and values
-//                 that are not finite are taken out and noted, to be put back into
-//                 the rows that see them
-//   warps 4-7, 8-11  softmax and output of tile 0, tile 1: thread = row = lane of
-//                 tensor memory
+//   warp 2        V tiles that some row does not see in full: rows behind the last
+//                 key are zeroed (0 x NaN would reach the sum), and values that
+//                 are not finite are taken out and noted, to be put back into the
+//                 rows that see them
+//   warp 3        the blocks
+//   warps 4-7, 8-11  Q, softmax and output of tile 0, tile 1: thread = row = lane
+//                 of tensor memory
 // Bound: the tensor cores and the exponentials (16 a clock and SM) alike take
-// 128 x 128 x 2 per 1024 cycles.
+// 1024 cycles for a tile's 128 rows x 128 keys x 128 dims.
 // Work is split over the keys when there are few rows: every split writes its
 // normalised fp32 output and log2 of its sum, merged by attn_merge_kernel.
-// Every wait is bounded (hq_common.cuh): after one that gave up the roles run on
-// without waiting, so that all of them end.
+// Every wait is bounded (hq_common.cuh): after one that gave up a role runs on to
+// the end of its block without waiting, and takes no other.
 #include "hq_attn.cuh"
 #include "hq_tmap.h"
 
@@ -56,7 +61,7 @@ struct TileLayout {
     static constexpr int kBlkBytes = 128 * 128;      // 128 rows of one block
     static constexpr int kTile = kBlk * kBlkBytes;   // 128 rows of Q, K or V
     static constexpr int kStages = DP == 128 ? 5 : 8;
-    static constexpr int kSmem = 2 * kTile + kStages * kTile + 1024;  // Q, ring, alignment slack
+    static constexpr int kShared = 2 * kTile + kStages * kTile;  // Q, the ring, then TileShared
 };
 
 struct alignas(64) TileParams {
@@ -72,22 +77,36 @@ struct alignas(64) TileParams {
     const int* table;
     long long table_stride;
     const int* kv_lens;
-    int T, B, Hq, G, D;
+    int T, B, Hq, Hk, G, D;
     int causal;
     float scale_log2;
     int page_size, box_rows, num_pages, max_pages;  // page_size 0: packed rows
     int prefix_len;                                 // > 0: all T rows over the pages table[0..]
-    int splits;
+    int blocks, splits;  // the grid: row blocks x Hk x splits
     int skip_rows;  // sequences of at most this many rows (tokens x G) are not this kernel's
     unsigned* err;
 };
 
+// A block of rows and its share of the keys.
+struct Item {
+    int first, n, len;       // the sequence: first row (token), tokens, keys
+    const int* table;        // its pages
+    int row0, hk, split;
+    int ni[2];               // key tiles of each row tile
+    int k_first, m_first;    // first key; first tile in which a row does not see every key
+    int stop;                // no more blocks
+};
+
 struct TileShared {
-    uint64_t full[8], empty[8], q_full, s_full[2], p_full[2], o_full[2], v_req, v_clean;
+    uint64_t full[8], empty[8], q_full[2], s_full[2], p_full[2], o_full[2], v_req, v_clean;
+    uint64_t item_full[2], item_empty[2], next;
+    uint4 next_block;
+    Item item[2];
     uint32_t tmem;
-    int seq, block;              // this CTA's sequence and 256-row block; seq -1: none
-    int any_bad;
-    int bad[3][128];             // first key whose value in that dim is NaN, +Inf, -Inf
+    // first key, counted from the block's first masked tile, whose value in a dim is
+    // NaN, +Inf, -Inf; 0xFFFF: none (masked tiles span less than 512 keys)
+    int any_bad[2];
+    uint16_t bad[2][3][128];
 };
 
 __device__ __forceinline__ void tma_load_4d(void* dst, const void* map, int c0, int c1, int c2, int c3, uint64_t* bar) {
@@ -138,25 +157,55 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
         : "memory");
 }
 
-// The sequence and 256-row block of this CTA: blocks are numbered through the
-// sequences, and taken last first (the last block of a causal prompt has the
-// most keys).  One warp; every lane returns the same.
-__device__ void find_block(const TileParams& p, int want, int& seq, int& block, unsigned* err) {
+// 16 columns from registers to this warp's lanes.
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+
+// Asks for the next block of the grid that no CTA has begun (16 bytes into `to`,
+// counted on `bar`); its index, or -1 if there is none.
+__device__ __forceinline__ void next_block_request(void* to, uint64_t* bar) {
+    mbar_arrive_expect_tx(bar, 16);
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                     smem_u32(to)),
+                 "r"(smem_u32(bar))
+                 : "memory");
+}
+__device__ __forceinline__ int next_block_answer(const void* at) {
+    const uint4 v = lds128(smem_u32(at));
+    uint32_t got, x;
+    asm volatile(
+        "{\n\t.reg .b128 h;\n\t.reg .pred p;\n\t.reg .b64 lo, hi;\n\t.reg .b32 y, z, w;\n\t"
+        "mov.b64 lo, {%2, %3};\n\tmov.b64 hi, {%4, %5};\n\tmov.b128 h, {lo, hi};\n\t"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\tmov.u32 %1, 0;\n\t"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, y, z, w}, h;\n\t}"
+        : "=r"(got), "=r"(x)
+        : "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w));
+    return got ? (int)x : -1;
+}
+
+// The sequence and 256-row block with the number `want`: blocks are numbered
+// through the sequences.  One warp; every lane returns the same.
+__device__ __forceinline__ int find_block(const TileParams& p, int want, int& block) {
     const int lane = threadIdx.x & 31;
     int before = 0;
-    seq = -1;
-    block = 0;
+#pragma unroll 1
     for (int s0 = 0; s0 < p.B; s0 += 32) {
         const int s = s0 + lane;
         int first = 0, n = 0, nb = 0;
         if (s < p.B) {
             bool ok = seq_rows(p.cu_q, s, p.T, first, n);
             if (ok && p.page_size) ok = len_ok(p.kv_lens[s], p.max_pages, p.page_size);
-            if (!ok) bad_index(err);
+            if (!ok) bad_index(p.err);
             else if ((long long)n * p.G > p.skip_rows) nb = (int)(((long long)n * p.G + 2 * kRows - 1) / (2 * kRows));
         }
         int incl = nb;
-#pragma unroll
+#pragma unroll 1
         for (int d = 1; d < 32; d <<= 1) {
             const int x = __shfl_up_sync(~0u, incl, d);
             if (lane >= d) incl += x;
@@ -165,12 +214,74 @@ __device__ void find_block(const TileParams& p, int want, int& seq, int& block, 
         const unsigned hit = __ballot_sync(~0u, want >= lo && want < lo + nb);
         if (hit) {
             const int l = __ffs(hit) - 1;
-            seq = s0 + l;
             block = want - __shfl_sync(~0u, lo, l);
-            return;
+            return s0 + l;
         }
         before += __shfl_sync(~0u, incl, 31);
     }
+    return -1;
+}
+
+// Block `index` of the grid: the last row blocks come first (under a causal mask
+// they have the most keys), then key/value heads, then key splits.
+__device__ __forceinline__ bool make_item(const TileParams& p, int index, Item& it) {
+    const int split = index % p.splits, rest = index / p.splits;
+    it.hk = rest % p.Hk;
+    it.split = split;
+    int block = p.blocks - 1 - rest / p.Hk, seq = 0;
+    if (p.prefix_len) {
+        it.first = 0;
+        it.n = p.T;
+        it.len = p.prefix_len;
+        it.table = p.table;
+    } else {
+        seq = find_block(p, block, block);
+        if (seq < 0) return false;
+        seq_rows(p.cu_q, seq, p.T, it.first, it.n);
+        it.len = p.page_size ? p.kv_lens[seq] : it.n;
+        it.table = p.table + seq * p.table_stride;
+    }
+    const int R = it.n * p.G, causal = p.causal && !p.prefix_len;  // fits: n_tokens * n_heads does
+    it.row0 = block * 2 * kRows;
+    auto seen = [&](int r) { return keys_seen(it.len, it.n, min(r, R - 1) / p.G, causal); };
+    const int end1 = (seen(it.row0 + 2 * kRows - 1) + kKeys - 1) / kKeys;
+    const int end0 = (seen(it.row0 + kRows - 1) + kKeys - 1) / kKeys;
+    const int a = (int)((long long)end1 * split / p.splits), b = (int)((long long)end1 * (split + 1) / p.splits);
+    it.ni[0] = max(0, min(b, end0) - a);
+    it.ni[1] = it.row0 + kRows < R ? b - a : 0;
+    it.k_first = a * kKeys;
+    it.m_first = max(0, seen(it.row0) / kKeys - a);
+    it.stop = 0;
+    return true;
+}
+
+// Whether one of the two 16-bit values of w is Inf or NaN.
+template <bool kBF16>
+__device__ __forceinline__ bool not_finite(uint32_t w) {
+    constexpr uint32_t kExp = kBF16 ? 0x7F80u : 0x7C00u;
+    return (w & kExp) == kExp || (w >> 16 & kExp) == kExp;
+}
+
+// Takes the values of w (dims d, d + 1 of key `key`) that are not finite out and
+// notes them.
+template <bool kBF16>
+__device__ __noinline__ uint32_t take_out(uint16_t (*bad)[128], int d, int key, uint32_t w) {
+    constexpr uint32_t kExp = kBF16 ? 0x7F80u : 0x7C00u;
+    for (int e = 0; e < 2; ++e) {
+        const uint32_t h = w >> (16 * e) & 0xFFFFu;
+        if ((h & kExp) != kExp) continue;
+        const int kind = (h & 0x7FFFu) != kExp ? 0 : (h & 0x8000u) ? 2 : 1;
+        unsigned* word = reinterpret_cast<unsigned*>(&bad[kind][(d + e) & ~1]);
+        const int sh = 16 * ((d + e) & 1);
+        unsigned old = *word;
+        while ((int)(old >> sh & 0xFFFFu) > key) {
+            const unsigned seen = atomicCAS(word, old, (old & ~(0xFFFFu << sh)) | (unsigned)key << sh);
+            if (seen == old) break;
+            old = seen;
+        }
+        w &= ~(0xFFFFu << (16 * e));
+    }
+    return w;
 }
 
 template <bool kBF16, int DP>
@@ -184,338 +295,384 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
     constexpr uint32_t kIdescS = umma_idesc_f16(kBF16, kRows, kKeys);
     constexpr uint32_t kIdescO = umma_idesc_f16(kBF16, kRows, DP) | (1u << 16);  // B: N contiguous
 
-    extern __shared__ uint8_t smem_raw[];
-    __shared__ TileShared sh;
-    uint8_t* qs = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    extern __shared__ __align__(1024) uint8_t smem[];
+    uint8_t* qs = smem;
     uint8_t* ring = qs + 2 * L::kTile;
+    TileShared& sh = *reinterpret_cast<TileShared*>(smem + L::kShared);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-    if (warp == 0) {
-        int seq = 0, block = (int)(gridDim.x - 1 - blockIdx.x);
-        if (!p.prefix_len) find_block(p, block, seq, block, p.err);
-        if (lane == 0) {
-            sh.seq = seq;
-            sh.block = block;
-            sh.any_bad = 0;
-        }
-    } else if (warp == 1) {
+    if (warp == 1) {
         if (lane == 0) {
             for (int i = 0; i < S; ++i) {
                 mbar_init(&sh.full[i], 1);
                 mbar_init(&sh.empty[i], 1);
             }
-            mbar_init(&sh.q_full, 256);
             for (int t = 0; t < 2; ++t) {
+                mbar_init(&sh.q_full[t], 128);
                 mbar_init(&sh.s_full[t], 1);
                 mbar_init(&sh.p_full[t], 128);
                 mbar_init(&sh.o_full[t], 1);
+                mbar_init(&sh.item_full[t], 1);
+                mbar_init(&sh.item_empty[t], 11);  // warps 0-2 and 4-11
             }
             mbar_init(&sh.v_req, 1);
-            mbar_init(&sh.v_clean, 64);
+            mbar_init(&sh.v_clean, 32);
+            mbar_init(&sh.next, 1);
             fence_mbarrier_init();
             fence_async_smem();
         }
         __syncwarp();
         tmem_alloc(&sh.tmem, kTmemCols);
         tmem_relinquish();
-    } else if (warp >= 4) {
-        for (int i = threadIdx.x - 128; i < 3 * 128; i += 256) (&sh.bad[0][0])[i] = INT_MAX;
+    } else if (warp == 2) {
+        for (int i = lane; i < 2 * 3 * 64; i += 32) reinterpret_cast<unsigned*>(&sh.bad[0][0][0])[i] = ~0u;
+        if (lane < 2) sh.any_bad[lane] = 0;
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sh.tmem;
-    const int seq = sh.seq;
+    bool ok = true;  // no wait of this role has given up
 
-    // This CTA's rows and keys (the same numbers in every thread).
-    int first = 0, n = 0, len = 0;
-    if (seq >= 0) {
-        if (p.prefix_len) {
-            n = p.T;
-            len = p.prefix_len;
-        } else {
-            seq_rows(p.cu_q, seq, p.T, first, n);
-            len = p.page_size ? p.kv_lens[seq] : n;
+    // Item k of this CTA is in slot k & 1.
+    auto item_wait = [&](int k) { return ok && (ok = wait_bar(&sh.item_full[k & 1], (uint32_t)(k >> 1) & 1u, p.err)); };
+
+    if (warp == 3) {
+        // -------------------------------------------------------- blocks
+        int index = (int)blockIdx.x;
+        uint32_t asked = 0;
+        for (int k = 0; ok;) {
+            if (lane == 0) next_block_request(&sh.next_block, &sh.next);
+            __syncwarp();
+            Item it;
+            if (make_item(p, index, it)) {
+                if (k >= 2) ok = wait_bar(&sh.item_empty[k & 1], (uint32_t)((k - 2) >> 1) & 1u, p.err);
+                __syncwarp();
+                if (sh.any_bad[k & 1]) {
+                    for (int i = lane; i < 3 * 64; i += 32) reinterpret_cast<unsigned*>(&sh.bad[k & 1][0][0])[i] = ~0u;
+                    __syncwarp();
+                }
+                if (lane == 0) {
+                    sh.any_bad[k & 1] = 0;
+                    sh.item[k & 1] = it;
+                    mbar_arrive(&sh.item_full[k & 1]);
+                }
+                __syncwarp();
+                ++k;
+            }
+            // also when a wait gave up: the answer lands before the CTA exits
+            const bool told = wait_bar(&sh.next, asked++ & 1u, p.err);
+            index = told ? next_block_answer(&sh.next_block) : -1;
+            ok = ok && told;
+            __syncwarp();
+            if (lane == 0) fence_async_smem();  // the answer is read before the next one is written
+            if (index >= 0) continue;
+            if (ok && k >= 2) ok = wait_bar(&sh.item_empty[k & 1], (uint32_t)((k - 2) >> 1) & 1u, p.err);
+            __syncwarp();
+            if (lane == 0) {
+                sh.item[k & 1].stop = 1;
+                mbar_arrive(&sh.item_full[k & 1]);
+            }
+            break;
         }
-    }
-    const int R = n * p.G;  // fits: n_tokens * n_heads does
-    const int row0 = sh.block * 2 * kRows;
-    const int hk = blockIdx.y, split = blockIdx.z;
-    const int causal = p.causal && !p.prefix_len;
-    auto seen_of = [&](int r) { return keys_seen(len, n, min(r, R - 1) / p.G, causal); };
-    int ni[2] = {0, 0}, k_first = 0, m_first = 0;  // key tiles of each row tile; first key; first tile with a mask
-    if (seq >= 0 && row0 < R) {
-        const int end1 = (seen_of(row0 + 2 * kRows - 1) + kKeys - 1) / kKeys;
-        const int end0 = (seen_of(row0 + kRows - 1) + kKeys - 1) / kKeys;
-        const int a = (int)((long long)end1 * split / p.splits), b = (int)((long long)end1 * (split + 1) / p.splits);
-        ni[0] = max(0, min(b, end0) - a);
-        ni[1] = row0 + kRows < R ? b - a : 0;
-        k_first = a * kKeys;
-        m_first = max(0, seen_of(row0) / kKeys - a);
-    }
-    const int nt = max(ni[0], ni[1]);
-
-    if (warp == 0) {
-        // ---------------------------------------------------------- loads
-        const int* table = p.prefix_len ? p.table : p.table + seq * p.table_stride;
+        __syncwarp();
+    } else if (warp == 0) {
+        // --------------------------------------------------------- loads
         const int boxes = kKeys / p.box_rows;
-        bool ok = true;
         int use = 0;
-        for (int i = 0; i < nt; ++i) {
-            const int k0 = k_first + i * kKeys;
-            const int live = min(boxes, (len - k0 + p.box_rows - 1) / p.box_rows);
-            for (int kv = 0; kv < 2; ++kv, ++use) {
-                const int slot = use % S;
-                if (ok) ok = mbar_wait(&sh.empty[slot], ((uint32_t)(use / S) & 1u) ^ 1u, p.err);
+        for (int k = 0; item_wait(k); ++k) {
+            const Item it = sh.item[k & 1];
+            if (it.stop) break;
+            const int nt = max(it.ni[0], it.ni[1]);
+#pragma unroll 1
+            for (int i = 0; i < 2 * nt; ++i, ++use) {  // K, V of tile 0, of tile 1, ...
+                const int k0 = it.k_first + (i >> 1) * kKeys, slot = use % S;
+                const int live = min(boxes, (it.len - k0 + p.box_rows - 1) / p.box_rows);
+                if (ok) ok = wait_bar(&sh.empty[slot], ((uint32_t)(use / S) & 1u) ^ 1u, p.err);
                 uint8_t* dst = ring + slot * L::kTile;
                 if (lane == 0) mbar_arrive_expect_tx(&sh.full[slot], (uint32_t)(live * L::kBlk * p.box_rows * 128));
                 __syncwarp();
-                for (int b = lane; b < live * L::kBlk; b += 32) {
-                    const int box = b / L::kBlk, blk = b % L::kBlk;
+                if (lane < live * L::kBlk) {
+                    const int box = lane / L::kBlk, blk = lane % L::kBlk;
                     const int key = k0 + box * p.box_rows;
-                    int token = first + key, page = 0;
+                    int token = it.first + key, page = 0;
                     if (p.page_size) {
                         token = key & (p.page_size - 1);
-                        page = table[key / p.page_size];
+                        page = it.table[key / p.page_size];
                         if (!page_ok(page, p.num_pages)) {
                             bad_index(p.err);
                             page = p.num_pages;  // out of range: the box reads zeros
                         }
                     }
-                    tma_load_4d(dst + blk * L::kBlkBytes + box * p.box_rows * 128, kv ? &p.v_map : &p.k_map, blk * 64, token,
-                                hk, page, &sh.full[slot]);
+                    tma_load_4d(dst + blk * L::kBlkBytes + box * p.box_rows * 128, i & 1 ? &p.v_map : &p.k_map, blk * 64,
+                                token, it.hk, page, &sh.full[slot]);
                 }
             }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.item_empty[k & 1]);
         }
         // Every stage filled here has been consumed (its commit has landed) before exit.
-        for (int j = max(0, use - S); j < use; ++j) mbar_wait(&sh.empty[j % S], (uint32_t)(j / S) & 1u, p.err);
+#pragma unroll 1
+        for (int j = max(0, use - S); j < use; ++j) wait_bar(&sh.empty[j % S], (uint32_t)(j / S) & 1u, p.err);
     } else if (warp == 1) {
-        // ------------------------------------------------------------ MMA
-        if (lane == 0 && nt > 0) {
-            bool ok = mbar_wait(&sh.q_full, 0, p.err);
-            auto wait_full = [&](int use) {
-                if (ok) ok = mbar_wait(&sh.full[use % S], (uint32_t)(use / S) & 1u, p.err);
-            };
-            auto qk = [&](int t, int use) {
-                const uint32_t qa = smem_u32(qs) + t * L::kTile, ka = smem_u32(ring) + (use % S) * L::kTile;
+        // ----------------------------------------------------------- MMA
+        if (lane == 0) {
+            const uint32_t ring_a = smem_u32(ring);
+            uint32_t use = 0, cleaned = 0, loaded[2] = {0, 0}, done[2] = {0, 0};
+            for (int k = 0; item_wait(k); ++k) {
+                if (sh.item[k & 1].stop) break;
+                const int n0 = sh.item[k & 1].ni[0], n1 = sh.item[k & 1].ni[1], m_first = sh.item[k & 1].m_first;
+                const int nt = max(n0, n1);
+                mbar_arrive(&sh.item_empty[k & 1]);
+                // step i: O += P V of key tile i, S = Q K^T of tile i + 1
+#pragma unroll 1
+                for (int i = -1; i < nt; ++i) {
+                    const uint32_t vu = use + 2 * i + 1, ku = vu + 1;
+                    if (i >= 0) {
+                        if (ok) ok = wait_bar(&sh.full[vu % S], (vu / S) & 1u, p.err);
+                        if (i >= m_first && ok) ok = wait_bar(&sh.v_clean, cleaned++ & 1u, p.err);
+                    }
+                    if (i + 1 < nt && ok) ok = wait_bar(&sh.full[ku % S], (ku / S) & 1u, p.err);
+                    const uint64_t vd = sw128_mn_desc(ring_a + (vu % S) * L::kTile);
+                    const uint64_t kd = sw128_kmajor_desc(ring_a + (ku % S) * L::kTile);
+#pragma unroll 1
+                    for (int t = 0; t < 2; ++t) {
+                        const int my = t ? n1 : n0;
+                        const uint32_t sp = tmem + 128u * t;
+                        if (i >= 0 && i < my) {
+                            if (ok) ok = wait_bar(&sh.p_full[t], done[t]++ & 1u, p.err);
+                            tc_fence_after();
 #pragma unroll
-                for (int k = 0; k < DP / 16; ++k) {
-                    const uint32_t off = (k >> 2) * L::kBlkBytes + (k & 3) * 32;
-                    umma_f16(tmem + 128u * t, sw128_kmajor_desc(qa + off), sw128_kmajor_desc(ka + off), kIdescS, k != 0);
+                            for (int j = 0; j < kKeys / 16; ++j)
+                                umma_ts_f16(tmem + kColO + (uint32_t)DP * t, sp + 8u * j, vd + j * (2048 >> 4), kIdescO,
+                                            (i | j) != 0);
+                            umma_commit(&sh.o_full[t]);
+                        }
+                        if (i + 1 < my) {
+                            if (i < 0 && ok) ok = wait_bar(&sh.q_full[t], loaded[t]++ & 1u, p.err);
+                            tc_fence_after();
+                            const uint64_t qd = sw128_kmajor_desc(smem_u32(qs) + t * L::kTile);
+#pragma unroll
+                            for (int j = 0; j < DP / 16; ++j) {
+                                const uint32_t off = ((j >> 2) * L::kBlkBytes + (j & 3) * 32) >> 4;
+                                umma_f16(sp, qd + off, kd + off, kIdescS, j != 0);
+                            }
+                            umma_commit(&sh.s_full[t]);
+                        }
+                    }
+                    if (i >= 0) umma_commit(&sh.empty[vu % S]);
+                    if (i + 1 < nt) {
+                        umma_commit(&sh.empty[ku % S]);
+                        if (i + 1 >= m_first) mbar_arrive(&sh.v_req);
+                    }
                 }
-                umma_commit(&sh.s_full[t]);
-            };
-            wait_full(0);
-            tc_fence_after();
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-                if (ni[t] > 0) qk(t, 0);
-            umma_commit(&sh.empty[0]);
-            if (m_first == 0) mbar_arrive(&sh.v_req);
-            for (int i = 0; i < nt; ++i) {
-                wait_full(2 * i + 1);
-                if (i + 1 < nt) wait_full(2 * i + 2);
-                if (i >= m_first && ok) ok = mbar_wait(&sh.v_clean, (uint32_t)(i - m_first) & 1u, p.err);
-                const uint32_t va = smem_u32(ring) + ((2 * i + 1) % S) * L::kTile;
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    if (i >= ni[t]) continue;
-                    if (ok) ok = mbar_wait(&sh.p_full[t], (uint32_t)i & 1u, p.err);
-                    tc_fence_after();
-#pragma unroll
-                    for (int k = 0; k < kKeys / 16; ++k)
-                        umma_ts_f16(tmem + kColO + (uint32_t)DP * t, tmem + 128u * t + 8u * k, sw128_mn_desc(va + k * 2048),
-                                    kIdescO, (i | k) != 0);
-                    umma_commit(&sh.o_full[t]);
-                    if (i + 1 < ni[t]) qk(t, 2 * i + 2);
-                }
-                umma_commit(&sh.empty[(2 * i + 1) % S]);
-                if (i + 1 < nt) {
-                    umma_commit(&sh.empty[(2 * i + 2) % S]);
-                    if (i + 1 >= m_first) mbar_arrive(&sh.v_req);
-                }
+                use += 2 * nt;
             }
         }
         __syncwarp();
-    } else if (warp < 4) {
+    } else if (warp == 2) {
         // ----------------------------------------- V tiles under a mask
-        // v_req comes once the tile's K has been used, so V's stage is in this
-        // use's phase or the one before it, and stays until v_clean.
-        const int tid = threadIdx.x - 64;
-        const int lim_min = nt > 0 ? seen_of(row0) : 0;
-        bool ok = true;
-        for (int i = m_first; i < nt; ++i) {
-            const int use = 2 * i + 1;
-            if (ok) ok = mbar_wait(&sh.v_req, (uint32_t)(i - m_first) & 1u, p.err);
-            if (ok) ok = mbar_wait(&sh.full[use % S], (uint32_t)(use / S) & 1u, p.err);
-            uint8_t* vt = ring + (use % S) * L::kTile;
-            const int k0 = k_first + i * kKeys;
-            const int valid = min(kKeys, len - k0), lo = min(valid, max(0, lim_min - k0));
-            // 16-byte chunk c of row r of a block lies at chunk c ^ (r & 7)
-            for (int x = tid; x < (kKeys - lo) * DP / 8; x += 64) {
-                const int r = lo + x / (DP / 8), c = x % (DP / 8);
-                uint4* at = reinterpret_cast<uint4*>(vt + (c >> 3) * L::kBlkBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4));
-                if (r >= valid) {
-                    *at = make_uint4(0u, 0u, 0u, 0u);
-                    continue;
-                }
-                uint4 v = *at;
-                constexpr uint32_t kExp = kBF16 ? 0x7F80u : 0x7C00u;
-                uint32_t w[4] = {v.x, v.y, v.z, v.w};
-                bool hit = false;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const uint32_t h = (w[e >> 1] >> (16 * (e & 1))) & 0xFFFFu;
-                    if ((h & kExp) == kExp) {
-                        const int kind = (h & 0x7FFFu) != kExp ? 0 : (h & 0x8000u) ? 2 : 1;
-                        atomicMin(&sh.bad[kind][c * 8 + e], k0 + r);
-                        w[e >> 1] &= ~(0xFFFFu << (16 * (e & 1)));
-                        hit = true;
+        // v_req comes once the tile's K has been used, so V's stage is in this use's
+        // phase or the one before it, and stays until v_clean.
+        uint32_t use = 0, asked = 0;
+        for (int k = 0; item_wait(k); ++k) {
+            const Item it = sh.item[k & 1];
+            if (it.stop) break;
+            const int nt = max(it.ni[0], it.ni[1]);
+            const int lim_min = keys_seen(it.len, it.n, it.row0 / p.G, p.causal && !p.prefix_len);
+            const int base = it.k_first + it.m_first * kKeys;
+#pragma unroll 1
+            for (int i = it.m_first; i < nt; ++i) {
+                const uint32_t vu = use + 2 * i + 1;
+                if (ok) ok = wait_bar(&sh.v_req, asked++ & 1u, p.err);
+                if (ok) ok = wait_bar(&sh.full[vu % S], (vu / S) & 1u, p.err);
+                __syncwarp();
+                const uint32_t vt = smem_u32(ring) + (vu % S) * L::kTile;
+                const int k0 = it.k_first + i * kKeys;
+                const int valid = min(kKeys, it.len - k0), lo = min(valid, max(0, lim_min - k0));
+                // 16-byte chunk c of row r of a block lies at chunk c ^ (r & 7)
+#pragma unroll 1
+                for (int x = lo * (DP / 8) + lane; x < kKeys * (DP / 8); x += 32) {
+                    const int r = x / (DP / 8), c = x % (DP / 8);
+                    const uint32_t at = vt + (c >> 3) * L::kBlkBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+                    if (r >= valid) {
+                        sts128(at, make_uint4(0u, 0u, 0u, 0u));
+                        continue;
+                    }
+                    uint4 v = lds128(at);
+                    if (not_finite<kBF16>(v.x) || not_finite<kBF16>(v.y) || not_finite<kBF16>(v.z) || not_finite<kBF16>(v.w)) {
+                        const int key = k0 + r - base;
+                        v.x = take_out<kBF16>(sh.bad[k & 1], c * 8, key, v.x);
+                        v.y = take_out<kBF16>(sh.bad[k & 1], c * 8 + 2, key, v.y);
+                        v.z = take_out<kBF16>(sh.bad[k & 1], c * 8 + 4, key, v.z);
+                        v.w = take_out<kBF16>(sh.bad[k & 1], c * 8 + 6, key, v.w);
+                        sts128(at, v);
+                        sh.any_bad[k & 1] = 1;
                     }
                 }
-                if (hit) {
-                    *at = make_uint4(w[0], w[1], w[2], w[3]);
-                    sh.any_bad = 1;
-                }
+                fence_async_smem();
+                mbar_arrive(&sh.v_clean);
             }
-            fence_async_smem();
-            mbar_arrive(&sh.v_clean);
+            use += 2 * nt;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.item_empty[k & 1]);
         }
     } else {
-        // ----------------------------------------------- softmax and output
+        // ------------------------------------------ Q, softmax and output
         const int t = (warp - 4) >> 2, i0 = (threadIdx.x - 128) & 127;
-        const int r = row0 + t * kRows + i0;
-        const bool live = r < R;
-        const int token = live ? r / p.G : 0, head = hk * p.G + (live ? r % p.G : 0);
-        const int lim = live ? seen_of(r) : seen_of(R - 1);
-        const int my = ni[t];
-        if (nt > 0) {  // this row of Q, zeros behind the last row and dim
-            const T16* q = static_cast<const T16*>(p.q) + (size_t)(first + token) * p.q_st + (size_t)head * p.q_sh;
-#pragma unroll
-            for (int c = 0; c < DP / 8; ++c) {
-                const uint4 v = live && c * 8 < p.D ? ldg128_nc(q + c * 8) : make_uint4(0u, 0u, 0u, 0u);
-                sts128(smem_u32(qs) + t * L::kTile + (c >> 3) * L::kBlkBytes + i0 * 128 + (((c & 7) ^ (i0 & 7)) << 4), v);
-            }
-            fence_async_smem();
-            mbar_arrive(&sh.q_full);
-        }
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
         const uint32_t ts = tmem + lanes + 128u * t, to = tmem + lanes + kColO + (uint32_t)DP * t;
-        bool ok = true;
-        float m = -INFINITY, l = 0.f;
-        for (int i = 0; i < my; ++i) {
-            if (ok) ok = mbar_wait(&sh.s_full[t], (uint32_t)i & 1u, p.err);
-            __syncwarp();
-            tc_fence_after();
-            const int cut = i >= m_first ? lim - (k_first + i * kKeys) : kKeys;  // columns from `cut` on are not seen
-            float mx = -INFINITY;
+        const int causal = p.causal && !p.prefix_len;
+        uint32_t steps = 0;  // key tiles of this row tile so far
+        Item it{};
+        bool live = false;
+        int token = 0, head = 0, lim = 0;
+        // Takes item k: this thread's row, and its row of Q into shared memory (the
+        // MMAs of the item before have read theirs).
+        auto take = [&](int k) {
+            if (!item_wait(k)) return false;
+            it = sh.item[k & 1];
+            if (it.stop) return false;
+            const int R = it.n * p.G, r = it.row0 + t * kRows + i0;
+            live = r < R;
+            const int tok = min(r, R - 1) / p.G;  // rows behind the last see what it sees
+            lim = keys_seen(it.len, it.n, tok, causal);
+            token = it.first + tok;
+            head = it.hk * p.G + (live ? r - tok * p.G : 0);
+            if (it.ni[t] > 0) {
+                const T16* q = static_cast<const T16*>(p.q) + (size_t)token * p.q_st + (size_t)head * p.q_sh;
+                const uint32_t dst = smem_u32(qs) + t * L::kTile + i0 * 128;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                float s[32];
-                tmem_ld32_now(ts + 32u * c, s);
-                if (cut < kKeys) {
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) s[e] = 32 * c + e < cut ? s[e] : -INFINITY;
+                for (int c = 0; c < DP / 8; ++c) {
+                    const uint4 v = live && c * 8 < p.D ? ldg128_nc(q + c * 8) : make_uint4(0u, 0u, 0u, 0u);
+                    sts128(dst + (c >> 3) * L::kBlkBytes + (((c & 7) ^ (i0 & 7)) << 4), v);
                 }
-#pragma unroll
-                for (int e = 0; e < 32; ++e) mx = fmaxf(mx, s[e]);
+                fence_async_smem();
+                mbar_arrive(&sh.q_full[t]);
             }
-            mx *= p.scale_log2;
-            const bool move = mx > m + 8.f;  // also from -inf; a first tile has no O yet
-            if (__any_sync(~0u, move && l > 0.f)) {
-                if (ok) ok = mbar_wait(&sh.o_full[t], (uint32_t)(i - 1) & 1u, p.err);
+            return true;
+        };
+        bool more = take(0);
+        for (int k = 0; more; ++k) {
+            float m = -INFINITY, l = 0.f;
+            const int my = it.ni[t];
+#pragma unroll 1
+            for (int i = 0; i < my; ++i) {
+                if (ok) ok = wait_bar(&sh.s_full[t], (steps + i) & 1u, p.err);
                 __syncwarp();
                 tc_fence_after();
-                const float f = move ? ex2(m - mx) : 1.f;
-#pragma unroll
-                for (int c = 0; c < DP / 32; ++c) {
-                    float o[32];
-                    uint32_t w[32];
-                    tmem_ld32_now(to + 32u * c, o);
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) w[e] = __float_as_uint(o[e] * f);
-                    tmem_st32(to + 32u * c, w);
-                }
-                l *= f;
-            }
-            if (move) m = mx;
-            const float sub = m == -INFINITY ? 0.f : m - kShift;
-            float sum = 0.f;
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                uint32_t w[32];
-#pragma unroll
-                for (int d = 0; d < 2; ++d) {
+                const int cut = i >= it.m_first ? lim - (it.k_first + i * kKeys) : kKeys;  // columns from here on are not seen
+                float mx = -INFINITY;
+#pragma unroll 1
+                for (int c = 0; c < 4; ++c) {
                     float s[32];
-                    tmem_ld32_now(ts + 64u * c + 32u * d, s);
+                    tmem_ld32_now(ts + 32u * c, s);
                     if (cut < kKeys) {
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) s[e] = 64 * c + 32 * d + e < cut ? s[e] : -INFINITY;
+                        for (int e = 0; e < 32; ++e) s[e] = 32 * c + e < cut ? s[e] : -INFINITY;
+                    }
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) mx = fmaxf(mx, s[e]);
+                }
+                mx *= p.scale_log2;
+                const bool move = mx > m + 8.f;  // also from -inf; a first tile has no O yet
+                if (__any_sync(~0u, move && l > 0.f)) {
+                    if (ok) ok = wait_bar(&sh.o_full[t], (steps + i - 1) & 1u, p.err);
+                    __syncwarp();
+                    tc_fence_after();
+                    const float f = move ? ex2(m - mx) : 1.f;
+#pragma unroll 1
+                    for (int c = 0; c < DP / 32; ++c) {
+                        float o[32];
+                        uint32_t w[32];
+                        tmem_ld32_now(to + 32u * c, o);
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) w[e] = __float_as_uint(o[e] * f);
+                        tmem_st32(to + 32u * c, w);
+                    }
+                    l *= f;
+                }
+                if (move) m = mx;
+                const float sub = m == -INFINITY ? 0.f : m - kShift;
+                float sum = 0.f;
+#pragma unroll 1
+                for (int c = 0; c < 4; ++c) {
+                    float s[32];
+                    uint32_t w[16];
+                    tmem_ld32_now(ts + 32u * c, s);
+                    if (cut < kKeys) {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) s[e] = 32 * c + e < cut ? s[e] : -INFINITY;
                     }
 #pragma unroll
                     for (int e = 0; e < 32; e += 2) {
                         const float a = ex2(fmaf(s[e], p.scale_log2, -sub)), b = ex2(fmaf(s[e + 1], p.scale_log2, -sub));
                         sum += a + b;
-                        w[16 * d + e / 2] = pack2<kBF16>(a, b);
+                        w[e / 2] = pack2<kBF16>(a, b);
+                    }
+                    tmem_st16(ts + 16u * c, w);
+                }
+                l += sum;
+                tmem_st_wait();
+                tc_fence_before();
+                mbar_arrive(&sh.p_full[t]);
+            }
+            steps += my;
+            if (my > 0) {
+                if (ok) ok = wait_bar(&sh.o_full[t], (steps - 1) & 1u, p.err);
+                __syncwarp();
+                tc_fence_after();
+            }
+            // what this block's output needs, before the next block's Q goes on its way
+            const size_t hrow = (size_t)token * p.Hq + head;
+            const size_t prow = (size_t)it.split * p.T * p.Hq + hrow;
+            T16* out = static_cast<T16*>(p.o) + (size_t)token * p.o_st + (size_t)head * p.o_sh;
+            const bool store = live, any_bad = sh.any_bad[k & 1] != 0;  // written before v_clean, which every PV waited for
+            const int see = lim, bad_lim = lim - (it.k_first + it.m_first * kKeys);
+            more = take(k + 1);
+            // l = 0: no key was seen (zeros), or every score was -inf (no softmax: NaN,
+            // which a merge settles where other splits have a sum).
+            const bool part = p.part_o != nullptr;
+            const float inv = l != 0.f ? 1.f / l : (!part && see > 0 ? NAN : 0.f);
+#pragma unroll 1
+            for (int c = 0; c < DP / 32; ++c) {
+                float o[32];
+                __syncwarp();
+                if (my > 0) tmem_ld32_now(to + 32u * c, o);
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] = my > 0 && l != 0.f ? o[e] * inv : inv;
+                if (any_bad) {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        if ((int)sh.bad[k & 1][1][32 * c + e] < bad_lim) o[e] += INFINITY;
+                        if ((int)sh.bad[k & 1][2][32 * c + e] < bad_lim) o[e] -= INFINITY;
+                        if ((int)sh.bad[k & 1][0][32 * c + e] < bad_lim) o[e] = NAN;
                     }
                 }
-                tmem_st32(ts + 32u * c, w);
-            }
-            l += sum;
-            tmem_st_wait();
-            tc_fence_before();
-            mbar_arrive(&sh.p_full[t]);
-        }
-        if (my > 0) {
-            if (ok) ok = mbar_wait(&sh.o_full[t], (uint32_t)(my - 1) & 1u, p.err);
-            __syncwarp();
-            tc_fence_after();
-        }
-        // l = 0: no key was seen (zeros), or every score was -inf (no softmax: NaN,
-        // which a merge settles where other splits have a sum).
-        const bool part = p.part_o != nullptr;
-        const float inv = l != 0.f ? 1.f / l : (!part && lim > 0 ? NAN : 0.f);
-        const size_t hrow = (size_t)(first + token) * p.Hq + head;
-        const bool any_bad = sh.any_bad != 0;  // written before v_clean, which every PV waited for
-#pragma unroll 1
-        for (int c = 0; c < DP / 32; ++c) {
-            float o[32];
-            __syncwarp();
-            if (my > 0) {
-                tmem_ld32_now(to + 32u * c, o);
+                if (!store) continue;
+                if (part) {
+                    float* dst = p.part_o + prow * p.D + 32 * c;
 #pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] = l != 0.f ? o[e] * inv : inv;
-            } else {
+                    for (int e = 0; e < 32; e += 4)
+                        if (32 * c + e < p.D)
+                            *reinterpret_cast<float4*>(dst + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                } else {
 #pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] = inv;
-            }
-            if (any_bad) {
-#pragma unroll
-                for (int e = 0; e < 32; ++e) {
-                    if (sh.bad[1][32 * c + e] < lim) o[e] += INFINITY;
-                    if (sh.bad[2][32 * c + e] < lim) o[e] -= INFINITY;
-                    if (sh.bad[0][32 * c + e] < lim) o[e] = NAN;
+                    for (int e = 0; e < 32; e += 8)
+                        if (32 * c + e < p.D)
+                            *reinterpret_cast<uint4*>(out + 32 * c + e) =
+                                make_uint4(pack2<kBF16>(o[e], o[e + 1]), pack2<kBF16>(o[e + 2], o[e + 3]),
+                                           pack2<kBF16>(o[e + 4], o[e + 5]), pack2<kBF16>(o[e + 6], o[e + 7]));
                 }
             }
-            if (live && part) {
-                float* dst = p.part_o + ((size_t)split * p.T * p.Hq + hrow) * p.D + 32 * c;
-#pragma unroll
-                for (int e = 0; e < 32; e += 4)
-                    if (32 * c + e < p.D) *reinterpret_cast<float4*>(dst + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-            } else if (live) {
-                T16* dst = static_cast<T16*>(p.o) + (size_t)(first + token) * p.o_st + (size_t)head * p.o_sh + 32 * c;
-#pragma unroll
-                for (int e = 0; e < 32; e += 8)
-                    if (32 * c + e < p.D)
-                        *reinterpret_cast<uint4*>(dst + e) =
-                            make_uint4(pack2<kBF16>(o[e], o[e + 1]), pack2<kBF16>(o[e + 2], o[e + 3]),
-                                       pack2<kBF16>(o[e + 4], o[e + 5]), pack2<kBF16>(o[e + 6], o[e + 7]));
+            if (store) {
+                const float l2 = l == 0.f ? -INFINITY : m - kShift + log2f(l);
+                if (part) p.part_l[prow] = l2;
+                else if (p.lse) p.lse[hrow] = l2 * 0.693147180559945309417f;
             }
-        }
-        if (live) {
-            const float l2 = l == 0.f ? -INFINITY : m - kShift + log2f(l);
-            if (part) p.part_l[(size_t)split * p.T * p.Hq + hrow] = l2;
-            else if (p.lse) p.lse[hrow] = l2 * 0.693147180559945309417f;
+            __syncwarp();
+            tc_fence_before();  // O is read before the next block's first PV, which p_full lets go
+            if (lane == 0) mbar_arrive(&sh.item_empty[k & 1]);
         }
     }
 
@@ -594,21 +751,21 @@ __global__ void __launch_bounds__(256) attn_merge_kernel(const MergeParams p) {
 int ceil_div(long long a, int b) { return (int)((a + b - 1) / b); }
 
 template <bool kBF16, int DP>
-cudaError_t launch_tile(const TileParams& p, int blocks, int Hk, int dev, cudaStream_t s) {
-    using L = TileLayout<DP>;
+cudaError_t launch_tile(const TileParams& p, int dev, cudaStream_t s) {
+    constexpr int kSmem = TileLayout<DP>::kShared + (int)sizeof(TileShared);
     auto fn = attn_tile_kernel<kBF16, DP>;
-    cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(fn), dev, L::kSmem);
+    cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(fn), dev, kSmem);
     if (e != cudaSuccess) return e;
-    fn<<<dim3(blocks, Hk, p.splits), kThreads, L::kSmem, s>>>(p);
+    const long long grid = (long long)p.blocks * p.Hk * p.splits;
+    if (grid > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
+    fn<<<(unsigned)grid, kThreads, kSmem, s>>>(p);
     return cudaGetLastError();
 }
 
-cudaError_t launch_tile_any(const AttnArgs& a, const TileParams& p, int blocks) {
+cudaError_t launch_tile_any(const AttnArgs& a, const TileParams& p) {
     if (a.D <= 64)
-        return a.dtype == DType::BF16 ? launch_tile<true, 64>(p, blocks, a.Hk, a.dev, a.stream)
-                                      : launch_tile<false, 64>(p, blocks, a.Hk, a.dev, a.stream);
-    return a.dtype == DType::BF16 ? launch_tile<true, 128>(p, blocks, a.Hk, a.dev, a.stream)
-                                  : launch_tile<false, 128>(p, blocks, a.Hk, a.dev, a.stream);
+        return a.dtype == DType::BF16 ? launch_tile<true, 64>(p, a.dev, a.stream) : launch_tile<false, 64>(p, a.dev, a.stream);
+    return a.dtype == DType::BF16 ? launch_tile<true, 128>(p, a.dev, a.stream) : launch_tile<false, 128>(p, a.dev, a.stream);
 }
 
 // Key splits of `blocks` x Hk CTAs over `keys` keys: enough to fill the SMs once,
@@ -682,6 +839,7 @@ cudaError_t launch_attn(const AttnArgs& a) {
         p.T = a.T;
         p.B = a.B;
         p.Hq = a.Hq;
+        p.Hk = a.Hk;
         p.G = a.G;
         p.D = a.D;
         p.causal = a.causal;
@@ -701,7 +859,8 @@ cudaError_t launch_attn(const AttnArgs& a) {
         x.splits = pl.prefix;
         x.part_o = plane_o;
         x.part_l = plane_l;
-        if ((e = launch_tile_any(a, x, row_blocks)) != cudaSuccess) return e;
+        x.blocks = row_blocks;
+        if ((e = launch_tile_any(a, x)) != cudaSuccess) return e;
     }
     if (pl.tile) {
         const bool part = pl.own + pl.prefix > 1;
@@ -712,8 +871,8 @@ cudaError_t launch_attn(const AttnArgs& a) {
         p.part_o = part ? plane_o + pl.prefix * rows * a.D : nullptr;
         p.part_l = part ? plane_l + pl.prefix * rows : nullptr;
         // every sequence may end inside a block
-        const int blocks = (int)std::min((long long)row_blocks + a.B, (long long)0x7fffffff);
-        if ((e = launch_tile_any(a, p, blocks)) != cudaSuccess) return e;
+        p.blocks = (int)std::min((long long)row_blocks + a.B, 0x7fffffffLL);
+        if ((e = launch_tile_any(a, p)) != cudaSuccess) return e;
         if (part) {
             MergeParams m{plane_o, plane_l, a.o, a.o_st, a.o_sh, a.lse, a.cu_q, a.kv_lens, a.T, a.B, a.Hq, a.D, a.causal,
                           a.prefix_len, pl.own + pl.prefix, a.page_size, a.max_pages, a.G, p.skip_rows};
