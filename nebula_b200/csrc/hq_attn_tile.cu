@@ -128,8 +128,26 @@ __device__ __forceinline__ uint64_t sw128_mn_desc(uint32_t addr) {
     return d;
 }
 
-// 32 columns of this warp's lanes; the wait is part of the statement, so nothing
-// that uses the registers can be moved before it.
+// All 128 columns of this warp's lanes, in four loads; the wait is part of the last
+// statement, which takes all registers, so nothing that uses them can be moved
+// before it.
+__device__ __forceinline__ void tmem_ld128_now(uint32_t taddr, float (&f)[128]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : "=f"(f[0]), "=f"(f[1]), "=f"(f[2]), "=f"(f[3]), "=f"(f[4]), "=f"(f[5]), "=f"(f[6]), "=f"(f[7]), "=f"(f[8]), "=f"(f[9]), "=f"(f[10]), "=f"(f[11]), "=f"(f[12]), "=f"(f[13]), "=f"(f[14]), "=f"(f[15]), "=f"(f[16]), "=f"(f[17]), "=f"(f[18]), "=f"(f[19]), "=f"(f[20]), "=f"(f[21]), "=f"(f[22]), "=f"(f[23]), "=f"(f[24]), "=f"(f[25]), "=f"(f[26]), "=f"(f[27]), "=f"(f[28]), "=f"(f[29]), "=f"(f[30]), "=f"(f[31])
+                 : "r"(taddr + 0u) : "memory");
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : "=f"(f[32]), "=f"(f[33]), "=f"(f[34]), "=f"(f[35]), "=f"(f[36]), "=f"(f[37]), "=f"(f[38]), "=f"(f[39]), "=f"(f[40]), "=f"(f[41]), "=f"(f[42]), "=f"(f[43]), "=f"(f[44]), "=f"(f[45]), "=f"(f[46]), "=f"(f[47]), "=f"(f[48]), "=f"(f[49]), "=f"(f[50]), "=f"(f[51]), "=f"(f[52]), "=f"(f[53]), "=f"(f[54]), "=f"(f[55]), "=f"(f[56]), "=f"(f[57]), "=f"(f[58]), "=f"(f[59]), "=f"(f[60]), "=f"(f[61]), "=f"(f[62]), "=f"(f[63])
+                 : "r"(taddr + 32u) : "memory");
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : "=f"(f[64]), "=f"(f[65]), "=f"(f[66]), "=f"(f[67]), "=f"(f[68]), "=f"(f[69]), "=f"(f[70]), "=f"(f[71]), "=f"(f[72]), "=f"(f[73]), "=f"(f[74]), "=f"(f[75]), "=f"(f[76]), "=f"(f[77]), "=f"(f[78]), "=f"(f[79]), "=f"(f[80]), "=f"(f[81]), "=f"(f[82]), "=f"(f[83]), "=f"(f[84]), "=f"(f[85]), "=f"(f[86]), "=f"(f[87]), "=f"(f[88]), "=f"(f[89]), "=f"(f[90]), "=f"(f[91]), "=f"(f[92]), "=f"(f[93]), "=f"(f[94]), "=f"(f[95])
+                 : "r"(taddr + 64u) : "memory");
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%128];\n\ttcgen05.wait::ld.sync.aligned;"
+                 : "=f"(f[96]), "=f"(f[97]), "=f"(f[98]), "=f"(f[99]), "=f"(f[100]), "=f"(f[101]), "=f"(f[102]), "=f"(f[103]), "=f"(f[104]), "=f"(f[105]), "=f"(f[106]), "=f"(f[107]), "=f"(f[108]), "=f"(f[109]), "=f"(f[110]), "=f"(f[111]), "=f"(f[112]), "=f"(f[113]), "=f"(f[114]), "=f"(f[115]), "=f"(f[116]), "=f"(f[117]), "=f"(f[118]), "=f"(f[119]), "=f"(f[120]), "=f"(f[121]), "=f"(f[122]), "=f"(f[123]), "=f"(f[124]), "=f"(f[125]), "=f"(f[126]), "=f"(f[127]),
+                   "+f"(f[0]), "+f"(f[1]), "+f"(f[2]), "+f"(f[3]), "+f"(f[4]), "+f"(f[5]), "+f"(f[6]), "+f"(f[7]), "+f"(f[8]), "+f"(f[9]), "+f"(f[10]), "+f"(f[11]), "+f"(f[12]), "+f"(f[13]), "+f"(f[14]), "+f"(f[15]), "+f"(f[16]), "+f"(f[17]), "+f"(f[18]), "+f"(f[19]), "+f"(f[20]), "+f"(f[21]), "+f"(f[22]), "+f"(f[23]), "+f"(f[24]), "+f"(f[25]), "+f"(f[26]), "+f"(f[27]), "+f"(f[28]), "+f"(f[29]), "+f"(f[30]), "+f"(f[31]), "+f"(f[32]), "+f"(f[33]), "+f"(f[34]), "+f"(f[35]), "+f"(f[36]), "+f"(f[37]), "+f"(f[38]), "+f"(f[39]), "+f"(f[40]), "+f"(f[41]), "+f"(f[42]), "+f"(f[43]), "+f"(f[44]), "+f"(f[45]), "+f"(f[46]), "+f"(f[47]), "+f"(f[48]), "+f"(f[49]), "+f"(f[50]), "+f"(f[51]), "+f"(f[52]), "+f"(f[53]), "+f"(f[54]), "+f"(f[55]), "+f"(f[56]), "+f"(f[57]), "+f"(f[58]), "+f"(f[59]), "+f"(f[60]), "+f"(f[61]), "+f"(f[62]), "+f"(f[63]), "+f"(f[64]), "+f"(f[65]), "+f"(f[66]), "+f"(f[67]), "+f"(f[68]), "+f"(f[69]), "+f"(f[70]), "+f"(f[71]), "+f"(f[72]), "+f"(f[73]), "+f"(f[74]), "+f"(f[75]), "+f"(f[76]), "+f"(f[77]), "+f"(f[78]), "+f"(f[79]), "+f"(f[80]), "+f"(f[81]), "+f"(f[82]), "+f"(f[83]), "+f"(f[84]), "+f"(f[85]), "+f"(f[86]), "+f"(f[87]), "+f"(f[88]), "+f"(f[89]), "+f"(f[90]), "+f"(f[91]), "+f"(f[92]), "+f"(f[93]), "+f"(f[94]), "+f"(f[95])
+                 : "r"(taddr + 96u) : "memory");
+}
+
+// 32 columns, likewise.
 __device__ __forceinline__ void tmem_ld32_now(uint32_t taddr, float (&f)[32]) {
     uint32_t r[32];
     asm volatile(
@@ -146,14 +164,13 @@ __device__ __forceinline__ void tmem_ld32_now(uint32_t taddr, float (&f)[32]) {
     for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(r[i]);
 }
 
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+__device__ __forceinline__ void tmem_ld16_now(uint32_t taddr, uint32_t (&r)[16]) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
-        "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
         : "memory");
 }
 
@@ -202,9 +219,9 @@ __device__ __forceinline__ int find_block(const TileParams& p, int want, int& bl
             bool ok = seq_rows(p.cu_q, s, p.T, first, n);
             if (ok && p.page_size) ok = len_ok(p.kv_lens[s], p.max_pages, p.page_size);
             if (!ok) bad_index(p.err);
-            else if ((long long)n * p.G > p.skip_rows) nb = (int)(((long long)n * p.G + 2 * kRows - 1) / (2 * kRows));
+            else if (n * p.G > p.skip_rows) nb = (int)(((unsigned)(n * p.G) + 2 * kRows - 1) / (2 * kRows));
         }
-        int incl = nb;
+        int incl = nb;  // n * G fits: n_tokens * n_heads does
 #pragma unroll 1
         for (int d = 1; d < 32; d <<= 1) {
             const int x = __shfl_up_sync(~0u, incl, d);
@@ -246,7 +263,7 @@ __device__ __forceinline__ bool make_item(const TileParams& p, int index, Item& 
     auto seen = [&](int r) { return keys_seen(it.len, it.n, min(r, R - 1) / p.G, causal); };
     const int end1 = (seen(it.row0 + 2 * kRows - 1) + kKeys - 1) / kKeys;
     const int end0 = (seen(it.row0 + kRows - 1) + kKeys - 1) / kKeys;
-    const int a = (int)((long long)end1 * split / p.splits), b = (int)((long long)end1 * (split + 1) / p.splits);
+    const int a = end1 * split / p.splits, b = end1 * (split + 1) / p.splits;  // end1 <= 2^24, splits <= 32
     it.ni[0] = max(0, min(b, end0) - a);
     it.ni[1] = it.row0 + kRows < R ? b - a : 0;
     it.k_first = a * kKeys;
@@ -255,33 +272,61 @@ __device__ __forceinline__ bool make_item(const TileParams& p, int index, Item& 
     return true;
 }
 
-// Whether one of the two 16-bit values of w is Inf or NaN.
+// Whether one of the eight 16-bit values of v is Inf or NaN: one step more in the
+// exponent's last place then reaches the sign's.
 template <bool kBF16>
-__device__ __forceinline__ bool not_finite(uint32_t w) {
-    constexpr uint32_t kExp = kBF16 ? 0x7F80u : 0x7C00u;
-    return (w & kExp) == kExp || (w >> 16 & kExp) == kExp;
+__device__ __forceinline__ bool not_finite(uint4 v) {
+    constexpr uint32_t kStep = kBF16 ? 0x00800080u : 0x04000400u, kAbs = 0x7FFF7FFFu;
+    return (((v.x & kAbs) + kStep) | ((v.y & kAbs) + kStep) | ((v.z & kAbs) + kStep) | ((v.w & kAbs) + kStep)) & 0x80008000u;
 }
 
-// Takes the values of w (dims d, d + 1 of key `key`) that are not finite out and
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ void fma2(float& x, float& y, float a, float b) {  // (x, y) = (x, y) a + b
+    asm("{\n\t.reg .b64 v, p, q;\n\tmov.b64 v, {%0, %1};\n\tmov.b64 p, {%2, %2};\n\tmov.b64 q, {%3, %3};\n\t"
+        "fma.rn.f32x2 v, v, p, q;\n\tmov.b64 {%0, %1}, v;\n\t}"
+        : "+f"(x), "+f"(y)
+        : "f"(a), "f"(b));
+}
+__device__ __forceinline__ void add2(float& x, float& y, float a, float b) {  // (x, y) += (a, b)
+    asm("{\n\t.reg .b64 v, p;\n\tmov.b64 v, {%0, %1};\n\tmov.b64 p, {%2, %3};\n\tadd.rn.f32x2 v, v, p;\n\t"
+        "mov.b64 {%0, %1}, v;\n\t}"
+        : "+f"(x), "+f"(y)
+        : "f"(a), "f"(b));
+}
+
+// A warpgroup's share of the registers that the block was launched with (168 a
+// thread): 80 + 2 x 208 <= 3 x 168.
+constexpr int kRegsLoad = 80, kRegsSoftmax = 208;
+template <int N>
+__device__ __forceinline__ void regs_down() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_up() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+// Takes the values of v (dims d .. d + 7 of key `key`) that are not finite out and
 // notes them.
 template <bool kBF16>
-__device__ __noinline__ uint32_t take_out(uint16_t (*bad)[128], int d, int key, uint32_t w) {
+__device__ __noinline__ void take_out(uint16_t (*bad)[128], int d, int key, uint4& v) {
     constexpr uint32_t kExp = kBF16 ? 0x7F80u : 0x7C00u;
-    for (int e = 0; e < 2; ++e) {
-        const uint32_t h = w >> (16 * e) & 0xFFFFu;
+    uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    for (int e = 0; e < 8; ++e) {
+        const int sh = 16 * (e & 1);
+        const uint32_t h = w[e >> 1] >> sh & 0xFFFFu;
         if ((h & kExp) != kExp) continue;
         const int kind = (h & 0x7FFFu) != kExp ? 0 : (h & 0x8000u) ? 2 : 1;
-        unsigned* word = reinterpret_cast<unsigned*>(&bad[kind][(d + e) & ~1]);
-        const int sh = 16 * ((d + e) & 1);
+        unsigned* word = reinterpret_cast<unsigned*>(&bad[kind][d + (e & ~1)]);
         unsigned old = *word;
         while ((int)(old >> sh & 0xFFFFu) > key) {
             const unsigned seen = atomicCAS(word, old, (old & ~(0xFFFFu << sh)) | (unsigned)key << sh);
             if (seen == old) break;
             old = seen;
         }
-        w &= ~(0xFFFFu << (16 * e));
+        w[e >> 1] &= ~(0xFFFFu << sh);
     }
-    return w;
+    v = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 template <bool kBF16, int DP>
@@ -339,6 +384,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
 
     if (warp == 3) {
         // -------------------------------------------------------- blocks
+        regs_down<kRegsLoad>();
         int index = (int)blockIdx.x;
         uint32_t asked = 0;
         for (int k = 0; ok;) {
@@ -378,6 +424,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
         __syncwarp();
     } else if (warp == 0) {
         // --------------------------------------------------------- loads
+        regs_down<kRegsLoad>();
         const int boxes = kKeys / p.box_rows;
         int use = 0;
         for (int k = 0; item_wait(k); ++k) {
@@ -416,6 +463,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
         for (int j = max(0, use - S); j < use; ++j) wait_bar(&sh.empty[j % S], (uint32_t)(j / S) & 1u, p.err);
     } else if (warp == 1) {
         // ----------------------------------------------------------- MMA
+        regs_down<kRegsLoad>();
         if (lane == 0) {
             const uint32_t ring_a = smem_u32(ring);
             uint32_t use = 0, cleaned = 0, loaded[2] = {0, 0}, done[2] = {0, 0};
@@ -474,12 +522,15 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
         // ----------------------------------------- V tiles under a mask
         // v_req comes once the tile's K has been used, so V's stage is in this use's
         // phase or the one before it, and stays until v_clean.
+        regs_down<kRegsLoad>();
         uint32_t use = 0, asked = 0;
         for (int k = 0; item_wait(k); ++k) {
             const Item it = sh.item[k & 1];
             if (it.stop) break;
             const int nt = max(it.ni[0], it.ni[1]);
-            const int lim_min = keys_seen(it.len, it.n, it.row0 / p.G, p.causal && !p.prefix_len);
+            const int causal = p.causal && !p.prefix_len, R = it.n * p.G;
+            const int lim_min = keys_seen(it.len, it.n, it.row0 / p.G, causal);
+            const int lim_max = keys_seen(it.len, it.n, (min(it.row0 + 2 * kRows, R) - 1) / p.G, causal);
             const int base = it.k_first + it.m_first * kKeys;
 #pragma unroll 1
             for (int i = it.m_first; i < nt; ++i) {
@@ -489,27 +540,24 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
                 __syncwarp();
                 const uint32_t vt = smem_u32(ring) + (vu % S) * L::kTile;
                 const int k0 = it.k_first + i * kKeys;
-                const int valid = min(kKeys, it.len - k0), lo = min(valid, max(0, lim_min - k0));
-                // 16-byte chunk c of row r of a block lies at chunk c ^ (r & 7)
-#pragma unroll 1
-                for (int x = lo * (DP / 8) + lane; x < kKeys * (DP / 8); x += 32) {
-                    const int r = x / (DP / 8), c = x % (DP / 8);
-                    const uint32_t at = vt + (c >> 3) * L::kBlkBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4);
-                    if (r >= valid) {
-                        sts128(at, make_uint4(0u, 0u, 0u, 0u));
-                        continue;
-                    }
+                // keys [lo, hi) are seen by some rows only, those behind by none
+                const int hi = min(kKeys, lim_max - k0), lo = min(hi, max(0, lim_min - k0));
+                constexpr int C = DP / 8, RS = 32 / C;  // 16-byte chunks of a row, rows of a step
+                const int c = lane % C;
+                // chunk c of row r of a block lies at chunk c ^ (r & 7)
+                const uint32_t col = vt + (c >> 3) * L::kBlkBytes;
+#pragma unroll 4
+                for (int r = lo + lane / C; r < hi; r += RS) {
+                    const uint32_t at = col + r * 128 + (((c & 7) ^ (r & 7)) << 4);
                     uint4 v = lds128(at);
-                    if (not_finite<kBF16>(v.x) || not_finite<kBF16>(v.y) || not_finite<kBF16>(v.z) || not_finite<kBF16>(v.w)) {
-                        const int key = k0 + r - base;
-                        v.x = take_out<kBF16>(sh.bad[k & 1], c * 8, key, v.x);
-                        v.y = take_out<kBF16>(sh.bad[k & 1], c * 8 + 2, key, v.y);
-                        v.z = take_out<kBF16>(sh.bad[k & 1], c * 8 + 4, key, v.z);
-                        v.w = take_out<kBF16>(sh.bad[k & 1], c * 8 + 6, key, v.w);
-                        sts128(at, v);
-                        sh.any_bad[k & 1] = 1;
-                    }
+                    if (!not_finite<kBF16>(v)) continue;
+                    take_out<kBF16>(sh.bad[k & 1], c * 8, k0 + r - base, v);
+                    sts128(at, v);
+                    sh.any_bad[k & 1] = 1;
                 }
+#pragma unroll 1
+                for (int r = hi + lane / C; r < kKeys; r += RS)
+                    sts128(col + r * 128 + (((c & 7) ^ (r & 7)) << 4), make_uint4(0u, 0u, 0u, 0u));
                 fence_async_smem();
                 mbar_arrive(&sh.v_clean);
             }
@@ -519,19 +567,19 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
         }
     } else {
         // ------------------------------------------ Q, softmax and output
+        regs_up<kRegsSoftmax>();
         const int t = (warp - 4) >> 2, i0 = (threadIdx.x - 128) & 127;
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
         const uint32_t ts = tmem + lanes + 128u * t, to = tmem + lanes + kColO + (uint32_t)DP * t;
         const int causal = p.causal && !p.prefix_len;
         uint32_t steps = 0;  // key tiles of this row tile so far
-        Item it{};
         bool live = false;
         int token = 0, head = 0, lim = 0;
         // Takes item k: this thread's row, and its row of Q into shared memory (the
         // MMAs of the item before have read theirs).
         auto take = [&](int k) {
             if (!item_wait(k)) return false;
-            it = sh.item[k & 1];
+            const Item& it = sh.item[k & 1];  // stays until this warp has arrived on item_empty
             if (it.stop) return false;
             const int R = it.n * p.G, r = it.row0 + t * kRows + i0;
             live = r < R;
@@ -540,12 +588,18 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
             token = it.first + tok;
             head = it.hk * p.G + (live ? r - tok * p.G : 0);
             if (it.ni[t] > 0) {
-                const T16* q = static_cast<const T16*>(p.q) + (size_t)token * p.q_st + (size_t)head * p.q_sh;
-                const uint32_t dst = smem_u32(qs) + t * L::kTile + i0 * 128;
-#pragma unroll
-                for (int c = 0; c < DP / 8; ++c) {
-                    const uint4 v = live && c * 8 < p.D ? ldg128_nc(q + c * 8) : make_uint4(0u, 0u, 0u, 0u);
-                    sts128(dst + (c >> 3) * L::kBlkBytes + (((c & 7) ^ (i0 & 7)) << 4), v);
+                // 16 lanes (DP 128) a row, so that a load takes whole lines; this warp's 32 rows
+                constexpr int C = DP / 8, RS = 32 / C;
+                const long long mine = live ? token * p.q_st + head * p.q_sh : -1;
+                const int c = lane % C, w0 = i0 & ~31;
+                const uint32_t dst = smem_u32(qs) + t * L::kTile + (c >> 3) * L::kBlkBytes;
+#pragma unroll 8
+                for (int i = 0; i < 32 / RS; ++i) {
+                    const int row = i * RS + lane / C;
+                    const long long off = __shfl_sync(~0u, mine, row);
+                    const uint4 v = off >= 0 && c * 8 < p.D ? ldg128_nc(static_cast<const T16*>(p.q) + off + c * 8)
+                                                            : make_uint4(0u, 0u, 0u, 0u);
+                    sts128(dst + (w0 + row) * 128 + (((c & 7) ^ (row & 7)) << 4), v);
                 }
                 fence_async_smem();
                 mbar_arrive(&sh.q_full[t]);
@@ -555,25 +609,24 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
         bool more = take(0);
         for (int k = 0; more; ++k) {
             float m = -INFINITY, l = 0.f;
-            const int my = it.ni[t];
+            const Item& it = sh.item[k & 1];
+            const int my = it.ni[t], k_first = it.k_first, m_first = it.m_first;
 #pragma unroll 1
             for (int i = 0; i < my; ++i) {
                 if (ok) ok = wait_bar(&sh.s_full[t], (steps + i) & 1u, p.err);
                 __syncwarp();
                 tc_fence_after();
-                const int cut = i >= it.m_first ? lim - (it.k_first + i * kKeys) : kKeys;  // columns from here on are not seen
-                float mx = -INFINITY;
-#pragma unroll 1
-                for (int c = 0; c < 4; ++c) {
-                    float s[32];
-                    tmem_ld32_now(ts + 32u * c, s);
-                    if (cut < kKeys) {
+                const int cut = i >= m_first ? lim - (k_first + i * kKeys) : kKeys;  // columns from here on are not seen
+                float s[128];
+                tmem_ld128_now(ts, s);
+                if (cut < kKeys) {
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) s[e] = 32 * c + e < cut ? s[e] : -INFINITY;
-                    }
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) mx = fmaxf(mx, s[e]);
+                    for (int e = 0; e < 128; ++e) s[e] = e < cut ? s[e] : -INFINITY;
                 }
+                float top[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+                for (int e = 4; e < 128; ++e) top[e & 3] = fmaxf(top[e & 3], s[e]);
+                float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
                 mx *= p.scale_log2;
                 const bool move = mx > m + 8.f;  // also from -inf; a first tile has no O yet
                 if (__any_sync(~0u, move && l > 0.f)) {
@@ -582,37 +635,33 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
                     tc_fence_after();
                     const float f = move ? ex2(m - mx) : 1.f;
 #pragma unroll 1
-                    for (int c = 0; c < DP / 32; ++c) {
-                        float o[32];
-                        uint32_t w[32];
-                        tmem_ld32_now(to + 32u * c, o);
+                    for (int c = 0; c < DP / 16; ++c) {
+                        uint32_t w[16];
+                        tmem_ld16_now(to + 16u * c, w);
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) w[e] = __float_as_uint(o[e] * f);
-                        tmem_st32(to + 32u * c, w);
+                        for (int e = 0; e < 16; ++e) w[e] = __float_as_uint(__uint_as_float(w[e]) * f);
+                        tmem_st16(to + 16u * c, w);
                     }
                     l *= f;
                 }
                 if (move) m = mx;
                 const float sub = m == -INFINITY ? 0.f : m - kShift;
-                float sum = 0.f;
-#pragma unroll 1
-                for (int c = 0; c < 4; ++c) {
-                    float s[32];
-                    uint32_t w[16];
-                    tmem_ld32_now(ts + 32u * c, s);
-                    if (cut < kKeys) {
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) s[e] = 32 * c + e < cut ? s[e] : -INFINITY;
-                    }
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t w[16];
 #pragma unroll
                     for (int e = 0; e < 32; e += 2) {
-                        const float a = ex2(fmaf(s[e], p.scale_log2, -sub)), b = ex2(fmaf(s[e + 1], p.scale_log2, -sub));
-                        sum += a + b;
-                        w[e / 2] = pack2<kBF16>(a, b);
+                        float x = s[32 * c + e], y = s[32 * c + e + 1];
+                        fma2(x, y, p.scale_log2, -sub);
+                        x = ex2(x);
+                        y = ex2(y);
+                        add2(sum[e & 2], sum[(e & 2) + 1], x, y);
+                        w[e / 2] = pack2<kBF16>(x, y);
                     }
                     tmem_st16(ts + 16u * c, w);
                 }
-                l += sum;
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                 tmem_st_wait();
                 tc_fence_before();
                 mbar_arrive(&sh.p_full[t]);
@@ -628,7 +677,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
             const size_t prow = (size_t)it.split * p.T * p.Hq + hrow;
             T16* out = static_cast<T16*>(p.o) + (size_t)token * p.o_st + (size_t)head * p.o_sh;
             const bool store = live, any_bad = sh.any_bad[k & 1] != 0;  // written before v_clean, which every PV waited for
-            const int see = lim, bad_lim = lim - (it.k_first + it.m_first * kKeys);
+            const int see = lim, bad_lim = lim - (k_first + m_first * kKeys);
             more = take(k + 1);
             // l = 0: no key was seen (zeros), or every score was -inf (no softmax: NaN,
             // which a merge settles where other splits have a sum).
