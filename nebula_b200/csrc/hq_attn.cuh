@@ -26,20 +26,23 @@ __device__ __forceinline__ void bad_index(unsigned* err) {
 }
 
 // mbar_wait (hq_common.cuh) in few instructions: kernels that wait in many places
-// and run for microseconds are bound by fetching their code.
-__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, unsigned* err) {
+// and run for microseconds are bound by fetching their code.  A wait of the block
+// that gives up records kDevTimeout and sets *gave_up (shared memory); those that
+// come after it give up at once where they would wait.
+__device__ __forceinline__ void wait_bar(uint64_t* bar, uint32_t parity, int* gave_up, unsigned* err) {
     unsigned long long t0 = 0;
 #pragma unroll 1
-    for (unsigned n = 0; !mbar_try_wait(bar, parity); ++n) {
+    for (unsigned n = 1; !mbar_try_wait(bar, parity); ++n) {
         if (n & 63u) continue;
+        if (*reinterpret_cast<volatile int*>(gave_up)) return;
         const unsigned long long t = globaltimer_ns();
-        if (n == 0) t0 = t;
+        if (t0 == 0) t0 = t;
         else if (t - t0 > kWaitBudgetNs) {
             record_error(err, kDevTimeout);
-            return false;
+            *reinterpret_cast<volatile int*>(gave_up) = 1;
+            return;
         }
     }
-    return true;
 }
 
 }  // namespace hq

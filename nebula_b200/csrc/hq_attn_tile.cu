@@ -17,26 +17,26 @@
 // since it was last moved: until then the sums stay exact in fp32 and P, at most
 // 2^8 (2^14 in fp16, see kShift), in range.
 //
-// CTAs stay on their SM: warp 3 asks the launch hardware for the next block of
+// CTAs stay on their SM: warp 0 asks the launch hardware for the next block of
 // the grid (cluster launch control) and works out its rows and keys while the
 // others are on the current one; the next block's Q and first keys are loaded, and
 // its first S computed, while this one's output is written.
-//   warp 0        loads: one TMA box per 64 dims and up to 128 keys of a page
-//                 (page numbers from the table), K and V tiles alternate in a ring
-//   warp 1        issues the MMAs (one thread); owns the tensor memory
-//   warp 2        V tiles that some row does not see in full: rows behind the last
+//   warp 0        the blocks, and their loads: one TMA box per 64 dims and up to 128
+//                 keys of a page (page numbers from the table), K and V tiles
+//                 alternate in a ring
+//   warp 1        issues the MMAs; owns the tensor memory
+//   warps 2, 3    V tiles that some row does not see in full: rows behind the last
 //                 key are zeroed (0 x NaN would reach the sum), and values that
 //                 are not finite are taken out and noted, to be put back into the
 //                 rows that see them
-//   warp 3        the blocks
 //   warps 4-7, 8-11  Q, softmax and output of tile 0, tile 1: thread = row = lane
 //                 of tensor memory
 // Bound: the tensor cores and the exponentials (16 a clock and SM) alike take
 // 1024 cycles for a tile's 128 rows x 128 keys x 128 dims.
 // Work is split over the keys when there are few rows: every split writes its
 // normalised fp32 output and log2 of its sum, merged by attn_merge_kernel.
-// Every wait is bounded (hq_common.cuh): after one that gave up a role runs on to
-// the end of its block without waiting, and takes no other.
+// Every wait is bounded: after one that gave up all roles run to the end of their
+// block without waiting, and take no other.
 #include "hq_attn.cuh"
 #include "hq_tmap.h"
 
@@ -106,6 +106,7 @@ struct TileShared {
     // first key, counted from the block's first masked tile, whose value in a dim is
     // NaN, +Inf, -Inf; 0xFFFF: none (masked tiles span less than 512 keys)
     int any_bad[2];
+    int gave_up;
     uint16_t bad[2][3][128];
 };
 
@@ -280,6 +281,27 @@ __device__ __forceinline__ bool not_finite(uint4 v) {
     return (((v.x & kAbs) + kStep) | ((v.y & kAbs) + kStep) | ((v.z & kAbs) + kStep) | ((v.w & kAbs) + kStep)) & 0x80008000u;
 }
 
+// D (tensor memory) [+]= A x B: A from shared memory, A from tensor memory.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+                 "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+                 : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+                 "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+                 : "memory");
+}
+
+// One lane of the warp (all lanes call it together).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t e;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e)::"memory");
+    return e != 0;
+}
+
 // Two fp32 operations in one instruction.
 __device__ __forceinline__ void fma2(float& x, float& y, float a, float b) {  // (x, y) = (x, y) a + b
     asm("{\n\t.reg .b64 v, p, q;\n\tmov.b64 v, {%0, %1};\n\tmov.b64 p, {%2, %2};\n\tmov.b64 q, {%3, %3};\n\t"
@@ -358,10 +380,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
                 mbar_init(&sh.p_full[t], 128);
                 mbar_init(&sh.o_full[t], 1);
                 mbar_init(&sh.item_full[t], 1);
-                mbar_init(&sh.item_empty[t], 11);  // warps 0-2 and 4-11
+                mbar_init(&sh.item_empty[t], 11);  // all warps but warp 0
             }
             mbar_init(&sh.v_req, 1);
-            mbar_init(&sh.v_clean, 32);
+            mbar_init(&sh.v_clean, 64);
             mbar_init(&sh.next, 1);
             fence_mbarrier_init();
             fence_async_smem();
@@ -372,27 +394,31 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
     } else if (warp == 2) {
         for (int i = lane; i < 2 * 3 * 64; i += 32) reinterpret_cast<unsigned*>(&sh.bad[0][0][0])[i] = ~0u;
         if (lane < 2) sh.any_bad[lane] = 0;
+        if (lane == 2) sh.gave_up = 0;
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sh.tmem;
-    bool ok = true;  // no wait of this role has given up
+    auto wait = [&](uint64_t* bar, uint32_t parity) { wait_bar(bar, parity & 1u, &sh.gave_up, p.err); };
+    auto gave_up = [&] { return *reinterpret_cast<volatile int*>(&sh.gave_up) != 0; };
+    // Item k of this CTA is in slot k & 1; false: there is none.
+    auto item_wait = [&](int k) {
+        wait(&sh.item_full[k & 1], (uint32_t)(k >> 1));
+        return !gave_up() && !sh.item[k & 1].stop;
+    };
 
-    // Item k of this CTA is in slot k & 1.
-    auto item_wait = [&](int k) { return ok && (ok = wait_bar(&sh.item_full[k & 1], (uint32_t)(k >> 1) & 1u, p.err)); };
-
-    if (warp == 3) {
-        // -------------------------------------------------------- blocks
+    if (warp == 0) {
+        // ----------------------------------------------- blocks and loads
         regs_down<kRegsLoad>();
-        int index = (int)blockIdx.x;
-        uint32_t asked = 0;
-        for (int k = 0; ok;) {
+        const int boxes = kKeys / p.box_rows;
+        int index = (int)blockIdx.x, use = 0;
+        for (int k = 0, asked = 0;; ++asked) {
             if (lane == 0) next_block_request(&sh.next_block, &sh.next);
             __syncwarp();
             Item it;
             if (make_item(p, index, it)) {
-                if (k >= 2) ok = wait_bar(&sh.item_empty[k & 1], (uint32_t)((k - 2) >> 1) & 1u, p.err);
+                if (k >= 2) wait(&sh.item_empty[k & 1], (uint32_t)((k - 2) >> 1));
                 __syncwarp();
                 if (sh.any_bad[k & 1]) {
                     for (int i = lane; i < 3 * 64; i += 32) reinterpret_cast<unsigned*>(&sh.bad[k & 1][0][0])[i] = ~0u;
@@ -405,120 +431,122 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
                 }
                 __syncwarp();
                 ++k;
-            }
-            // also when a wait gave up: the answer lands before the CTA exits
-            const bool told = wait_bar(&sh.next, asked++ & 1u, p.err);
-            index = told ? next_block_answer(&sh.next_block) : -1;
-            ok = ok && told;
-            __syncwarp();
-            if (lane == 0) fence_async_smem();  // the answer is read before the next one is written
-            if (index >= 0) continue;
-            if (ok && k >= 2) ok = wait_bar(&sh.item_empty[k & 1], (uint32_t)((k - 2) >> 1) & 1u, p.err);
-            __syncwarp();
-            if (lane == 0) {
-                sh.item[k & 1].stop = 1;
-                mbar_arrive(&sh.item_full[k & 1]);
-            }
-            break;
-        }
-        __syncwarp();
-    } else if (warp == 0) {
-        // --------------------------------------------------------- loads
-        regs_down<kRegsLoad>();
-        const int boxes = kKeys / p.box_rows;
-        int use = 0;
-        for (int k = 0; item_wait(k); ++k) {
-            const Item it = sh.item[k & 1];
-            if (it.stop) break;
-            const int nt = max(it.ni[0], it.ni[1]);
+                const int nt = max(it.ni[0], it.ni[1]);
 #pragma unroll 1
-            for (int i = 0; i < 2 * nt; ++i, ++use) {  // K, V of tile 0, of tile 1, ...
-                const int k0 = it.k_first + (i >> 1) * kKeys, slot = use % S;
-                const int live = min(boxes, (it.len - k0 + p.box_rows - 1) / p.box_rows);
-                if (ok) ok = wait_bar(&sh.empty[slot], ((uint32_t)(use / S) & 1u) ^ 1u, p.err);
-                uint8_t* dst = ring + slot * L::kTile;
-                if (lane == 0) mbar_arrive_expect_tx(&sh.full[slot], (uint32_t)(live * L::kBlk * p.box_rows * 128));
-                __syncwarp();
-                if (lane < live * L::kBlk) {
-                    const int box = lane / L::kBlk, blk = lane % L::kBlk;
-                    const int key = k0 + box * p.box_rows;
-                    int token = it.first + key, page = 0;
-                    if (p.page_size) {
-                        token = key & (p.page_size - 1);
-                        page = it.table[key / p.page_size];
-                        if (!page_ok(page, p.num_pages)) {
-                            bad_index(p.err);
-                            page = p.num_pages;  // out of range: the box reads zeros
+                for (int i = 0; i < 2 * nt; ++i, ++use) {  // K, V of tile 0, of tile 1, ...
+                    const int k0 = it.k_first + (i >> 1) * kKeys, slot = use % S;
+                    const int live = min(boxes, (it.len - k0 + p.box_rows - 1) / p.box_rows);
+                    wait(&sh.empty[slot], ((uint32_t)(use / S) & 1u) ^ 1u);
+                    uint8_t* dst = ring + slot * L::kTile;
+                    if (lane == 0) mbar_arrive_expect_tx(&sh.full[slot], (uint32_t)(live * L::kBlk * p.box_rows * 128));
+                    __syncwarp();
+                    if (lane < live * L::kBlk) {
+                        const int box = lane / L::kBlk, blk = lane % L::kBlk;
+                        const int key = k0 + box * p.box_rows;
+                        int token = it.first + key, page = 0;
+                        if (p.page_size) {
+                            token = key & (p.page_size - 1);
+                            page = it.table[key / p.page_size];
+                            if (!page_ok(page, p.num_pages)) {
+                                bad_index(p.err);
+                                page = p.num_pages;  // out of range: the box reads zeros
+                            }
                         }
+                        tma_load_4d(dst + blk * L::kBlkBytes + box * p.box_rows * 128, i & 1 ? &p.v_map : &p.k_map, blk * 64,
+                                    token, it.hk, page, &sh.full[slot]);
                     }
-                    tma_load_4d(dst + blk * L::kBlkBytes + box * p.box_rows * 128, i & 1 ? &p.v_map : &p.k_map, blk * 64,
-                                token, it.hk, page, &sh.full[slot]);
                 }
             }
+            wait(&sh.next, (uint32_t)asked);
+            __syncwarp();
+            index = gave_up() ? -1 : next_block_answer(&sh.next_block);
+            if (index < 0) {
+                if (k >= 2) wait(&sh.item_empty[k & 1], (uint32_t)((k - 2) >> 1));
+                __syncwarp();
+                if (lane == 0) {
+                    sh.item[k & 1].stop = 1;
+                    mbar_arrive(&sh.item_full[k & 1]);
+                }
+                break;
+            }
+            if (lane == 0) fence_async_smem();  // the answer is read before the next one is written
+        }
+        __syncwarp();
+        // Every stage filled here has been consumed (its commits have landed) before exit.
+#pragma unroll 1
+        for (int j = max(0, use - S); j < use; ++j) wait(&sh.empty[j % S], (uint32_t)(j / S));
+    } else if (warp == 1) {
+        // ----------------------------------------------------------- MMAs
+        // The whole warp walks the loops, on values that the compiler can see to be
+        // the same in all lanes, and one lane issues: operands then stay in uniform
+        // registers.  (One thread in a branch of its own took 60 to 90 cycles an MMA,
+        // more than the MMA.)
+        regs_down<kRegsLoad>();
+        auto same = [](int x) { return __shfl_sync(~0u, x, 0); };
+        const uint32_t tm = (uint32_t)same((int)tmem), ring_a = smem_u32(ring), q_a = smem_u32(qs);
+        uint32_t use = 0, cleaned = 0, loaded[2] = {0, 0}, done[2] = {0, 0};
+        for (int k = 0; item_wait(k); ++k) {
+            const int n0 = same(sh.item[k & 1].ni[0]), n1 = same(sh.item[k & 1].ni[1]), m_first = same(sh.item[k & 1].m_first);
+            const int nt = max(n0, n1);
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.item_empty[k & 1]);
-        }
-        // Every stage filled here has been consumed (its commit has landed) before exit.
+            // Step i: O += P V of key tile i, S = Q K^T of tile i + 1, for both row tiles.
 #pragma unroll 1
-        for (int j = max(0, use - S); j < use; ++j) wait_bar(&sh.empty[j % S], (uint32_t)(j / S) & 1u, p.err);
-    } else if (warp == 1) {
-        // ----------------------------------------------------------- MMA
-        regs_down<kRegsLoad>();
-        if (lane == 0) {
-            const uint32_t ring_a = smem_u32(ring);
-            uint32_t use = 0, cleaned = 0, loaded[2] = {0, 0}, done[2] = {0, 0};
-            for (int k = 0; item_wait(k); ++k) {
-                if (sh.item[k & 1].stop) break;
-                const int n0 = sh.item[k & 1].ni[0], n1 = sh.item[k & 1].ni[1], m_first = sh.item[k & 1].m_first;
-                const int nt = max(n0, n1);
-                mbar_arrive(&sh.item_empty[k & 1]);
-                // step i: O += P V of key tile i, S = Q K^T of tile i + 1
-#pragma unroll 1
-                for (int i = -1; i < nt; ++i) {
-                    const uint32_t vu = use + 2 * i + 1, ku = vu + 1;
-                    if (i >= 0) {
-                        if (ok) ok = wait_bar(&sh.full[vu % S], (vu / S) & 1u, p.err);
-                        if (i >= m_first && ok) ok = wait_bar(&sh.v_clean, cleaned++ & 1u, p.err);
-                    }
-                    if (i + 1 < nt && ok) ok = wait_bar(&sh.full[ku % S], (ku / S) & 1u, p.err);
-                    const uint64_t vd = sw128_mn_desc(ring_a + (vu % S) * L::kTile);
-                    const uint64_t kd = sw128_kmajor_desc(ring_a + (ku % S) * L::kTile);
-#pragma unroll 1
-                    for (int t = 0; t < 2; ++t) {
-                        const int my = t ? n1 : n0;
-                        const uint32_t sp = tmem + 128u * t;
-                        if (i >= 0 && i < my) {
-                            if (ok) ok = wait_bar(&sh.p_full[t], done[t]++ & 1u, p.err);
-                            tc_fence_after();
+            for (int i = -1; i < nt; ++i) {
+                const uint32_t vu = use + 2 * i + 1, ku = vu + 1;
+                const uint32_t va = ring_a + (vu % S) * L::kTile, ka = ring_a + (ku % S) * L::kTile;
+                if (i >= 0) {
+                    wait(&sh.full[vu % S], vu / S);
+                    if (i >= m_first) wait(&sh.v_clean, cleaned++);
+                }
+                if (i + 1 < nt) wait(&sh.full[ku % S], ku / S);
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const int my = t ? n1 : n0;
+                    const uint32_t sp = tm + 128u * t, op = tm + kColO + (uint32_t)DP * t;
+                    if (i >= 0 && i < my) {
+                        wait(&sh.p_full[t], done[t]++);
+                        __syncwarp();
+                        tc_fence_after();
+                        if (elect_one()) {
+                            const uint64_t vd = sw128_mn_desc(va);
 #pragma unroll
                             for (int j = 0; j < kKeys / 16; ++j)
-                                umma_ts_f16(tmem + kColO + (uint32_t)DP * t, sp + 8u * j, vd + j * (2048 >> 4), kIdescO,
-                                            (i | j) != 0);
+                                mma_ts(op, sp + 8u * j, vd + j * (2048 >> 4), kIdescO, (i | j) != 0);
                             umma_commit(&sh.o_full[t]);
                         }
-                        if (i + 1 < my) {
-                            if (i < 0 && ok) ok = wait_bar(&sh.q_full[t], loaded[t]++ & 1u, p.err);
-                            tc_fence_after();
-                            const uint64_t qd = sw128_kmajor_desc(smem_u32(qs) + t * L::kTile);
+                        __syncwarp();
+                    }
+                    if (i + 1 < my) {
+                        if (i < 0) {
+                            wait(&sh.q_full[t], loaded[t]++);
+                            __syncwarp();
+                        }
+                        tc_fence_after();
+                        if (elect_one()) {
+                            const uint64_t qd = sw128_kmajor_desc(q_a + t * L::kTile), kd = sw128_kmajor_desc(ka);
 #pragma unroll
                             for (int j = 0; j < DP / 16; ++j) {
                                 const uint32_t off = ((j >> 2) * L::kBlkBytes + (j & 3) * 32) >> 4;
-                                umma_f16(sp, qd + off, kd + off, kIdescS, j != 0);
+                                mma_ss(sp, qd + off, kd + off, kIdescS, j != 0);
                             }
                             umma_commit(&sh.s_full[t]);
                         }
+                        __syncwarp();
                     }
+                }
+                if (elect_one()) {
                     if (i >= 0) umma_commit(&sh.empty[vu % S]);
                     if (i + 1 < nt) {
                         umma_commit(&sh.empty[ku % S]);
                         if (i + 1 >= m_first) mbar_arrive(&sh.v_req);
                     }
                 }
-                use += 2 * nt;
+                __syncwarp();
             }
+            use += 2 * nt;
         }
-        __syncwarp();
-    } else if (warp == 2) {
+    } else if (warp < 4) {
         // ----------------------------------------- V tiles under a mask
         // v_req comes once the tile's K has been used, so V's stage is in this use's
         // phase or the one before it, and stays until v_clean.
@@ -526,7 +554,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
         uint32_t use = 0, asked = 0;
         for (int k = 0; item_wait(k); ++k) {
             const Item it = sh.item[k & 1];
-            if (it.stop) break;
             const int nt = max(it.ni[0], it.ni[1]);
             const int causal = p.causal && !p.prefix_len, R = it.n * p.G;
             const int lim_min = keys_seen(it.len, it.n, it.row0 / p.G, causal);
@@ -535,19 +562,19 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
 #pragma unroll 1
             for (int i = it.m_first; i < nt; ++i) {
                 const uint32_t vu = use + 2 * i + 1;
-                if (ok) ok = wait_bar(&sh.v_req, asked++ & 1u, p.err);
-                if (ok) ok = wait_bar(&sh.full[vu % S], (vu / S) & 1u, p.err);
+                wait(&sh.v_req, asked++);
+                wait(&sh.full[vu % S], (vu / S));
                 __syncwarp();
                 const uint32_t vt = smem_u32(ring) + (vu % S) * L::kTile;
                 const int k0 = it.k_first + i * kKeys;
                 // keys [lo, hi) are seen by some rows only, those behind by none
                 const int hi = min(kKeys, lim_max - k0), lo = min(hi, max(0, lim_min - k0));
-                constexpr int C = DP / 8, RS = 32 / C;  // 16-byte chunks of a row, rows of a step
-                const int c = lane % C;
+                constexpr int C = DP / 8, RS = 64 / C;  // 16-byte chunks of a row, rows of a step
+                const int x = threadIdx.x - 64, c = x % C;
                 // chunk c of row r of a block lies at chunk c ^ (r & 7)
                 const uint32_t col = vt + (c >> 3) * L::kBlkBytes;
 #pragma unroll 4
-                for (int r = lo + lane / C; r < hi; r += RS) {
+                for (int r = lo + x / C; r < hi; r += RS) {
                     const uint32_t at = col + r * 128 + (((c & 7) ^ (r & 7)) << 4);
                     uint4 v = lds128(at);
                     if (!not_finite<kBF16>(v)) continue;
@@ -556,7 +583,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
                     sh.any_bad[k & 1] = 1;
                 }
 #pragma unroll 1
-                for (int r = hi + lane / C; r < kKeys; r += RS)
+                for (int r = hi + x / C; r < kKeys; r += RS)
                     sts128(col + r * 128 + (((c & 7) ^ (r & 7)) << 4), make_uint4(0u, 0u, 0u, 0u));
                 fence_async_smem();
                 mbar_arrive(&sh.v_clean);
@@ -580,7 +607,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
         auto take = [&](int k) {
             if (!item_wait(k)) return false;
             const Item& it = sh.item[k & 1];  // stays until this warp has arrived on item_empty
-            if (it.stop) return false;
             const int R = it.n * p.G, r = it.row0 + t * kRows + i0;
             live = r < R;
             const int tok = min(r, R - 1) / p.G;  // rows behind the last see what it sees
@@ -613,7 +639,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
             const int my = it.ni[t], k_first = it.k_first, m_first = it.m_first;
 #pragma unroll 1
             for (int i = 0; i < my; ++i) {
-                if (ok) ok = wait_bar(&sh.s_full[t], (steps + i) & 1u, p.err);
+                wait(&sh.s_full[t], (steps + i));
                 __syncwarp();
                 tc_fence_after();
                 const int cut = i >= m_first ? lim - (k_first + i * kKeys) : kKeys;  // columns from here on are not seen
@@ -630,7 +656,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
                 mx *= p.scale_log2;
                 const bool move = mx > m + 8.f;  // also from -inf; a first tile has no O yet
                 if (__any_sync(~0u, move && l > 0.f)) {
-                    if (ok) ok = wait_bar(&sh.o_full[t], (steps + i - 1) & 1u, p.err);
+                    wait(&sh.o_full[t], (steps + i - 1));
                     __syncwarp();
                     tc_fence_after();
                     const float f = move ? ex2(m - mx) : 1.f;
@@ -668,7 +694,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
             }
             steps += my;
             if (my > 0) {
-                if (ok) ok = wait_bar(&sh.o_full[t], (steps - 1) & 1u, p.err);
+                wait(&sh.o_full[t], (steps - 1));
                 __syncwarp();
                 tc_fence_after();
             }
