@@ -98,7 +98,7 @@ struct Item {
 };
 
 struct TileShared {
-    uint64_t full[8], empty[8], q_full[2], s_full[2], p_full[2], o_full[2], v_req, v_clean;
+    uint64_t full[8], empty[8], q_full[2], s_full[2], p_full[2][2], o_full[2], v_req, v_clean;
     uint64_t item_full[2], item_empty[2], next;
     uint4 next_block;
     Item item[2];
@@ -317,8 +317,8 @@ __device__ __forceinline__ void add2(float& x, float& y, float a, float b) {  //
 }
 
 // A warpgroup's share of the registers that the block was launched with (168 a
-// thread): 80 + 2 x 208 <= 3 x 168.
-constexpr int kRegsLoad = 80, kRegsSoftmax = 208;
+// thread): 72 + 2 x 216 = 3 x 168.
+constexpr int kRegsLoad = 72, kRegsSoftmax = 216;
 template <int N>
 __device__ __forceinline__ void regs_down() {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
@@ -377,7 +377,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
             for (int t = 0; t < 2; ++t) {
                 mbar_init(&sh.q_full[t], 128);
                 mbar_init(&sh.s_full[t], 1);
-                mbar_init(&sh.p_full[t], 128);
+                mbar_init(&sh.p_full[t][0], 128);
+                mbar_init(&sh.p_full[t][1], 128);
                 mbar_init(&sh.o_full[t], 1);
                 mbar_init(&sh.item_full[t], 1);
                 mbar_init(&sh.item_empty[t], 11);  // all warps but warp 0
@@ -505,17 +506,22 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
                     const int my = t ? n1 : n0;
                     const uint32_t sp = tm + 128u * t, op = tm + kColO + (uint32_t)DP * t;
                     if (i >= 0 && i < my) {
-                        wait(&sh.p_full[t], done[t]++);
-                        __syncwarp();
-                        tc_fence_after();
-                        if (elect_one()) {
-                            const uint64_t vd = sw128_mn_desc(va);
+                        // P comes in halves of 64 keys
 #pragma unroll
-                            for (int j = 0; j < kKeys / 16; ++j)
-                                mma_ts(op, sp + 8u * j, vd + j * (2048 >> 4), kIdescO, (i | j) != 0);
-                            umma_commit(&sh.o_full[t]);
+                        for (int h = 0; h < 2; ++h) {
+                            wait(&sh.p_full[t][h], done[t]);
+                            __syncwarp();
+                            tc_fence_after();
+                            if (elect_one()) {
+                                const uint64_t vd = sw128_mn_desc(va);
+#pragma unroll
+                                for (int j = 4 * h; j < 4 * h + 4; ++j)
+                                    mma_ts(op, sp + 8u * j, vd + j * (2048 >> 4), kIdescO, (i | j) != 0);
+                                if (h) umma_commit(&sh.o_full[t]);
+                            }
+                            __syncwarp();
                         }
-                        __syncwarp();
+                        ++done[t];
                     }
                     if (i + 1 < my) {
                         if (i < 0) {
@@ -686,11 +692,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
                         w[e / 2] = pack2<kBF16>(x, y);
                     }
                     tmem_st16(ts + 16u * c, w);
+                    if (c & 1) {  // half of P is there
+                        tmem_st_wait();
+                        tc_fence_before();
+                        mbar_arrive(&sh.p_full[t][c >> 1]);
+                    }
                 }
                 l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                tmem_st_wait();
-                tc_fence_before();
-                mbar_arrive(&sh.p_full[t]);
             }
             steps += my;
             if (my > 0) {
