@@ -25,6 +25,21 @@ __device__ __forceinline__ void bad_index(unsigned* err) {
     if (err) atomicCAS(err, 0u, (unsigned)kDevBadIndex);
 }
 
+// 16-byte asynchronous copy into shared memory; zeros where there is nothing to copy.
+__device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, bool have) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(have ? 16 : 0) : "memory");
+}
+
+// Whether the phase is over, without waiting.
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok)
+                 : "r"(smem_u32(bar)), "r"(parity)
+                 : "memory");
+    return ok != 0;
+}
+
 // mbar_wait (hq_common.cuh) in few instructions: kernels that wait in many places
 // and run for microseconds are bound by fetching their code.  A wait of the block
 // that gives up records kDevTimeout and sets *gave_up (shared memory); those that

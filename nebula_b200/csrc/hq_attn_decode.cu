@@ -108,9 +108,6 @@ __device__ __forceinline__ void next_unit(const DecodeParams& p, Place& at) {
     while (at.seq.tiles == 0);
 }
 
-__device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, bool have) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(have ? 16 : 0) : "memory");
-}
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_async_wait() {

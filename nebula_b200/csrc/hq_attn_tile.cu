@@ -606,48 +606,63 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
         const uint32_t ts = tmem + lanes + 128u * t, to = tmem + lanes + kColO + (uint32_t)DP * t;
         const int causal = p.causal && !p.prefix_len;
         uint32_t steps = 0;  // key tiles of this row tile so far
-        bool live = false;
-        int token = 0, head = 0, lim = 0;
-        // Takes item k: this thread's row, and its row of Q into shared memory (the
-        // MMAs of the item before have read theirs).
+        // Takes item k: this thread's row, and requests its warp's rows of Q (the MMAs of
+        // the item before have read theirs).  16 lanes (DP 128) a row, so that a request
+        // takes whole lines; rows behind the last and dims behind D are zeros.
+        int next_token = 0, next_head = 0, next_lim = 0;
+        bool next_live = false;
         auto take = [&](int k) {
             if (!item_wait(k)) return false;
             const Item& it = sh.item[k & 1];  // stays until this warp has arrived on item_empty
             const int R = it.n * p.G, r = it.row0 + t * kRows + i0;
-            live = r < R;
+            next_live = r < R;
             const int tok = min(r, R - 1) / p.G;  // rows behind the last see what it sees
-            lim = keys_seen(it.len, it.n, tok, causal);
-            token = it.first + tok;
-            head = it.hk * p.G + (live ? r - tok * p.G : 0);
+            next_lim = keys_seen(it.len, it.n, tok, causal);
+            next_token = it.first + tok;
+            next_head = it.hk * p.G + (next_live ? r - tok * p.G : 0);
             if (it.ni[t] > 0) {
-                // 16 lanes (DP 128) a row, so that a load takes whole lines; this warp's 32 rows
                 constexpr int C = DP / 8, RS = 32 / C;
-                const long long mine = live ? token * p.q_st + head * p.q_sh : -1;
+                const long long mine = next_live ? next_token * p.q_st + next_head * p.q_sh : -1;
                 const int c = lane % C, w0 = i0 & ~31;
                 const uint32_t dst = smem_u32(qs) + t * L::kTile + (c >> 3) * L::kBlkBytes;
-#pragma unroll 8
+#pragma unroll 4
                 for (int i = 0; i < 32 / RS; ++i) {
                     const int row = i * RS + lane / C;
                     const long long off = __shfl_sync(~0u, mine, row);
-                    const uint4 v = off >= 0 && c * 8 < p.D ? ldg128_nc(static_cast<const T16*>(p.q) + off + c * 8)
-                                                            : make_uint4(0u, 0u, 0u, 0u);
-                    sts128(dst + (w0 + row) * 128 + (((c & 7) ^ (row & 7)) << 4), v);
+                    const bool have = off >= 0 && c * 8 < p.D;
+                    cp_async16_zfill(dst + (w0 + row) * 128 + (((c & 7) ^ (row & 7)) << 4),
+                                     static_cast<const T16*>(p.q) + (have ? off + c * 8 : 0), have);
                 }
-                fence_async_smem();
-                mbar_arrive(&sh.q_full[t]);
             }
             return true;
         };
+        // Hands the Q that take() requested to the MMAs.
+        auto hand_q = [&](int k) {
+            if (sh.item[k & 1].ni[t] <= 0) return;
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            fence_async_smem();
+            mbar_arrive(&sh.q_full[t]);
+        };
         bool more = take(0);
+        if (more) hand_q(0);
         for (int k = 0; more; ++k) {
             float m = -INFINITY, l = 0.f;
             const Item& it = sh.item[k & 1];
             const int my = it.ni[t], k_first = it.k_first, m_first = it.m_first;
+            const int token = next_token, head = next_head, lim = next_lim;
+            const bool live = next_live;
+            bool took = false;
 #pragma unroll 1
             for (int i = 0; i < my; ++i) {
-                wait(&sh.s_full[t], (steps + i));
+                wait(&sh.s_full[t], steps + i);
                 __syncwarp();
                 tc_fence_after();
+                if (i == my - 1 && __all_sync(~0u, mbar_test(&sh.item_full[(k + 1) & 1], (uint32_t)((k + 1) >> 1) & 1u))) {
+                    // the last S is there, so Q has been read: the next one can be on its way.
+                    // (Not waited for: the next block may be published only after this one.)
+                    more = take(k + 1);
+                    took = true;
+                }
                 const int cut = i >= m_first ? lim - (k_first + i * kKeys) : kKeys;  // columns from here on are not seen
                 float s[128];
                 tmem_ld128_now(ts, s);
@@ -679,44 +694,58 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
                 if (move) m = mx;
                 const float sub = m == -INFINITY ? 0.f : m - kShift;
                 float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                auto exponentials = [&](int c) {  // of 32 columns
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
+                    for (int e = 32 * c; e < 32 * c + 32; e += 2) {
+                        fma2(s[e], s[e + 1], p.scale_log2, -sub);
+                        s[e] = ex2(s[e]);
+                        s[e + 1] = ex2(s[e + 1]);
+                    }
+                };
+                auto put = [&](int c) {
                     uint32_t w[16];
 #pragma unroll
                     for (int e = 0; e < 32; e += 2) {
-                        float x = s[32 * c + e], y = s[32 * c + e + 1];
-                        fma2(x, y, p.scale_log2, -sub);
-                        x = ex2(x);
-                        y = ex2(y);
-                        add2(sum[e & 2], sum[(e & 2) + 1], x, y);
-                        w[e / 2] = pack2<kBF16>(x, y);
+                        add2(sum[e & 2], sum[(e & 2) + 1], s[32 * c + e], s[32 * c + e + 1]);
+                        w[e / 2] = pack2<kBF16>(s[32 * c + e], s[32 * c + e + 1]);
                     }
                     tmem_st16(ts + 16u * c, w);
-                    if (c & 1) {  // half of P is there
-                        tmem_st_wait();
-                        tc_fence_before();
-                        mbar_arrive(&sh.p_full[t][c >> 1]);
-                    }
-                }
+                };
+                auto hand_over = [&](int half) {
+                    tmem_st_wait();
+                    tc_fence_before();
+                    mbar_arrive(&sh.p_full[t][half]);
+                };
+                // the function unit has the next columns' exponentials while these are stored
+                exponentials(0);
+                exponentials(1);
+                put(0);
+                exponentials(2);
+                put(1);
+                hand_over(0);
+                exponentials(3);
+                put(2);
+                put(3);
+                hand_over(1);
                 l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
             }
             steps += my;
-            if (my > 0) {
-                wait(&sh.o_full[t], (steps - 1));
-                __syncwarp();
-                tc_fence_after();
-            }
-            // what this block's output needs, before the next block's Q goes on its way
             const size_t hrow = (size_t)token * p.Hq + head;
             const size_t prow = (size_t)it.split * p.T * p.Hq + hrow;
             T16* out = static_cast<T16*>(p.o) + (size_t)token * p.o_st + (size_t)head * p.o_sh;
-            const bool store = live, any_bad = sh.any_bad[k & 1] != 0;  // written before v_clean, which every PV waited for
-            const int see = lim, bad_lim = lim - (k_first + m_first * kKeys);
-            more = take(k + 1);
+            const int bad_lim = lim - (k_first + m_first * kKeys);
+            if (!took) more = take(k + 1);
+            if (more) hand_q(k + 1);
+            if (my > 0) {
+                wait(&sh.o_full[t], steps - 1);
+                __syncwarp();
+                tc_fence_after();
+            }
+            const bool any_bad = sh.any_bad[k & 1] != 0;  // written before v_clean, which every PV waited for
             // l = 0: no key was seen (zeros), or every score was -inf (no softmax: NaN,
             // which a merge settles where other splits have a sum).
             const bool part = p.part_o != nullptr;
-            const float inv = l != 0.f ? 1.f / l : (!part && see > 0 ? NAN : 0.f);
+            const float inv = l != 0.f ? 1.f / l : (!part && lim > 0 ? NAN : 0.f);
 #pragma unroll 1
             for (int c = 0; c < DP / 32; ++c) {
                 float o[32];
@@ -732,7 +761,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
                         if ((int)sh.bad[k & 1][0][32 * c + e] < bad_lim) o[e] = NAN;
                     }
                 }
-                if (!store) continue;
+                if (!live) continue;
                 if (part) {
                     float* dst = p.part_o + prow * p.D + 32 * c;
 #pragma unroll
@@ -748,7 +777,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
                                            pack2<kBF16>(o[e + 4], o[e + 5]), pack2<kBF16>(o[e + 6], o[e + 7]));
                 }
             }
-            if (store) {
+            if (live) {
                 const float l2 = l == 0.f ? -INFINITY : m - kShift + log2f(l);
                 if (part) p.part_l[prow] = l2;
                 else if (p.lse) p.lse[hrow] = l2 * 0.693147180559945309417f;
