@@ -207,46 +207,63 @@ __device__ __forceinline__ int next_block_answer(const void* at) {
     return got ? (int)x : -1;
 }
 
-// The sequence and 256-row block with the number `want`: blocks are numbered
-// through the sequences.  One warp; every lane returns the same.
+// The sequence and 256-row block with the number `want`: the blocks of all sequences
+// by their place in their sequence, the last places first (under a causal mask they
+// have the most keys, and the CTAs end together when the longest work comes first;
+// 12 prompts of 172 to 1500 tokens: 61 us in the order of the sequences).
+// -1: there are fewer blocks.  One warp; every lane returns the same.
 __device__ __forceinline__ int find_block(const TileParams& p, int want, int& block) {
     const int lane = threadIdx.x & 31;
-    int before = 0;
+    auto blocks_of = [&](int s) {  // n * G fits: n_tokens * n_heads does
+        int first = 0, n = 0;
+        if (s >= p.B) return 0;
+        bool ok = seq_rows(p.cu_q, s, p.T, first, n);
+        if (ok && p.page_size) ok = len_ok(p.kv_lens[s], p.max_pages, p.page_size);
+        if (!ok) bad_index(p.err);
+        return ok && n * p.G > p.skip_rows ? (int)(((unsigned)(n * p.G) + 2 * kRows - 1) / (2 * kRows)) : 0;
+    };
+    const int mine = blocks_of(lane);  // the first 32 sequences'
+    // blocks with a place below b
+    auto below = [&](int b) {
+        int sum = min(mine, b);
+#pragma unroll 1
+        for (int s = lane + 32; s < p.B; s += 32) sum += min(blocks_of(s), b);
+        return __reduce_add_sync(~0u, sum);
+    };
+    int most = mine;
+#pragma unroll 1
+    for (int s = lane + 32; s < p.B; s += 32) most = max(most, blocks_of(s));
+    most = __reduce_max_sync(~0u, most);
+    int rank = below(most) - 1 - want;
+    if (rank < 0) return -1;
+    int lo = 0, hi = most;  // below(lo) <= rank < below(hi)
+#pragma unroll 1
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (below(mid) <= rank) lo = mid;
+        else hi = mid;
+    }
+    block = lo;
+    if (lo > 0) rank -= below(lo);
+    // the sequence with that rank among those that have such a block
 #pragma unroll 1
     for (int s0 = 0; s0 < p.B; s0 += 32) {
-        const int s = s0 + lane;
-        int first = 0, n = 0, nb = 0;
-        if (s < p.B) {
-            bool ok = seq_rows(p.cu_q, s, p.T, first, n);
-            if (ok && p.page_size) ok = len_ok(p.kv_lens[s], p.max_pages, p.page_size);
-            if (!ok) bad_index(p.err);
-            else if (n * p.G > p.skip_rows) nb = (int)(((unsigned)(n * p.G) + 2 * kRows - 1) / (2 * kRows));
-        }
-        int incl = nb;  // n * G fits: n_tokens * n_heads does
-#pragma unroll 1
-        for (int d = 1; d < 32; d <<= 1) {
-            const int x = __shfl_up_sync(~0u, incl, d);
-            if (lane >= d) incl += x;
-        }
-        const int lo = before + incl - nb;
-        const unsigned hit = __ballot_sync(~0u, want >= lo && want < lo + nb);
-        if (hit) {
-            const int l = __ffs(hit) - 1;
-            block = want - __shfl_sync(~0u, lo, l);
-            return s0 + l;
-        }
-        before += __shfl_sync(~0u, incl, 31);
+        const bool has = (s0 ? blocks_of(s0 + lane) : mine) > lo;
+        const unsigned all = __ballot_sync(~0u, has);
+        const unsigned hit = __ballot_sync(~0u, has && __popc(all & ((1u << lane) - 1u)) == rank);
+        if (hit) return s0 + __ffs(hit) - 1;
+        rank -= __popc(all);
     }
     return -1;
 }
 
-// Block `index` of the grid: the last row blocks come first (under a causal mask
-// they have the most keys), then key/value heads, then key splits.
+// Block `index` of the grid: row blocks as find_block numbers them, then key/value
+// heads, then key splits.
 __device__ __forceinline__ bool make_item(const TileParams& p, int index, Item& it) {
     const int split = index % p.splits, rest = index / p.splits;
     it.hk = rest % p.Hk;
     it.split = split;
-    int block = p.blocks - 1 - rest / p.Hk, seq = 0;
+    int block = rest / p.Hk, seq = 0;
     if (p.prefix_len) {
         it.first = 0;
         it.n = p.T;
