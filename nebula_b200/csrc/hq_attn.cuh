@@ -25,6 +25,20 @@ __device__ __forceinline__ void bad_index(unsigned* err) {
     if (err) atomicCAS(err, 0u, (unsigned)kDevBadIndex);
 }
 
+// Whether one of the eight 16-bit values of v is Inf or NaN: one step more in the
+// exponent's last place then reaches the sign's.
+template <bool kBF16>
+__device__ __forceinline__ bool not_finite(uint4 v) {
+    constexpr uint32_t kStep = kBF16 ? 0x00800080u : 0x04000400u, kAbs = 0x7FFF7FFFu;
+    return (((v.x & kAbs) + kStep) | ((v.y & kAbs) + kStep) | ((v.z & kAbs) + kStep) | ((v.w & kAbs) + kStep)) & 0x80008000u;
+}
+
+__device__ __forceinline__ float ld_dsmem_f1(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+
 // 16-byte asynchronous copy into shared memory; zeros where there is nothing to copy.
 __device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, bool have) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(have ? 16 : 0) : "memory");

@@ -37,13 +37,41 @@ struct AttnArgs {
 // kernel's, where it is launched; all others the tile kernel's.
 constexpr int kDecodeRows = 16;
 
+// Launches a kernel; with `overlap` it may start while the kernel before it on the
+// stream still runs (programmatic dependent launch), for whose results it then waits
+// itself.
+template <typename P>
+cudaError_t launch_overlapped(void (*fn)(P), unsigned grid, unsigned threads, size_t smem, cudaStream_t s, bool overlap,
+                              const P& p) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = overlap ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, fn, p);
+}
+
+// How the decode kernel's CTAs share the items, the (sequence, key/value head)s.
+enum DecodeMode : int { kFlat = 0, kWhole = 1, kCluster = 2 };
+struct DecodePlan {
+    int mode, ctas, cluster;
+};
+DecodePlan decode_plan(int B, int Hk, int max_kv, int sms);
+
 // What a call launches, and the workspace that its partial results take.
 struct AttnPlan {
     bool decode, tile;
-    int prefix;         // key splits of the shared prefix (0: none)
-    int own;            // key splits of the tile kernel
-    int ctas, whole;    // decode kernel: CTAs; no (sequence, head) is split
-    size_t planes;      // partials of every (row, head): prefix, tile, decode
+    int prefix;          // key splits of the shared prefix (0: none)
+    int own;             // key splits of the tile kernel
+    DecodePlan dec;
+    bool join;           // partials of the decode kernel are joined by a kernel
+    size_t planes;       // partials of every (row, head): prefix, tile, decode
+    size_t slots;        // rows of the decode kernel's slots
     size_t bytes;
 };
 AttnPlan attn_plan(int T, int B, int max_q, int Hq, int Hk, int D, bool paged, int max_kv, int prefix_len, int sms);
@@ -51,13 +79,13 @@ cudaError_t launch_attn(const AttnArgs& a);
 
 // The decode kernel's partial results and those of the prefix that they join.
 struct DecodeParts {
-    int ctas, whole, only;
+    DecodePlan plan;
+    int only, overlap;
     float *slot_o, *slot_l;  // [ctas][2][16][D], [ctas][2][16]
-    float *own_o, *own_l;    // [T * Hq][D], [T * Hq]; null without a prefix
+    float *own_o, *own_l;    // [T * Hq][D], [T * Hq]: with a prefix and kFlat
     const float *pre_o, *pre_l;
     int prefix_splits;
 };
-int decode_ctas(int B, int Hk, int max_kv, int sms);
 cudaError_t launch_attn_decode(const AttnArgs& a, const DecodeParts& parts);
 cudaError_t launch_attn_join(const AttnArgs& a, const DecodeParts& parts);
 

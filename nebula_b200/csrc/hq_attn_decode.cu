@@ -2,12 +2,9 @@
 // single tokens (the rows of a sequence and key/value head, tokens x G, are at
 // most 16), bound by reading the cache once.
 //
-// Work is cut into units of 128 keys of one (sequence, key/value head).  The
-// units of all sequences stand in one line (sequence, head, keys) of which every
-// CTA takes an equal share, whatever the lengths: each CTA sums up the lengths
-// itself, so no plan is made beforehand and a captured call follows them.  A warp
-// takes 16 keys of each unit, which lie in one page, through a ring of its own in
-// shared memory (cp.async, three units of 8 KB ahead; nothing but its own copies
+// Work is cut into units of 128 keys of one (sequence, key/value head), an item.  A
+// warp takes 16 keys of each unit, which lie in one page, through a ring of its own
+// in shared memory (cp.async, three units of 8 KB ahead; nothing but its own copies
 // to wait for): 128 KB in flight per SM, several times bandwidth x latency.
 //   S = Q K^T  mma.sync m16n8k16, the 16 rows (padded) x 16 keys
 //   P = 2^(c S - m), a running maximum m (moved, with O and the sum, only when
@@ -15,9 +12,17 @@
 //   O += P V   mma.sync, P straight from S's registers
 // The tensor rate is no bound here: 16 rows x 128 dims x 2 products a key need a
 // tenth of the rate that mma.sync has while 512 bytes of it arrive.
-// Where the CTA's share leaves a (sequence, head), its warps' sums are joined in
-// shared memory; one that no other CTA shares is written out, the others leave
-// normalised fp32 partials (at most two a CTA), joined by attn_join_kernel.
+// At an item's end the warps' sums are joined in shared memory.  Who takes which
+// units (DecodeMode; decode_plan chooses):
+//   kCluster  few items: a cluster of CTAs each, which join through distributed
+//             shared memory
+//   kWhole    each CTA the items that begin in its share of the line of all units
+//   kFlat     each CTA an equal share of the line, whatever the lengths: items that
+//             CTAs share leave normalised fp32 partials (at most two a CTA), joined
+//             by attn_join_kernel
+// The CTAs work their share out from the lengths on the device, so no plan is made
+// beforehand and a captured call follows them.  With a shared prefix its partials
+// (tile kernel) are joined with the item's own before it is written.
 #include "hq_attn.cuh"
 
 #include <algorithm>
@@ -58,11 +63,14 @@ struct DecodeParams {
     int T, B, Hq, Hk, G, D;
     int page_size, page_shift, num_pages, max_pages;
     float scale_log2;
-    int only;   // no other kernel takes the sequences of more rows
-    int whole;  // no (sequence, head) is shared between CTAs
-    // partials: two slots of 16 rows a CTA; with a shared prefix the (sequence,
-    // head)s of one CTA leave theirs by row in own_o, own_l [T * Hq]
+    int only;  // no other kernel takes the sequences of more rows
+    int mode, cluster;
+    // partials of items that CTAs share: two slots of 16 rows a CTA; with a prefix the
+    // other items' by row in own_o, own_l [T * Hq] (kFlat)
     float *slot_o, *slot_l, *own_o, *own_l;
+    const float *pre_o, *pre_l;  // the prefix's [prefix_splits][T * Hq]
+    int prefix_splits, prefix_len;
+    int overlap;  // launched while the kernel before it runs
     unsigned* err;
 };
 
@@ -141,6 +149,39 @@ __device__ __forceinline__ long long block_sum(long long x, long long* scratch) 
     return x;
 }
 
+// One row's partial results on their way to the output: sums of 2^(x - top) v in
+// acc (four dims d .. d + 3 of this lane) and of 2^(x - top) in sum.
+struct Row {
+    float acc[4], sum, top;
+};
+
+// Joins the prefix's partials of row `row` to it.
+__device__ __forceinline__ void join_prefix(const float* pre_o, const float* pre_l, int splits, size_t rows, size_t row, int D,
+                                            int d, Row& x) {
+    const int lane = threadIdx.x & 31;
+    const float l2 = lane < splits ? pre_l[lane * rows + row] : -INFINITY;  // splits <= 32
+    float top = fmaxf(x.top, l2);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+    const float base = top == -INFINITY ? 0.f : top;
+    const float f = ex2(x.top - base), w = ex2(l2 - base);
+    x.sum *= f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x.acc[e] *= f;
+#pragma unroll 4
+    for (int s = 0; s < splits; ++s) {
+        const float ws = __shfl_sync(~0u, w, s);
+        x.sum += ws;
+        if (d >= D) continue;
+        const float4 o = *reinterpret_cast<const float4*>(pre_o + (s * rows + row) * D + d);
+        x.acc[0] += ws * o.x;
+        x.acc[1] += ws * o.y;
+        x.acc[2] += ws * o.z;
+        x.acc[3] += ws * o.w;
+    }
+    x.top = top;
+}
+
 template <bool kBF16, int DP>
 __global__ void __launch_bounds__(kThreads, 1) attn_decode_kernel(const __grid_constant__ DecodeParams p) {
     using L = DecodeLayout<DP>;
@@ -158,119 +199,285 @@ __global__ void __launch_bounds__(kThreads, 1) attn_decode_kernel(const __grid_c
     float* join = reinterpret_cast<float*>(smem + L::kRing);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int g = lane >> 2, t4 = lane & 3;
+    const size_t rows = (size_t)p.T * p.Hq;
     pdl_launch_dependents();
 
-    // ------------------------------------------- this CTA's share of the line
-    Seq mine{};
-    long long count = 0;
-    for (int s = tid; s < p.B; s += kThreads) {
-        mine = seq_of(p, s);
-        count += (long long)mine.tiles * p.Hk;
-    }
-    const long long total = block_sum(count, s_scan);
-    const long long ctas = min((long long)gridDim.x, total);  // that have work, one unit at least
-    if (blockIdx.x >= ctas) return;
-    long long u0 = total * blockIdx.x / ctas, u1 = total * (blockIdx.x + 1) / ctas;
     if (tid < 2 * DP) (&s_bad[0][0])[tid] = 0;
     if (tid == 0) s_any_bad = 0;
-    long long before = 0;
-    for (int s0 = 0; s0 < p.B; s0 += kThreads) {
-        const int s = s0 + tid;
-        if (p.B > kThreads) mine = s < p.B ? seq_of(p, s) : Seq{};
-        const long long n = (long long)mine.tiles * p.Hk;
-        long long incl = n;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const long long x = __shfl_up_sync(~0u, incl, d);
-            if (lane >= d) incl += x;
-        }
-        __syncthreads();
-        if (lane == 31) s_scan[warp] = incl;
-        __syncthreads();
-        long long lo = before + incl - n, all = before;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-            if (w < warp) lo += s_scan[w];
-            all += s_scan[w];
-        }
-        for (int e = 0; e < 2; ++e) {
-            const long long u = e ? u1 : u0;
-            if (n > 0 && u >= lo && u < lo + n)
-                s_place[e] = Place{s, (int)((u - lo) / mine.tiles), (int)((u - lo) % mine.tiles), mine};
-        }
-        before = all;
-        if (before > u1) break;
-    }
-    __syncthreads();
 
-    Place at = s_place[0];
-    if (p.whole) {  // the (sequence, head)s that begin in this CTA's share
-        if (at.tile > 0) {
-            u0 += at.seq.tiles - at.tile;
-            if (u0 < total) {
-                at.tile = at.seq.tiles - 1;
-                next_unit(p, at);
-            }
+    Place at;
+    int units;
+    if (p.mode == kCluster) {
+        const int item = blockIdx.x / p.cluster, rank = blockIdx.x % p.cluster;
+        at.s = item / p.Hk;
+        at.h = item % p.Hk;
+        at.seq = seq_of(p, at.s);
+        if (at.seq.tiles == 0) {  // in all CTAs of the cluster
+            if (p.overlap) pdl_wait();
+            return;
         }
-        const Place end = s_place[1];
-        if (u1 < total && end.tile > 0) u1 += end.seq.tiles - end.tile;
-        if (u0 >= u1) return;
+        const int a = (int)((long long)at.seq.tiles * rank / p.cluster);
+        units = (int)((long long)at.seq.tiles * (rank + 1) / p.cluster) - a;
+        at.tile = a;
+        __syncthreads();
+    } else {
+        // ----------------------------------- this CTA's share of the line
+        Seq mine{};
+        long long count = 0;
+#pragma unroll 1
+        for (int s = tid; s < p.B; s += kThreads) {
+            mine = seq_of(p, s);
+            count += (long long)mine.tiles * p.Hk;
+        }
+        const long long total = block_sum(count, s_scan);
+        const long long ctas = min((long long)gridDim.x, total);  // that have work, one unit at least
+        if (blockIdx.x >= ctas) {
+            if (p.overlap) pdl_wait();
+            return;
+        }
+        long long u0 = total * blockIdx.x / ctas, u1 = total * (blockIdx.x + 1) / ctas;
+        long long before = 0;
+#pragma unroll 1
+        for (int s0 = 0; s0 < p.B; s0 += kThreads) {
+            const int s = s0 + tid;
+            if (p.B > kThreads) mine = s < p.B ? seq_of(p, s) : Seq{};
+            const long long n = (long long)mine.tiles * p.Hk;
+            long long incl = n;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const long long x = __shfl_up_sync(~0u, incl, d);
+                if (lane >= d) incl += x;
+            }
+            __syncthreads();
+            if (lane == 31) s_scan[warp] = incl;
+            __syncthreads();
+            long long lo = before + incl - n, all = before;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                if (w < warp) lo += s_scan[w];
+                all += s_scan[w];
+            }
+#pragma unroll 1
+            for (int e = 0; e < 2; ++e) {
+                const long long u = e ? u1 : u0;
+                if (n > 0 && u >= lo && u < lo + n) {
+                    s_place[e] = Place{s, (int)((u - lo) / mine.tiles), (int)((u - lo) % mine.tiles), mine};
+                }
+            }
+            before = all;
+            if (before > u1) break;
+        }
+        __syncthreads();
+        at = s_place[0];
+        if (p.mode == kWhole) {  // the items that begin in this CTA's share
+            if (at.tile > 0) {
+                u0 += at.seq.tiles - at.tile;
+                if (u0 < total) {
+                    at.tile = at.seq.tiles - 1;
+                    next_unit(p, at);
+                }
+            }
+            const Place end = s_place[1];
+            if (u1 < total && end.tile > 0) u1 += end.seq.tiles - end.tile;
+        }
+        units = u0 < u1 ? (int)(u1 - u0) : 0;
+        if (units == 0) {
+            if (p.overlap) pdl_wait();
+            return;
+        }
     }
+
     Place ahead = at;  // `at`: the unit in work; `ahead`: the next one to load
     const uint32_t ring = smem_u32(smem) + warp * NS * L::kStage;
     auto page_of = [&](const Place& x) {
         const int key = x.tile * kUnit + warp * kSlice;
         return key < x.seq.len ? __ldg(p.table + x.s * p.table_stride + (key >> p.page_shift)) : 0;
     };
-    int page = page_of(ahead);
-    // Requests this warp's keys of unit `ahead` into stage `st`; rows behind the last
-    // key and dims behind D are filled with zeros.
-    auto load = [&](int st) {
-        const int key = ahead.tile * kUnit + warp * kSlice;
-        if (key < ahead.seq.len) {
-            bool ok = page_ok(page, p.num_pages);
-            if (!ok) bad_index(p.err);
-            const long long pg = ok ? page : 0;
-            const int slot = key & (p.page_size - 1);
-            const T16* k = static_cast<const T16*>(p.k) + pg * p.k_sp + slot * p.k_st + ahead.h * p.k_sh;
-            const T16* v = static_cast<const T16*>(p.v) + pg * p.v_sp + slot * p.v_st + ahead.h * p.v_sh;
-            const int live = ok ? ahead.seq.len - key : 0;
-            const uint32_t dst = ring + st * L::kStage;
+    int page = units > 0 ? page_of(ahead) : 0;
+
+    uint32_t qf[DP / 16][4];
+    float o[DP / 8][4];
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    int lim[2] = {0, 0}, lim_min = 0, R = at.seq.n * p.G, tile0 = at.tile;
+    bool first_seg = true, fresh = true, waited = !p.overlap;
+
+    // Ends the item in work: joins the warps and writes it, or its partial.
+    auto leave = [&](bool whole) {
 #pragma unroll
-            for (int i = 0; i < kSlice * kChunks / 32; ++i) {
-                const int x = i * 32 + lane, r = x / kChunks, c = x % kChunks;
-                const bool have = r < live && c * 8 < p.D;
-                const uint32_t off = r * RB + ((c ^ (r & 7)) << 4);
-                cp_async16_zfill(dst + off, have ? k + r * p.k_st + c * 8 : k, have);
-                cp_async16_zfill(dst + kSlice * RB + off, have ? v + r * p.v_st + c * 8 : v, have);
+        for (int e = 0; e < 2; ++e) {
+            l[e] += __shfl_xor_sync(~0u, l[e], 1);
+            l[e] += __shfl_xor_sync(~0u, l[e], 2);
+            if (t4 == 0) {
+                s_m[warp][g + 8 * e] = m[e];
+                s_l[warp][g + 8 * e] = l[e];
             }
         }
-        cp_async_commit();
+        if (p.prefix_splits && p.mode != kFlat && !waited) {  // the prefix's partials are complete
+            pdl_wait();
+            waited = true;
+        }
+        // A cluster's partials: [16][DP] sums, [16] maxima and sums, where the ring was
+        // (every warp is past its last unit at the barrier below).
+        float* part = reinterpret_cast<float*>(smem);
+        const int d = 4 * lane;
+        // row r of the item from its joined sums
+        auto write = [&](int r, Row& x) {
+            const int tok = r / p.G, hd = at.h * p.G + r % p.G;
+            const int see = keys_seen(at.seq.len, at.seq.n, tok, 1);
+            const size_t row = (size_t)(at.seq.first + tok) * p.Hq + hd;
+            const bool out = whole && !p.own_o;
+            if (out && p.prefix_splits) {
+                x.top -= kShift;
+                join_prefix(p.pre_o, p.pre_l, p.prefix_splits, rows, row, p.D, d, x);
+                x.top += kShift;
+            }
+            // no key: zeros; scores that are all -inf: NaN, or left to the join
+            const float inv = x.sum != 0.f ? 1.f / x.sum : (out && see + p.prefix_len > 0 ? NAN : 0.f);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x.acc[e] = x.sum != 0.f ? x.acc[e] * inv : inv;
+            const float l2 = x.sum == 0.f ? -INFINITY : x.top - kShift + log2f(x.sum);
+            if (out) {
+                if (d < p.D)
+                    *reinterpret_cast<uint2*>(static_cast<T16*>(p.o) + (size_t)(at.seq.first + tok) * p.o_st +
+                                              (size_t)hd * p.o_sh + d) =
+                        make_uint2(pack2<kBF16>(x.acc[0], x.acc[1]), pack2<kBF16>(x.acc[2], x.acc[3]));
+                if (lane == 0 && p.lse) p.lse[row] = l2 * 0.693147180559945309417f;
+            } else {
+                const size_t slot = (size_t)(2 * blockIdx.x + (first_seg ? 0 : 1)) * kMaxRows + r;
+                float* dst = whole ? p.own_o + row * p.D : p.slot_o + slot * p.D;
+                if (d < p.D) *reinterpret_cast<float4*>(dst + d) = make_float4(x.acc[0], x.acc[1], x.acc[2], x.acc[3]);
+                if (lane == 0) (whole ? p.own_l[row] : p.slot_l[slot]) = l2;
+            }
+        };
+#pragma unroll 1
+        for (int half = 0; 8 * half < R; ++half) {
+            if (g + 8 * half < R) {
+#pragma unroll
+                for (int i = 0; i < DP / 8; ++i)
+                    *reinterpret_cast<float2*>(join + (warp * 8 + g) * L::kPitch + 8 * i + 2 * t4) =
+                        half ? make_float2(o[i][2], o[i][3]) : make_float2(o[i][0], o[i][1]);
+            }
+            __syncthreads();
+            // one warp a row, four dims a lane
+            const int r = 8 * half + warp;
+            if (r < R) {
+                Row x{};
+                x.top = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) x.top = fmaxf(x.top, s_m[w][r]);
+                const float base = x.top == -INFINITY ? 0.f : x.top;
+#pragma unroll 4
+                for (int w = 0; w < kWarps; ++w) {
+                    const float f = ex2(s_m[w][r] - base);
+                    x.sum += f * s_l[w][r];
+                    if (d < DP) {
+                        const float2* src = reinterpret_cast<const float2*>(join + (w * 8 + warp) * L::kPitch + d);
+                        const float2 a = src[0], b = src[1];
+                        x.acc[0] += f * a.x;
+                        x.acc[1] += f * a.y;
+                        x.acc[2] += f * b.x;
+                        x.acc[3] += f * b.y;
+                    }
+                }
+                if (s_any_bad && d < DP) {
+                    // of the last 16 keys, the first `vis` are seen
+                    const int vis = keys_seen(at.seq.len, at.seq.n, r / p.G, 1) - (at.seq.len - 16);
+                    const unsigned mask = vis >= 16 ? 0xFFFFu : vis > 0 ? (1u << vis) - 1u : 0u;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const unsigned b0 = s_bad[0][d + e], b1 = s_bad[1][d + e];
+                        if ((b0 >> 16) & mask) x.acc[e] += INFINITY;
+                        if (b1 & mask) x.acc[e] -= INFINITY;
+                        if (b0 & mask) x.acc[e] = NAN;
+                    }
+                }
+                if (p.mode == kCluster) {
+                    if (d < DP) *reinterpret_cast<float4*>(part + r * DP + d) = make_float4(x.acc[0], x.acc[1], x.acc[2], x.acc[3]);
+                    if (lane == 0) {
+                        part[kMaxRows * DP + r] = x.top;
+                        part[kMaxRows * DP + kMaxRows + r] = x.sum;
+                    }
+                } else {
+                    write(r, x);
+                }
+            }
+            __syncthreads();
+        }
+        if (p.mode == kCluster) {
+            cluster_sync();
+            // the rows over all warps of the cluster
+#pragma unroll 1
+            for (int r = (int)cluster_ctarank() * kWarps + warp; r < R; r += p.cluster * kWarps) {
+                Row x{};
+                const uint32_t base = smem_u32(part);
+                const bool have = lane < p.cluster;  // lane q: CTA q
+                const uint32_t ml = mapa_shared(base + (kMaxRows * DP + r) * 4, have ? lane : 0);
+                const float mq = have ? ld_dsmem_f1(ml) : -INFINITY, lq = have ? ld_dsmem_f1(ml + kMaxRows * 4) : 0.f;
+                x.top = mq;
+#pragma unroll
+                for (int k = 16; k; k >>= 1) x.top = fmaxf(x.top, __shfl_xor_sync(~0u, x.top, k));
+                const float f = ex2(mq - (x.top == -INFINITY ? 0.f : x.top));
+                x.sum = f * lq;
+#pragma unroll
+                for (int k = 16; k; k >>= 1) x.sum += __shfl_xor_sync(~0u, x.sum, k);
+#pragma unroll 4
+                for (int q = 0; q < p.cluster; ++q) {
+                    const float fq = __shfl_sync(~0u, f, q);
+                    if (d >= DP) continue;
+                    const float4 y = ld_dsmem_f4(mapa_shared(base + (r * DP + d) * 4, q));
+                    x.acc[0] += fq * y.x;
+                    x.acc[1] += fq * y.y;
+                    x.acc[2] += fq * y.z;
+                    x.acc[3] += fq * y.w;
+                }
+                write(r, x);
+            }
+            cluster_sync();  // the others' partials have been read
+        } else if (s_any_bad) {  // the same in all threads since the barriers above
+            __syncthreads();
+            if (tid < 2 * DP) (&s_bad[0][0])[tid] = 0;
+            if (tid == 0) s_any_bad = 0;
+            __syncthreads();
+        }
+        first_seg = false;
+        fresh = true;
     };
 
-    const int units = (int)(u1 - u0);
+    // A CTA of a cluster may have no unit; it takes one empty step.
+    const int steps = max(units, 1);
     int loaded = 0;
-    auto load_next = [&]() {
+#pragma unroll 1
+    for (int u = 1 - NS; u < steps; ++u) {
+        // Requests this warp's keys of the next unit; rows behind the last key and dims
+        // behind D are filled with zeros.
         if (loaded < units) {
-            load(loaded % NS);
+            const int key = ahead.tile * kUnit + warp * kSlice;
+            if (key < ahead.seq.len) {
+                const bool ok = page_ok(page, p.num_pages);
+                if (!ok) bad_index(p.err);
+                const long long pg = ok ? page : 0;
+                const int slot = key & (p.page_size - 1);
+                const T16* k = static_cast<const T16*>(p.k) + pg * p.k_sp + slot * p.k_st + ahead.h * p.k_sh;
+                const T16* v = static_cast<const T16*>(p.v) + pg * p.v_sp + slot * p.v_st + ahead.h * p.v_sh;
+                const int live = ok ? ahead.seq.len - key : 0;
+                const uint32_t dst = ring + loaded % NS * L::kStage;
+#pragma unroll
+                for (int i = 0; i < kSlice * kChunks / 32; ++i) {
+                    const int x = i * 32 + lane, r = x / kChunks, c = x % kChunks;
+                    const bool have = r < live && c * 8 < p.D;
+                    const uint32_t off = r * RB + ((c ^ (r & 7)) << 4);
+                    cp_async16_zfill(dst + off, have ? k + r * p.k_st + c * 8 : k, have);
+                    cp_async16_zfill(dst + kSlice * RB + off, have ? v + r * p.v_st + c * 8 : v, have);
+                }
+            }
             if (++loaded < units) {
                 next_unit(p, ahead);
                 page = page_of(ahead);
             }
-        } else {
-            cp_async_commit();
         }
-    };
-#pragma unroll
-    for (int i = 0; i < NS - 1; ++i) load_next();
-
-    uint32_t qf[DP / 16][4];
-    float o[DP / 8][4];
-    float m[2], l[2];
-    int lim[2], lim_min = 0, R = 0, tile0 = 0;
-    bool first_seg = true, fresh = true;
-    for (int u = 0; u < units; ++u) {
-        if (fresh) {  // a new (sequence, head): its rows of Q, rows g and g + 8 in this lane
+        cp_async_commit();
+        if (u < 0) continue;
+        if (fresh) {  // a new item: its rows of Q, rows g and g + 8 in this lane
             fresh = false;
             R = at.seq.n * p.G;
             tile0 = at.tile;
@@ -279,7 +486,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_decode_kernel(const __grid_c
             for (int e = 0; e < 2; ++e) {
                 const int r = g + 8 * e;
                 const bool live = r < R;
-                const int tok = live ? r / p.G : 0, hd = at.h * p.G + (live ? r % p.G : 0);
+                const int tok = live ? r / p.G : 0, hd = at.h * p.G + (live ? r - tok * p.G : 0);
                 lim[e] = live ? keys_seen(at.seq.len, at.seq.n, tok, 1) : at.seq.len;
                 m[e] = -INFINITY;
                 l[e] = 0.f;
@@ -297,41 +504,37 @@ __global__ void __launch_bounds__(kThreads, 1) attn_decode_kernel(const __grid_c
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
         }
-        load_next();
         cp_async_wait<NS - 1>();
         __syncwarp();
         const int key0 = at.tile * kUnit + warp * kSlice;
-        if (key0 < at.seq.len) {
-            const uint32_t kst = ring + (u % NS) * L::kStage, vst = kst + kSlice * RB;
+        if (u < units && key0 < at.seq.len) {
+            const uint32_t kst = ring + u % NS * L::kStage, vst = kst + kSlice * RB;
             const bool masked = key0 + kSlice > lim_min;
             if (masked && at.seq.n > 1) {
                 // Values that only some rows see and that are not finite would reach the
                 // others as 0 x NaN: taken out here, put back into the rows that see them
                 // at the end.  Only the last n <= 16 keys can be such.
                 const int lo = max(0, lim_min - key0), hi = min(kSlice, at.seq.len - key0);
+#pragma unroll 1
                 for (int x = lane; x < (hi - lo) * kChunks; x += 32) {
                     const int r = lo + x / kChunks, c = x % kChunks;
                     const uint32_t a = vst + r * RB + ((c ^ (r & 7)) << 4);
                     const uint4 v4 = lds128(a);
+                    if (!not_finite<kBF16>(v4)) continue;
                     uint32_t w[4] = {v4.x, v4.y, v4.z, v4.w};
                     constexpr uint32_t kExp = kBF16 ? 0x7F80u : 0x7C00u;
-                    bool hit = false;
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         const uint32_t h = (w[e >> 1] >> (16 * (e & 1))) & 0xFFFFu;
-                        if ((h & kExp) == kExp) {
-                            const unsigned bit = 1u << (key0 + r - (at.seq.len - 16));
-                            if ((h & 0x7FFFu) != kExp) atomicOr(&s_bad[0][c * 8 + e], bit);
-                            else if (h & 0x8000u) atomicOr(&s_bad[1][c * 8 + e], bit);
-                            else atomicOr(&s_bad[0][c * 8 + e], bit << 16);
-                            w[e >> 1] &= ~(0xFFFFu << (16 * (e & 1)));
-                            hit = true;
-                        }
+                        if ((h & kExp) != kExp) continue;
+                        const unsigned bit = 1u << (key0 + r - (at.seq.len - 16));
+                        if ((h & 0x7FFFu) != kExp) atomicOr(&s_bad[0][c * 8 + e], bit);
+                        else if (h & 0x8000u) atomicOr(&s_bad[1][c * 8 + e], bit);
+                        else atomicOr(&s_bad[0][c * 8 + e], bit << 16);
+                        w[e >> 1] &= ~(0xFFFFu << (16 * (e & 1)));
                     }
-                    if (hit) {
-                        sts128(a, make_uint4(w[0], w[1], w[2], w[3]));
-                        s_any_bad = 1;
-                    }
+                    sts128(a, make_uint4(w[0], w[1], w[2], w[3]));
+                    s_any_bad = 1;
                 }
                 __syncwarp();
             }
@@ -351,14 +554,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_decode_kernel(const __grid_c
                     for (int e = 0; e < 4; ++e)
                         if (key0 + 8 * nt + 2 * t4 + (e & 1) >= lim[e >> 1]) s[nt][e] = -INFINITY;
             }
-            float mx[2], f[2];
+            float f[2];
             bool move = false;
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 float x = fmaxf(fmaxf(s[0][2 * e], s[0][2 * e + 1]), fmaxf(s[1][2 * e], s[1][2 * e + 1]));
                 x = fmaxf(x, __shfl_xor_sync(~0u, x, 1));
                 x = fmaxf(x, __shfl_xor_sync(~0u, x, 2)) * p.scale_log2;
-                mx[e] = x;
                 f[e] = 1.f;
                 if (x > m[e] + 8.f) {
                     f[e] = ex2(m[e] - x);
@@ -398,102 +600,17 @@ __global__ void __launch_bounds__(kThreads, 1) attn_decode_kernel(const __grid_c
                 mma_16816<kBF16>(o[2 * i + 1], pf, b[2], b[3]);
             }
         }
-        __syncwarp();  // the stage is read; the next load_next() may fill it
-
-        if (at.tile + 1 == at.seq.tiles || u + 1 == units) {
-            // ------------------------------------------ leave this (sequence, head)
-            const bool whole = tile0 == 0 && at.tile + 1 == at.seq.tiles;
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                l[e] += __shfl_xor_sync(~0u, l[e], 1);
-                l[e] += __shfl_xor_sync(~0u, l[e], 2);
-                if (t4 == 0) {
-                    s_m[warp][g + 8 * e] = m[e];
-                    s_l[warp][g + 8 * e] = l[e];
-                }
-            }
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                if (8 * half >= R) break;
-                if (g + 8 * half < R) {
-#pragma unroll
-                    for (int i = 0; i < DP / 8; ++i)
-                        *reinterpret_cast<float2*>(join + (warp * 8 + g) * L::kPitch + 8 * i + 2 * t4) =
-                            make_float2(o[i][2 * half], o[i][2 * half + 1]);
-                }
-                __syncthreads();
-                // one warp a row, four dims a lane
-                const int r = 8 * half + warp, d = 4 * lane;
-                if (r < R) {
-                    float top = -INFINITY;
-#pragma unroll
-                    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_m[w][r]);
-                    const float base = top == -INFINITY ? 0.f : top;
-                    float sum = 0.f, acc[4] = {};
-#pragma unroll
-                    for (int w = 0; w < kWarps; ++w) {
-                        const float x = ex2(s_m[w][r] - base);
-                        sum += x * s_l[w][r];
-                        if (d < DP) {
-                            const float2* src = reinterpret_cast<const float2*>(join + (w * 8 + warp) * L::kPitch + d);
-                            const float2 a = src[0], b = src[1];
-                            acc[0] += x * a.x;
-                            acc[1] += x * a.y;
-                            acc[2] += x * b.x;
-                            acc[3] += x * b.y;
-                        }
-                    }
-                    const int tok = r / p.G, hd = at.h * p.G + r % p.G;
-                    const int see = keys_seen(at.seq.len, at.seq.n, tok, 1);
-                    const size_t row = (size_t)(at.seq.first + tok) * p.Hq + hd;
-                    const bool out = whole && !p.own_o;
-                    // no key: zeros; scores that are all -inf: NaN, or left to the join
-                    const float inv = sum != 0.f ? 1.f / sum : (out && see > 0 ? NAN : 0.f);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[e] = sum != 0.f ? acc[e] * inv : inv;
-                    if (s_any_bad && d < DP) {
-                        const int vis = see - (at.seq.len - 16);  // of the last 16 keys, the first `vis` are seen
-                        const unsigned mask = vis >= 16 ? 0xFFFFu : vis > 0 ? (1u << vis) - 1u : 0u;
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const unsigned b0 = s_bad[0][d + e], b1 = s_bad[1][d + e];
-                            if ((b0 >> 16) & mask) acc[e] += INFINITY;
-                            if (b1 & mask) acc[e] -= INFINITY;
-                            if (b0 & mask) acc[e] = NAN;
-                        }
-                    }
-                    const float l2 = sum == 0.f ? -INFINITY : top - kShift + log2f(sum);
-                    if (out) {
-                        if (d < p.D)
-                            *reinterpret_cast<uint2*>(static_cast<T16*>(p.o) + (size_t)(at.seq.first + tok) * p.o_st +
-                                                      (size_t)hd * p.o_sh + d) =
-                                make_uint2(pack2<kBF16>(acc[0], acc[1]), pack2<kBF16>(acc[2], acc[3]));
-                        if (lane == 0 && p.lse) p.lse[row] = l2 * 0.693147180559945309417f;
-                    } else {
-                        const size_t slot = (size_t)(2 * blockIdx.x + (first_seg ? 0 : 1)) * kMaxRows + r;
-                        float* dst = whole ? p.own_o + row * p.D : p.slot_o + slot * p.D;
-                        if (d < p.D) *reinterpret_cast<float4*>(dst + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
-                        if (lane == 0) (whole ? p.own_l[row] : p.slot_l[slot]) = l2;
-                    }
-                }
-                __syncthreads();
-            }
-            if (s_any_bad) {  // uniform: written before the barriers above
-                __syncthreads();
-                if (tid < 2 * DP) (&s_bad[0][0])[tid] = 0;
-                if (tid == 0) s_any_bad = 0;
-                __syncthreads();
-            }
-            first_seg = false;
-            fresh = true;
-        }
+        __syncwarp();  // the stage is read; the next request may fill it
+        if (at.tile + 1 == at.seq.tiles || u + 1 == steps)
+            leave(p.mode == kCluster || (tile0 == 0 && at.tile + 1 == at.seq.tiles));
         if (u + 1 < units) next_unit(p, at);
     }
     cp_async_wait<0>();
+    if (!waited) pdl_wait();  // what waits for this kernel waits for the one before it, too
 }
 
-// Joins the partials of every (sequence, head) that more than one CTA worked on,
-// and with a shared prefix of every one, with the prefix's.  One block each; the
+// kFlat: joins the partials of every item that more than one CTA worked on, and with
+// a shared prefix of every one, with the prefix's.  One block each; the
 // partials' weights first, then warp w adds up every eighth partial.
 struct JoinParams {
     const float *slot_o, *slot_l, *own_o, *own_l;
@@ -505,7 +622,7 @@ struct JoinParams {
     const int* kv_lens;
     int T, B, Hq, Hk, G, D;
     int page_size, max_pages;
-    int ctas, whole, prefix_splits, prefix_len;
+    int ctas, prefix_splits, prefix_len;
 };
 
 template <bool kBF16>
@@ -531,7 +648,7 @@ __global__ void __launch_bounds__(kThreads) attn_join_kernel(const JoinParams p)
     const long long ctas = min((long long)p.ctas, total);
     const long long ub = before + (long long)hk * me.tiles, ue = ub + me.tiles;
     const int c0 = (int)(((ub + 1) * ctas - 1) / total), c1 = (int)((ue * ctas - 1) / total);
-    const bool whole = p.whole || c0 == c1;
+    const bool whole = c0 == c1;
     if (whole && !p.prefix_splits) return;
     const int own = whole ? 1 : c1 - c0 + 1, parts = own + p.prefix_splits;
     const int R = me.n * p.G;
@@ -620,15 +737,51 @@ cudaError_t launch_one(const DecodeParams& p, int ctas, int dev, cudaStream_t s)
     auto fn = attn_decode_kernel<kBF16, DP>;
     cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(fn), dev, DecodeLayout<DP>::kSmem);
     if (e != cudaSuccess) return e;
-    fn<<<ctas, kThreads, DecodeLayout<DP>::kSmem, s>>>(p);
-    return cudaGetLastError();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)ctas);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = (size_t)DecodeLayout<DP>::kSmem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    cfg.attrs = attr;
+    if (p.cluster > 1) {
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = (unsigned)p.cluster;
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        cfg.numAttrs = 1;
+    }
+    if (p.overlap) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+        ++cfg.numAttrs;
+    }
+    return cudaLaunchKernelEx(&cfg, fn, p);
 }
 
 }  // namespace
 
-int decode_ctas(int B, int Hk, int max_kv, int sms) {
-    const long long units = (long long)B * Hk * std::max(1, (max_kv + kUnit - 1) / kUnit);
-    return (int)std::min<long long>(sms, units);
+DecodePlan decode_plan(int B, int Hk, int max_kv, int sms) {
+    const long long items = (long long)B * Hk;
+    const int tiles = std::max(1, (max_kv + kUnit - 1) / kUnit);
+    DecodePlan pl{};
+    pl.cluster = 1;
+    // A cluster per item while they fill no more than the SMs and no CTA has more than
+    // 8 units (1024 keys, 0.5 MB): beyond, a share of every SM is faster in spite of
+    // the join's launch.
+    int cs = 1;
+    while (cs < 8 && items * cs * 2 <= sms && cs < tiles) cs *= 2;
+    if (cs > 1 && tiles <= 8 * cs) {
+        pl.mode = kCluster;
+        pl.cluster = cs;
+        pl.ctas = (int)items * cs;
+        return pl;
+    }
+    // Whole items where a CTA's longest share stays within 16 units (1 MB).
+    const long long share = (items + sms - 1) / sms * tiles;
+    pl.mode = share <= 16 ? kWhole : kFlat;
+    pl.ctas = (int)std::min<long long>(sms, pl.mode == kWhole ? items : items * tiles);
+    return pl;
 }
 
 cudaError_t launch_attn_decode(const AttnArgs& a, const DecodeParts& parts) {
@@ -664,28 +817,33 @@ cudaError_t launch_attn_decode(const AttnArgs& a, const DecodeParts& parts) {
     p.max_pages = a.max_pages;
     p.scale_log2 = a.scale * 1.44269504088896340736f;
     p.only = parts.only;
-    p.whole = parts.whole;
+    p.mode = parts.plan.mode;
+    p.cluster = parts.plan.cluster;
     p.slot_o = parts.slot_o;
     p.slot_l = parts.slot_l;
     p.own_o = parts.own_o;
     p.own_l = parts.own_l;
+    p.pre_o = parts.pre_o;
+    p.pre_l = parts.pre_l;
+    p.prefix_splits = parts.prefix_splits;
+    p.prefix_len = a.prefix_len;
+    p.overlap = parts.overlap;
     p.err = a.err;
+    const int ctas = parts.plan.ctas;
     if (a.D <= 64)
-        return a.dtype == DType::BF16 ? launch_one<true, 64>(p, parts.ctas, a.dev, a.stream)
-                                      : launch_one<false, 64>(p, parts.ctas, a.dev, a.stream);
-    return a.dtype == DType::BF16 ? launch_one<true, 128>(p, parts.ctas, a.dev, a.stream)
-                                  : launch_one<false, 128>(p, parts.ctas, a.dev, a.stream);
+        return a.dtype == DType::BF16 ? launch_one<true, 64>(p, ctas, a.dev, a.stream) : launch_one<false, 64>(p, ctas, a.dev, a.stream);
+    return a.dtype == DType::BF16 ? launch_one<true, 128>(p, ctas, a.dev, a.stream) : launch_one<false, 128>(p, ctas, a.dev, a.stream);
 }
 
 cudaError_t launch_attn_join(const AttnArgs& a, const DecodeParts& parts) {
     JoinParams j{parts.slot_o, parts.slot_l, parts.own_o, parts.own_l, parts.pre_o, parts.pre_l, a.o, a.o_st, a.o_sh, a.lse,
-                 a.cu_q, a.kv_lens, a.T, a.B, a.Hq, a.Hk, a.G, a.D, a.page_size, a.max_pages, parts.ctas, parts.whole,
+                 a.cu_q, a.kv_lens, a.T, a.B, a.Hq, a.Hk, a.G, a.D, a.page_size, a.max_pages, parts.plan.ctas,
                  parts.prefix_splits, a.prefix_len};
     auto fn = a.dtype == DType::BF16 ? attn_join_kernel<true> : attn_join_kernel<false>;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)a.B, (unsigned)a.Hk);
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = (size_t)(parts.ctas + parts.prefix_splits) * kMaxRows * 4;
+    cfg.dynamicSmemBytes = (size_t)(parts.plan.ctas + parts.prefix_splits) * kMaxRows * 4;
     cfg.stream = a.stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

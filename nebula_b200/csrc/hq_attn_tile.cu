@@ -83,6 +83,7 @@ struct alignas(64) TileParams {
     int page_size, box_rows, num_pages, max_pages;  // page_size 0: packed rows
     int prefix_len;                                 // > 0: all T rows over the pages table[0..]
     int blocks, splits;  // the grid: row blocks x Hk x splits
+    int overlap;    // launched while the kernel before it runs
     int skip_rows;  // sequences of at most this many rows (tokens x G) are not this kernel's
     unsigned* err;
 };
@@ -290,14 +291,6 @@ __device__ __forceinline__ bool make_item(const TileParams& p, int index, Item& 
     return true;
 }
 
-// Whether one of the eight 16-bit values of v is Inf or NaN: one step more in the
-// exponent's last place then reaches the sign's.
-template <bool kBF16>
-__device__ __forceinline__ bool not_finite(uint4 v) {
-    constexpr uint32_t kStep = kBF16 ? 0x00800080u : 0x04000400u, kAbs = 0x7FFF7FFFu;
-    return (((v.x & kAbs) + kStep) | ((v.y & kAbs) + kStep) | ((v.z & kAbs) + kStep) | ((v.w & kAbs) + kStep)) & 0x80008000u;
-}
-
 // D (tensor memory) [+]= A x B: A from shared memory, A from tensor memory.
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
@@ -385,6 +378,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
     TileShared& sh = *reinterpret_cast<TileShared*>(smem + L::kShared);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
+    pdl_launch_dependents();
     if (warp == 1) {
         if (lane == 0) {
             for (int i = 0; i < S; ++i) {
@@ -805,6 +799,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
         }
     }
 
+    if (p.overlap) pdl_wait();  // what waits for this kernel waits for the one before it, too
     tc_fence_before();
     __syncthreads();
     if (warp == 1) {
@@ -887,8 +882,7 @@ cudaError_t launch_tile(const TileParams& p, int dev, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     const long long grid = (long long)p.blocks * p.Hk * p.splits;
     if (grid > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
-    fn<<<(unsigned)grid, kThreads, kSmem, s>>>(p);
-    return cudaGetLastError();
+    return launch_overlapped(fn, (unsigned)grid, kThreads, kSmem, s, p.overlap, p);
 }
 
 cudaError_t launch_tile_any(const AttnArgs& a, const TileParams& p) {
@@ -931,25 +925,23 @@ AttnPlan attn_plan(int T, int B, int max_q, int Hq, int Hk, int D, bool paged, i
     pl.own = pl.tile ? key_splits(rows, Hk, max_kv, sms) : 0;
     pl.planes = pl.prefix;
     if (pl.tile && pl.own + pl.prefix > 1) pl.planes += pl.own;
-    size_t slots = 0;
     if (pl.decode) {
-        pl.ctas = decode_ctas(B, Hk, max_kv, sms);
-        // A join costs a launch: lengths that a CTA reads in less time are not split.
-        pl.whole = max_kv <= 256;
-        if (pl.prefix) ++pl.planes;
-        if (!pl.whole) slots = (size_t)pl.ctas * 2 * kDecodeRows;
+        pl.dec = decode_plan(B, Hk, max_kv, sms);
+        pl.join = pl.dec.mode == kFlat;
+        if (pl.join) pl.slots = (size_t)pl.dec.ctas * 2 * kDecodeRows;
+        if (pl.join && pl.prefix) ++pl.planes;
     }
-    pl.bytes = ((pl.planes * T * Hq + slots) * (D + 1) * 4 + 255) & ~(size_t)255;
+    pl.bytes = ((pl.planes * T * Hq + pl.slots) * (D + 1) * 4 + 255) & ~(size_t)255;
     return pl;
 }
 
 cudaError_t launch_attn(const AttnArgs& a) {
     const AttnPlan pl = attn_plan(a.T, a.B, a.max_q, a.Hq, a.Hk, a.D, a.page_size > 0, a.max_kv, a.prefix_len, a.sm_count);
     // workspace: outputs of the planes, of the decode slots, then the sums of both
-    const size_t rows = (size_t)a.T * a.Hq, slots = pl.decode && !pl.whole ? (size_t)pl.ctas * 2 * kDecodeRows : 0;
+    const size_t rows = (size_t)a.T * a.Hq;
     float* plane_o = reinterpret_cast<float*>(a.ws);
     float* slot_o = plane_o + pl.planes * rows * a.D;
-    float* plane_l = slot_o + slots * a.D;
+    float* plane_l = slot_o + pl.slots * a.D;
     float* slot_l = plane_l + pl.planes * rows;
 
     cudaError_t e = cudaSuccess;
@@ -996,37 +988,38 @@ cudaError_t launch_attn(const AttnArgs& a) {
         p.table = a.table;
         p.table_stride = a.table_stride;
         p.splits = pl.own;
+        p.overlap = pl.prefix > 0;
         p.skip_rows = pl.decode ? kDecodeRows : 0;
         p.part_o = part ? plane_o + pl.prefix * rows * a.D : nullptr;
         p.part_l = part ? plane_l + pl.prefix * rows : nullptr;
         // every sequence may end inside a block
         p.blocks = (int)std::min((long long)row_blocks + a.B, 0x7fffffffLL);
         if ((e = launch_tile_any(a, p)) != cudaSuccess) return e;
-        if (part) {
-            MergeParams m{plane_o, plane_l, a.o, a.o_st, a.o_sh, a.lse, a.cu_q, a.kv_lens, a.T, a.B, a.Hq, a.D, a.causal,
-                          a.prefix_len, pl.own + pl.prefix, a.page_size, a.max_pages, a.G, p.skip_rows};
-            const unsigned grid = (unsigned)((rows + 7) / 8);
-            if (a.dtype == DType::BF16) attn_merge_kernel<true><<<grid, 256, 0, a.stream>>>(m);
-            else attn_merge_kernel<false><<<grid, 256, 0, a.stream>>>(m);
-            if ((e = cudaGetLastError()) != cudaSuccess) return e;
-        }
     }
     if (pl.decode) {
         DecodeParts d{};
-        d.ctas = pl.ctas;
-        d.whole = pl.whole;
+        d.plan = pl.dec;
         d.only = !pl.tile;
+        d.overlap = pl.prefix || pl.tile;  // the kernel before it is this call's own
         d.slot_o = slot_o;
         d.slot_l = slot_l;
         if (pl.prefix) {
-            d.own_o = plane_o + (pl.planes - 1) * rows * a.D;
-            d.own_l = plane_l + (pl.planes - 1) * rows;
+            if (pl.join) {
+                d.own_o = plane_o + (pl.planes - 1) * rows * a.D;
+                d.own_l = plane_l + (pl.planes - 1) * rows;
+            }
             d.pre_o = plane_o;
             d.pre_l = plane_l;
             d.prefix_splits = pl.prefix;
         }
         if ((e = launch_attn_decode(a, d)) != cudaSuccess) return e;
-        if (!pl.whole || pl.prefix) e = launch_attn_join(a, d);
+        if (pl.join && (e = launch_attn_join(a, d)) != cudaSuccess) return e;
+    }
+    if (pl.tile && pl.own + pl.prefix > 1) {
+        MergeParams m{plane_o, plane_l, a.o, a.o_st, a.o_sh, a.lse, a.cu_q, a.kv_lens, a.T, a.B, a.Hq, a.D, a.causal,
+                      a.prefix_len, pl.own + pl.prefix, a.page_size, a.max_pages, a.G, p.skip_rows};
+        auto fn = a.dtype == DType::BF16 ? attn_merge_kernel<true> : attn_merge_kernel<false>;
+        e = launch_overlapped(fn, (unsigned)((rows + 7) / 8), 256, 0, a.stream, true, m);
     }
     return e;
 }

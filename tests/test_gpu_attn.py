@@ -298,7 +298,7 @@ def test_paged_on_another_stream():
     s = torch.cuda.Stream()
     outs = [run_paged(c, stream=s) for _ in range(4)]
     s.synchronize()
-    assert all(torch.equal(o, outs[0]) for o in outs) and torch.equal(outs[0][:2], want[:2])
+    assert all(torch.equal(o[:2], want[:2]) for o in outs)  # rows 2 and 3 belong to no sequence
 
 
 @pytest.mark.parametrize("prefix", [0, 300])
