@@ -60,8 +60,9 @@ cudaError_t launch_overlapped(void (*fn)(P), unsigned grid, unsigned threads, si
 enum DecodeMode : int { kFlat = 0, kWhole = 1, kCluster = 2 };
 struct DecodePlan {
     int mode, ctas, cluster;
+    int group;  // warps of an item
 };
-DecodePlan decode_plan(int B, int Hk, int max_kv, int sms);
+DecodePlan decode_plan(int B, int Hk, int max_q, int max_kv, int sms);
 
 // What a call launches, and the workspace that its partial results take.
 struct AttnPlan {

@@ -53,8 +53,8 @@ hq_status check_shape(const hq_attn_shape* s, bool attention) {
     if (!attention) return HQ_OK;
     if (s->n_heads <= 0 || s->n_heads % s->n_kv_heads)
         return fail(HQ_ERR_UNSUPPORTED_SHAPE, "n_heads=%d must be a multiple of n_kv_heads=%d", s->n_heads, s->n_kv_heads);
-    if ((long long)s->n_tokens * s->n_heads > 0x7fffffffLL)
-        return fail(HQ_ERR_UNSUPPORTED_SHAPE, "n_tokens * n_heads must fit 31 bits");
+    if ((long long)s->n_tokens * s->n_heads > 0x7fffffffLL || (long long)s->n_seqs * s->n_heads > 0x7fffffffLL)
+        return fail(HQ_ERR_UNSUPPORTED_SHAPE, "n_tokens * n_heads and n_seqs * n_heads must fit 31 bits");
     if (!(s->scale > 0.f) || !std::isfinite(s->scale)) return fail(HQ_ERR_INVALID_ARG, "scale must be positive and finite");
     return HQ_OK;
 }

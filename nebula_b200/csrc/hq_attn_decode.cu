@@ -2,13 +2,15 @@
 // single tokens (the rows of a sequence and key/value head, tokens x G, are at
 // most 16), bound by reading the cache once.
 //
-// Work is cut into units of 128 keys of one (sequence, key/value head), an item.  A
+// An item is one (sequence, key/value head); W warps work on it (8, a CTA; fewer
+// where there are more items than CTAs and they are short), in units of 16 W keys.  A
 // warp takes 16 keys of each unit, which lie in one page, through a ring of its own
 // in shared memory (cp.async, three units of 8 KB ahead; nothing but its own copies
 // to wait for): 128 KB in flight per SM, several times bandwidth x latency.
 //   S = Q K^T  mma.sync m16n8k16, the 16 rows (padded) x 16 keys
-//   P = 2^(c S - m), a running maximum m (moved, with O and the sum, only when
-//              it has grown by more than 2^8) and sum per warp and row
+//   P = 2^(c S - m), a running maximum m and sum per warp and row; m is moved, with O
+//              and the sum, only when a score is above it by more than 2^8, which a
+//              vote tells: lanes need not agree on each unit's maximum
 //   O += P V   mma.sync, P straight from S's registers
 // The tensor rate is no bound here: 16 rows x 128 dims x 2 products a key need a
 // tenth of the rate that mma.sync has while 512 bytes of it arrive.
@@ -16,10 +18,10 @@
 // units (DecodeMode; decode_plan chooses):
 //   kCluster  few items: a cluster of CTAs each, which join through distributed
 //             shared memory
-//   kWhole    each CTA the items that begin in its share of the line of all units
-//   kFlat     each CTA an equal share of the line, whatever the lengths: items that
-//             CTAs share leave normalised fp32 partials (at most two a CTA), joined
-//             by attn_join_kernel
+//   kWhole    each group of W warps every so manieth item
+//   kFlat     each CTA an equal share of the line of all units, whatever the lengths:
+//             items that CTAs share leave normalised fp32 partials (at most two a
+//             CTA), joined by attn_join_kernel
 // The CTAs work their share out from the lengths on the device, so no plan is made
 // beforehand and a captured call follows them.  With a shared prefix its partials
 // (tile kernel) are joined with the item's own before it is written.
@@ -35,7 +37,7 @@ namespace {
 constexpr int kWarps = 8;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kSlice = 16;                 // keys of a warp in a unit
-constexpr int kUnit = kSlice * kWarps;
+constexpr int kUnit = kSlice * kWarps;     // keys of a unit of a whole CTA
 constexpr int kMaxRows = kDecodeRows;      // 16: the MMA's M
 
 template <int DP>
@@ -65,6 +67,8 @@ struct DecodeParams {
     float scale_log2;
     int only;  // no other kernel takes the sequences of more rows
     int mode, cluster;
+    int group;  // W: warps of an item
+    int max_rows;  // rows (tokens x G) that this kernel takes of a sequence
     // partials of items that CTAs share: two slots of 16 rows a CTA; with a prefix the
     // other items' by row in own_o, own_l [T * Hq] (kFlat)
     float *slot_o, *slot_l, *own_o, *own_l;
@@ -79,25 +83,20 @@ struct Seq {
 };
 
 // Sequence s, tiles 0 if it is not this kernel's.
-__device__ __forceinline__ Seq seq_of(const int* cu_q, const int* kv_lens, int T, int G, int max_pages, int page_size, int s,
-                                      unsigned* err) {
+__device__ __forceinline__ Seq seq_of(const int* cu_q, const int* kv_lens, int T, int G, int max_rows, int max_pages,
+                                      int page_size, int unit, int s, unsigned* err) {
     Seq q{};
     if (!seq_rows(cu_q, s, T, q.first, q.n)) {
         bad_index(err);
         return q;
     }
-    if (q.n <= 0 || (long long)q.n * G > kMaxRows) return q;
+    if (q.n <= 0 || (long long)q.n * G > max_rows) return q;
     q.len = kv_lens[s];
     if (!len_ok(q.len, max_pages, page_size)) {
         bad_index(err);
         return q;
     }
-    q.tiles = max(1, (q.len + kUnit - 1) / kUnit);
-    return q;
-}
-__device__ __forceinline__ Seq seq_of(const DecodeParams& p, int s) {
-    const Seq q = seq_of(p.cu_q, p.kv_lens, p.T, p.G, p.max_pages, p.page_size, s, p.err);
-    if (p.only && q.n > 0 && q.tiles == 0) bad_index(p.err);  // more rows than the caller's bound, or a bad length
+    q.tiles = max(1, (int)((unsigned)(q.len + unit - 1) / (unsigned)unit));
     return q;
 }
 
@@ -106,15 +105,6 @@ struct Place {
     int s, h, tile;
     Seq seq;
 };
-
-__device__ __forceinline__ void next_unit(const DecodeParams& p, Place& at) {
-    if (++at.tile < at.seq.tiles) return;
-    at.tile = 0;
-    if (++at.h < p.Hk) return;
-    at.h = 0;
-    do at.seq = ++at.s < p.B ? seq_of(p, at.s) : Seq{0, 0, 0, 1};
-    while (at.seq.tiles == 0);
-}
 
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -168,16 +158,24 @@ __device__ __forceinline__ void join_prefix(const float* pre_o, const float* pre
     x.sum *= f;
 #pragma unroll
     for (int e = 0; e < 4; ++e) x.acc[e] *= f;
-#pragma unroll 4
-    for (int s = 0; s < splits; ++s) {
-        const float ws = __shfl_sync(~0u, w, s);
-        x.sum += ws;
-        if (d >= D) continue;
-        const float4 o = *reinterpret_cast<const float4*>(pre_o + (s * rows + row) * D + d);
-        x.acc[0] += ws * o.x;
-        x.acc[1] += ws * o.y;
-        x.acc[2] += ws * o.z;
-        x.acc[3] += ws * o.w;
+    // eight partials requested at a time
+#pragma unroll 1
+    for (int s0 = 0; s0 < splits; s0 += 8) {
+        float4 o[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            o[i] = s0 + i < splits && d < D ? *reinterpret_cast<const float4*>(pre_o + ((s0 + i) * rows + row) * D + d)
+                                            : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float ws = __shfl_sync(~0u, w, (s0 + i) & 31);
+            if (s0 + i >= splits) continue;
+            x.sum += ws;
+            x.acc[0] += ws * o[i].x;
+            x.acc[1] += ws * o[i].y;
+            x.acc[2] += ws * o[i].z;
+            x.acc[3] += ws * o[i].w;
+        }
     }
     x.top = top;
 }
@@ -192,33 +190,61 @@ __global__ void __launch_bounds__(kThreads, 1) attn_decode_kernel(const __grid_c
 
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ long long s_scan[kWarps];
-    __shared__ Place s_place[2];
+    __shared__ Place s_start;
     __shared__ float s_m[kWarps][kMaxRows], s_l[kWarps][kMaxRows];
     __shared__ unsigned s_bad[2][DP];  // keys (bit j: key len - 16 + j) whose value in that dim is NaN | +Inf << 16, -Inf
     __shared__ int s_any_bad;
     float* join = reinterpret_cast<float*>(smem + L::kRing);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int g = lane >> 2, t4 = lane & 3;
+    const int W = p.group, gw = warp & (W - 1), w0 = warp - gw;  // this warp in its group, the group's first
+    const int unit = kSlice * W;
     const size_t rows = (size_t)p.T * p.Hq;
     pdl_launch_dependents();
+
+    auto seq_at = [&](int s) {
+        const Seq q = seq_of(p.cu_q, p.kv_lens, p.T, p.G, p.max_rows, p.max_pages, p.page_size, unit, s, p.err);
+        if (p.only && q.n > 0 && q.tiles == 0) bad_index(p.err);  // more rows than the caller's bound, or a bad length
+        return q;
+    };
+    auto group_sync = [&] {
+        if (W == 1) __syncwarp();
+        else named_bar_sync(1 + w0 / W, 32 * W);
+    };
 
     if (tid < 2 * DP) (&s_bad[0][0])[tid] = 0;
     if (tid == 0) s_any_bad = 0;
 
-    Place at;
-    int units;
-    if (p.mode == kCluster) {
-        const int item = blockIdx.x / p.cluster, rank = blockIdx.x % p.cluster;
-        at.s = item / p.Hk;
-        at.h = item % p.Hk;
-        at.seq = seq_of(p, at.s);
+    Place at{};
+    int units = 0x7fffffff;                                            // of this CTA's share
+    const int slots = gridDim.x * (kWarps / W);                        // kWhole: groups
+    int item = blockIdx.x * (kWarps / W) + w0 / W;
+    // kWhole: the group's next item that has work; s = B: none
+    auto next_item = [&](Place& x, int& i) {
+        const int items = p.B * p.Hk;
+        for (; i < items; i += slots) {
+            x.s = i / p.Hk;
+            x.h = i - x.s * p.Hk;
+            x.tile = 0;
+            x.seq = seq_at(x.s);
+            if (x.seq.tiles) return;
+        }
+        x.s = p.B;
+    };
+    if (p.mode == kWhole) {
+        next_item(at, item);
+        __syncthreads();
+    } else if (p.mode == kCluster) {
+        const int it = blockIdx.x / p.cluster, rank = blockIdx.x % p.cluster;
+        at.s = it / p.Hk;
+        at.h = it - at.s * p.Hk;
+        at.seq = seq_at(at.s);
         if (at.seq.tiles == 0) {  // in all CTAs of the cluster
             if (p.overlap) pdl_wait();
             return;
         }
-        const int a = (int)((long long)at.seq.tiles * rank / p.cluster);
-        units = (int)((long long)at.seq.tiles * (rank + 1) / p.cluster) - a;
-        at.tile = a;
+        at.tile = (int)((long long)at.seq.tiles * rank / p.cluster);
+        units = (int)((long long)at.seq.tiles * (rank + 1) / p.cluster) - at.tile;
         __syncthreads();
     } else {
         // ----------------------------------- this CTA's share of the line
@@ -226,7 +252,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_decode_kernel(const __grid_c
         long long count = 0;
 #pragma unroll 1
         for (int s = tid; s < p.B; s += kThreads) {
-            mine = seq_of(p, s);
+            mine = seq_at(s);
             count += (long long)mine.tiles * p.Hk;
         }
         const long long total = block_sum(count, s_scan);
@@ -235,12 +261,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_decode_kernel(const __grid_c
             if (p.overlap) pdl_wait();
             return;
         }
-        long long u0 = total * blockIdx.x / ctas, u1 = total * (blockIdx.x + 1) / ctas;
+        const long long u0 = total * blockIdx.x / ctas;
+        units = (int)(total * (blockIdx.x + 1) / ctas - u0);
         long long before = 0;
 #pragma unroll 1
         for (int s0 = 0; s0 < p.B; s0 += kThreads) {
             const int s = s0 + tid;
-            if (p.B > kThreads) mine = s < p.B ? seq_of(p, s) : Seq{};
+            if (p.B > kThreads) mine = s < p.B ? seq_at(s) : Seq{};
             const long long n = (long long)mine.tiles * p.Hk;
             long long incl = n;
 #pragma unroll
@@ -257,48 +284,50 @@ __global__ void __launch_bounds__(kThreads, 1) attn_decode_kernel(const __grid_c
                 if (w < warp) lo += s_scan[w];
                 all += s_scan[w];
             }
-#pragma unroll 1
-            for (int e = 0; e < 2; ++e) {
-                const long long u = e ? u1 : u0;
-                if (n > 0 && u >= lo && u < lo + n) {
-                    s_place[e] = Place{s, (int)((u - lo) / mine.tiles), (int)((u - lo) % mine.tiles), mine};
-                }
-            }
+            if (n > 0 && u0 >= lo && u0 < lo + n)
+                s_start = Place{s, (int)((u0 - lo) / mine.tiles), (int)((u0 - lo) % mine.tiles), mine};
             before = all;
-            if (before > u1) break;
+            if (before > u0) break;
         }
         __syncthreads();
-        at = s_place[0];
-        if (p.mode == kWhole) {  // the items that begin in this CTA's share
-            if (at.tile > 0) {
-                u0 += at.seq.tiles - at.tile;
-                if (u0 < total) {
-                    at.tile = at.seq.tiles - 1;
-                    next_unit(p, at);
-                }
-            }
-            const Place end = s_place[1];
-            if (u1 < total && end.tile > 0) u1 += end.seq.tiles - end.tile;
-        }
-        units = u0 < u1 ? (int)(u1 - u0) : 0;
-        if (units == 0) {
-            if (p.overlap) pdl_wait();
+        at = s_start;
+    }
+    // The unit after x (of this CTA's share, while there are any); s = B behind the last.
+    auto next_unit = [&](Place& x, int& i) {
+        if (++x.tile < x.seq.tiles) return;
+        if (p.mode == kWhole) {
+            i += slots;
+            next_item(x, i);
             return;
         }
-    }
+        x.tile = 0;
+        if (++x.h < p.Hk) return;
+        x.h = 0;
+        do {
+            if (++x.s >= p.B) return;
+            x.seq = seq_at(x.s);
+        } while (x.seq.tiles == 0);
+    };
 
     Place ahead = at;  // `at`: the unit in work; `ahead`: the next one to load
+    int ahead_item = item;
     const uint32_t ring = smem_u32(smem) + warp * NS * L::kStage;
     auto page_of = [&](const Place& x) {
-        const int key = x.tile * kUnit + warp * kSlice;
-        return key < x.seq.len ? __ldg(p.table + x.s * p.table_stride + (key >> p.page_shift)) : 0;
+        const int key = x.tile * unit + gw * kSlice;
+        return x.s < p.B && key < x.seq.len ? __ldg(p.table + x.s * p.table_stride + (key >> p.page_shift)) : 0;
     };
     int page = units > 0 ? page_of(ahead) : 0;
+    // This lane's 16-byte chunk of a step's rows r0, r0 + RS, ...: where it is read, and
+    // where it goes (chunk c of row r at chunk c ^ (r & 7)).
+    constexpr int RS = 32 / kChunks;
+    const int chunk = lane % kChunks, r0 = lane / kChunks;
+    const long long k_lane = r0 * p.k_st + chunk * 8, v_lane = r0 * p.v_st + chunk * 8;
+    const uint32_t s_lane = r0 * RB + ((chunk ^ r0) << 4);
 
     uint32_t qf[DP / 16][4];
     float o[DP / 8][4];
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-    int lim[2] = {0, 0}, lim_min = 0, R = at.seq.n * p.G, tile0 = at.tile;
+    int lim[2] = {0, 0}, lim_min = 0, tile0 = 0;
     bool first_seg = true, fresh = true, waited = !p.overlap;
 
     // Ends the item in work: joins the warps and writes it, or its partial.
@@ -312,6 +341,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_decode_kernel(const __grid_c
                 s_l[warp][g + 8 * e] = l[e];
             }
         }
+        const int R = at.seq.n * p.G;
         if (p.prefix_splits && p.mode != kFlat && !waited) {  // the prefix's partials are complete
             pdl_wait();
             waited = true;
@@ -357,21 +387,21 @@ __global__ void __launch_bounds__(kThreads, 1) attn_decode_kernel(const __grid_c
                     *reinterpret_cast<float2*>(join + (warp * 8 + g) * L::kPitch + 8 * i + 2 * t4) =
                         half ? make_float2(o[i][2], o[i][3]) : make_float2(o[i][0], o[i][1]);
             }
-            __syncthreads();
+            group_sync();
             // one warp a row, four dims a lane
-            const int r = 8 * half + warp;
-            if (r < R) {
+#pragma unroll 1
+            for (int r = 8 * half + gw; r < min(R, 8 * half + 8); r += W) {
                 Row x{};
                 x.top = -INFINITY;
-#pragma unroll
-                for (int w = 0; w < kWarps; ++w) x.top = fmaxf(x.top, s_m[w][r]);
+#pragma unroll 4
+                for (int w = 0; w < W; ++w) x.top = fmaxf(x.top, s_m[w0 + w][r]);
                 const float base = x.top == -INFINITY ? 0.f : x.top;
 #pragma unroll 4
-                for (int w = 0; w < kWarps; ++w) {
-                    const float f = ex2(s_m[w][r] - base);
-                    x.sum += f * s_l[w][r];
+                for (int w = 0; w < W; ++w) {
+                    const float f = ex2(s_m[w0 + w][r] - base);
+                    x.sum += f * s_l[w0 + w][r];
                     if (d < DP) {
-                        const float2* src = reinterpret_cast<const float2*>(join + (w * 8 + warp) * L::kPitch + d);
+                        const float2* src = reinterpret_cast<const float2*>(join + ((w0 + w) * 8 + (r & 7)) * L::kPitch + d);
                         const float2 a = src[0], b = src[1];
                         x.acc[0] += f * a.x;
                         x.acc[1] += f * a.y;
@@ -401,7 +431,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_decode_kernel(const __grid_c
                     write(r, x);
                 }
             }
-            __syncthreads();
+            group_sync();
         }
         if (p.mode == kCluster) {
             cluster_sync();
@@ -433,7 +463,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_decode_kernel(const __grid_c
                 write(r, x);
             }
             cluster_sync();  // the others' partials have been read
-        } else if (s_any_bad) {  // the same in all threads since the barriers above
+        } else if (s_any_bad) {  // W = 8: the same in all threads since the barriers above
             __syncthreads();
             if (tid < 2 * DP) (&s_bad[0][0])[tid] = 0;
             if (tid == 0) s_any_bad = 0;
@@ -443,43 +473,48 @@ __global__ void __launch_bounds__(kThreads, 1) attn_decode_kernel(const __grid_c
         fresh = true;
     };
 
-    // A CTA of a cluster may have no unit; it takes one empty step.
-    const int steps = max(units, 1);
-    int loaded = 0;
+    // The request of one unit runs NS - 1 units ahead of the work.  A CTA of a cluster
+    // may have no unit; it takes one empty step.
+    int loaded = 0, load_st = 0, work_st = 0;
 #pragma unroll 1
-    for (int u = 1 - NS; u < steps; ++u) {
-        // Requests this warp's keys of the next unit; rows behind the last key and dims
-        // behind D are filled with zeros.
-        if (loaded < units) {
-            const int key = ahead.tile * kUnit + warp * kSlice;
+    for (int u = 1 - NS;; ++u) {
+        if (loaded < units && ahead.s < p.B) {
+            // This warp's keys of unit `ahead`; rows behind the last key and dims behind D
+            // are filled with zeros.
+            const int key = ahead.tile * unit + gw * kSlice;
             if (key < ahead.seq.len) {
                 const bool ok = page_ok(page, p.num_pages);
                 if (!ok) bad_index(p.err);
                 const long long pg = ok ? page : 0;
-                const int slot = key & (p.page_size - 1);
+                const int slot = key & (p.page_size - 1), live = ok ? ahead.seq.len - key : 0;
                 const T16* k = static_cast<const T16*>(p.k) + pg * p.k_sp + slot * p.k_st + ahead.h * p.k_sh;
                 const T16* v = static_cast<const T16*>(p.v) + pg * p.v_sp + slot * p.v_st + ahead.h * p.v_sh;
-                const int live = ok ? ahead.seq.len - key : 0;
-                const uint32_t dst = ring + loaded % NS * L::kStage;
+                const uint32_t dst = ring + load_st * L::kStage + s_lane;
+                const bool dims = chunk * 8 < p.D;
+                const T16 *kl = k + k_lane, *vl = v + v_lane;
 #pragma unroll
-                for (int i = 0; i < kSlice * kChunks / 32; ++i) {
-                    const int x = i * 32 + lane, r = x / kChunks, c = x % kChunks;
-                    const bool have = r < live && c * 8 < p.D;
-                    const uint32_t off = r * RB + ((c ^ (r & 7)) << 4);
-                    cp_async16_zfill(dst + off, have ? k + r * p.k_st + c * 8 : k, have);
-                    cp_async16_zfill(dst + kSlice * RB + off, have ? v + r * p.v_st + c * 8 : v, have);
+                for (int i = 0; i < kSlice / RS; ++i) {
+                    const bool have = dims && r0 + i * RS < live;
+                    const uint32_t to = (dst ^ ((i * RS & 7) << 4)) + i * RS * RB;
+                    cp_async16_zfill(to, have ? kl : k, have);
+                    cp_async16_zfill(to + kSlice * RB, have ? vl : v, have);
+                    kl += RS * p.k_st;
+                    vl += RS * p.v_st;
                 }
             }
+            load_st = load_st + 1 == NS ? 0 : load_st + 1;
             if (++loaded < units) {
-                next_unit(p, ahead);
+                next_unit(ahead, ahead_item);
                 page = page_of(ahead);
             }
         }
         cp_async_commit();
         if (u < 0) continue;
+        const bool work = u < loaded;
+        if (!work && (p.mode != kCluster || u > 0)) break;
         if (fresh) {  // a new item: its rows of Q, rows g and g + 8 in this lane
             fresh = false;
-            R = at.seq.n * p.G;
+            const int R = at.seq.n * p.G;
             tile0 = at.tile;
             lim_min = keys_seen(at.seq.len, at.seq.n, 0, 1);
 #pragma unroll
@@ -506,9 +541,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_decode_kernel(const __grid_c
         }
         cp_async_wait<NS - 1>();
         __syncwarp();
-        const int key0 = at.tile * kUnit + warp * kSlice;
-        if (u < units && key0 < at.seq.len) {
-            const uint32_t kst = ring + u % NS * L::kStage, vst = kst + kSlice * RB;
+        const int key0 = at.tile * unit + gw * kSlice;
+        if (work && key0 < at.seq.len) {
+            const uint32_t kst = ring + work_st * L::kStage, vst = kst + kSlice * RB;
             const bool masked = key0 + kSlice > lim_min;
             if (masked && at.seq.n > 1) {
                 // Values that only some rows see and that are not finite would reach the
@@ -538,39 +573,40 @@ __global__ void __launch_bounds__(kThreads, 1) attn_decode_kernel(const __grid_c
                 }
                 __syncwarp();
             }
-            float s[2][4] = {};
+            float s[2][4] = {}, s2[2][4] = {};  // even and odd steps: two chains an n-tile
             const int kr = ((lane >> 4) << 3) + (lane & 7), kc = (lane >> 3) & 1;
 #pragma unroll
-            for (int k = 0; k < DP / 16; ++k) {
+            for (int k = 0; k < DP / 16; k += 2) {
                 uint32_t b[4];
                 ldsm4(kst + kr * RB + (((2 * k + kc) ^ (kr & 7)) << 4), b);
                 mma_16816<kBF16>(s[0], qf[k], b[0], b[1]);
                 mma_16816<kBF16>(s[1], qf[k], b[2], b[3]);
+                ldsm4(kst + kr * RB + (((2 * k + 2 + kc) ^ (kr & 7)) << 4), b);
+                mma_16816<kBF16>(s2[0], qf[k + 1], b[0], b[1]);
+                mma_16816<kBF16>(s2[1], qf[k + 1], b[2], b[3]);
             }
-            if (masked) {
 #pragma unroll
-                for (int nt = 0; nt < 2; ++nt)
+            for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (key0 + 8 * nt + 2 * t4 + (e & 1) >= lim[e >> 1]) s[nt][e] = -INFINITY;
-            }
-            float f[2];
-            bool move = false;
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                float x = fmaxf(fmaxf(s[0][2 * e], s[0][2 * e + 1]), fmaxf(s[1][2 * e], s[1][2 * e + 1]));
-                x = fmaxf(x, __shfl_xor_sync(~0u, x, 1));
-                x = fmaxf(x, __shfl_xor_sync(~0u, x, 2)) * p.scale_log2;
-                f[e] = 1.f;
-                if (x > m[e] + 8.f) {
-                    f[e] = ex2(m[e] - x);
-                    m[e] = x;
-                    move = true;
+                for (int e = 0; e < 4; ++e) {
+                    s[nt][e] = (s[nt][e] + s2[nt][e]) * p.scale_log2;
+                    if (masked && key0 + 8 * nt + 2 * t4 + (e & 1) >= lim[e >> 1]) s[nt][e] = -INFINITY;
                 }
-            }
-            if (__any_sync(~0u, move)) {
-                l[0] *= f[0];
-                l[1] *= f[1];
+            float x[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                x[e] = fmaxf(fmaxf(s[0][2 * e], s[0][2 * e + 1]), fmaxf(s[1][2 * e], s[1][2 * e + 1]));
+            if (__any_sync(~0u, x[0] > m[0] + 8.f || x[1] > m[1] + 8.f)) {
+                float f[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    x[e] = fmaxf(x[e], __shfl_xor_sync(~0u, x[e], 1));
+                    x[e] = fmaxf(x[e], __shfl_xor_sync(~0u, x[e], 2));
+                    x[e] = fmaxf(x[e], m[e]);
+                    f[e] = ex2(m[e] - (x[e] == -INFINITY ? 0.f : x[e]));
+                    m[e] = x[e];
+                    l[e] *= f[e];
+                }
 #pragma unroll
                 for (int i = 0; i < DP / 8; ++i) {
                     o[i][0] *= f[0];
@@ -585,8 +621,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_decode_kernel(const __grid_c
                 const float sub = m[e] == -INFINITY ? 0.f : m[e] - kShift;
 #pragma unroll
                 for (int nt = 0; nt < 2; ++nt) {
-                    const float a = ex2(fmaf(s[nt][2 * e], p.scale_log2, -sub));
-                    const float b = ex2(fmaf(s[nt][2 * e + 1], p.scale_log2, -sub));
+                    const float a = ex2(s[nt][2 * e] - sub), b = ex2(s[nt][2 * e + 1] - sub);
                     l[e] += a + b;
                     pf[e + 2 * nt] = pack2<kBF16>(a, b);
                 }
@@ -601,9 +636,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_decode_kernel(const __grid_c
             }
         }
         __syncwarp();  // the stage is read; the next request may fill it
-        if (at.tile + 1 == at.seq.tiles || u + 1 == steps)
-            leave(p.mode == kCluster || (tile0 == 0 && at.tile + 1 == at.seq.tiles));
-        if (u + 1 < units) next_unit(p, at);
+        work_st = work_st + 1 == NS ? 0 : work_st + 1;
+        if (at.tile + 1 == at.seq.tiles || u + 1 >= units) leave(p.mode != kFlat || (tile0 == 0 && at.tile + 1 == at.seq.tiles));
+        if (u + 1 < units) next_unit(at, item);
     }
     cp_async_wait<0>();
     if (!waited) pdl_wait();  // what waits for this kernel waits for the one before it, too
@@ -622,7 +657,7 @@ struct JoinParams {
     const int* kv_lens;
     int T, B, Hq, Hk, G, D;
     int page_size, max_pages;
-    int ctas, prefix_splits, prefix_len;
+    int max_rows, ctas, prefix_splits, prefix_len;
 };
 
 template <bool kBF16>
@@ -634,11 +669,14 @@ __global__ void __launch_bounds__(kThreads) attn_join_kernel(const JoinParams p)
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int s = blockIdx.x, hk = blockIdx.y;
     pdl_wait();
-    const Seq me = seq_of(p.cu_q, p.kv_lens, p.T, p.G, p.max_pages, p.page_size, s, nullptr);
+    auto seq_at = [&](int x) {
+        return seq_of(p.cu_q, p.kv_lens, p.T, p.G, p.max_rows, p.max_pages, p.page_size, kUnit, x, nullptr);
+    };
+    const Seq me = seq_at(s);
     if (me.tiles == 0) return;
     long long before = 0, total = 0;
     for (int x = tid; x < p.B; x += kThreads) {
-        const long long n = (long long)seq_of(p.cu_q, p.kv_lens, p.T, p.G, p.max_pages, p.page_size, x, nullptr).tiles * p.Hk;
+        const long long n = (long long)seq_at(x).tiles * p.Hk;
         total += n;
         if (x < s) before += n;
     }
@@ -732,6 +770,11 @@ __global__ void __launch_bounds__(kThreads) attn_join_kernel(const JoinParams p)
     }
 }
 
+// Rows (tokens x G) of a sequence that the kernels take: alone, up to the caller's bound.
+int max_rows(const AttnArgs& a, const DecodeParts& parts) {
+    return parts.only ? std::min(kMaxRows, a.max_q * a.G) : kMaxRows;  // alone: max_q * G <= 16
+}
+
 template <bool kBF16, int DP>
 cudaError_t launch_one(const DecodeParams& p, int ctas, int dev, cudaStream_t s) {
     auto fn = attn_decode_kernel<kBF16, DP>;
@@ -761,11 +804,12 @@ cudaError_t launch_one(const DecodeParams& p, int ctas, int dev, cudaStream_t s)
 
 }  // namespace
 
-DecodePlan decode_plan(int B, int Hk, int max_kv, int sms) {
+DecodePlan decode_plan(int B, int Hk, int max_q, int max_kv, int sms) {
     const long long items = (long long)B * Hk;
     const int tiles = std::max(1, (max_kv + kUnit - 1) / kUnit);
     DecodePlan pl{};
     pl.cluster = 1;
+    pl.group = kWarps;
     // A cluster per item while they fill no more than the SMs and no CTA has more than
     // 8 units (1024 keys, 0.5 MB): beyond, a share of every SM is faster in spite of
     // the join's launch.
@@ -777,10 +821,20 @@ DecodePlan decode_plan(int B, int Hk, int max_kv, int sms) {
         pl.ctas = (int)items * cs;
         return pl;
     }
-    // Whole items where a CTA's longest share stays within 16 units (1 MB).
-    const long long share = (items + sms - 1) / sms * tiles;
-    pl.mode = share <= 16 ? kWhole : kFlat;
-    pl.ctas = (int)std::min<long long>(sms, pl.mode == kWhole ? items : items * tiles);
+    // Whole items where no group has more than 24 units of work, with so many warps an
+    // item that one round takes all items if it can.  (Groups of fewer than 8 warps
+    // have no room for values that only some of a sequence's rows see: one row each.)
+    int W = kWarps;
+    while (W > 1 && max_q == 1 && items * W > (long long)sms * kWarps) W /= 2;
+    const long long slots = (long long)sms * (kWarps / W), rounds = (items + slots - 1) / slots;
+    if (rounds * std::max(1, (max_kv + kSlice * W - 1) / (kSlice * W)) <= 24) {
+        pl.mode = kWhole;
+        pl.group = W;
+        pl.ctas = (int)std::min<long long>(sms, (items + kWarps / W - 1) / (kWarps / W));
+        return pl;
+    }
+    pl.mode = kFlat;
+    pl.ctas = (int)std::min<long long>(sms, items * tiles);
     return pl;
 }
 
@@ -819,6 +873,8 @@ cudaError_t launch_attn_decode(const AttnArgs& a, const DecodeParts& parts) {
     p.only = parts.only;
     p.mode = parts.plan.mode;
     p.cluster = parts.plan.cluster;
+    p.group = parts.plan.group;
+    p.max_rows = max_rows(a, parts);
     p.slot_o = parts.slot_o;
     p.slot_l = parts.slot_l;
     p.own_o = parts.own_o;
@@ -837,8 +893,8 @@ cudaError_t launch_attn_decode(const AttnArgs& a, const DecodeParts& parts) {
 
 cudaError_t launch_attn_join(const AttnArgs& a, const DecodeParts& parts) {
     JoinParams j{parts.slot_o, parts.slot_l, parts.own_o, parts.own_l, parts.pre_o, parts.pre_l, a.o, a.o_st, a.o_sh, a.lse,
-                 a.cu_q, a.kv_lens, a.T, a.B, a.Hq, a.Hk, a.G, a.D, a.page_size, a.max_pages, parts.plan.ctas,
-                 parts.prefix_splits, a.prefix_len};
+                 a.cu_q, a.kv_lens, a.T, a.B, a.Hq, a.Hk, a.G, a.D, a.page_size, a.max_pages, max_rows(a, parts),
+                 parts.plan.ctas, parts.prefix_splits, a.prefix_len};
     auto fn = a.dtype == DType::BF16 ? attn_join_kernel<true> : attn_join_kernel<false>;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)a.B, (unsigned)a.Hk);

@@ -926,7 +926,7 @@ AttnPlan attn_plan(int T, int B, int max_q, int Hq, int Hk, int D, bool paged, i
     pl.planes = pl.prefix;
     if (pl.tile && pl.own + pl.prefix > 1) pl.planes += pl.own;
     if (pl.decode) {
-        pl.dec = decode_plan(B, Hk, max_kv, sms);
+        pl.dec = decode_plan(B, Hk, max_q, max_kv, sms);
         pl.join = pl.dec.mode == kFlat;
         if (pl.join) pl.slots = (size_t)pl.dec.ctas * 2 * kDecodeRows;
         if (pl.join && pl.prefix) ++pl.planes;
