@@ -74,4 +74,74 @@ __device__ __forceinline__ void wait_bar(uint64_t* bar, uint32_t parity, int* ga
     }
 }
 
+// A box of the 4-D tensor map into shared memory; its bytes count on `bar`.
+__device__ __forceinline__ void tma_load_4d(void* dst, const void* map, int c0, int c1, int c2, int c3, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::
+            "r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(smem_u32(bar))
+        : "memory");
+}
+
+__device__ __forceinline__ float warp_max(float x) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) x = fmaxf(x, __shfl_xor_sync(~0u, x, o));
+    return x;
+}
+__device__ __forceinline__ float warp_sum(float x) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(~0u, x, o);
+    return x;
+}
+
+// One row's partial results on their way to the output: sums of 2^(x - top) v in
+// acc (four dims d .. d + 3 of this lane) and of 2^(x - top) in sum.
+struct Row {
+    float acc[4], sum, top;
+};
+
+// Joins n partials to it: normalised outputs po[at(i)][D], log2 of their sums pl[at(i)].
+// 32 sums at a time (a lane each), eight outputs requested at a time.
+template <typename At>
+__device__ __forceinline__ void join_parts(Row& x, int n, const float* po, const float* pl, int D, int d, At at) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll 1
+    for (int c = 0; c < n; c += 32) {
+        const float l2 = c + lane < n ? pl[at(c + lane)] : -INFINITY;
+        const float top = fmaxf(x.top, warp_max(l2));
+        const float base = top == -INFINITY ? 0.f : top;
+        const float f = ex2(x.top - base), w = ex2(l2 - base);
+        x.top = top;
+        x.sum = x.sum * f + warp_sum(w);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x.acc[e] *= f;
+#pragma unroll 1
+        for (int s = 0; s < min(32, n - c); s += 8) {
+            float4 o[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                o[i] = c + s + i < n && d < D ? *reinterpret_cast<const float4*>(po + at(c + s + i) * D + d)
+                                              : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float ws = __shfl_sync(~0u, w, s + i);
+                x.acc[0] += ws * o[i].x;
+                x.acc[1] += ws * o[i].y;
+                x.acc[2] += ws * o[i].z;
+                x.acc[3] += ws * o[i].w;
+            }
+        }
+    }
+}
+
+// Normalises it; log2 of its sum.  A row without any weight is 0 where it sees no key,
+// and NaN (0 / 0) where its scores are all -inf.
+__device__ __forceinline__ float finish_row(Row& x, bool sees) {
+    const bool some = x.sum != 0.f;
+    const float inv = some ? 1.f / x.sum : sees ? NAN : 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x.acc[e] = some ? x.acc[e] * inv : inv;
+    return some ? x.top + log2f(x.sum) : -INFINITY;
+}
+
 }  // namespace hq

@@ -3,6 +3,8 @@
 
 #include "hq_internal.h"
 
+#include <cuda.h>
+
 namespace hq {
 
 struct AttnArgs {
@@ -55,6 +57,9 @@ cudaError_t launch_overlapped(void (*fn)(P), unsigned grid, unsigned threads, si
     cfg.numAttrs = overlap ? 1 : 0;
     return cudaLaunchKernelEx(&cfg, fn, p);
 }
+
+// Tensor maps of the keys and values, boxes of 64 dims x box_rows tokens.
+cudaError_t kv_maps(const AttnArgs& a, int box_rows, CUtensorMap* k_map, CUtensorMap* v_map);
 
 // How the decode kernel's CTAs share the items, the (sequence, key/value head)s.
 enum DecodeMode : int { kFlat = 0, kWhole = 1, kCluster = 2 };

@@ -5,8 +5,9 @@
 // An item is one (sequence, key/value head); W warps work on it (8, a CTA; fewer
 // where there are more items than CTAs and they are short), in units of 16 W keys.  A
 // warp takes 16 keys of each unit, which lie in one page, through a ring of its own
-// in shared memory (cp.async, three units of 8 KB ahead; nothing but its own copies
-// to wait for): 128 KB in flight per SM, several times bandwidth x latency.
+// in shared memory (TMA boxes of 16 keys x 64 dims, two units of 8 KB ahead; nothing
+// but its own copies to wait for): 128 KB in flight per SM, several times bandwidth x
+// latency.  (cp.async instead of TMA took 700 of a unit's 2200 cycles to issue.)
 //   S = Q K^T  mma.sync m16n8k16, the 16 rows (padded) x 16 keys
 //   P = 2^(c S - m), a running maximum m and sum per warp and row; m is moved, with O
 //              and the sum, only when a score is above it by more than 2^8, which a
@@ -25,9 +26,13 @@
 // The CTAs work their share out from the lengths on the device, so no plan is made
 // beforehand and a captured call follows them.  With a shared prefix its partials
 // (tile kernel) are joined with the item's own before it is written.
+// A short call is bound by fetching this code: it is kept in loops, each step in one
+// place.
 #include "hq_attn.cuh"
+#include "hq_tmap.h"
 
 #include <algorithm>
+#include <cstring>
 #include <type_traits>
 
 namespace hq {
@@ -43,21 +48,20 @@ constexpr int kMaxRows = kDecodeRows;      // 16: the MMA's M
 template <int DP>
 struct DecodeLayout {
     static constexpr int kStages = 384 / DP;            // 3 (DP 128) or 6: 24 KB a warp
-    static constexpr int kStage = 2 * kSlice * DP * 2;  // K, then V
+    static constexpr int kBlk = DP / 64;                // 64-dim blocks of 128-byte rows
+    static constexpr int kHalf = kBlk * kSlice * 128;   // K or V of a stage
+    static constexpr int kStage = 2 * kHalf;
     static constexpr int kRing = kWarps * kStages * kStage;
-    static constexpr int kPitch = DP + 2;               // floats of a row in the join buffer
-    static constexpr int kJoin = kWarps * 8 * kPitch * 4;
-    static constexpr int kSmem = kRing + kJoin;
+    static constexpr int kJoin = kWarps * 8 * DP * 4;   // 8 rows of every warp
 };
 
-struct DecodeParams {
+struct alignas(64) DecodeParams {
+    CUtensorMap k_map, v_map;  // {dim, token, head, page}, boxes of 64 x 16
     const void* q;
     long long q_st, q_sh;
     void* o;
     long long o_st, o_sh;
     float* lse;
-    const void *k, *v;
-    long long k_sp, k_st, k_sh, v_sp, v_st, v_sh;
     const int* cu_q;
     const int* table;
     long long table_stride;
@@ -100,17 +104,11 @@ __device__ __forceinline__ Seq seq_of(const int* cu_q, const int* kv_lens, int T
     return q;
 }
 
-// A place in the line of units.
+// A unit of an item.
 struct Place {
     int s, h, tile;
     Seq seq;
 };
-
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
 
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -139,68 +137,39 @@ __device__ __forceinline__ long long block_sum(long long x, long long* scratch) 
     return x;
 }
 
-// One row's partial results on their way to the output: sums of 2^(x - top) v in
-// acc (four dims d .. d + 3 of this lane) and of 2^(x - top) in sum.
-struct Row {
-    float acc[4], sum, top;
+template <int DP>
+struct DecodeShared {
+    uint64_t full[kWarps][DecodeLayout<DP>::kStages];
+    Place place[kWarps][DecodeLayout<DP>::kStages];  // the unit in a stage
+    float m[kWarps][kMaxRows], l[kWarps][kMaxRows];
+    unsigned bad[2][DP];  // keys (bit j: key len - 16 + j) whose value in that dim is NaN | +Inf << 16, -Inf
+    int any_bad, gave_up;
 };
-
-// Joins the prefix's partials of row `row` to it.
-__device__ __forceinline__ void join_prefix(const float* pre_o, const float* pre_l, int splits, size_t rows, size_t row, int D,
-                                            int d, Row& x) {
-    const int lane = threadIdx.x & 31;
-    const float l2 = lane < splits ? pre_l[lane * rows + row] : -INFINITY;  // splits <= 32
-    float top = fmaxf(x.top, l2);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-    const float base = top == -INFINITY ? 0.f : top;
-    const float f = ex2(x.top - base), w = ex2(l2 - base);
-    x.sum *= f;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) x.acc[e] *= f;
-    // eight partials requested at a time
-#pragma unroll 1
-    for (int s0 = 0; s0 < splits; s0 += 8) {
-        float4 o[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            o[i] = s0 + i < splits && d < D ? *reinterpret_cast<const float4*>(pre_o + ((s0 + i) * rows + row) * D + d)
-                                            : make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float ws = __shfl_sync(~0u, w, (s0 + i) & 31);
-            if (s0 + i >= splits) continue;
-            x.sum += ws;
-            x.acc[0] += ws * o[i].x;
-            x.acc[1] += ws * o[i].y;
-            x.acc[2] += ws * o[i].z;
-            x.acc[3] += ws * o[i].w;
-        }
-    }
-    x.top = top;
-}
 
 template <bool kBF16, int DP>
 __global__ void __launch_bounds__(kThreads, 1) attn_decode_kernel(const __grid_constant__ DecodeParams p) {
     using L = DecodeLayout<DP>;
     using T16 = typename std::conditional<kBF16, __nv_bfloat16, __half>::type;
     constexpr float kShift = kBF16 ? 0.f : 6.f;  // fp16: P scaled by 2^6, as is the sum
-    constexpr int NS = L::kStages, RB = 2 * DP;  // RB: bytes of a key's row
-    constexpr int kChunks = DP / 8;
+    constexpr int NS = L::kStages;
 
-    extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ long long s_scan[kWarps];
-    __shared__ Place s_start;
-    __shared__ float s_m[kWarps][kMaxRows], s_l[kWarps][kMaxRows];
-    __shared__ unsigned s_bad[2][DP];  // keys (bit j: key len - 16 + j) whose value in that dim is NaN | +Inf << 16, -Inf
-    __shared__ int s_any_bad;
-    float* join = reinterpret_cast<float*>(smem + L::kRing);
+    extern __shared__ __align__(1024) uint8_t smem[];
+    DecodeShared<DP>& sh = *reinterpret_cast<DecodeShared<DP>*>(smem + L::kRing + L::kJoin);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int g = lane >> 2, t4 = lane & 3;
     const int W = p.group, gw = warp & (W - 1), w0 = warp - gw;  // this warp in its group, the group's first
     const int unit = kSlice * W;
     const size_t rows = (size_t)p.T * p.Hq;
     pdl_launch_dependents();
+
+    if (lane == 0) {
+        for (int i = 0; i < NS; ++i) mbar_init(&sh.full[warp][i], 1);
+        fence_mbarrier_init();
+        fence_async_smem();
+    }
+    if (tid < 2 * DP) (&sh.bad[0][0])[tid] = 0;
+    if (tid == 0) sh.any_bad = sh.gave_up = 0;
+    __syncthreads();
 
     auto seq_at = [&](int s) {
         const Seq q = seq_of(p.cu_q, p.kv_lens, p.T, p.G, p.max_rows, p.max_pages, p.page_size, unit, s, p.err);
@@ -212,42 +181,27 @@ __global__ void __launch_bounds__(kThreads, 1) attn_decode_kernel(const __grid_c
         else named_bar_sync(1 + w0 / W, 32 * W);
     };
 
-    if (tid < 2 * DP) (&s_bad[0][0])[tid] = 0;
-    if (tid == 0) s_any_bad = 0;
-
-    Place at{};
-    int units = 0x7fffffff;                                            // of this CTA's share
-    const int slots = gridDim.x * (kWarps / W);                        // kWhole: groups
+    // `next` runs through the units of this warp's share; it begins before the first.
+    Place next{};
+    int units = 0x7fffffff;                          // in the share
+    const int slots = gridDim.x * (kWarps / W);      // kWhole: groups, and the next item of this one
     int item = blockIdx.x * (kWarps / W) + w0 / W;
-    // kWhole: the group's next item that has work; s = B: none
-    auto next_item = [&](Place& x, int& i) {
-        const int items = p.B * p.Hk;
-        for (; i < items; i += slots) {
-            x.s = i / p.Hk;
-            x.h = i - x.s * p.Hk;
-            x.tile = 0;
-            x.seq = seq_at(x.s);
-            if (x.seq.tiles) return;
-        }
-        x.s = p.B;
-    };
-    if (p.mode == kWhole) {
-        next_item(at, item);
-        __syncthreads();
-    } else if (p.mode == kCluster) {
+    if (p.mode == kCluster) {
         const int it = blockIdx.x / p.cluster, rank = blockIdx.x % p.cluster;
-        at.s = it / p.Hk;
-        at.h = it - at.s * p.Hk;
-        at.seq = seq_at(at.s);
-        if (at.seq.tiles == 0) {  // in all CTAs of the cluster
+        next.s = it / p.Hk;
+        next.h = it - next.s * p.Hk;
+        next.seq = seq_at(next.s);
+        const int a = (int)((unsigned)(next.seq.tiles * rank) / (unsigned)p.cluster);  // tiles <= 2^24, a cluster 8
+        units = (int)((unsigned)(next.seq.tiles * (rank + 1)) / (unsigned)p.cluster) - a;
+        next.tile = a - 1;
+        if (next.seq.tiles == 0) {  // in all CTAs of the cluster
             if (p.overlap) pdl_wait();
             return;
         }
-        at.tile = (int)((long long)at.seq.tiles * rank / p.cluster);
-        units = (int)((long long)at.seq.tiles * (rank + 1) / p.cluster) - at.tile;
-        __syncthreads();
-    } else {
+    } else if (p.mode == kFlat) {
         // ----------------------------------- this CTA's share of the line
+        long long* scan = reinterpret_cast<long long*>(smem + L::kRing);
+        Place* start = reinterpret_cast<Place*>(scan + kWarps);
         Seq mine{};
         long long count = 0;
 #pragma unroll 1
@@ -255,7 +209,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_decode_kernel(const __grid_c
             mine = seq_at(s);
             count += (long long)mine.tiles * p.Hk;
         }
-        const long long total = block_sum(count, s_scan);
+        const long long total = block_sum(count, scan);
         const long long ctas = min((long long)gridDim.x, total);  // that have work, one unit at least
         if (blockIdx.x >= ctas) {
             if (p.overlap) pdl_wait();
@@ -265,256 +219,112 @@ __global__ void __launch_bounds__(kThreads, 1) attn_decode_kernel(const __grid_c
         units = (int)(total * (blockIdx.x + 1) / ctas - u0);
         long long before = 0;
 #pragma unroll 1
-        for (int s0 = 0; s0 < p.B; s0 += kThreads) {
+        for (int s0 = 0; s0 < p.B && before <= u0; s0 += kThreads) {
             const int s = s0 + tid;
             if (p.B > kThreads) mine = s < p.B ? seq_at(s) : Seq{};
             const long long n = (long long)mine.tiles * p.Hk;
             long long incl = n;
-#pragma unroll
+#pragma unroll 1
             for (int d = 1; d < 32; d <<= 1) {
                 const long long x = __shfl_up_sync(~0u, incl, d);
                 if (lane >= d) incl += x;
             }
             __syncthreads();
-            if (lane == 31) s_scan[warp] = incl;
+            if (lane == 31) scan[warp] = incl;
             __syncthreads();
-            long long lo = before + incl - n, all = before;
-#pragma unroll
+            long long lo = before + incl - n;
+#pragma unroll 1
             for (int w = 0; w < kWarps; ++w) {
-                if (w < warp) lo += s_scan[w];
-                all += s_scan[w];
+                if (w < warp) lo += scan[w];
+                before += scan[w];
             }
             if (n > 0 && u0 >= lo && u0 < lo + n)
-                s_start = Place{s, (int)((u0 - lo) / mine.tiles), (int)((u0 - lo) % mine.tiles), mine};
-            before = all;
-            if (before > u0) break;
+                *start = Place{s, (int)((u0 - lo) / mine.tiles), (int)((u0 - lo) % mine.tiles) - 1, mine};
         }
         __syncthreads();
-        at = s_start;
+        next = *start;
+        __syncthreads();
+    } else {
+        item -= slots;
     }
-    // The unit after x (of this CTA's share, while there are any); s = B behind the last.
-    auto next_unit = [&](Place& x, int& i) {
-        if (++x.tile < x.seq.tiles) return;
-        if (p.mode == kWhole) {
-            i += slots;
-            next_item(x, i);
-            return;
-        }
-        x.tile = 0;
-        if (++x.h < p.Hk) return;
-        x.h = 0;
-        do {
-            if (++x.s >= p.B) return;
-            x.seq = seq_at(x.s);
-        } while (x.seq.tiles == 0);
-    };
 
-    Place ahead = at;  // `at`: the unit in work; `ahead`: the next one to load
-    int ahead_item = item;
     const uint32_t ring = smem_u32(smem) + warp * NS * L::kStage;
-    auto page_of = [&](const Place& x) {
-        const int key = x.tile * unit + gw * kSlice;
-        return x.s < p.B && key < x.seq.len ? __ldg(p.table + x.s * p.table_stride + (key >> p.page_shift)) : 0;
-    };
-    int page = units > 0 ? page_of(ahead) : 0;
-    // This lane's 16-byte chunk of a step's rows r0, r0 + RS, ...: where it is read, and
-    // where it goes (chunk c of row r at chunk c ^ (r & 7)).
-    constexpr int RS = 32 / kChunks;
-    const int chunk = lane % kChunks, r0 = lane / kChunks;
-    const long long k_lane = r0 * p.k_st + chunk * 8, v_lane = r0 * p.v_st + chunk * 8;
-    const uint32_t s_lane = r0 * RB + ((chunk ^ r0) << 4);
+    float* join = reinterpret_cast<float*>(smem + L::kRing);
+    // A cluster CTA's joined rows for the others: [16][DP] sums, [16] maxima and sums,
+    // where the ring was (every warp is past its last unit by then).
+    float* part = reinterpret_cast<float*>(smem);
+    const int d = 4 * lane;  // the dims that this lane joins and writes
 
     uint32_t qf[DP / 16][4];
     float o[DP / 8][4];
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
     int lim[2] = {0, 0}, lim_min = 0, tile0 = 0;
-    bool first_seg = true, fresh = true, waited = !p.overlap;
-
-    // Ends the item in work: joins the warps and writes it, or its partial.
-    auto leave = [&](bool whole) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            l[e] += __shfl_xor_sync(~0u, l[e], 1);
-            l[e] += __shfl_xor_sync(~0u, l[e], 2);
-            if (t4 == 0) {
-                s_m[warp][g + 8 * e] = m[e];
-                s_l[warp][g + 8 * e] = l[e];
-            }
-        }
-        const int R = at.seq.n * p.G;
-        if (p.prefix_splits && p.mode != kFlat && !waited) {  // the prefix's partials are complete
-            pdl_wait();
-            waited = true;
-        }
-        // A cluster's partials: [16][DP] sums, [16] maxima and sums, where the ring was
-        // (every warp is past its last unit at the barrier below).
-        float* part = reinterpret_cast<float*>(smem);
-        const int d = 4 * lane;
-        // row r of the item from its joined sums
-        auto write = [&](int r, Row& x) {
-            const int tok = r / p.G, hd = at.h * p.G + r % p.G;
-            const int see = keys_seen(at.seq.len, at.seq.n, tok, 1);
-            const size_t row = (size_t)(at.seq.first + tok) * p.Hq + hd;
-            const bool out = whole && !p.own_o;
-            if (out && p.prefix_splits) {
-                x.top -= kShift;
-                join_prefix(p.pre_o, p.pre_l, p.prefix_splits, rows, row, p.D, d, x);
-                x.top += kShift;
-            }
-            // no key: zeros; scores that are all -inf: NaN, or left to the join
-            const float inv = x.sum != 0.f ? 1.f / x.sum : (out && see + p.prefix_len > 0 ? NAN : 0.f);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x.acc[e] = x.sum != 0.f ? x.acc[e] * inv : inv;
-            const float l2 = x.sum == 0.f ? -INFINITY : x.top - kShift + log2f(x.sum);
-            if (out) {
-                if (d < p.D)
-                    *reinterpret_cast<uint2*>(static_cast<T16*>(p.o) + (size_t)(at.seq.first + tok) * p.o_st +
-                                              (size_t)hd * p.o_sh + d) =
-                        make_uint2(pack2<kBF16>(x.acc[0], x.acc[1]), pack2<kBF16>(x.acc[2], x.acc[3]));
-                if (lane == 0 && p.lse) p.lse[row] = l2 * 0.693147180559945309417f;
-            } else {
-                const size_t slot = (size_t)(2 * blockIdx.x + (first_seg ? 0 : 1)) * kMaxRows + r;
-                float* dst = whole ? p.own_o + row * p.D : p.slot_o + slot * p.D;
-                if (d < p.D) *reinterpret_cast<float4*>(dst + d) = make_float4(x.acc[0], x.acc[1], x.acc[2], x.acc[3]);
-                if (lane == 0) (whole ? p.own_l[row] : p.slot_l[slot]) = l2;
-            }
-        };
+    bool first_seg = true, fresh = true, waited = !p.overlap, have = false;
+    int page = 0, loaded = 0, load_st = 0, work_st = 0;
+    uint32_t phase = 0;
+    // Step u works on the warp's unit u, requests unit u + NS - 1 and finds the one after
+    // it.  A CTA of a cluster may have no unit; it takes one empty step.
 #pragma unroll 1
-        for (int half = 0; 8 * half < R; ++half) {
-            if (g + 8 * half < R) {
-#pragma unroll
-                for (int i = 0; i < DP / 8; ++i)
-                    *reinterpret_cast<float2*>(join + (warp * 8 + g) * L::kPitch + 8 * i + 2 * t4) =
-                        half ? make_float2(o[i][2], o[i][3]) : make_float2(o[i][0], o[i][1]);
-            }
-            group_sync();
-            // one warp a row, four dims a lane
-#pragma unroll 1
-            for (int r = 8 * half + gw; r < min(R, 8 * half + 8); r += W) {
-                Row x{};
-                x.top = -INFINITY;
-#pragma unroll 4
-                for (int w = 0; w < W; ++w) x.top = fmaxf(x.top, s_m[w0 + w][r]);
-                const float base = x.top == -INFINITY ? 0.f : x.top;
-#pragma unroll 4
-                for (int w = 0; w < W; ++w) {
-                    const float f = ex2(s_m[w0 + w][r] - base);
-                    x.sum += f * s_l[w0 + w][r];
-                    if (d < DP) {
-                        const float2* src = reinterpret_cast<const float2*>(join + ((w0 + w) * 8 + (r & 7)) * L::kPitch + d);
-                        const float2 a = src[0], b = src[1];
-                        x.acc[0] += f * a.x;
-                        x.acc[1] += f * a.y;
-                        x.acc[2] += f * b.x;
-                        x.acc[3] += f * b.y;
-                    }
+    for (int u = -NS;; ++u) {
+        if (have) {
+            // This warp's 16 keys of `next`: whole, their page has them.
+            const int key = next.tile * unit + gw * kSlice;
+            Place* mark = &sh.place[warp][load_st];
+            if (lane == 0) *mark = next;
+            if (key < next.seq.len) {
+                if (!page_ok(page, p.num_pages)) {
+                    bad_index(p.err);
+                    page = p.num_pages;  // out of range: the boxes read zeros
                 }
-                if (s_any_bad && d < DP) {
-                    // of the last 16 keys, the first `vis` are seen
-                    const int vis = keys_seen(at.seq.len, at.seq.n, r / p.G, 1) - (at.seq.len - 16);
-                    const unsigned mask = vis >= 16 ? 0xFFFFu : vis > 0 ? (1u << vis) - 1u : 0u;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const unsigned b0 = s_bad[0][d + e], b1 = s_bad[1][d + e];
-                        if ((b0 >> 16) & mask) x.acc[e] += INFINITY;
-                        if (b1 & mask) x.acc[e] -= INFINITY;
-                        if (b0 & mask) x.acc[e] = NAN;
-                    }
-                }
-                if (p.mode == kCluster) {
-                    if (d < DP) *reinterpret_cast<float4*>(part + r * DP + d) = make_float4(x.acc[0], x.acc[1], x.acc[2], x.acc[3]);
-                    if (lane == 0) {
-                        part[kMaxRows * DP + r] = x.top;
-                        part[kMaxRows * DP + kMaxRows + r] = x.sum;
-                    }
-                } else {
-                    write(r, x);
-                }
-            }
-            group_sync();
-        }
-        if (p.mode == kCluster) {
-            cluster_sync();
-            // the rows over all warps of the cluster
-#pragma unroll 1
-            for (int r = (int)cluster_ctarank() * kWarps + warp; r < R; r += p.cluster * kWarps) {
-                Row x{};
-                const uint32_t base = smem_u32(part);
-                const bool have = lane < p.cluster;  // lane q: CTA q
-                const uint32_t ml = mapa_shared(base + (kMaxRows * DP + r) * 4, have ? lane : 0);
-                const float mq = have ? ld_dsmem_f1(ml) : -INFINITY, lq = have ? ld_dsmem_f1(ml + kMaxRows * 4) : 0.f;
-                x.top = mq;
-#pragma unroll
-                for (int k = 16; k; k >>= 1) x.top = fmaxf(x.top, __shfl_xor_sync(~0u, x.top, k));
-                const float f = ex2(mq - (x.top == -INFINITY ? 0.f : x.top));
-                x.sum = f * lq;
-#pragma unroll
-                for (int k = 16; k; k >>= 1) x.sum += __shfl_xor_sync(~0u, x.sum, k);
-#pragma unroll 4
-                for (int q = 0; q < p.cluster; ++q) {
-                    const float fq = __shfl_sync(~0u, f, q);
-                    if (d >= DP) continue;
-                    const float4 y = ld_dsmem_f4(mapa_shared(base + (r * DP + d) * 4, q));
-                    x.acc[0] += fq * y.x;
-                    x.acc[1] += fq * y.y;
-                    x.acc[2] += fq * y.z;
-                    x.acc[3] += fq * y.w;
-                }
-                write(r, x);
-            }
-            cluster_sync();  // the others' partials have been read
-        } else if (s_any_bad) {  // W = 8: the same in all threads since the barriers above
-            __syncthreads();
-            if (tid < 2 * DP) (&s_bad[0][0])[tid] = 0;
-            if (tid == 0) s_any_bad = 0;
-            __syncthreads();
-        }
-        first_seg = false;
-        fresh = true;
-    };
-
-    // The request of one unit runs NS - 1 units ahead of the work.  A CTA of a cluster
-    // may have no unit; it takes one empty step.
-    int loaded = 0, load_st = 0, work_st = 0;
-#pragma unroll 1
-    for (int u = 1 - NS;; ++u) {
-        if (loaded < units && ahead.s < p.B) {
-            // This warp's keys of unit `ahead`; rows behind the last key and dims behind D
-            // are filled with zeros.
-            const int key = ahead.tile * unit + gw * kSlice;
-            if (key < ahead.seq.len) {
-                const bool ok = page_ok(page, p.num_pages);
-                if (!ok) bad_index(p.err);
-                const long long pg = ok ? page : 0;
-                const int slot = key & (p.page_size - 1), live = ok ? ahead.seq.len - key : 0;
-                const T16* k = static_cast<const T16*>(p.k) + pg * p.k_sp + slot * p.k_st + ahead.h * p.k_sh;
-                const T16* v = static_cast<const T16*>(p.v) + pg * p.v_sp + slot * p.v_st + ahead.h * p.v_sh;
-                const uint32_t dst = ring + load_st * L::kStage + s_lane;
-                const bool dims = chunk * 8 < p.D;
-                const T16 *kl = k + k_lane, *vl = v + v_lane;
-#pragma unroll
-                for (int i = 0; i < kSlice / RS; ++i) {
-                    const bool have = dims && r0 + i * RS < live;
-                    const uint32_t to = (dst ^ ((i * RS & 7) << 4)) + i * RS * RB;
-                    cp_async16_zfill(to, have ? kl : k, have);
-                    cp_async16_zfill(to + kSlice * RB, have ? vl : v, have);
-                    kl += RS * p.k_st;
-                    vl += RS * p.v_st;
+                uint64_t* bar = &sh.full[warp][load_st];
+                uint8_t* dst = smem + warp * NS * L::kStage + load_st * L::kStage;
+                if (lane == 0) mbar_arrive_expect_tx(bar, L::kStage);
+                __syncwarp();
+                if (lane < 2 * L::kBlk) {
+                    const int kv = lane / L::kBlk, blk = lane % L::kBlk;
+                    tma_load_4d(dst + kv * L::kHalf + blk * kSlice * 128, kv ? &p.v_map : &p.k_map, blk * 64,
+                                key & (p.page_size - 1), next.h, page, bar);
                 }
             }
             load_st = load_st + 1 == NS ? 0 : load_st + 1;
-            if (++loaded < units) {
-                next_unit(ahead, ahead_item);
-                page = page_of(ahead);
-            }
+            ++loaded;
         }
-        cp_async_commit();
+        have = false;
+        if (loaded < units && next.s < p.B) {
+            bool found = ++next.tile < next.seq.tiles;
+            if (!found) {
+                next.tile = 0;
+#pragma unroll 1
+                while (true) {  // the next item with work
+                    if (p.mode == kWhole) {
+                        item += slots;
+                        next.s = item / p.Hk;
+                        next.h = item - next.s * p.Hk;
+                    } else if (++next.h == p.Hk) {
+                        next.h = 0;
+                        ++next.s;
+                    }
+                    if (next.s >= p.B) break;
+                    if (p.mode == kWhole || next.h == 0) next.seq = seq_at(next.s);
+                    if (next.seq.tiles > 0) {
+                        found = true;
+                        break;
+                    }
+                    next.h = p.Hk - 1;  // none of this sequence's
+                }
+            }
+            have = found;
+            const int key = next.tile * unit + gw * kSlice;
+            if (found && key < next.seq.len) page = __ldg(p.table + next.s * p.table_stride + (key >> p.page_shift));
+        }
         if (u < 0) continue;
         const bool work = u < loaded;
         if (!work && (p.mode != kCluster || u > 0)) break;
+        __syncwarp();
+        const Place at = work ? sh.place[warp][work_st] : Place{next.s, next.h, next.tile, next.seq};
+        const int R = at.seq.n * p.G;
         if (fresh) {  // a new item: its rows of Q, rows g and g + 8 in this lane
             fresh = false;
-            const int R = at.seq.n * p.G;
             tile0 = at.tile;
             lim_min = keys_seen(at.seq.len, at.seq.n, 0, 1);
 #pragma unroll
@@ -530,8 +340,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_decode_kernel(const __grid_c
                 for (int k = 0; k < DP / 16; ++k)
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
-                        const int d = 16 * k + 8 * x + 2 * t4;
-                        qf[k][e + 2 * x] = live && d < p.D ? __ldg(reinterpret_cast<const uint32_t*>(q + d)) : 0u;
+                        const int dim = 16 * k + 8 * x + 2 * t4;
+                        qf[k][e + 2 * x] = live && dim < p.D ? __ldg(reinterpret_cast<const uint32_t*>(q + dim)) : 0u;
                     }
             }
 #pragma unroll
@@ -539,38 +349,49 @@ __global__ void __launch_bounds__(kThreads, 1) attn_decode_kernel(const __grid_c
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
         }
-        cp_async_wait<NS - 1>();
-        __syncwarp();
         const int key0 = at.tile * unit + gw * kSlice;
         if (work && key0 < at.seq.len) {
-            const uint32_t kst = ring + work_st * L::kStage, vst = kst + kSlice * RB;
+            wait_bar(&sh.full[warp][work_st], phase >> work_st & 1u, &sh.gave_up, p.err);
+            phase ^= 1u << work_st;
+            __syncwarp();
+            // 16-byte chunk c of key r of a 64-dim block lies at chunk c ^ (r & 7)
+            const uint32_t kst = ring + work_st * L::kStage, vst = kst + L::kHalf;
             const bool masked = key0 + kSlice > lim_min;
-            if (masked && at.seq.n > 1) {
-                // Values that only some rows see and that are not finite would reach the
-                // others as 0 x NaN: taken out here, put back into the rows that see them
-                // at the end.  Only the last n <= 16 keys can be such.
+            if (masked) {
+                // Rows of V behind the last key are zeroed: 0 x NaN would reach the sum.
+                // So would values that only some rows see: those are taken out, and put
+                // back into the rows that see them at the end.  Only the last n <= 16
+                // keys can be such.
                 const int lo = max(0, lim_min - key0), hi = min(kSlice, at.seq.len - key0);
 #pragma unroll 1
-                for (int x = lane; x < (hi - lo) * kChunks; x += 32) {
-                    const int r = lo + x / kChunks, c = x % kChunks;
-                    const uint32_t a = vst + r * RB + ((c ^ (r & 7)) << 4);
-                    const uint4 v4 = lds128(a);
-                    if (!not_finite<kBF16>(v4)) continue;
-                    uint32_t w[4] = {v4.x, v4.y, v4.z, v4.w};
-                    constexpr uint32_t kExp = kBF16 ? 0x7F80u : 0x7C00u;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const uint32_t h = (w[e >> 1] >> (16 * (e & 1))) & 0xFFFFu;
-                        if ((h & kExp) != kExp) continue;
-                        const unsigned bit = 1u << (key0 + r - (at.seq.len - 16));
-                        if ((h & 0x7FFFu) != kExp) atomicOr(&s_bad[0][c * 8 + e], bit);
-                        else if (h & 0x8000u) atomicOr(&s_bad[1][c * 8 + e], bit);
-                        else atomicOr(&s_bad[0][c * 8 + e], bit << 16);
-                        w[e >> 1] &= ~(0xFFFFu << (16 * (e & 1)));
+                for (int x = lo * (DP / 8) + lane; x < kSlice * (DP / 8); x += 32) {
+                    const int r = x / (DP / 8), c = x % (DP / 8);
+                    const uint32_t a = vst + (c >> 3) * kSlice * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+                    uint4 v4 = r < hi ? lds128(a) : make_uint4(0u, 0u, 0u, 0u);
+                    if (r < hi && !not_finite<kBF16>(v4)) continue;
+                    if (r < hi) {
+                        uint32_t w[4] = {v4.x, v4.y, v4.z, v4.w};
+                        constexpr uint32_t kExp = kBF16 ? 0x7F80u : 0x7C00u;
+#pragma unroll 1
+                        for (int e = 0; e < 8; ++e) {
+                            const int i = e >> 1, sft = 16 * (e & 1);
+                            const uint32_t word = i == 0 ? w[0] : i == 1 ? w[1] : i == 2 ? w[2] : w[3], h = word >> sft & 0xFFFFu;
+                            if ((h & kExp) != kExp) continue;
+                            const unsigned bit = 1u << (key0 + r - (at.seq.len - 16));
+                            const bool nan = (h & 0x7FFFu) != kExp, minus = h & 0x8000u;
+                            atomicOr(&sh.bad[!nan && minus][c * 8 + e], !nan && !minus ? bit << 16 : bit);
+                            const uint32_t keep = ~(0xFFFFu << sft);
+                            w[0] &= i == 0 ? keep : ~0u;
+                            w[1] &= i == 1 ? keep : ~0u;
+                            w[2] &= i == 2 ? keep : ~0u;
+                            w[3] &= i == 3 ? keep : ~0u;
+                        }
+                        v4 = make_uint4(w[0], w[1], w[2], w[3]);
+                        sh.any_bad = 1;
                     }
-                    sts128(a, make_uint4(w[0], w[1], w[2], w[3]));
-                    s_any_bad = 1;
+                    sts128(a, v4);
                 }
+                fence_async_smem();  // before the next request fills the stage
                 __syncwarp();
             }
             float s[2][4] = {}, s2[2][4] = {};  // even and odd steps: two chains an n-tile
@@ -578,10 +399,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_decode_kernel(const __grid_c
 #pragma unroll
             for (int k = 0; k < DP / 16; k += 2) {
                 uint32_t b[4];
-                ldsm4(kst + kr * RB + (((2 * k + kc) ^ (kr & 7)) << 4), b);
+                const uint32_t row = kst + (k >> 2) * kSlice * 128 + kr * 128;
+                ldsm4(row + ((((2 * k & 7) + kc) ^ (kr & 7)) << 4), b);
                 mma_16816<kBF16>(s[0], qf[k], b[0], b[1]);
                 mma_16816<kBF16>(s[1], qf[k], b[2], b[3]);
-                ldsm4(kst + kr * RB + (((2 * k + 2 + kc) ^ (kr & 7)) << 4), b);
+                ldsm4(row + ((((2 * k + 2 & 7) + kc) ^ (kr & 7)) << 4), b);
                 mma_16816<kBF16>(s2[0], qf[k + 1], b[0], b[1]);
                 mma_16816<kBF16>(s2[1], qf[k + 1], b[2], b[3]);
             }
@@ -630,23 +452,144 @@ __global__ void __launch_bounds__(kThreads, 1) attn_decode_kernel(const __grid_c
 #pragma unroll
             for (int i = 0; i < DP / 16; ++i) {
                 uint32_t b[4];
-                ldsm4_t(vst + vr * RB + (((2 * i + vc) ^ (vr & 7)) << 4), b);
+                ldsm4_t(vst + (i >> 2) * kSlice * 128 + vr * 128 + ((((2 * i & 7) + vc) ^ (vr & 7)) << 4), b);
                 mma_16816<kBF16>(o[2 * i], pf, b[0], b[1]);
                 mma_16816<kBF16>(o[2 * i + 1], pf, b[2], b[3]);
             }
         }
         __syncwarp();  // the stage is read; the next request may fill it
         work_st = work_st + 1 == NS ? 0 : work_st + 1;
-        if (at.tile + 1 == at.seq.tiles || u + 1 >= units) leave(p.mode != kFlat || (tile0 == 0 && at.tile + 1 == at.seq.tiles));
-        if (u + 1 < units) next_unit(at, item);
+        if (at.tile + 1 < at.seq.tiles && u + 1 < units) continue;
+
+        // ------------------------------------------------- the item's end
+        const bool whole = p.mode != kFlat || (tile0 == 0 && at.tile + 1 == at.seq.tiles);
+        if (p.prefix_splits && p.mode != kFlat && !waited) {  // the prefix's partials are complete
+            pdl_wait();
+            waited = true;
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            l[e] += __shfl_xor_sync(~0u, l[e], 1);
+            l[e] += __shfl_xor_sync(~0u, l[e], 2);
+            if (t4 == 0) {
+                sh.m[warp][g + 8 * e] = m[e];
+                sh.l[warp][g + 8 * e] = l[e];
+            }
+        }
+        // Rows 8 half .. 8 half + 7 of the group's warps are joined, one warp a row, four
+        // dims a lane; in a cluster then the CTAs' joined rows.
+        const int levels = p.mode == kCluster ? 2 : 1;
+#pragma unroll 1
+        for (int pass = 0; pass < (R > 8 ? 2 : 1) + levels - 1; ++pass) {
+            const bool across = p.mode == kCluster && pass == (R > 8 ? 2 : 1);  // the CTAs of a cluster
+            int r = 8 * pass + gw, step = W, end = min(R, 8 * pass + 8), sources = W;
+            if (across) {
+                cluster_sync();
+                r = (int)cluster_ctarank() * kWarps + warp;
+                step = p.cluster * kWarps;
+                end = R;
+                sources = p.cluster;
+            } else {
+                if (g + 8 * pass < R) {
+                    float* to = join + (warp * 8 + g) * DP;
+#pragma unroll
+                    for (int i = 0; i < DP / 8; ++i)
+                        *reinterpret_cast<float2*>(to + ((8 * i + 2 * t4) ^ (8 * g & (DP - 1)))) =
+                            pass ? make_float2(o[i][2], o[i][3]) : make_float2(o[i][0], o[i][1]);
+                }
+                group_sync();
+            }
+#pragma unroll 1
+            for (; r < end; r += step) {
+                const int tok = r / p.G, hd = at.h * p.G + r - tok * p.G;
+                const int see = keys_seen(at.seq.len, at.seq.n, tok, 1);
+                const size_t row = (size_t)(at.seq.first + tok) * p.Hq + hd;
+                // source `lane`: its maximum and sum; all their maximum and sum
+                Row x{};
+                float mq = -INFINITY, lq = 0.f;
+                if (lane < sources) {
+                    if (across) {
+                        const uint32_t ml = mapa_shared(smem_u32(part + kMaxRows * DP + r), lane);
+                        mq = ld_dsmem_f1(ml);
+                        lq = ld_dsmem_f1(ml + kMaxRows * 4);
+                    } else {
+                        mq = sh.m[w0 + lane][r];
+                        lq = sh.l[w0 + lane][r];
+                    }
+                }
+                x.top = warp_max(mq);
+                const float f = ex2(mq - (x.top == -INFINITY ? 0.f : x.top));
+                x.sum = warp_sum(f * lq);
+#pragma unroll 2
+                for (int q = 0; q < sources; ++q) {
+                    const float fq = __shfl_sync(~0u, f, q);
+                    if (d >= DP) continue;
+                    const float4 y = across ? ld_dsmem_f4(mapa_shared(smem_u32(part + r * DP + d), q))
+                                            : *reinterpret_cast<const float4*>(join + ((w0 + q) * 8 + (r & 7)) * DP +
+                                                                               (d ^ (8 * (r & 7) & (DP - 1))));
+                    x.acc[0] += fq * y.x;
+                    x.acc[1] += fq * y.y;
+                    x.acc[2] += fq * y.z;
+                    x.acc[3] += fq * y.w;
+                }
+                if (!across && sh.any_bad && d < DP) {
+                    const int vis = see - (at.seq.len - 16);  // of the last 16 keys, the first `vis` are seen
+                    const unsigned mask = vis >= 16 ? 0xFFFFu : vis > 0 ? (1u << vis) - 1u : 0u;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const unsigned b0 = sh.bad[0][d + e], b1 = sh.bad[1][d + e];
+                        if ((b0 >> 16) & mask) x.acc[e] += INFINITY;
+                        if (b1 & mask) x.acc[e] -= INFINITY;
+                        if (b0 & mask) x.acc[e] = NAN;
+                    }
+                }
+                if (p.mode == kCluster && !across) {
+                    if (d < DP) *reinterpret_cast<float4*>(part + r * DP + d) = make_float4(x.acc[0], x.acc[1], x.acc[2], x.acc[3]);
+                    if (lane == 0) {
+                        part[kMaxRows * DP + r] = x.top;
+                        part[kMaxRows * DP + kMaxRows + r] = x.sum;
+                    }
+                    continue;
+                }
+                const bool out = whole && !p.own_o;
+                x.top -= kShift;
+                if (out && p.prefix_splits)
+                    join_parts(x, p.prefix_splits, p.pre_o, p.pre_l, p.D, d, [&](int i) { return i * rows + row; });
+                // no key: zeros; scores that are all -inf: NaN, or left to the join
+                const float l2 = finish_row(x, out && see + p.prefix_len > 0);
+                if (out) {
+                    if (d < p.D)
+                        *reinterpret_cast<uint2*>(static_cast<T16*>(p.o) + (size_t)(at.seq.first + tok) * p.o_st +
+                                                  (size_t)hd * p.o_sh + d) =
+                            make_uint2(pack2<kBF16>(x.acc[0], x.acc[1]), pack2<kBF16>(x.acc[2], x.acc[3]));
+                    if (lane == 0 && p.lse) p.lse[row] = l2 * 0.693147180559945309417f;
+                } else {
+                    const size_t slot = (size_t)(2 * blockIdx.x + (first_seg ? 0 : 1)) * kMaxRows + r;
+                    float* dst = whole ? p.own_o + row * p.D : p.slot_o + slot * p.D;
+                    if (d < p.D) *reinterpret_cast<float4*>(dst + d) = make_float4(x.acc[0], x.acc[1], x.acc[2], x.acc[3]);
+                    if (lane == 0) (whole ? p.own_l[row] : p.slot_l[slot]) = l2;
+                }
+            }
+            if (across) cluster_sync();  // the others' rows have been read
+            else group_sync();
+        }
+        if (p.mode != kCluster && sh.any_bad) {  // W = 8: the same in all threads since the barriers above
+            __syncthreads();
+            if (tid < 2 * DP) (&sh.bad[0][0])[tid] = 0;
+            if (tid == 0) sh.any_bad = 0;
+            __syncthreads();
+        }
+        first_seg = false;
+        fresh = true;
     }
-    cp_async_wait<0>();
+    if (sh.gave_up) {  // copies still in flight land before the CTA exits
+        for (int i = 0; i < NS; ++i) mbar_wait(&sh.full[warp][i], phase >> i & 1u, p.err);
+    }
     if (!waited) pdl_wait();  // what waits for this kernel waits for the one before it, too
 }
 
 // kFlat: joins the partials of every item that more than one CTA worked on, and with
-// a shared prefix of every one, with the prefix's.  One block each; the
-// partials' weights first, then warp w adds up every eighth partial.
+// a shared prefix of every one, with the prefix's.  One block an item, one warp a row.
 struct JoinParams {
     const float *slot_o, *slot_l, *own_o, *own_l;
     const float *pre_o, *pre_l;  // [prefix_splits][T * Hq]
@@ -662,10 +605,7 @@ struct JoinParams {
 
 template <bool kBF16>
 __global__ void __launch_bounds__(kThreads) attn_join_kernel(const JoinParams p) {
-    extern __shared__ __align__(16) float weights[];  // [partials][16]
-    __shared__ float buf[kWarps][8][128];
     __shared__ long long scan[kWarps];
-    __shared__ float s_sum[kMaxRows], s_top[kMaxRows];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int s = blockIdx.x, hk = blockIdx.y;
     pdl_wait();
@@ -675,6 +615,7 @@ __global__ void __launch_bounds__(kThreads) attn_join_kernel(const JoinParams p)
     const Seq me = seq_at(s);
     if (me.tiles == 0) return;
     long long before = 0, total = 0;
+#pragma unroll 1
     for (int x = tid; x < p.B; x += kThreads) {
         const long long n = (long long)seq_at(x).tiles * p.Hk;
         total += n;
@@ -686,87 +627,30 @@ __global__ void __launch_bounds__(kThreads) attn_join_kernel(const JoinParams p)
     const long long ctas = min((long long)p.ctas, total);
     const long long ub = before + (long long)hk * me.tiles, ue = ub + me.tiles;
     const int c0 = (int)(((ub + 1) * ctas - 1) / total), c1 = (int)((ue * ctas - 1) / total);
-    const bool whole = c0 == c1;
-    if (whole && !p.prefix_splits) return;
-    const int own = whole ? 1 : c1 - c0 + 1, parts = own + p.prefix_splits;
-    const int R = me.n * p.G;
+    if (c0 == c1 && !p.prefix_splits) return;
+    const int R = me.n * p.G, d = 4 * lane;
     const size_t rows = (size_t)p.T * p.Hq;
-    const bool mid = ub != total * c0 / ctas;  // CTA c0 begins with another (sequence, head)
-    auto row_of = [&](int r) { return (size_t)(me.first + r / p.G) * p.Hq + hk * p.G + r % p.G; };
-    auto slot_of = [&](int i) { return (size_t)(2 * (c0 + i) + (i == 0 && mid ? 1 : 0)) * kMaxRows; };
-    for (int x = tid; x < parts * kMaxRows; x += kThreads) {
-        const int i = x / kMaxRows, r = x % kMaxRows;
-        if (r < R)
-            weights[x] = i >= own ? p.pre_l[(i - own) * rows + row_of(r)] : whole ? p.own_l[row_of(r)] : p.slot_l[slot_of(i) + r];
-    }
-    __syncthreads();
+    const bool mid = ub != total * c0 / ctas;  // CTA c0 begins with another item
+#pragma unroll 1
     for (int r = warp; r < R; r += kWarps) {
-        float top = -INFINITY, sum = 0.f;
-        for (int i = lane; i < parts; i += 32) top = fmaxf(top, weights[i * kMaxRows + r]);
-        for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
-        const float base = top == -INFINITY ? 0.f : top;
-        for (int i = lane; i < parts; i += 32) {
-            const float w = ex2(weights[i * kMaxRows + r] - base);
-            weights[i * kMaxRows + r] = w;
-            sum += w;
+        const int tok = r / p.G, hd = hk * p.G + r - tok * p.G;
+        const size_t row = (size_t)(me.first + tok) * p.Hq + hd;
+        Row x{};
+        x.top = -INFINITY;
+#pragma unroll 1
+        for (int k = 0; k < (p.prefix_splits ? 2 : 1); ++k) {
+            const bool whole = c0 == c1;
+            const float* po = k ? p.pre_o : whole ? p.own_o : p.slot_o;
+            const float* pl = k ? p.pre_l : whole ? p.own_l : p.slot_l;
+            join_parts(x, k ? p.prefix_splits : c1 - c0 + 1, po, pl, p.D, d, [&](int i) {
+                return k ? i * rows + row : whole ? row : (size_t)(2 * (c0 + i) + (i == 0 && mid ? 1 : 0)) * kMaxRows + r;
+            });
         }
-        for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
-        if (lane == 0) {
-            s_sum[r] = sum;
-            s_top[r] = top;
-        }
-    }
-    __syncthreads();
-    const int d = 4 * lane;
-    for (int r0 = 0; r0 < R; r0 += 8) {
-        const int nr = min(8, R - r0);
-        float acc[8][4] = {};
-        if (d < p.D) {
-            for (int i = warp; i < parts; i += kWarps) {
-                const float* src = i >= own ? p.pre_o + (i - own) * rows * p.D
-                                            : whole ? p.own_o : p.slot_o + slot_of(i) * p.D;
-#pragma unroll
-                for (int r = 0; r < 8; ++r) {
-                    if (r >= nr) continue;
-                    const size_t at = i >= own || whole ? row_of(r0 + r) : (size_t)(r0 + r);
-                    const float4 x = *reinterpret_cast<const float4*>(src + at * p.D + d);
-                    const float w = weights[i * kMaxRows + r0 + r];
-                    acc[r][0] += w * x.x;
-                    acc[r][1] += w * x.y;
-                    acc[r][2] += w * x.z;
-                    acc[r][3] += w * x.w;
-                }
-            }
-        }
-#pragma unroll
-        for (int r = 0; r < 8; ++r)
-            *reinterpret_cast<float4*>(&buf[warp][r][d]) = make_float4(acc[r][0], acc[r][1], acc[r][2], acc[r][3]);
-        __syncthreads();
-        if (warp < nr) {
-            const int r = r0 + warp;
-            float x[4] = {};
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                const float4 y = *reinterpret_cast<const float4*>(&buf[w][warp][d]);
-                x[0] += y.x;
-                x[1] += y.y;
-                x[2] += y.z;
-                x[3] += y.w;
-            }
-            const int tok = r / p.G;
-            const float sum = s_sum[r];
-            const float inv =
-                sum != 0.f ? 1.f / sum : (p.prefix_len + keys_seen(me.len, me.n, tok, 1) > 0 ? NAN : 0.f);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = sum != 0.f ? x[e] * inv : inv;
-            if (d < p.D)
-                *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.o) + (size_t)(me.first + tok) * p.o_st +
-                                          (size_t)(hk * p.G + r % p.G) * p.o_sh + d) =
-                    make_uint2(pack2<kBF16>(x[0], x[1]), pack2<kBF16>(x[2], x[3]));
-            if (p.lse && lane == 0)
-                p.lse[row_of(r)] = sum == 0.f ? -INFINITY : (s_top[r] + log2f(sum)) * 0.693147180559945309417f;
-        }
-        __syncthreads();
+        const float l2 = finish_row(x, p.prefix_len + keys_seen(me.len, me.n, tok, 1) > 0);
+        if (d < p.D)
+            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.o) + (size_t)(me.first + tok) * p.o_st + (size_t)hd * p.o_sh +
+                                      d) = make_uint2(pack2<kBF16>(x.acc[0], x.acc[1]), pack2<kBF16>(x.acc[2], x.acc[3]));
+        if (p.lse && lane == 0) p.lse[row] = l2 * 0.693147180559945309417f;
     }
 }
 
@@ -777,13 +661,14 @@ int max_rows(const AttnArgs& a, const DecodeParts& parts) {
 
 template <bool kBF16, int DP>
 cudaError_t launch_one(const DecodeParams& p, int ctas, int dev, cudaStream_t s) {
+    constexpr int kSmem = DecodeLayout<DP>::kRing + DecodeLayout<DP>::kJoin + (int)sizeof(DecodeShared<DP>);
     auto fn = attn_decode_kernel<kBF16, DP>;
-    cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(fn), dev, DecodeLayout<DP>::kSmem);
+    cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(fn), dev, kSmem);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)ctas);
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = (size_t)DecodeLayout<DP>::kSmem;
+    cfg.dynamicSmemBytes = (size_t)kSmem;
     cfg.stream = s;
     cudaLaunchAttribute attr[2];
     cfg.attrs = attr;
@@ -839,7 +724,10 @@ DecodePlan decode_plan(int B, int Hk, int max_q, int max_kv, int sms) {
 }
 
 cudaError_t launch_attn_decode(const AttnArgs& a, const DecodeParts& parts) {
-    DecodeParams p{};
+    DecodeParams p;
+    memset(&p, 0, sizeof p);
+    cudaError_t e = kv_maps(a, kSlice, &p.k_map, &p.v_map);
+    if (e != cudaSuccess) return e;
     p.q = a.q;
     p.q_st = a.q_st;
     p.q_sh = a.q_sh;
@@ -847,14 +735,6 @@ cudaError_t launch_attn_decode(const AttnArgs& a, const DecodeParts& parts) {
     p.o_st = a.o_st;
     p.o_sh = a.o_sh;
     p.lse = a.lse;
-    p.k = a.k;
-    p.v = a.v;
-    p.k_sp = a.k_sp;
-    p.k_st = a.k_st;
-    p.k_sh = a.k_sh;
-    p.v_sp = a.v_sp;
-    p.v_st = a.v_st;
-    p.v_sh = a.v_sh;
     p.cu_q = a.cu_q;
     p.table = a.table;
     p.table_stride = a.table_stride;
@@ -899,7 +779,6 @@ cudaError_t launch_attn_join(const AttnArgs& a, const DecodeParts& parts) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)a.B, (unsigned)a.Hk);
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = (size_t)(parts.plan.ctas + parts.prefix_splits) * kMaxRows * 4;
     cfg.stream = a.stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

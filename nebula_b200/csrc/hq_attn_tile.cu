@@ -17,10 +17,12 @@
 // since it was last moved: until then the sums stay exact in fp32 and P, at most
 // 2^8 (2^14 in fp16, see kShift), in range.
 //
-// CTAs stay on their SM: warp 0 asks the launch hardware for the next block of
-// the grid (cluster launch control) and works out its rows and keys while the
-// others are on the current one; the next block's Q and first keys are loaded, and
-// its first S computed, while this one's output is written.
+// CTAs stay on their SM: warp 0 takes the next block of the grid and works out its
+// rows and keys while the others are on the current one; the next block's Q and first
+// keys are loaded, and its first S computed, while this one's output is written.
+// Where there are more blocks than SMs it asks the launch hardware for the next
+// (cluster launch control), so that CTAs share them as they get done; else every CTA
+// has its own, and blocks that the lengths leave without rows cost nothing.
 //   warp 0        the blocks, and their loads: one TMA box per 64 dims and up to 128
 //                 keys of a page (page numbers from the table), K and V tiles
 //                 alternate in a ring
@@ -83,6 +85,7 @@ struct alignas(64) TileParams {
     int page_size, box_rows, num_pages, max_pages;  // page_size 0: packed rows
     int prefix_len;                                 // > 0: all T rows over the pages table[0..]
     int blocks, splits;  // the grid: row blocks x Hk x splits
+    int ask;        // blocks are shared out by cluster launch control
     int overlap;    // launched while the kernel before it runs
     int skip_rows;  // sequences of at most this many rows (tokens x G) are not this kernel's
     unsigned* err;
@@ -110,14 +113,6 @@ struct TileShared {
     int gave_up;
     uint16_t bad[2][3][128];
 };
-
-__device__ __forceinline__ void tma_load_4d(void* dst, const void* map, int c0, int c1, int c2, int c3, uint64_t* bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::
-            "r"(smem_u32(dst)),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(smem_u32(bar))
-        : "memory");
-}
 
 // Shared-memory matrix descriptor, N contiguous (V as the B operand): 128-byte
 // swizzle, 64-element blocks kBlkBytes apart, groups of 8 keys 1024 bytes apart.
@@ -425,11 +420,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
         regs_down<kRegsLoad>();
         const int boxes = kKeys / p.box_rows;
         int index = (int)blockIdx.x, use = 0;
+        bool any = true;
         for (int k = 0, asked = 0;; ++asked) {
-            if (lane == 0) next_block_request(&sh.next_block, &sh.next);
+            if (p.ask && lane == 0) next_block_request(&sh.next_block, &sh.next);
             __syncwarp();
             Item it;
-            if (make_item(p, index, it)) {
+            const bool found = any && make_item(p, index, it);
+            any = found;  // the numbers behind one without rows have none either
+            if (found) {
                 if (k >= 2) wait(&sh.item_empty[k & 1], (uint32_t)((k - 2) >> 1));
                 __syncwarp();
                 if (sh.any_bad[k & 1]) {
@@ -469,9 +467,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
                     }
                 }
             }
-            wait(&sh.next, (uint32_t)asked);
-            __syncwarp();
-            index = gave_up() ? -1 : next_block_answer(&sh.next_block);
+            if (p.ask) {
+                wait(&sh.next, (uint32_t)asked);
+                __syncwarp();
+                index = gave_up() ? -1 : next_block_answer(&sh.next_block);
+            } else {
+                const bool last = index >= p.blocks * p.Hk * p.splits - (int)gridDim.x;
+                index = last || !any || gave_up() ? -1 : index + (int)gridDim.x;
+            }
             if (index < 0) {
                 if (k >= 2) wait(&sh.item_empty[k & 1], (uint32_t)((k - 2) >> 1));
                 __syncwarp();
@@ -486,7 +489,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
         __syncwarp();
         // Every stage filled here has been consumed (its commits have landed) before exit.
 #pragma unroll 1
-        for (int j = max(0, use - S); j < use; ++j) wait(&sh.empty[j % S], (uint32_t)(j / S));
+        for (int j = max(0, use - S); j < use; ++j) mbar_wait(&sh.empty[j % S], (uint32_t)(j / S) & 1u, p.err);
     } else if (warp == 1) {
         // ----------------------------------------------------------- MMAs
         // The whole warp walks the loops, on values that the compiler can see to be
@@ -809,8 +812,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
 }
 
 // Merges the splits of every row: out = sum_s w_s o_s / sum_s w_s, w_s = 2^(l_s - max l)
-// for split s's normalised output o_s and log2 of its sum l_s.  One warp a row and
-// head, four dims a lane; reads each partial once.
+// for split s's normalised output o_s and log2 of its sum l_s.  One warp a row and head.
 struct MergeParams {
     const float *part_o, *part_l;
     void* o;
@@ -845,50 +847,36 @@ __global__ void __launch_bounds__(256) attn_merge_kernel(const MergeParams p) {
         if (hit) seen = __shfl_sync(~0u, k, __ffs(hit) - 1);
     }
     if (seen < 0) return;
-    float m = -INFINITY;
-    for (int s = lane; s < p.splits; s += 32) m = fmaxf(m, p.part_l[s * rows + row]);
-    for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, d));
-    const float base = m == -INFINITY ? 0.f : m;
-    const bool have = 4 * lane < p.D;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    float l = 0.f;
-#pragma unroll 4
-    for (int s = 0; s < p.splits; ++s) {
-        const float w = ex2(p.part_l[s * rows + row] - base);
-        l += w;
-        if (!have) continue;
-        const float4 x = *reinterpret_cast<const float4*>(p.part_o + (s * rows + row) * p.D + 4 * lane);
-        o.x += w * x.x;
-        o.y += w * x.y;
-        o.z += w * x.z;
-        o.w += w * x.w;
+    Row x{};
+    x.top = -INFINITY;
+    const int d = 4 * lane;
+    join_parts(x, p.splits, p.part_o, p.part_l, p.D, d, [&](int s) { return s * rows + row; });
+    const float l2 = finish_row(x, seen + p.prefix_len > 0);
+    if (d < p.D) {
+        uint16_t* dst = static_cast<uint16_t*>(p.o) + (size_t)t * p.o_st + (size_t)h * p.o_sh + d;
+        *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<kBF16>(x.acc[0], x.acc[1]), pack2<kBF16>(x.acc[2], x.acc[3]));
     }
-    const float inv = l != 0.f ? 1.f / l : (seen + p.prefix_len > 0 ? NAN : 0.f);
-    if (l == 0.f) o = make_float4(1.f, 1.f, 1.f, 1.f);
-    if (have) {
-        uint16_t* dst = static_cast<uint16_t*>(p.o) + (size_t)t * p.o_st + (size_t)h * p.o_sh + 4 * lane;
-        *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<kBF16>(o.x * inv, o.y * inv), pack2<kBF16>(o.z * inv, o.w * inv));
-    }
-    if (p.lse && lane == 0) p.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.693147180559945309417f;
+    if (p.lse && lane == 0) p.lse[row] = l2 * 0.693147180559945309417f;
 }
 
 int ceil_div(long long a, int b) { return (int)((a + b - 1) / b); }
 
 template <bool kBF16, int DP>
-cudaError_t launch_tile(const TileParams& p, int dev, cudaStream_t s) {
+cudaError_t launch_tile(const TileParams& p, int dev, int sms, cudaStream_t s) {
     constexpr int kSmem = TileLayout<DP>::kShared + (int)sizeof(TileShared);
     auto fn = attn_tile_kernel<kBF16, DP>;
     cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(fn), dev, kSmem);
     if (e != cudaSuccess) return e;
-    const long long grid = (long long)p.blocks * p.Hk * p.splits;
-    if (grid > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
+    const long long all = (long long)p.blocks * p.Hk * p.splits;
+    if (all > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
+    const long long grid = p.ask ? all : std::min<long long>(all, sms);
     return launch_overlapped(fn, (unsigned)grid, kThreads, kSmem, s, p.overlap, p);
 }
 
 cudaError_t launch_tile_any(const AttnArgs& a, const TileParams& p) {
     if (a.D <= 64)
-        return a.dtype == DType::BF16 ? launch_tile<true, 64>(p, a.dev, a.stream) : launch_tile<false, 64>(p, a.dev, a.stream);
-    return a.dtype == DType::BF16 ? launch_tile<true, 128>(p, a.dev, a.stream) : launch_tile<false, 128>(p, a.dev, a.stream);
+        return a.dtype == DType::BF16 ? launch_tile<true, 64>(p, a.dev, a.sm_count, a.stream) : launch_tile<false, 64>(p, a.dev, a.sm_count, a.stream);
+    return a.dtype == DType::BF16 ? launch_tile<true, 128>(p, a.dev, a.sm_count, a.stream) : launch_tile<false, 128>(p, a.dev, a.sm_count, a.stream);
 }
 
 // Key splits of `blocks` x Hk CTAs over `keys` keys: enough to fill the SMs once,
@@ -899,7 +887,9 @@ int key_splits(long long rows, int Hk, int keys, int sms) {
     return (int)std::max(1LL, std::min({(long long)sms / items, (long long)by_keys, 32LL}));
 }
 
-cudaError_t kv_maps(const AttnArgs& a, TileParams& p) {
+}  // namespace
+
+cudaError_t kv_maps(const AttnArgs& a, int box_rows, CUtensorMap* k_map, CUtensorMap* v_map) {
     // A dimension of one element takes any legal stride.
     const uint64_t any = 16;
     const uint64_t tokens = a.page_size ? a.page_size : a.T, pages = a.page_size ? a.num_pages : 1;
@@ -907,13 +897,11 @@ cudaError_t kv_maps(const AttnArgs& a, TileParams& p) {
     auto one = [&](CUtensorMap* m, const void* base, long long st, long long sh, long long sp) {
         const uint64_t strides[3] = {tokens > 1 ? 2 * (uint64_t)st : any, a.Hk > 1 ? 2 * (uint64_t)sh : any,
                                      pages > 1 ? 2 * (uint64_t)sp : any};
-        return make_tmap_4d(m, base, dims, strides, (uint32_t)p.box_rows);
+        return make_tmap_4d(m, base, dims, strides, (uint32_t)box_rows);
     };
-    cudaError_t e = one(&p.k_map, a.k, a.k_st, a.k_sh, a.k_sp);
-    return e != cudaSuccess ? e : one(&p.v_map, a.v, a.v_st, a.v_sh, a.v_sp);
+    cudaError_t e = one(k_map, a.k, a.k_st, a.k_sh, a.k_sp);
+    return e != cudaSuccess ? e : one(v_map, a.v, a.v_st, a.v_sh, a.v_sp);
 }
-
-}  // namespace
 
 AttnPlan attn_plan(int T, int B, int max_q, int Hq, int Hk, int D, bool paged, int max_kv, int prefix_len, int sms) {
     AttnPlan pl{};
@@ -970,7 +958,7 @@ cudaError_t launch_attn(const AttnArgs& a) {
         p.num_pages = a.num_pages;
         p.max_pages = a.max_pages;
         p.err = a.err;
-        if ((e = kv_maps(a, p)) != cudaSuccess) return e;
+        if ((e = kv_maps(a, p.box_rows, &p.k_map, &p.v_map)) != cudaSuccess) return e;
     }
     const int row_blocks = ceil_div((long long)a.T * a.G, 2 * kRows);
     if (pl.prefix) {
@@ -981,6 +969,7 @@ cudaError_t launch_attn(const AttnArgs& a) {
         x.part_o = plane_o;
         x.part_l = plane_l;
         x.blocks = row_blocks;
+        x.ask = (long long)row_blocks * a.Hk * x.splits > a.sm_count;
         if ((e = launch_tile_any(a, x)) != cudaSuccess) return e;
     }
     if (pl.tile) {
@@ -994,6 +983,7 @@ cudaError_t launch_attn(const AttnArgs& a) {
         p.part_l = part ? plane_l + pl.prefix * rows : nullptr;
         // every sequence may end inside a block
         p.blocks = (int)std::min((long long)row_blocks + a.B, 0x7fffffffLL);
+        p.ask = (long long)row_blocks * a.Hk * p.splits > a.sm_count;
         if ((e = launch_tile_any(a, p)) != cudaSuccess) return e;
     }
     if (pl.decode) {
