@@ -60,6 +60,9 @@ cudaError_t launch_overlapped(void (*fn)(P), unsigned grid, unsigned threads, si
 
 // Tensor maps of the keys and values, boxes of 64 dims x box_rows tokens.
 cudaError_t kv_maps(const AttnArgs& a, int box_rows, CUtensorMap* k_map, CUtensorMap* v_map);
+// Pages of 128 dims with the dims as two blocks of 64, both in a box: {64, token, block,
+// head, page}; the boxes lie in shared memory as two of kv_maps'.
+cudaError_t kv_maps_128(const AttnArgs& a, int box_rows, CUtensorMap* k_map, CUtensorMap* v_map);
 
 // How the decode kernel's CTAs share the items, the (sequence, key/value head)s.
 enum DecodeMode : int { kFlat = 0, kWhole = 1, kCluster = 2 };

@@ -5,9 +5,9 @@
 // An item is one (sequence, key/value head); W warps work on it (8, a CTA; fewer
 // where there are more items than CTAs and they are short), in units of 16 W keys.  A
 // warp takes 16 keys of each unit, which lie in one page, through a ring of its own
-// in shared memory (TMA boxes of 16 keys x 64 dims, two units of 8 KB ahead; nothing
-// but its own copies to wait for): 128 KB in flight per SM, several times bandwidth x
-// latency.  (cp.async instead of TMA took 700 of a unit's 2200 cycles to issue.)
+// in shared memory (a TMA box of 16 keys each of K and V, two units of 8 KB ahead;
+// nothing but its own copies to wait for): 128 KB in flight per SM, several times
+// bandwidth x latency.
 //   S = Q K^T  mma.sync m16n8k16, the 16 rows (padded) x 16 keys
 //   P = 2^(c S - m), a running maximum m and sum per warp and row; m is moved, with O
 //              and the sum, only when a score is above it by more than 2^8, which a
@@ -56,7 +56,7 @@ struct DecodeLayout {
 };
 
 struct alignas(64) DecodeParams {
-    CUtensorMap k_map, v_map;  // {dim, token, head, page}, boxes of 64 x 16
+    CUtensorMap k_map, v_map;  // {64 dims, token, 64-dim block, head, page}: see kv_maps
     const void* q;
     long long q_st, q_sh;
     void* o;
@@ -69,6 +69,7 @@ struct alignas(64) DecodeParams {
     int T, B, Hq, Hk, G, D;
     int page_size, page_shift, num_pages, max_pages;
     float scale_log2;
+    int whole_box;  // the maps have all dims in a box
     int only;  // no other kernel takes the sequences of more rows
     int mode, cluster;
     int group;  // W: warps of an item
@@ -259,7 +260,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_decode_kernel(const __grid_c
     float o[DP / 8][4];
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
     int lim[2] = {0, 0}, lim_min = 0, tile0 = 0;
-    bool first_seg = true, fresh = true, waited = !p.overlap, have = false;
+    bool first_seg = true, fresh = true, waited = !p.overlap, have = false, starts = false;
+    Place at{};
     int page = 0, loaded = 0, load_st = 0, work_st = 0;
     uint32_t phase = 0;
     // Step u works on the warp's unit u, requests unit u + NS - 1 and finds the one after
@@ -269,21 +271,27 @@ __global__ void __launch_bounds__(kThreads, 1) attn_decode_kernel(const __grid_c
         if (have) {
             // This warp's 16 keys of `next`: whole, their page has them.
             const int key = next.tile * unit + gw * kSlice;
-            Place* mark = &sh.place[warp][load_st];
-            if (lane == 0) *mark = next;
-            if (key < next.seq.len) {
-                if (!page_ok(page, p.num_pages)) {
-                    bad_index(p.err);
-                    page = p.num_pages;  // out of range: the boxes read zeros
-                }
-                uint64_t* bar = &sh.full[warp][load_st];
-                uint8_t* dst = smem + warp * NS * L::kStage + load_st * L::kStage;
-                if (lane == 0) mbar_arrive_expect_tx(bar, L::kStage);
-                __syncwarp();
-                if (lane < 2 * L::kBlk) {
-                    const int kv = lane / L::kBlk, blk = lane % L::kBlk;
-                    tma_load_4d(dst + kv * L::kHalf + blk * kSlice * 128, kv ? &p.v_map : &p.k_map, blk * 64,
-                                key & (p.page_size - 1), next.h, page, bar);
+            if (lane == 0) {
+                if (starts) sh.place[warp][load_st] = next;
+                if (key < next.seq.len) {
+                    if (!page_ok(page, p.num_pages)) {
+                        bad_index(p.err);
+                        page = p.num_pages;  // out of range: the boxes read zeros
+                    }
+                    uint64_t* bar = &sh.full[warp][load_st];
+                    uint8_t* dst = smem + (warp * NS + load_st) * L::kStage;
+                    const int slot = key & (p.page_size - 1);
+                    mbar_arrive_expect_tx(bar, L::kStage);
+                    if (p.whole_box) {
+                        tma_load_5d(dst, &p.k_map, 0, slot, 0, next.h, page, bar);
+                        tma_load_5d(dst + L::kHalf, &p.v_map, 0, slot, 0, next.h, page, bar);
+                    } else {
+#pragma unroll 1
+                        for (int b = 0; b < L::kBlk; ++b) {
+                            tma_load_4d(dst + b * kSlice * 128, &p.k_map, 64 * b, slot, next.h, page, bar);
+                            tma_load_4d(dst + L::kHalf + b * kSlice * 128, &p.v_map, 64 * b, slot, next.h, page, bar);
+                        }
+                    }
                 }
             }
             load_st = load_st + 1 == NS ? 0 : load_st + 1;
@@ -314,14 +322,21 @@ __global__ void __launch_bounds__(kThreads, 1) attn_decode_kernel(const __grid_c
                 }
             }
             have = found;
+            starts = next.tile == 0 || loaded == 0;
             const int key = next.tile * unit + gw * kSlice;
             if (found && key < next.seq.len) page = __ldg(p.table + next.s * p.table_stride + (key >> p.page_shift));
         }
         if (u < 0) continue;
         const bool work = u < loaded;
         if (!work && (p.mode != kCluster || u > 0)) break;
-        __syncwarp();
-        const Place at = work ? sh.place[warp][work_st] : Place{next.s, next.h, next.tile, next.seq};
+        if (!fresh) {
+            ++at.tile;
+        } else if (work) {
+            __syncwarp();
+            at = sh.place[warp][work_st];
+        } else {
+            at = next;
+        }
         const int R = at.seq.n * p.G;
         if (fresh) {  // a new item: its rows of Q, rows g and g + 8 in this lane
             fresh = false;
@@ -665,6 +680,7 @@ cudaError_t launch_one(const DecodeParams& p, int ctas, int dev, cudaStream_t s)
     auto fn = attn_decode_kernel<kBF16, DP>;
     cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(fn), dev, kSmem);
     if (e != cudaSuccess) return e;
+    static_assert(kSmem <= 227 * 1024, "shared memory of an SM");
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)ctas);
     cfg.blockDim = dim3(kThreads);
@@ -726,7 +742,8 @@ DecodePlan decode_plan(int B, int Hk, int max_q, int max_kv, int sms) {
 cudaError_t launch_attn_decode(const AttnArgs& a, const DecodeParts& parts) {
     DecodeParams p;
     memset(&p, 0, sizeof p);
-    cudaError_t e = kv_maps(a, kSlice, &p.k_map, &p.v_map);
+    p.whole_box = a.D == 128;
+    cudaError_t e = p.whole_box ? kv_maps_128(a, kSlice, &p.k_map, &p.v_map) : kv_maps(a, kSlice, &p.k_map, &p.v_map);
     if (e != cudaSuccess) return e;
     p.q = a.q;
     p.q_st = a.q_st;

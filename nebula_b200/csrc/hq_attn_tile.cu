@@ -864,6 +864,8 @@ int ceil_div(long long a, int b) { return (int)((a + b - 1) / b); }
 template <bool kBF16, int DP>
 cudaError_t launch_tile(const TileParams& p, int dev, int sms, cudaStream_t s) {
     constexpr int kSmem = TileLayout<DP>::kShared + (int)sizeof(TileShared);
+    static_assert(kSmem <= 227 * 1024, "shared memory of an SM");
+    static_assert(kSmem <= 227 * 1024, "shared memory of an SM");
     auto fn = attn_tile_kernel<kBF16, DP>;
     cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(fn), dev, kSmem);
     if (e != cudaSuccess) return e;
@@ -894,10 +896,24 @@ cudaError_t kv_maps(const AttnArgs& a, int box_rows, CUtensorMap* k_map, CUtenso
     const uint64_t any = 16;
     const uint64_t tokens = a.page_size ? a.page_size : a.T, pages = a.page_size ? a.num_pages : 1;
     const uint64_t dims[4] = {(uint64_t)a.D, tokens, (uint64_t)a.Hk, pages};
+    const uint32_t box[4] = {64, (uint32_t)box_rows, 1, 1};
     auto one = [&](CUtensorMap* m, const void* base, long long st, long long sh, long long sp) {
         const uint64_t strides[3] = {tokens > 1 ? 2 * (uint64_t)st : any, a.Hk > 1 ? 2 * (uint64_t)sh : any,
                                      pages > 1 ? 2 * (uint64_t)sp : any};
-        return make_tmap_4d(m, base, dims, strides, (uint32_t)box_rows);
+        return make_tmap_16bit(m, base, 4, dims, strides, box);
+    };
+    cudaError_t e = one(k_map, a.k, a.k_st, a.k_sh, a.k_sp);
+    return e != cudaSuccess ? e : one(v_map, a.v, a.v_st, a.v_sh, a.v_sp);
+}
+
+cudaError_t kv_maps_128(const AttnArgs& a, int box_rows, CUtensorMap* k_map, CUtensorMap* v_map) {
+    const uint64_t any = 16;
+    const uint64_t dims[5] = {64, (uint64_t)a.page_size, 2, (uint64_t)a.Hk, (uint64_t)a.num_pages};
+    const uint32_t box[5] = {64, (uint32_t)box_rows, 2, 1, 1};
+    auto one = [&](CUtensorMap* m, const void* base, long long st, long long sh, long long sp) {
+        const uint64_t strides[4] = {2 * (uint64_t)st, 128, a.Hk > 1 ? 2 * (uint64_t)sh : any,
+                                     a.num_pages > 1 ? 2 * (uint64_t)sp : any};
+        return make_tmap_16bit(m, base, 5, dims, strides, box);
     };
     cudaError_t e = one(k_map, a.k, a.k_st, a.k_sh, a.k_sp);
     return e != cudaSuccess ? e : one(v_map, a.v, a.v_st, a.v_sh, a.v_sp);

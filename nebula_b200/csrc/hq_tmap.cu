@@ -36,15 +36,19 @@ cudaError_t make_tmap_2d(CUtensorMap* out, const void* base, CUtensorMapDataType
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
-cudaError_t make_tmap_4d(CUtensorMap* out, const void* base, const uint64_t (&dims)[4], const uint64_t (&strides)[3],
-                         uint32_t rows) {
+cudaError_t make_tmap_16bit(CUtensorMap* out, const void* base, int rank, const uint64_t* dims, const uint64_t* strides,
+                            const uint32_t* box) {
     auto fn = encode_fn();
     if (!fn) return cudaErrorNotSupported;
-    cuuint64_t d[4] = {dims[0], dims[1], dims[2], dims[3]};
-    cuuint64_t st[3] = {strides[0], strides[1], strides[2]};
-    cuuint32_t box[4] = {64, rows, 1, 1};
-    cuuint32_t estride[4] = {1, 1, 1, 1};
-    CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void*>(base), d, st, box, estride,
+    cuuint64_t d[5], st[4];
+    cuuint32_t bx[5], estride[5];
+    for (int i = 0; i < rank; ++i) {
+        d[i] = dims[i];
+        bx[i] = box[i];
+        estride[i] = 1;
+        if (i + 1 < rank) st[i] = strides[i];
+    }
+    CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT16, (cuuint32_t)rank, const_cast<void*>(base), d, st, bx, estride,
                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;

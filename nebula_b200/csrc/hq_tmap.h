@@ -14,9 +14,10 @@ cudaError_t make_tmap_2d(CUtensorMap* out, const void* base, CUtensorMapDataType
                          uint64_t outer, uint64_t row_bytes, uint32_t box_inner, uint32_t box_outer,
                          CUtensorMapSwizzle swizzle);
 
-// 4-D tensor of 16-bit elements, innermost dimension first; strides of dimensions
-// 1..3 in bytes (multiples of 16).  128-byte swizzle, boxes of 64 x rows x 1 x 1.
-cudaError_t make_tmap_4d(CUtensorMap* out, const void* base, const uint64_t (&dims)[4], const uint64_t (&strides)[3],
-                         uint32_t rows);
+// Tensor of 16-bit elements of `rank` (3 to 5) dimensions, innermost first; strides of
+// dimensions 1 .. rank - 1 in bytes (multiples of 16).  128-byte swizzle: the box's
+// innermost dimension is 64.
+cudaError_t make_tmap_16bit(CUtensorMap* out, const void* base, int rank, const uint64_t* dims, const uint64_t* strides,
+                            const uint32_t* box);
 
 }  // namespace hq
