@@ -13,6 +13,18 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+__device__ __forceinline__ float lg2(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ float rcp(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 template <bool kBF16>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     uint32_t w;
@@ -146,10 +158,10 @@ __device__ __forceinline__ void join_parts(Row& x, int n, const float* po, const
 // and NaN (0 / 0) where its scores are all -inf.
 __device__ __forceinline__ float finish_row(Row& x, bool sees) {
     const bool some = x.sum != 0.f;
-    const float inv = some ? 1.f / x.sum : sees ? NAN : 0.f;
+    const float inv = some ? rcp(x.sum) : sees ? NAN : 0.f;
 #pragma unroll
     for (int e = 0; e < 4; ++e) x.acc[e] = some ? x.acc[e] * inv : inv;
-    return some ? x.top + log2f(x.sum) : -INFINITY;
+    return some ? x.top + lg2(x.sum) : -INFINITY;
 }
 
 }  // namespace hq

@@ -35,8 +35,10 @@ struct AttnArgs {
     cudaStream_t stream;
 };
 
-// Sequences of at most kDecodeRows rows (tokens x G) over pages are the decode
-// kernel's, where it is launched; all others the tile kernel's.
+// Sequences of at most AttnPlan::dec_rows rows (tokens x G) over pages are the decode
+// kernel's, all others the tile kernel's.  Alone, the decode kernel takes up to
+// kDecodeRows; beside the tile kernel up to 8, the fewest that it computes, if they
+// hold a token.
 constexpr int kDecodeRows = 16;
 
 // Launches a kernel; with `overlap` it may start while the kernel before it on the
@@ -78,6 +80,7 @@ struct AttnPlan {
     int prefix;          // key splits of the shared prefix (0: none)
     int own;             // key splits of the tile kernel
     DecodePlan dec;
+    int dec_rows;
     bool join;           // partials of the decode kernel are joined by a kernel
     size_t planes;       // partials of every (row, head): prefix, tile, decode
     size_t slots;        // rows of the decode kernel's slots
@@ -89,7 +92,7 @@ cudaError_t launch_attn(const AttnArgs& a);
 // The decode kernel's partial results and those of the prefix that they join.
 struct DecodeParts {
     DecodePlan plan;
-    int only, overlap;
+    int rows, only, overlap;
     float *slot_o, *slot_l;  // [ctas][2][16][D], [ctas][2][16]
     float *own_o, *own_l;    // [T * Hq][D], [T * Hq]: with a prefix and kFlat
     const float *pre_o, *pre_l;

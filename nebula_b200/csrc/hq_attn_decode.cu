@@ -8,13 +8,15 @@
 // in shared memory (a TMA box of 16 keys each of K and V, two units of 8 KB ahead;
 // nothing but its own copies to wait for): 128 KB in flight per SM, several times
 // bandwidth x latency.
-//   S = Q K^T  mma.sync m16n8k16, the 16 rows (padded) x 16 keys
-//   P = 2^(c S - m), a running maximum m and sum per warp and row; m is moved, with O
-//              and the sum, only when a score is above it by more than 2^8, which a
-//              vote tells: lanes need not agree on each unit's maximum
-//   O += P V   mma.sync, P straight from S's registers
-// The tensor rate is no bound here: 16 rows x 128 dims x 2 products a key need a
-// tenth of the rate that mma.sync has while 512 bytes of it arrive.
+//   S^T = K Q^T    mma.sync m16n8k16: 16 keys x 8 rows (or 2 x 8)
+//   P^T = 2^(c S - m), a running maximum m and sum per warp and row; m is moved, with O
+//                  and the sum, only when a score is above it by more than 2^8, which
+//                  a vote tells: lanes need not agree on each unit's maximum
+//   O^T += V^T P^T mma.sync, V^T by transposing loads, P^T by an 8 x 8 transpose of the
+//                  registers
+// The tensor rate is no bound here, but with two warps a scheduler the instructions of
+// a unit are: with the few rows as the MMA's N side there are half as many as with the
+// rows as its M side, padded to 16.
 // At an item's end the warps' sums are joined in shared memory.  Who takes which
 // units (DecodeMode; decode_plan chooses):
 //   kCluster  few items: a cluster of CTAs each, which join through distributed
@@ -43,7 +45,7 @@ constexpr int kWarps = 8;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kSlice = 16;                 // keys of a warp in a unit
 constexpr int kUnit = kSlice * kWarps;     // keys of a unit of a whole CTA
-constexpr int kMaxRows = kDecodeRows;      // 16: the MMA's M
+constexpr int kMaxRows = kDecodeRows;      // 16
 
 template <int DP>
 struct DecodeLayout {
@@ -68,7 +70,7 @@ struct alignas(64) DecodeParams {
     const int* kv_lens;
     int T, B, Hq, Hk, G, D;
     int page_size, page_shift, num_pages, max_pages;
-    float scale_log2;
+    float scale_log2, inv_scale_log2;
     int whole_box;  // the maps have all dims in a box
     int only;  // no other kernel takes the sequences of more rows
     int mode, cluster;
@@ -124,6 +126,13 @@ __device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
                  : "memory");
 }
 
+// 8 x 8 16-bit values, a row in four lanes, transposed.
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
 // Sum of x over the block; `scratch`: kWarps values.  Two barriers.
 __device__ __forceinline__ long long block_sum(long long x, long long* scratch) {
     const int lane = threadIdx.x & 31;
@@ -147,7 +156,7 @@ struct DecodeShared {
     int any_bad, gave_up;
 };
 
-template <bool kBF16, int DP>
+template <bool kBF16, int DP, int NT>  // NT: groups of 8 rows
 __global__ void __launch_bounds__(kThreads, 1) attn_decode_kernel(const __grid_constant__ DecodeParams p) {
     using L = DecodeLayout<DP>;
     using T16 = typename std::conditional<kBF16, __nv_bfloat16, __half>::type;
@@ -256,10 +265,19 @@ __global__ void __launch_bounds__(kThreads, 1) attn_decode_kernel(const __grid_c
     float* part = reinterpret_cast<float*>(smem);
     const int d = 4 * lane;  // the dims that this lane joins and writes
 
-    uint32_t qf[DP / 16][4];
-    float o[DP / 8][4];
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-    int lim[2] = {0, 0}, lim_min = 0, tile0 = 0;
+    // This lane's part of Q^T (row g of each group), of O^T (dims 16 i + g, + 8; rows
+    // 2 t4, + 1), and rows 2 t4, + 1's maximum, sum, limit of keys, and the score above
+    // which the maximum is moved.
+    uint32_t qf[NT][DP / 16][2];
+    float o[NT][DP / 16][4];
+    float m[NT][2], l[NT][2], high[NT][2];
+    int lim[NT][2], lim_min = 0, tile0 = 0;
+    const int* pages = nullptr;  // of `next`
+    // 16-byte chunk c of key r of a 64-dim block lies at chunk c ^ (r & 7): this lane's
+    // addresses within K and V of a stage for the matrices of dims 0 .. 15
+    const int kr = (lane >> 3 & 1) * 8 + (lane & 7), vr = (lane >> 4) * 8 + (lane & 7);
+    const uint32_t ka = ring + kr * 128 + (((lane >> 4) ^ (kr & 7)) << 4);
+    const uint32_t va = ring + L::kHalf + vr * 128 + (((lane >> 3 & 1) ^ (vr & 7)) << 4);
     bool first_seg = true, fresh = true, waited = !p.overlap, have = false, starts = false;
     Place at{};
     int page = 0, loaded = 0, load_st = 0, work_st = 0;
@@ -324,7 +342,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_decode_kernel(const __grid_c
             have = found;
             starts = next.tile == 0 || loaded == 0;
             const int key = next.tile * unit + gw * kSlice;
-            if (found && key < next.seq.len) page = __ldg(p.table + next.s * p.table_stride + (key >> p.page_shift));
+            if (starts) pages = p.table + next.s * p.table_stride;
+            if (found && key < next.seq.len) page = __ldg(pages + (key >> p.page_shift));
         }
         if (u < 0) continue;
         const bool work = u < loaded;
@@ -338,39 +357,42 @@ __global__ void __launch_bounds__(kThreads, 1) attn_decode_kernel(const __grid_c
             at = next;
         }
         const int R = at.seq.n * p.G;
-        if (fresh) {  // a new item: its rows of Q, rows g and g + 8 in this lane
+        if (fresh) {  // a new item: its rows of Q
             fresh = false;
             tile0 = at.tile;
             lim_min = keys_seen(at.seq.len, at.seq.n, 0, 1);
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int r = g + 8 * e;
+            for (int nt = 0; nt < NT; ++nt) {
+                const int r = 8 * nt + g;
                 const bool live = r < R;
                 const int tok = live ? r / p.G : 0, hd = at.h * p.G + (live ? r - tok * p.G : 0);
-                lim[e] = live ? keys_seen(at.seq.len, at.seq.n, tok, 1) : at.seq.len;
-                m[e] = -INFINITY;
-                l[e] = 0.f;
                 const T16* q = static_cast<const T16*>(p.q) + (size_t)(at.seq.first + tok) * p.q_st + (size_t)hd * p.q_sh;
 #pragma unroll
                 for (int k = 0; k < DP / 16; ++k)
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
                         const int dim = 16 * k + 8 * x + 2 * t4;
-                        qf[k][e + 2 * x] = live && dim < p.D ? __ldg(reinterpret_cast<const uint32_t*>(q + dim)) : 0u;
+                        qf[nt][k][x] = live && dim < p.D ? __ldg(reinterpret_cast<const uint32_t*>(q + dim)) : 0u;
                     }
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int row = 8 * nt + 2 * t4 + e;
+                    lim[nt][e] = keys_seen(at.seq.len, at.seq.n, min(row, R - 1) / p.G, 1);
+                    m[nt][e] = high[nt][e] = -INFINITY;
+                    l[nt][e] = 0.f;
+                }
+#pragma unroll
+                for (int i = 0; i < DP / 16; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[nt][i][e] = 0.f;
             }
-#pragma unroll
-            for (int i = 0; i < DP / 8; ++i)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
         }
         const int key0 = at.tile * unit + gw * kSlice;
         if (work && key0 < at.seq.len) {
             wait_bar(&sh.full[warp][work_st], phase >> work_st & 1u, &sh.gave_up, p.err);
             phase ^= 1u << work_st;
             __syncwarp();
-            // 16-byte chunk c of key r of a 64-dim block lies at chunk c ^ (r & 7)
-            const uint32_t kst = ring + work_st * L::kStage, vst = kst + L::kHalf;
+            const uint32_t st = work_st * L::kStage, vst = ring + st + L::kHalf;
             const bool masked = key0 + kSlice > lim_min;
             if (masked) {
                 // Rows of V behind the last key are zeroed: 0 x NaN would reach the sum.
@@ -409,67 +431,63 @@ __global__ void __launch_bounds__(kThreads, 1) attn_decode_kernel(const __grid_c
                 fence_async_smem();  // before the next request fills the stage
                 __syncwarp();
             }
-            float s[2][4] = {}, s2[2][4] = {};  // even and odd steps: two chains an n-tile
-            const int kr = ((lane >> 4) << 3) + (lane & 7), kc = (lane >> 3) & 1;
+            float s[NT][4] = {}, s2[NT][4] = {};  // even and odd steps: two chains
 #pragma unroll
-            for (int k = 0; k < DP / 16; k += 2) {
-                uint32_t b[4];
-                const uint32_t row = kst + (k >> 2) * kSlice * 128 + kr * 128;
-                ldsm4(row + ((((2 * k & 7) + kc) ^ (kr & 7)) << 4), b);
-                mma_16816<kBF16>(s[0], qf[k], b[0], b[1]);
-                mma_16816<kBF16>(s[1], qf[k], b[2], b[3]);
-                ldsm4(row + ((((2 * k + 2 & 7) + kc) ^ (kr & 7)) << 4), b);
-                mma_16816<kBF16>(s2[0], qf[k + 1], b[0], b[1]);
-                mma_16816<kBF16>(s2[1], qf[k + 1], b[2], b[3]);
+            for (int k = 0; k < DP / 16; ++k) {
+                uint32_t a[4];
+                ldsm4(((ka + st) ^ ((2 * k & 7) << 4)) + (k >> 2) * kSlice * 128, a);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) mma_16816<kBF16>(k & 1 ? s2[nt] : s[nt], a, qf[nt][k][0], qf[nt][k][1]);
             }
+            bool above = false;
 #pragma unroll
-            for (int nt = 0; nt < 2; ++nt)
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    s[nt][e] = (s[nt][e] + s2[nt][e]) * p.scale_log2;
-                    if (masked && key0 + 8 * nt + 2 * t4 + (e & 1) >= lim[e >> 1]) s[nt][e] = -INFINITY;
+                    s[nt][e] += s2[nt][e];
+                    if (masked && key0 + g + 8 * (e >> 1) >= lim[nt][e & 1]) s[nt][e] = -INFINITY;
+                    above = above || s[nt][e] > high[nt][e & 1];
                 }
-            float x[2];
+            if (__any_sync(~0u, above)) {
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
-                x[e] = fmaxf(fmaxf(s[0][2 * e], s[0][2 * e + 1]), fmaxf(s[1][2 * e], s[1][2 * e + 1]));
-            if (__any_sync(~0u, x[0] > m[0] + 8.f || x[1] > m[1] + 8.f)) {
-                float f[2];
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    x[e] = fmaxf(x[e], __shfl_xor_sync(~0u, x[e], 1));
-                    x[e] = fmaxf(x[e], __shfl_xor_sync(~0u, x[e], 2));
-                    x[e] = fmaxf(x[e], m[e]);
-                    f[e] = ex2(m[e] - (x[e] == -INFINITY ? 0.f : x[e]));
-                    m[e] = x[e];
-                    l[e] *= f[e];
-                }
+                    for (int e = 0; e < 2; ++e) {
+                        float x = fmaxf(s[nt][e], s[nt][e + 2]);
+                        x = fmaxf(x, __shfl_xor_sync(~0u, x, 4));
+                        x = fmaxf(x, __shfl_xor_sync(~0u, x, 8));
+                        x = fmaxf(x, __shfl_xor_sync(~0u, x, 16)) * p.scale_log2;
+                        x = fmaxf(x, m[nt][e]);
+                        const float f = ex2(m[nt][e] - (x == -INFINITY ? 0.f : x));
+                        m[nt][e] = x;
+                        high[nt][e] = (x + 8.f) * p.inv_scale_log2;
+                        l[nt][e] *= f;
 #pragma unroll
-                for (int i = 0; i < DP / 8; ++i) {
-                    o[i][0] *= f[0];
-                    o[i][1] *= f[0];
-                    o[i][2] *= f[1];
-                    o[i][3] *= f[1];
-                }
+                        for (int i = 0; i < DP / 16; ++i) {
+                            o[nt][i][e] *= f;
+                            o[nt][i][e + 2] *= f;
+                        }
+                    }
             }
-            uint32_t pf[4];
+            uint32_t pf[NT][2];
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const float sub = m[e] == -INFINITY ? 0.f : m[e] - kShift;
+            for (int nt = 0; nt < NT; ++nt) {
+                float w[4];
 #pragma unroll
-                for (int nt = 0; nt < 2; ++nt) {
-                    const float a = ex2(s[nt][2 * e] - sub), b = ex2(s[nt][2 * e + 1] - sub);
-                    l[e] += a + b;
-                    pf[e + 2 * nt] = pack2<kBF16>(a, b);
+                for (int e = 0; e < 4; ++e) {
+                    const float sub = m[nt][e & 1] == -INFINITY ? 0.f : kShift - m[nt][e & 1];
+                    w[e] = ex2(fmaf(s[nt][e], p.scale_log2, sub));
+                    l[nt][e & 1] += w[e];
                 }
+                pf[nt][0] = transpose8x8(pack2<kBF16>(w[0], w[1]));
+                pf[nt][1] = transpose8x8(pack2<kBF16>(w[2], w[3]));
             }
-            const int vr = (((lane >> 3) & 1) << 3) + (lane & 7), vc = lane >> 4;
 #pragma unroll
             for (int i = 0; i < DP / 16; ++i) {
-                uint32_t b[4];
-                ldsm4_t(vst + (i >> 2) * kSlice * 128 + vr * 128 + ((((2 * i & 7) + vc) ^ (vr & 7)) << 4), b);
-                mma_16816<kBF16>(o[2 * i], pf, b[0], b[1]);
-                mma_16816<kBF16>(o[2 * i + 1], pf, b[2], b[3]);
+                uint32_t a[4];
+                ldsm4_t(((va + st) ^ ((2 * i & 7) << 4)) + (i >> 2) * kSlice * 128, a);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) mma_16816<kBF16>(o[nt][i], a, pf[nt][0], pf[nt][1]);
             }
         }
         __syncwarp();  // the stage is read; the next request may fill it
@@ -483,15 +501,19 @@ __global__ void __launch_bounds__(kThreads, 1) attn_decode_kernel(const __grid_c
             waited = true;
         }
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            l[e] += __shfl_xor_sync(~0u, l[e], 1);
-            l[e] += __shfl_xor_sync(~0u, l[e], 2);
-            if (t4 == 0) {
-                sh.m[warp][g + 8 * e] = m[e];
-                sh.l[warp][g + 8 * e] = l[e];
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float x = l[nt][e];
+                x += __shfl_xor_sync(~0u, x, 4);
+                x += __shfl_xor_sync(~0u, x, 8);
+                x += __shfl_xor_sync(~0u, x, 16);
+                if (g == 0) {
+                    sh.m[warp][8 * nt + 2 * t4 + e] = m[nt][e];
+                    sh.l[warp][8 * nt + 2 * t4 + e] = x;
+                }
             }
-        }
-        // Rows 8 half .. 8 half + 7 of the group's warps are joined, one warp a row, four
+        // Rows 8 pass .. 8 pass + 7 of the group's warps are joined, one warp a row, four
         // dims a lane; in a cluster then the CTAs' joined rows.
         const int levels = p.mode == kCluster ? 2 : 1;
 #pragma unroll 1
@@ -505,12 +527,16 @@ __global__ void __launch_bounds__(kThreads, 1) attn_decode_kernel(const __grid_c
                 end = R;
                 sources = p.cluster;
             } else {
-                if (g + 8 * pass < R) {
-                    float* to = join + (warp * 8 + g) * DP;
 #pragma unroll
-                    for (int i = 0; i < DP / 8; ++i)
-                        *reinterpret_cast<float2*>(to + ((8 * i + 2 * t4) ^ (8 * g & (DP - 1)))) =
-                            pass ? make_float2(o[i][2], o[i][3]) : make_float2(o[i][0], o[i][1]);
+                for (int e = 0; e < 2; ++e) {
+                    const int row = 2 * t4 + e, flip = 8 * row & (DP - 1);  // dim d of row r at d ^ 8 r: the four rows of a store in two halves of the banks
+                    float* to = join + (warp * 8 + row) * DP;
+                    if (row + 8 * pass >= R) continue;
+#pragma unroll
+                    for (int i = 0; i < DP / 16; ++i) {
+                        to[(16 * i + g) ^ flip] = NT > 1 && pass ? o[NT - 1][i][e] : o[0][i][e];
+                        to[(16 * i + g + 8) ^ flip] = NT > 1 && pass ? o[NT - 1][i][e + 2] : o[0][i][e + 2];
+                    }
                 }
                 group_sync();
             }
@@ -669,15 +695,10 @@ __global__ void __launch_bounds__(kThreads) attn_join_kernel(const JoinParams p)
     }
 }
 
-// Rows (tokens x G) of a sequence that the kernels take: alone, up to the caller's bound.
-int max_rows(const AttnArgs& a, const DecodeParts& parts) {
-    return parts.only ? std::min(kMaxRows, a.max_q * a.G) : kMaxRows;  // alone: max_q * G <= 16
-}
-
-template <bool kBF16, int DP>
+template <bool kBF16, int DP, int NT>
 cudaError_t launch_one(const DecodeParams& p, int ctas, int dev, cudaStream_t s) {
     constexpr int kSmem = DecodeLayout<DP>::kRing + DecodeLayout<DP>::kJoin + (int)sizeof(DecodeShared<DP>);
-    auto fn = attn_decode_kernel<kBF16, DP>;
+    auto fn = attn_decode_kernel<kBF16, DP, NT>;
     cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(fn), dev, kSmem);
     if (e != cudaSuccess) return e;
     static_assert(kSmem <= 227 * 1024, "shared memory of an SM");
@@ -701,6 +722,15 @@ cudaError_t launch_one(const DecodeParams& p, int ctas, int dev, cudaStream_t s)
         ++cfg.numAttrs;
     }
     return cudaLaunchKernelEx(&cfg, fn, p);
+}
+
+template <int NT>
+cudaError_t launch_any(const AttnArgs& a, const DecodeParams& p, int ctas) {
+    if (a.D <= 64)
+        return a.dtype == DType::BF16 ? launch_one<true, 64, NT>(p, ctas, a.dev, a.stream)
+                                      : launch_one<false, 64, NT>(p, ctas, a.dev, a.stream);
+    return a.dtype == DType::BF16 ? launch_one<true, 128, NT>(p, ctas, a.dev, a.stream)
+                                  : launch_one<false, 128, NT>(p, ctas, a.dev, a.stream);
 }
 
 }  // namespace
@@ -767,11 +797,12 @@ cudaError_t launch_attn_decode(const AttnArgs& a, const DecodeParts& parts) {
     p.num_pages = a.num_pages;
     p.max_pages = a.max_pages;
     p.scale_log2 = a.scale * 1.44269504088896340736f;
+    p.inv_scale_log2 = 1.f / p.scale_log2;
     p.only = parts.only;
     p.mode = parts.plan.mode;
     p.cluster = parts.plan.cluster;
     p.group = parts.plan.group;
-    p.max_rows = max_rows(a, parts);
+    p.max_rows = parts.rows;
     p.slot_o = parts.slot_o;
     p.slot_l = parts.slot_l;
     p.own_o = parts.own_o;
@@ -782,15 +813,12 @@ cudaError_t launch_attn_decode(const AttnArgs& a, const DecodeParts& parts) {
     p.prefix_len = a.prefix_len;
     p.overlap = parts.overlap;
     p.err = a.err;
-    const int ctas = parts.plan.ctas;
-    if (a.D <= 64)
-        return a.dtype == DType::BF16 ? launch_one<true, 64>(p, ctas, a.dev, a.stream) : launch_one<false, 64>(p, ctas, a.dev, a.stream);
-    return a.dtype == DType::BF16 ? launch_one<true, 128>(p, ctas, a.dev, a.stream) : launch_one<false, 128>(p, ctas, a.dev, a.stream);
+    return parts.rows > 8 ? launch_any<2>(a, p, parts.plan.ctas) : launch_any<1>(a, p, parts.plan.ctas);
 }
 
 cudaError_t launch_attn_join(const AttnArgs& a, const DecodeParts& parts) {
     JoinParams j{parts.slot_o, parts.slot_l, parts.own_o, parts.own_l, parts.pre_o, parts.pre_l, a.o, a.o_st, a.o_sh, a.lse,
-                 a.cu_q, a.kv_lens, a.T, a.B, a.Hq, a.Hk, a.G, a.D, a.page_size, a.max_pages, max_rows(a, parts),
+                 a.cu_q, a.kv_lens, a.T, a.B, a.Hq, a.Hk, a.G, a.D, a.page_size, a.max_pages, parts.rows,
                  parts.plan.ctas, parts.prefix_splits, a.prefix_len};
     auto fn = a.dtype == DType::BF16 ? attn_join_kernel<true> : attn_join_kernel<false>;
     cudaLaunchConfig_t cfg = {};

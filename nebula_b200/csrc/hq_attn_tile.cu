@@ -931,6 +931,7 @@ AttnPlan attn_plan(int T, int B, int max_q, int Hq, int Hk, int D, bool paged, i
     if (pl.tile && pl.own + pl.prefix > 1) pl.planes += pl.own;
     if (pl.decode) {
         pl.dec = decode_plan(B, Hk, max_q, max_kv, sms);
+        pl.dec_rows = !pl.tile ? max_q * G : G <= 8 ? 8 : kDecodeRows;
         pl.join = pl.dec.mode == kFlat;
         if (pl.join) pl.slots = (size_t)pl.dec.ctas * 2 * kDecodeRows;
         if (pl.join && pl.prefix) ++pl.planes;
@@ -994,7 +995,7 @@ cudaError_t launch_attn(const AttnArgs& a) {
         p.table_stride = a.table_stride;
         p.splits = pl.own;
         p.overlap = pl.prefix > 0;
-        p.skip_rows = pl.decode ? kDecodeRows : 0;
+        p.skip_rows = pl.decode ? pl.dec_rows : 0;
         p.part_o = part ? plane_o + pl.prefix * rows * a.D : nullptr;
         p.part_l = part ? plane_l + pl.prefix * rows : nullptr;
         // every sequence may end inside a block
@@ -1006,6 +1007,7 @@ cudaError_t launch_attn(const AttnArgs& a) {
         DecodeParts d{};
         d.plan = pl.dec;
         d.only = !pl.tile;
+        d.rows = pl.dec_rows;
         d.overlap = pl.prefix || pl.tile;  // the kernel before it is this call's own
         d.slot_o = slot_o;
         d.slot_l = slot_l;
