@@ -39,94 +39,105 @@ def _bad(msg: str):
     raise HQError(_lib.HQ_ERR_INVALID_ARG, msg)
 
 
-def _rows(t: torch.Tensor, name: str, like: torch.Tensor, shape: tuple) -> bytes:
-    """hq_rows of a [tokens, heads, head_dim] tensor beside `like`."""
+def _rows(t: torch.Tensor, name: str, dtype, dev: int, shape: tuple) -> bytes:
+    """hq_rows of a [tokens, heads, head_dim] tensor."""
     if t.shape != shape:
         _bad(f"{name} must be {list(shape)}, got {list(t.shape)}")
-    if t.dtype is not like.dtype or t.get_device() != like.get_device():
-        _bad(f"{name}: {t.dtype} on {t.device} beside {like.dtype} on {like.device}")
+    if t.dtype is not dtype or t.get_device() != dev:
+        _bad(f"{name}: {t.dtype} on {t.device} beside {dtype} on device {dev}")
     st, sh, sd = t.stride()
     if sd != 1 and shape[2] > 1:
         _bad(f"{name}: head_dim must be contiguous")
     return _ROWS(t.data_ptr(), st, sh)
 
 
-def _index(t: torch.Tensor | None, name: str, n: int, like: torch.Tensor):
+def _index(t: torch.Tensor | None, name: str, n: int, dev: int):
     """Device address of n contiguous int32 (None: null)."""
     if t is None:
         return None
-    if t.dtype is not torch.int32 or t.get_device() != like.get_device() or t.dim() != 1 or t.shape[0] != n or \
-            (n > 1 and t.stride(0) != 1):
-        _bad(f"{name} must be {n} contiguous int32 on {like.device}, got {t.dtype} {list(t.shape)} on {t.device}")
+    if t.dtype is not torch.int32 or t.get_device() != dev or t.shape != (n,) or (n > 1 and t.stride(0) != 1):
+        _bad(f"{name} must be {n} contiguous int32 on device {dev}, got {t.dtype} {list(t.shape)} on {t.device}")
     return t.data_ptr()
 
 
-def _view(k_pages, v_pages, page_table, kv_lens, like, D: int) -> tuple:
+def _view(k_pages, v_pages, page_table, kv_lens, dtype, dev: int, D: int) -> tuple:
     """(hq_kv_view, sequences, pages of a row of the table, page_size, kv_heads)."""
     shape = k_pages.shape
     if len(shape) != 4 or shape[3] != D:
         _bad(f"k_pages must be [num_pages, page_size, kv_heads, {D}], got {list(shape)}")
     if v_pages.shape != shape:
         _bad(f"key pages {list(shape)} and value pages {list(v_pages.shape)} differ")
-    dev, dt = like.get_device(), like.dtype
-    if k_pages.dtype is not dt or v_pages.dtype is not dt or k_pages.get_device() != dev or v_pages.get_device() != dev:
-        _bad(f"pages of {k_pages.dtype}, {v_pages.dtype} on {k_pages.device}, {v_pages.device} beside {dt} on {like.device}")
+    if k_pages.dtype is not dtype or v_pages.dtype is not dtype or k_pages.get_device() != dev or \
+            v_pages.get_device() != dev:
+        _bad(f"pages of {k_pages.dtype}, {v_pages.dtype} on {k_pages.device}, {v_pages.device} beside {dtype} on device {dev}")
     kp, kt, kh, kd = k_pages.stride()
     vp, vt, vh, vd = v_pages.stride()
     if (kd != 1 or vd != 1) and D > 1:
         _bad("pages: head_dim must be contiguous")
-    if page_table.dim() != 2 or page_table.dtype is not torch.int32 or page_table.get_device() != dev:
-        _bad(f"page_table must be [sequences, pages] int32 on {like.device}")
-    B, pages = page_table.shape
+    table = page_table.shape
+    if len(table) != 2 or page_table.dtype is not torch.int32 or page_table.get_device() != dev:
+        _bad(f"page_table must be [sequences, pages] int32 on device {dev}")
+    B, pages = table
     stride, inner = page_table.stride()
     if inner != 1 and pages > 1:
         _bad("page_table rows must be contiguous")
     return _VIEW(k_pages.data_ptr(), kp, kt, kh, v_pages.data_ptr(), vp, vt, vh, shape[0], shape[1], page_table.data_ptr(),
-                 stride, pages, _index(kv_lens, "kv_lens", B, like) or 0), B, pages, shape[1], shape[2]
+                 stride, pages, _index(kv_lens, "kv_lens", B, dev)), B, pages, shape[1], shape[2]
 
 
-def _dtype(q: torch.Tensor) -> int:
-    dt = _DT.get(q.dtype)
+def _kind(q: torch.Tensor, what: str) -> tuple:
+    """(dtype, its number, device) of [tokens, heads, head_dim] rows."""
+    dtype, dev = q.dtype, q.get_device()
+    dt = _DT.get(dtype)
     if dt is None:
-        _bad(f"unsupported dtype {q.dtype}")
-    if not q.is_cuda:
+        _bad(f"unsupported dtype {dtype}")
+    if dev < 0:
         _bad(f"tensors must be on a CUDA device, got {q.device}")
-    return dt
+    if q.dim() != 3:
+        _bad(f"{what} must be [tokens, heads, head_dim], got {list(q.shape)}")
+    return dtype, dt, dev
 
 
-def _on(q: torch.Tensor, stream):
-    """None where the tensors' device is current and the call goes on its current stream; else what makes it so (the
-    call's allocations are then that stream's, too)."""
+def _elsewhere(dev: int, stream):
+    """None where device `dev` is current and the call goes on its current stream; else what makes it so (the call's
+    allocations are then that stream's, too)."""
     if stream is not None:
-        if stream.device != q.device:
-            _bad(f"a stream of {stream.device} for tensors on {q.device}")
+        if stream.device.index != dev:
+            _bad(f"a stream of {stream.device} for tensors on device {dev}")
         return torch.cuda.stream(stream)
-    return None if q.get_device() == torch._C._cuda_getDevice() else torch.cuda.device(q.device)
+    return None if dev == torch._C._cuda_getDevice() else torch.cuda.device(dev)
 
 
-def _raw_stream(q: torch.Tensor) -> int:
-    """Handle of the device's current stream (torch.cuda.current_stream builds an object for it, ten times slower)."""
-    return torch._C._cuda_getCurrentRawStream(q.get_device())
+#: Handle of a device's current stream (torch.cuda.current_stream builds an object for it, ten times slower).
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
-def _lse(lse, q, heads):
+def _lse(lse, dev: int, shape: tuple):
     if lse is None:
         return None
-    if lse.dtype is not torch.float32 or lse.shape != (q.shape[0], heads) or not lse.is_contiguous() or \
-            lse.get_device() != q.get_device():
-        _bad(f"lse must be contiguous float32 [{q.shape[0]}, {heads}] on {q.device}")
+    if lse.dtype is not torch.float32 or lse.shape != shape or not lse.is_contiguous() or lse.get_device() != dev:
+        _bad(f"lse must be contiguous float32 {list(shape)} on device {dev}")
     return lse.data_ptr()
 
 
-def _workspace(need: int, workspace, q) -> tuple:
+def _workspace(need: int, workspace, q: torch.Tensor, dev: int) -> tuple:
     """(tensor kept until the call is enqueued, address, bytes)."""
     if workspace is None:
         if not need:
             return None, None, 0
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-    elif workspace.get_device() != q.get_device() or not workspace.is_contiguous():
-        _bad(f"workspace must be contiguous on {q.device}")
+        workspace = q.new_empty(need // 2)
+        return workspace, workspace.data_ptr(), need
+    if workspace.get_device() != dev or not workspace.is_contiguous():
+        _bad(f"workspace must be contiguous on device {dev}")
     return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
+
+
+def _output(out, q: torch.Tensor, dtype, dev: int, shape: tuple) -> tuple:
+    """(tensor, hq_rows) of the output."""
+    if out is not None:
+        return out, _rows(out, "out", dtype, dev, shape)
+    out = q.new_empty(shape)
+    return out, _ROWS(out.data_ptr(), shape[1] * shape[2], shape[2])
 
 
 def attn_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, max_seqlen: int, *,
@@ -135,26 +146,24 @@ def attn_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: t
     """Attention within packed sequences: q [T, Hq, D], k and v [T, Hkv, D]; sequence s is the rows
     cu_seqlens[s] .. cu_seqlens[s+1]-1, at most max_seqlen of them.  Rows behind the last sequence keep what `out`
     holds.  lse: optional [T, Hq] float32 output (ln of the softmax denominator)."""
-    dt = _dtype(q)
-    if q.dim() != 3 or k.dim() != 3 or cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1:
-        _bad("q, k, v must be [tokens, heads, head_dim], cu_seqlens [sequences + 1]")
-    ctx = _on(q, stream)
+    dtype, dt, dev = _kind(q, "q")
+    ctx = _elsewhere(dev, stream)
     if ctx is not None:
         with ctx:
             return attn_prompt(q, k, v, cu_seqlens, max_seqlen, causal=causal, scale=scale, out=out, lse=lse,
                                workspace=workspace)
-    T, Hq, D = full = q.shape
+    if k.dim() != 3 or cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1:
+        _bad("k and v must be [tokens, kv_heads, head_dim], cu_seqlens [sequences + 1]")
+    T, Hq, D = shape = q.shape
     Hk, B = k.shape[1], cu_seqlens.shape[0] - 1
     kv = (T, Hk, D)
-    rk, rv, rq = _rows(k, "k", q, kv), _rows(v, "v", q, kv), _rows(q, "q", q, full)
-    cu = _index(cu_seqlens, "cu_seqlens", B + 1, q)
     sh = _SHAPE(T, B, max_seqlen, Hq, Hk, D, dt, D ** -0.5 if scale is None else scale)
-    if out is None:
-        out = torch.empty(full, dtype=q.dtype, device=q.device)
+    out, ro = _output(out, q, dtype, dev, shape)
     L = lib()
-    ws, ws_p, ws_n = _workspace(L.hq_attn_prompt_workspace_size(sh), workspace, q)
-    check(L.hq_attn_prompt(sh, rq, rk, rv, cu, int(causal), _rows(out, "out", q, full), _lse(lse, q, Hq), ws_p, ws_n,
-                           _raw_stream(q)))
+    ws, ws_p, ws_n = _workspace(L.hq_attn_prompt_workspace_size(sh), workspace, q, dev)
+    check(L.hq_attn_prompt(sh, _rows(q, "q", dtype, dev, shape), _rows(k, "k", dtype, dev, kv), _rows(v, "v", dtype, dev, kv),
+                           _index(cu_seqlens, "cu_seqlens", B + 1, dev), int(causal), ro, _lse(lse, dev, (T, Hq)), ws_p, ws_n,
+                           _raw_stream(dev)))
     return out
 
 
@@ -167,33 +176,28 @@ def attn_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pa
     (cu_q None: row s alone), at most max_q_len, and kv_lens[s] keys, its rows' own last (kv_append writes them
     first).  Row i of n sees keys 0 .. kv_lens[s] - n + i, after the prefix_len keys of the pages prefix_table that
     every sequence shares.  max_kv_len: a bound of kv_lens that sizes the launch."""
-    dt = _dtype(q)
-    if q.dim() != 3:
-        _bad("q must be [tokens, heads, head_dim]")
-    ctx = _on(q, stream)
+    dtype, dt, dev = _kind(q, "q")
+    ctx = _elsewhere(dev, stream)
     if ctx is not None:
         with ctx:
             return attn_paged(q, k_pages, v_pages, page_table, kv_lens, cu_q, max_q_len, max_kv_len=max_kv_len,
                               prefix_table=prefix_table, prefix_len=prefix_len, scale=scale, out=out, lse=lse,
                               workspace=workspace)
-    T, Hq, D = full = q.shape
-    view, B, pages, page_size, Hk = _view(k_pages, v_pages, page_table, kv_lens, q, D)
-    rq = _rows(q, "q", q, full)
-    cu = _index(cu_q, "cu_q", B + 1, q)
+    T, Hq, D = shape = q.shape
+    view, B, pages, page_size, Hk = _view(k_pages, v_pages, page_table, kv_lens, dtype, dev, D)
     if max_kv_len is None:
         max_kv_len = pages * page_size
     pt = None
     if prefix_len:
         if prefix_table is None or prefix_table.dim() != 1 or prefix_table.shape[0] * page_size < prefix_len:
             _bad(f"prefix_table does not hold {prefix_len} keys")
-        pt = _index(prefix_table, "prefix_table", prefix_table.shape[0], q)
+        pt = _index(prefix_table, "prefix_table", prefix_table.shape[0], dev)
     sh = _SHAPE(T, B, max_q_len, Hq, Hk, D, dt, D ** -0.5 if scale is None else scale)
-    if out is None:
-        out = torch.empty(full, dtype=q.dtype, device=q.device)
+    out, ro = _output(out, q, dtype, dev, shape)
     L = lib()
-    ws, ws_p, ws_n = _workspace(L.hq_attn_paged_workspace_size(sh, max_kv_len, prefix_len), workspace, q)
-    check(L.hq_attn_paged(sh, rq, view, cu, max_kv_len, pt, prefix_len, _rows(out, "out", q, full), _lse(lse, q, Hq), ws_p,
-                          ws_n, _raw_stream(q)))
+    ws, ws_p, ws_n = _workspace(L.hq_attn_paged_workspace_size(sh, max_kv_len, prefix_len), workspace, q, dev)
+    check(L.hq_attn_paged(sh, _rows(q, "q", dtype, dev, shape), view, _index(cu_q, "cu_q", B + 1, dev), max_kv_len, pt,
+                          prefix_len, ro, _lse(lse, dev, (T, Hq)), ws_p, ws_n, _raw_stream(dev)))
     return out
 
 
@@ -202,30 +206,28 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: 
               stream=None) -> None:
     """Writes the rows of k and v [T, Hkv, D] into their pages: row i of the n rows of sequence s becomes its key
     kv_lens[s] - n + i."""
-    dt = _dtype(k)
-    if k.dim() != 3:
-        _bad("k and v must be [tokens, kv_heads, head_dim]")
-    ctx = _on(k, stream)
+    dtype, dt, dev = _kind(k, "k")
+    ctx = _elsewhere(dev, stream)
     if ctx is not None:
         with ctx:
             return kv_append(k, v, k_pages, v_pages, page_table, kv_lens, cu_q)
-    T, Hk, D = full = k.shape
-    view, B, _, _, heads = _view(k_pages, v_pages, page_table, kv_lens, k, D)
+    T, Hk, D = shape = k.shape
+    view, B, _, _, heads = _view(k_pages, v_pages, page_table, kv_lens, dtype, dev, D)
     if heads != Hk:
         _bad(f"{Hk} heads into pages of {heads}")
-    cu = _index(cu_q, "cu_q", B + 1, k)
-    check(lib().hq_kv_append(_SHAPE(T, B, T, Hk, Hk, D, dt, 1.0), _rows(k, "k", k, full), _rows(v, "v", k, full), view, cu,
-                             _raw_stream(k)))
+    check(lib().hq_kv_append(_SHAPE(T, B, T, Hk, Hk, D, dt, 1.0), _rows(k, "k", dtype, dev, shape),
+                             _rows(v, "v", dtype, dev, shape), view, _index(cu_q, "cu_q", B + 1, dev), _raw_stream(dev)))
 
 
-def _moves(src, dst) -> np.ndarray:
+def _moves(src, dst) -> bytes:
+    """hq_page_move[n]."""
     n = len(src)
     if len(dst) != n:
         _bad(f"{n} source pages and {len(dst)} destinations")
     both = np.empty((n, 2), np.int32)
     both[:, 0] = src
     both[:, 1] = dst
-    return both
+    return both.tobytes()  # (its .ctypes.data costs as much as all of this)
 
 
 def _page_bytes(shape, stride, size: int) -> int:
@@ -247,13 +249,14 @@ def kv_copy_pages(pools, src, dst, *, stream=None) -> None:
     if not pools:
         return
     first = pools[0]
-    if not first.is_cuda:
+    dev = first.get_device()
+    if dev < 0:
         _bad(f"pools must be on a CUDA device, got {first.device}")
-    ctx = _on(first, stream)
+    ctx = _elsewhere(dev, stream)
     if ctx is not None:
         with ctx:
             return kv_copy_pages(pools, src, dst)
-    dev, bases, geometry = first.get_device(), [], None
+    bases, geometry = [], None
     for t in pools:
         shape, stride, size = t.shape, t.stride(), t.element_size()
         if t.get_device() != dev or len(shape) not in (4, 5):
@@ -267,11 +270,11 @@ def kv_copy_pages(pools, src, dst, *, stream=None) -> None:
         p = t.data_ptr()
         if at:
             step = stride[0] * size
-            bases.extend(range(p, p + shape[0] * step, step) if step else [p] * shape[0])
+            bases += [p + i * step for i in range(shape[0])]
         else:
             bases.append(p)
     check(lib().hq_kv_copy_pages(struct.pack(f"@{len(bases)}P", *bases), len(bases), geometry[1], geometry[2], geometry[0],
-                                 both.ctypes.data, len(both), _raw_stream(first)))
+                                 both, len(src), _raw_stream(dev)))
 
 
 class PagePool:

@@ -12,6 +12,7 @@ from nebula_b200 import _lib
 from nebula_b200 import attention as at
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+F16 = torch.float16
 P = 0x10000  # an aligned address that no refused call follows
 
 
@@ -141,19 +142,19 @@ def test_python_refusals():
         at.kv_copy_pages([], [1], [])
     for bad in (k[:2], k[:, :1], k[..., :32], k.float()):
         with pytest.raises(E):
-            at._rows(bad, "k", q, (3, 2, 64))
+            at._rows(bad, "k", F16, -1, (3, 2, 64))
     with pytest.raises(E, match="contiguous"):
-        at._rows(torch.zeros((3, 2, 128), dtype=torch.float16)[..., ::2], "k", q, (3, 2, 64))
+        at._rows(torch.zeros((3, 2, 128), dtype=F16)[..., ::2], "k", F16, -1, (3, 2, 64))
     for bad in (cu.long(), cu[:1], torch.zeros(4, dtype=torch.int32)[::2], cu[None]):
         with pytest.raises(E, match="contiguous int32"):
-            at._index(bad, "cu", 2, q)
+            at._index(bad, "cu", 2, -1)
     pages, table, lens = torch.zeros((5, 16, 2, 64), dtype=torch.float16), torch.zeros((1, 1), dtype=torch.int32), cu[:1]
-    at._view(pages, pages, table, lens, q, 64)
+    at._view(pages, pages, table, lens, F16, -1, 64)
     for bad in ((pages, pages[:4], table, lens), (pages[0], pages[0], table, lens), (pages.float(), pages, table, lens),
                 (pages, pages, table[0], lens), (pages, pages, table.long(), lens), (pages, pages, table, cu),
                 (pages[..., ::2], pages[..., ::2], table, lens)):
         with pytest.raises(E):
-            at._view(*bad, q, 64)
+            at._view(*bad, F16, -1, 64)
     with pytest.raises(E, match="one block"):
         at._page_bytes((16, 2, 64), (256, 64, 1), 2)
     assert at._page_bytes((16, 2, 64), (64, 1024, 1), 2) == 4096
