@@ -113,8 +113,10 @@ struct KvAppendArgs {
     const int* kv_lens;
     const int* cu_q;
     unsigned* err;
+    int per_head, page_shift;  // set by the launch: 16-byte vectors of a head, and
+    unsigned head_mul;         // 2^32 / per_head rounded up
 };
-cudaError_t launch_kv_append(const KvAppendArgs& a, cudaStream_t s);
+cudaError_t launch_kv_append(KvAppendArgs a, cudaStream_t s);
 
 struct PageMove {
     int src, dst;
