@@ -447,14 +447,22 @@ HQ_API int hq_kv_pool_free_pages(const hq_kv_pool* p);
 /* A new, empty sequence, or one that shares all pages of `seq`; -1 on failure. */
 HQ_API int hq_kv_pool_new_seq(hq_kv_pool* p);
 HQ_API int hq_kv_pool_fork(hq_kv_pool* p, int seq);
-/* Room for n_tokens more keys.  Where the sequence's last page is partly filled
- * and shared, it gets one of its own: *n_moves is then 1 and *move the copy that
- * the caller makes (hq_kv_copy_pages) before it appends; else *n_moves is 0. */
-HQ_API hq_status hq_kv_pool_extend(hq_kv_pool* p, int seq, int n_tokens, hq_page_move* move, int* n_moves);
+/* Room for n_tokens[i] more keys of each sequence seqs[i], for all of the n or,
+ * where the pages do not suffice, for none.  A sequence whose last page is partly
+ * filled and shared gets one of its own: moves (room for n) then holds the copies
+ * that the caller makes (hq_kv_copy_pages) before it appends, *n_moves of them. */
+HQ_API hq_status hq_kv_pool_extend(hq_kv_pool* p, const int32_t* seqs, const int32_t* n_tokens, int n,
+                                   hq_page_move* moves, int* n_moves);
 HQ_API hq_status hq_kv_pool_free(hq_kv_pool* p, int seq);
 /* Length in keys, and pages (copies up to max_pages of them); -1: no such sequence. */
 HQ_API int hq_kv_pool_seq_len(const hq_kv_pool* p, int seq);
 HQ_API int hq_kv_pool_seq_pages(const hq_kv_pool* p, int seq, int32_t* pages, int max_pages);
+/* The page_table [n][max_pages] and kv_lens [n] (nullable) of an hq_kv_view, on
+ * the host; entries behind a sequence's last page are 0, and pages beyond
+ * max_pages are left out.  Returns the most pages that one of them has, -1 on
+ * failure. */
+HQ_API int hq_kv_pool_tables(const hq_kv_pool* p, const int32_t* seqs, int n, int32_t* page_table, int max_pages,
+                             int32_t* kv_lens);
 /* Renumbers the pages in use to 0 .. n-1 and writes the copies that this takes
  * (at most as many as there are pages in use; no page is both read and written). */
 HQ_API hq_status hq_kv_pool_compact(hq_kv_pool* p, hq_page_move* moves, int max_moves, int* n_moves);

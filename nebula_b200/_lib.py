@@ -58,7 +58,8 @@ SIGNATURES = {
     "hq_kv_pool_free_pages": (_i, [_vp]),
     "hq_kv_pool_new_seq": (_i, [_vp]),
     "hq_kv_pool_fork": (_i, [_vp, _i]),
-    "hq_kv_pool_extend": (_i, [_vp, _i, _i, _vp, _vp]),
+    "hq_kv_pool_extend": (_i, [_vp, _vp, _vp, _i, _vp, _vp]),
+    "hq_kv_pool_tables": (_i, [_vp, _vp, _i, _vp, _i, _vp]),
     "hq_kv_pool_free": (_i, [_vp, _i]),
     "hq_kv_pool_seq_len": (_i, [_vp, _i]),
     "hq_kv_pool_seq_pages": (_i, [_vp, _i, _vp, _i]),

@@ -314,13 +314,18 @@ class PagePool:
             _bad(f"no sequence {seq}")
         return s
 
-    def extend(self, seq: int, n_tokens: int) -> list[tuple[int, int]]:
-        """Room for n_tokens more keys; returns the page copies, (source, destination), to make first."""
-        move, n = (ctypes.c_int32 * 2)(), ctypes.c_int(0)
-        status = lib().hq_kv_pool_extend(self._h, seq, n_tokens, move, ctypes.byref(n))
+    def extend(self, seqs, counts) -> list[tuple[int, int]]:
+        """Room for counts[i] more keys of seqs[i] (integers, or lists of them), for all or for none; returns the page
+        copies, (source, destination), to make first."""
+        seqs, counts = np.atleast_1d(np.asarray(seqs, np.int32)), np.atleast_1d(np.asarray(counts, np.int32))
+        if seqs.ndim != 1 or seqs.shape != counts.shape:
+            _bad(f"{seqs.size} sequences and {counts.size} counts")
+        moves, n = np.empty((max(1, seqs.size), 2), np.int32), ctypes.c_int(0)
+        status = lib().hq_kv_pool_extend(self._h, seqs.ctypes.data, counts.ctypes.data, seqs.size, moves.ctypes.data,
+                                         ctypes.byref(n))
         if status != _lib.HQ_OK:
-            raise HQError(status, f"sequence {seq} by {n_tokens} keys, {self.free_pages} pages free")
-        return [(move[0], move[1])] if n.value else []
+            raise HQError(status, f"sequences {seqs.tolist()} by {counts.tolist()} keys, {self.free_pages} pages free")
+        return [tuple(m) for m in moves[: n.value].tolist()]
 
     def free(self, seq: int) -> None:
         status = lib().hq_kv_pool_free(self._h, seq)
@@ -340,6 +345,17 @@ class PagePool:
         out = np.empty(n, np.int32)
         lib().hq_kv_pool_seq_pages(self._h, seq, out.ctypes.data, n)
         return out
+
+    def tables(self, seqs) -> tuple[np.ndarray, np.ndarray]:
+        """(page table [n, pages], lengths [n]) of the sequences, int32 on the host."""
+        seqs = np.asarray(seqs, np.int32).reshape(-1)
+        L, lens = lib(), np.empty(seqs.size, np.int32)
+        pages = int(L.hq_kv_pool_tables(self._h, seqs.ctypes.data, seqs.size, None, 0, lens.ctypes.data))
+        if pages < 0:
+            _bad(f"no such sequence among {seqs.tolist()}")
+        table = np.empty((seqs.size, pages), np.int32)
+        L.hq_kv_pool_tables(self._h, seqs.ctypes.data, seqs.size, table.ctypes.data, pages, None)
+        return table, lens
 
     def compact(self) -> list[tuple[int, int]]:
         """Renumbers the pages in use to 0 .. n-1; returns the page copies to make."""
@@ -369,14 +385,9 @@ class KVCache:
         self.pool.free(seq)
 
     def extend(self, seqs, counts, stream=None) -> None:
-        """Room for counts[i] more keys of seqs[i]; pages that forks still share are copied, all layers in one call.
-        Where the pages run out, the sequences before the failing one keep their room."""
-        moves = []
-        try:
-            for s, n in zip(seqs, counts):
-                moves += self.pool.extend(s, n)
-        finally:
-            self._copy(moves, stream)
+        """Room for counts[i] more keys of seqs[i], for all or for none; pages that forks still share are copied, all
+        layers in one call."""
+        self._copy(self.pool.extend(seqs, counts), stream)
 
     def compact(self, stream=None) -> int:
         """Moves the pages in use to the front; returns how many moved."""
@@ -390,11 +401,6 @@ class KVCache:
 
     def tables(self, seqs) -> tuple[torch.Tensor, torch.Tensor, int]:
         """(page_table [n, pages] int32, kv_lens [n] int32, longest) of the sequences, on the cache's device."""
-        lists = [self.pool.seq_pages(s) for s in seqs]
-        lens = [self.pool.seq_len(s) for s in seqs]
-        host = np.zeros((len(lists), max([len(p) for p in lists], default=0) + 1), np.int32)  # last column: lengths
-        for row, p, n in zip(host, lists, lens):
-            row[: len(p)] = p
-            row[-1] = n
-        dev = torch.from_numpy(host).to(self.k.device)
-        return dev[:, :-1], dev[:, -1].contiguous(), max(lens, default=0)
+        table, lens = self.pool.tables(seqs)
+        dev = torch.from_numpy(np.concatenate([table.reshape(-1), lens])).to(self.k.device)  # one copy for both
+        return dev[: table.size].view(table.shape), dev[table.size:], int(lens.max(initial=0))

@@ -1,5 +1,6 @@
 """Split-fuse continuous batching over libhq.so (hq_batcher_*): the scheduling of hydrogen::SplitFuseBatcher
-(batcher.hpp:98-199, split_fuse.cpp:70-193) with a step executor that runs real hq_gemm layers at the fused M.
+(batcher.hpp:98-199, split_fuse.cpp:70-193) with a step executor that runs real hq_gemm layers at the fused M
+and, with a paged cache, the step's attention between them.
 """
 from __future__ import annotations
 
@@ -56,11 +57,33 @@ class FusedBatch:
     assembly_overhead_us: float
 
 
+@dataclass
+class AttentionStep:
+    """Where a fused batch's rows stand in the cache, as attention.attn_paged and kv_append take it (device tensors;
+    sequence i is the i-th chunk that has rows)."""
+    rows: int
+    cu_q: object
+    page_table: object
+    kv_lens: object
+    max_q_len: int
+    max_kv_len: int
+    prefix_table: object
+    prefix_len: int
+
+
 class SplitFuseBatcher:
     """SplitFuseBatcher's scheduling surface: submit_request, assemble_step_batch, update_step_completion,
-    has_active_work, num_active_requests, reset; plus execute_step over real quantized layers."""
+    has_active_work, num_active_requests, reset; plus execute_step over real quantized layers.
 
-    def __init__(self, max_prefill_chunk_tokens=64, max_decode_streams=16, max_batch_tokens=512):
+    With a ``cache`` (attention.KVCache) the batcher keeps the requests' keys and values there: plan_attention makes
+    room for a batch's rows, attend runs a layer's attention, update_step_completion frees what completed requests
+    held.  ``prefix``: a sequence of the cache whose keys every request sees before its own.  All device work belongs
+    on one stream, and the cache is compacted between steps only."""
+
+    def __init__(self, max_prefill_chunk_tokens=64, max_decode_streams=16, max_batch_tokens=512, *, cache=None,
+                 prefix=None):
+        self.cache, self.prefix = cache, prefix
+        self._seqs = {}  # request -> (its sequence, keys that it began with)
         cfg = _Config(max_prefill_chunk_tokens, max_decode_streams, max_batch_tokens)
         self._h = lib().hq_batcher_create(ctypes.byref(cfg))
         if not self._h:
@@ -79,9 +102,22 @@ class SplitFuseBatcher:
 
     def reset(self):
         lib().hq_batcher_reset(self._h)
+        for request in list(self._seqs):
+            self._release(request)
 
-    def submit_request(self, prompt_tokens: int, max_decode_tokens: int) -> int:
-        return int(lib().hq_batcher_submit(self._h, prompt_tokens, max_decode_tokens))
+    def submit_request(self, prompt_tokens: int, max_decode_tokens: int, parent: int | None = None) -> int:
+        """parent: an active request whose keys so far the new one continues; their pages are shared until either
+        writes to them, and prompt_tokens counts the tokens after them."""
+        if parent is not None and parent not in self._seqs:
+            raise ValueError(f"request {parent} holds no keys")
+        request = int(lib().hq_batcher_submit(self._h, prompt_tokens, max_decode_tokens))
+        if parent is not None:
+            seq = self.cache.fork(self._seqs[parent][0])
+            self._seqs[request] = seq, self.cache.pool.seq_len(seq)
+        return request
+
+    def _release(self, request: int):
+        self.cache.free(self._seqs.pop(request)[0])
 
     def assemble_step_batch(self) -> FusedBatch:
         cap = int(lib().hq_batcher_active_requests(self._h)) + 2
@@ -98,6 +134,47 @@ class SplitFuseBatcher:
         arr = (_Chunk * max(1, len(batch.chunks)))(
             *[_Chunk(c.request_id, c.start_token, c.num_tokens, int(c.is_prefill)) for c in batch.chunks])
         check(lib().hq_batcher_complete(self._h, arr, len(batch.chunks)))
+        for c in batch.chunks:
+            if c.request_id in self._seqs and self.request_state(c.request_id)["status"] == COMPLETED:
+                self._release(c.request_id)
+
+    def plan_attention(self, batch: FusedBatch) -> AttentionStep:
+        """Room in the cache for the batch's rows, for all or (HQ_ERR_OUT_OF_PAGES) for none, and their places.  To be
+        called before the batch's attend; again for the same batch it gives the same."""
+        import numpy as np
+        import torch
+        cache = self.cache
+        if cache is None:
+            raise ValueError("the batcher has no cache")
+        chunks = [c for c in batch.chunks if c.num_tokens]
+        for c in chunks:
+            if c.request_id not in self._seqs:
+                self._seqs[c.request_id] = cache.new_seq(), 0
+        seqs = [self._seqs[c.request_id][0] for c in chunks]
+        ends = [self._seqs[c.request_id][1] + c.start_token + c.num_tokens for c in chunks]
+        cache.extend(seqs, [max(0, e - cache.pool.seq_len(s)) for s, e in zip(seqs, ends)])
+        table, _ = cache.pool.tables(seqs)
+        prefix = cache.pool.seq_pages(self.prefix) if self.prefix is not None else np.empty(0, np.int32)
+        n = len(seqs)
+        counts = [c.num_tokens for c in chunks]
+        host = np.concatenate([table.reshape(-1), prefix, np.array(ends, np.int32),
+                               np.cumsum([0] + counts, dtype=np.int32)])
+        dev = torch.from_numpy(host).to(cache.k.device)  # one copy for all four
+        pages, pre, lens, cu = dev.split([table.size, prefix.size, n, n + 1])
+        return AttentionStep(sum(counts), cu, pages.view(table.shape), lens, max(counts, default=0), max(ends, default=0), pre,
+                             cache.pool.seq_len(self.prefix) if self.prefix is not None else 0)
+
+    def attend(self, step: AttentionStep, layer: int, q, k, v, *, scale=None, out=None, workspace=None, stream=None):
+        """One layer's attention of a planned step: k and v [rows, Hkv, D] go into the layer's pages, then q
+        [rows, Hq, D] attends to its sequences' keys.  Returns [rows, Hq, D]."""
+        from . import attention
+        if q.shape[0] != step.rows:
+            raise ValueError(f"{q.shape[0]} rows for a step of {step.rows}")
+        kp, vp = self.cache.k[layer], self.cache.v[layer]
+        attention.kv_append(k, v, kp, vp, step.page_table, step.kv_lens, step.cu_q, stream=stream)
+        return attention.attn_paged(q, kp, vp, step.page_table, step.kv_lens, step.cu_q, step.max_q_len,
+                                    max_kv_len=step.max_kv_len, prefix_table=step.prefix_table,
+                                    prefix_len=step.prefix_len, scale=scale, out=out, workspace=workspace, stream=stream)
 
     def has_active_work(self) -> bool:
         return bool(lib().hq_batcher_has_work(self._h))

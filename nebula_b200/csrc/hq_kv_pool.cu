@@ -92,18 +92,19 @@ HQ_API int hq_kv_pool_fork(hq_kv_pool* p, int seq) {
     }
 }
 
-HQ_API hq_status hq_kv_pool_extend(hq_kv_pool* p, int seq, int n_tokens, hq_page_move* move, int* n_moves) {
-    if (!p || !move || !n_moves || n_tokens < 0 || !p->has(seq)) return HQ_ERR_INVALID_ARG;
-    Seq& s = p->seqs[seq];
-    if ((long long)s.len + n_tokens > 0x7fffffffLL) return HQ_ERR_UNSUPPORTED_SHAPE;
-    *n_moves = 0;
-    if (n_tokens == 0) return HQ_OK;
-    const bool copy = s.len % p->page_size && p->refs[s.pages.back()] > 1;
-    const size_t want = ((size_t)s.len + n_tokens + p->page_size - 1) / p->page_size;
-    const size_t fresh = want - s.pages.size() + (copy ? 1 : 0);
-    if (fresh > p->free_pages.size()) return HQ_ERR_OUT_OF_PAGES;
+HQ_API hq_status hq_kv_pool_extend(hq_kv_pool* p, const int32_t* seqs, const int32_t* n_tokens, int n, hq_page_move* moves,
+                                   int* n_moves) {
+    if (!p || n < 0 || !n_moves || (n > 0 && (!seqs || !n_tokens || !moves))) return HQ_ERR_INVALID_ARG;
+    for (int i = 0; i < n; ++i)
+        if (n_tokens[i] < 0 || !p->has(seqs[i])) return HQ_ERR_INVALID_ARG;
+    struct Before {
+        int len;
+        size_t pages;
+        int32_t shared;  // the last page, where it was replaced by a copy; else -1
+    };
+    std::vector<Before> before;
     try {
-        s.pages.reserve(want);
+        before.reserve((size_t)n);
     } catch (const std::bad_alloc&) {
         return HQ_ERR_OUT_OF_MEMORY;
     }
@@ -114,16 +115,52 @@ HQ_API hq_status hq_kv_pool_extend(hq_kv_pool* p, int seq, int n_tokens, hq_page
         ++p->in_use;
         return g;
     };
-    if (copy) {
-        const int old = s.pages.back();
-        const int g = take();
-        --p->refs[old];
-        s.pages.back() = g;
-        *move = hq_page_move{old, g};
-        *n_moves = 1;
+    auto give = [p](int32_t g) {
+        p->refs[g] = 0;
+        p->free_pages.push(g);  // within the room that the heap had when every page was free
+        --p->in_use;
+    };
+    hq_status status = HQ_OK;
+    int copies = 0;
+    for (int i = 0; i < n && status == HQ_OK; ++i) {
+        Seq& s = p->seqs[seqs[i]];
+        Before was{s.len, s.pages.size(), -1};
+        if ((long long)s.len + n_tokens[i] > 0x7fffffffLL) status = HQ_ERR_UNSUPPORTED_SHAPE;
+        else if (n_tokens[i] > 0) {
+            const bool copy = s.len % p->page_size && p->refs[s.pages.back()] > 1;
+            const size_t want = ((size_t)s.len + n_tokens[i] + p->page_size - 1) / p->page_size;
+            if (want - s.pages.size() + (copy ? 1 : 0) > p->free_pages.size()) status = HQ_ERR_OUT_OF_PAGES;
+            else
+                try {
+                    s.pages.reserve(want);
+                    if (copy) {
+                        was.shared = s.pages.back();
+                        s.pages.back() = take();
+                        --p->refs[was.shared];
+                        moves[copies++] = hq_page_move{was.shared, s.pages.back()};
+                    }
+                    while (s.pages.size() < want) s.pages.push_back(take());
+                    s.len += n_tokens[i];
+                } catch (const std::bad_alloc&) {  // of the reserve: nothing was taken
+                    status = HQ_ERR_OUT_OF_MEMORY;
+                }
+        }
+        if (status == HQ_OK) before.push_back(was);
     }
-    while (s.pages.size() < want) s.pages.push_back(take());
-    s.len += n_tokens;
+    if (status != HQ_OK) {  // last one first: a sequence may be named twice
+        for (int i = (int)before.size() - 1; i >= 0; --i) {
+            Seq& s = p->seqs[seqs[i]];
+            for (; s.pages.size() > before[i].pages; s.pages.pop_back()) give(s.pages.back());
+            if (before[i].shared >= 0) {
+                give(s.pages.back());
+                s.pages.back() = before[i].shared;
+                ++p->refs[before[i].shared];
+            }
+            s.len = before[i].len;
+        }
+        return status;
+    }
+    *n_moves = copies;
     return HQ_OK;
 }
 
@@ -153,6 +190,25 @@ HQ_API int hq_kv_pool_seq_pages(const hq_kv_pool* p, int seq, int32_t* pages, in
     const Seq& s = p->seqs[seq];
     std::copy_n(s.pages.begin(), std::min((size_t)max_pages, s.pages.size()), pages);
     return (int)s.pages.size();
+}
+
+HQ_API int hq_kv_pool_tables(const hq_kv_pool* p, const int32_t* seqs, int n, int32_t* page_table, int max_pages,
+                             int32_t* kv_lens) {
+    if (!p || n < 0 || max_pages < 0 || (n > 0 && !seqs) || (n > 0 && max_pages > 0 && !page_table)) return -1;
+    size_t most = 0;
+    for (int i = 0; i < n; ++i) {
+        if (!p->has(seqs[i])) return -1;
+        most = std::max(most, p->seqs[seqs[i]].pages.size());
+    }
+    for (int i = 0; i < n; ++i) {
+        const Seq& s = p->seqs[seqs[i]];
+        int32_t* row = page_table + (size_t)i * max_pages;
+        const size_t m = std::min((size_t)max_pages, s.pages.size());
+        std::copy_n(s.pages.begin(), m, row);
+        std::fill(row + m, row + max_pages, 0);
+        if (kv_lens) kv_lens[i] = s.len;
+    }
+    return (int)most;
 }
 
 HQ_API hq_status hq_kv_pool_compact(hq_kv_pool* p, hq_page_move* moves, int max_moves, int* n_moves) {

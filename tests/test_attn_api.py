@@ -270,7 +270,55 @@ def test_pool_against_plain_lists(seed):
         assert pool.free_pages == len(plain.free())
         for s, (pages, n) in plain.seqs.items():
             assert pool.seq_len(s) == n and pool.seq_pages(s).tolist() == list(pages)
+        seqs = r.sample(sorted(plain.seqs), r.randint(0, len(plain.seqs)))
+        table, lens = pool.tables(seqs)
+        assert lens.tolist() == [plain.seqs[s][1] for s in seqs]
+        assert table.shape == (len(seqs), max([len(plain.seqs[s][0]) for s in seqs], default=0))
+        assert all(row.tolist() == list(plain.seqs[s][0]) + [0] * (table.shape[1] - len(plain.seqs[s][0]))
+                   for row, s in zip(table, seqs))
     pool.close()
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_pool_extends_all_or_none(seed):
+    """Several sequences at once, some named twice, are the single extensions in their order, or change nothing."""
+    r = random.Random(seed)
+    page, num = 16, 12
+    refused = 0
+    for _ in range(60):
+        pool, plain = at.PagePool(num, page), PlainPool(num, page)
+        for _ in range(r.randint(1, 6)):
+            if plain.seqs and r.random() < 0.6:
+                parent = r.choice(sorted(plain.seqs))
+                plain.seqs[pool.fork(parent)] = plain.seqs[parent]
+            else:
+                s = pool.new_seq()
+                plain.seqs[s] = ([], 0)
+                n = r.randint(0, 2 * page)
+                assert pool.extend(s, n) == (plain.extend(s, n) or [])
+        seqs = r.choices(sorted(plain.seqs), k=r.randint(0, 8))
+        counts = [r.choice([0, 1, 5, page, 2 * page, 4 * page]) for _ in seqs]
+        before = dict(plain.seqs), pool.free_pages
+        moves = []
+        for s, n in zip(seqs, counts):
+            m = plain.extend(s, n)
+            if m is None:
+                plain.seqs, moves = before[0], None
+                break
+            moves += m
+        if moves is None:
+            refused += 1
+            with pytest.raises(_lib.HQError, match="HQ_ERR_OUT_OF_PAGES"):
+                pool.extend(seqs, counts)
+        else:
+            assert pool.extend(seqs, counts) == moves
+        assert pool.free_pages == len(plain.free())
+        for s, (pages, n) in plain.seqs.items():
+            assert pool.seq_len(s) == n and pool.seq_pages(s).tolist() == list(pages)
+        s = pool.new_seq()  # what is free is handed out as before, lowest page first
+        assert pool.extend(s, pool.free_pages * page) == [] and pool.seq_pages(s).tolist() == plain.free()
+        pool.close()
+    assert 0 < refused < 60
 
 
 def test_pool_refuses_unknown_sequences():
@@ -282,13 +330,18 @@ def test_pool_refuses_unknown_sequences():
                 call(bad)
     with pytest.raises(_lib.HQError, match="HQ_ERR_INVALID_ARG"):
         pool.extend(s, -1)
+    for bad in (([s, s], [1]), ([s, s + 1], [1, 1]), ([s, s], [1, -1])):
+        with pytest.raises(_lib.HQError, match="HQ_ERR_INVALID_ARG"):
+            pool.extend(*bad)
+    with pytest.raises(_lib.HQError, match="HQ_ERR_INVALID_ARG"):
+        pool.tables([s, s + 1])
     with pytest.raises(_lib.HQError, match="HQ_ERR_OUT_OF_PAGES"):
         pool.extend(s, 65)
     assert pool.seq_len(s) == 0 and pool.free_pages == 4
     L, n = _lib.lib(), ctypes.c_int(-5)
     assert L.hq_kv_pool_create(0, 16) is None and L.hq_kv_pool_create(1 << 28, 16) is None
     assert L.hq_kv_pool_new_seq(None) == -1 and L.hq_kv_pool_fork(None, 0) == -1 and L.hq_kv_pool_free_pages(None) == 0
-    assert L.hq_kv_pool_extend(None, 0, 1, None, None) == _lib.HQ_ERR_INVALID_ARG
+    assert L.hq_kv_pool_extend(None, None, None, 0, None, None) == _lib.HQ_ERR_INVALID_ARG
     # a compaction that has no room for its moves changes nothing
     a, b = pool.new_seq(), pool.new_seq()
     pool.extend(a, 16), pool.extend(b, 16)
