@@ -37,10 +37,10 @@ __device__ __forceinline__ void bad_index(unsigned* err) {
     if (err) atomicCAS(err, 0u, (unsigned)kDevBadIndex);
 }
 
-// Whether one of the eight 16-bit values of v is Inf or NaN: one step more in the
+// Not 0 where one of the eight 16-bit values of v is Inf or NaN: one step more in the
 // exponent's last place then reaches the sign's.
 template <bool kBF16>
-__device__ __forceinline__ bool not_finite(uint4 v) {
+__device__ __forceinline__ uint32_t not_finite(uint4 v) {
     constexpr uint32_t kStep = kBF16 ? 0x00800080u : 0x04000400u, kAbs = 0x7FFF7FFFu;
     return (((v.x & kAbs) + kStep) | ((v.y & kAbs) + kStep) | ((v.z & kAbs) + kStep) | ((v.w & kAbs) + kStep)) & 0x80008000u;
 }

@@ -62,8 +62,9 @@ struct TileLayout {
     static constexpr int kBlk = DP / 64;             // 64-dim blocks of 128-byte rows
     static constexpr int kBlkBytes = 128 * 128;      // 128 rows of one block
     static constexpr int kTile = kBlk * kBlkBytes;   // 128 rows of Q, K or V
-    static constexpr int kStages = DP == 128 ? 5 : 8;
-    static constexpr int kShared = 2 * kTile + kStages * kTile;  // Q, the ring, then TileShared
+    static constexpr int kStages = DP == 128 ? 4 : 8;
+    static constexpr int kOut = 2 * kTile + kStages * kTile;  // Q, the ring, then 4 KB of output a softmax warp
+    static constexpr int kShared = kOut + 8 * 4096;           // and TileShared
 };
 
 struct alignas(64) TileParams {
@@ -593,18 +594,26 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
                 const int x = threadIdx.x - 64, c = x % C;
                 // chunk c of row r of a block lies at chunk c ^ (r & 7)
                 const uint32_t col = vt + (c >> 3) * L::kBlkBytes;
-#pragma unroll 4
-                for (int r = lo + x / C; r < hi; r += RS) {
-                    const uint32_t at = col + r * 128 + (((c & 7) ^ (r & 7)) << 4);
-                    uint4 v = lds128(at);
-                    if (!not_finite<kBF16>(v)) continue;
-                    take_out<kBF16>(sh.bad[k & 1], c * 8, k0 + r - base, v);
-                    sts128(at, v);
-                    sh.any_bad[k & 1] = 1;
+                auto at = [&](int r) { return col + r * 128 + (((c & 7) ^ (r & 7)) << 4); };
+                // Eight rows at a time: a look at each by itself took 5000 cycles a tile, more
+                // than its softmax.  (A row behind hi is zeroed below, whatever it holds.)
+#pragma unroll 1
+                for (int r0 = (lo & ~7) + x / C; r0 < hi; r0 += 8 * RS) {
+                    uint32_t any = 0;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) any |= not_finite<kBF16>(lds128(at(min(r0 + j * RS, kKeys - 1))));
+                    if (!any) continue;
+#pragma unroll 1
+                    for (int r = r0; r < min(hi, r0 + 8 * RS); r += RS) {
+                        uint4 v = lds128(at(r));
+                        if (r < lo || !not_finite<kBF16>(v)) continue;
+                        take_out<kBF16>(sh.bad[k & 1], c * 8, k0 + r - base, v);
+                        sts128(at(r), v);
+                        sh.any_bad[k & 1] = 1;
+                    }
                 }
 #pragma unroll 1
-                for (int r = hi + x / C; r < kKeys; r += RS)
-                    sts128(col + r * 128 + (((c & 7) ^ (r & 7)) << 4), make_uint4(0u, 0u, 0u, 0u));
+                for (int r = hi + x / C; r < kKeys; r += RS) sts128(at(r), make_uint4(0u, 0u, 0u, 0u));
                 fence_async_smem();
                 mbar_arrive(&sh.v_clean);
             }
@@ -680,9 +689,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
                 const int cut = i >= m_first ? lim - (k_first + i * kKeys) : kKeys;  // columns from here on are not seen
                 float s[128];
                 tmem_ld128_now(ts, s);
-                if (cut < kKeys) {
+                if (i >= m_first) {
 #pragma unroll
-                    for (int e = 0; e < 128; ++e) s[e] = e < cut ? s[e] : -INFINITY;
+                    for (int c = 0; c < 128; c += 32)
+                        if (cut < c + 32) {
+#pragma unroll
+                            for (int e = c; e < c + 32; ++e) s[e] = e < cut ? s[e] : -INFINITY;
+                        }
                 }
                 float top[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
@@ -746,7 +759,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
             steps += my;
             const size_t hrow = (size_t)token * p.Hq + head;
             const size_t prow = (size_t)it.split * p.T * p.Hq + hrow;
-            T16* out = static_cast<T16*>(p.o) + (size_t)token * p.o_st + (size_t)head * p.o_sh;
             const int bad_lim = lim - (k_first + m_first * kKeys);
             if (!took) more = take(k + 1);
             if (more) hand_q(k + 1);
@@ -760,10 +772,16 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
             // which a merge settles where other splits have a sum).
             const bool part = p.part_o != nullptr;
             const float inv = l != 0.f ? 1.f / l : (!part && lim > 0 ? NAN : 0.f);
+            // 128 bytes of each row at a time go through shared memory, so that a store takes
+            // whole lines: a thread's own row in 16-byte stores took 3 us of a block of 8 steps
+            // that took 21.
+            const uint32_t stage = smem_u32(smem + L::kOut) + (warp - 4) * 4096;
+            uint8_t* const to_out = part ? reinterpret_cast<uint8_t*>(p.part_o) : static_cast<uint8_t*>(p.o);
+            const long long mine = !live ? -1 : part ? (long long)prow * p.D * 4 : 2 * (token * p.o_st + head * p.o_sh);
+            const int per = part ? 4 : 8;  // values of 16 bytes
 #pragma unroll 1
             for (int c = 0; c < DP / 32; ++c) {
                 float o[32];
-                __syncwarp();
                 if (my > 0) tmem_ld32_now(to + 32u * c, o);
 #pragma unroll
                 for (int e = 0; e < 32; ++e) o[e] = my > 0 && l != 0.f ? o[e] * inv : inv;
@@ -775,21 +793,31 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
                         if ((int)sh.bad[k & 1][0][32 * c + e] < bad_lim) o[e] = NAN;
                     }
                 }
-                if (!live) continue;
+                const uint32_t row = stage + lane * 128;  // chunk c of row r lies at chunk c ^ (r & 7)
                 if (part) {
-                    float* dst = p.part_o + prow * p.D + 32 * c;
 #pragma unroll
                     for (int e = 0; e < 32; e += 4)
-                        if (32 * c + e < p.D)
-                            *reinterpret_cast<float4*>(dst + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                        sts128(row + ((e / 4 ^ (lane & 7)) << 4),
+                               make_uint4(__float_as_uint(o[e]), __float_as_uint(o[e + 1]), __float_as_uint(o[e + 2]),
+                                          __float_as_uint(o[e + 3])));
                 } else {
 #pragma unroll
                     for (int e = 0; e < 32; e += 8)
-                        if (32 * c + e < p.D)
-                            *reinterpret_cast<uint4*>(out + 32 * c + e) =
-                                make_uint4(pack2<kBF16>(o[e], o[e + 1]), pack2<kBF16>(o[e + 2], o[e + 3]),
-                                           pack2<kBF16>(o[e + 4], o[e + 5]), pack2<kBF16>(o[e + 6], o[e + 7]));
+                        sts128(row + (((4 * (c & 1) + e / 8) ^ (lane & 7)) << 4),
+                               make_uint4(pack2<kBF16>(o[e], o[e + 1]), pack2<kBF16>(o[e + 2], o[e + 3]),
+                                          pack2<kBF16>(o[e + 4], o[e + 5]), pack2<kBF16>(o[e + 6], o[e + 7])));
+                    if (!(c & 1)) continue;
                 }
+                __syncwarp();
+                const int ch = lane & 7, dim = (part ? 32 * c : 32 * (c - 1)) + per * ch;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int r = 4 * i + (lane >> 3);
+                    const long long off = __shfl_sync(~0u, mine, r);
+                    if (off >= 0 && dim < p.D)
+                        *reinterpret_cast<uint4*>(to_out + off + dim * (16 / per)) = lds128(stage + r * 128 + ((ch ^ (r & 7)) << 4));
+                }
+                __syncwarp();
             }
             if (live) {
                 const float l2 = l == 0.f ? -INFINITY : m - kShift + log2f(l);
@@ -864,7 +892,6 @@ int ceil_div(long long a, int b) { return (int)((a + b - 1) / b); }
 template <bool kBF16, int DP>
 cudaError_t launch_tile(const TileParams& p, int dev, int sms, cudaStream_t s) {
     constexpr int kSmem = TileLayout<DP>::kShared + (int)sizeof(TileShared);
-    static_assert(kSmem <= 227 * 1024, "shared memory of an SM");
     static_assert(kSmem <= 227 * 1024, "shared memory of an SM");
     auto fn = attn_tile_kernel<kBF16, DP>;
     cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(fn), dev, kSmem);
