@@ -51,21 +51,6 @@ __device__ __forceinline__ float ld_dsmem_f1(uint32_t addr) {
     return v;
 }
 
-// 16-byte asynchronous copy into shared memory; zeros where there is nothing to copy.
-__device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, bool have) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(have ? 16 : 0) : "memory");
-}
-
-// Whether the phase is over, without waiting.
-__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-                 : "=r"(ok)
-                 : "r"(smem_u32(bar)), "r"(parity)
-                 : "memory");
-    return ok != 0;
-}
-
 // mbar_wait (hq_common.cuh) in few instructions: kernels that wait in many places
 // and run for microseconds are bound by fetching their code.  A wait of the block
 // that gives up records kDevTimeout and sets *gave_up (shared memory); those that
@@ -87,6 +72,14 @@ __device__ __forceinline__ void wait_bar(uint64_t* bar, uint32_t parity, int* ga
 }
 
 // A box of the tensor map into shared memory; its bytes count on `bar`.
+__device__ __forceinline__ void tma_load_3d(void* dst, const void* map, int c0, int c1, int c2, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+            smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(bar))
+        : "memory");
+}
+
 __device__ __forceinline__ void tma_load_4d(void* dst, const void* map, int c0, int c1, int c2, int c3, uint64_t* bar) {
     asm volatile(
         "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::

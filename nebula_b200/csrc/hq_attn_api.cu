@@ -53,6 +53,8 @@ hq_status check_shape(const hq_attn_shape* s, bool attention) {
     if (!attention) return HQ_OK;
     if (s->n_heads <= 0 || s->n_heads % s->n_kv_heads)
         return fail(HQ_ERR_UNSUPPORTED_SHAPE, "n_heads=%d must be a multiple of n_kv_heads=%d", s->n_heads, s->n_kv_heads);
+    if (s->n_heads / s->n_kv_heads > 128)
+        return fail(HQ_ERR_UNSUPPORTED_SHAPE, "%d query heads a key/value head, more than 128", s->n_heads / s->n_kv_heads);
     if ((long long)s->n_tokens * s->n_heads > 0x7fffffffLL || (long long)s->n_seqs * s->n_heads > 0x7fffffffLL)
         return fail(HQ_ERR_UNSUPPORTED_SHAPE, "n_tokens * n_heads and n_seqs * n_heads must fit 31 bits");
     if (!(s->scale > 0.f) || !std::isfinite(s->scale)) return fail(HQ_ERR_INVALID_ARG, "scale must be positive and finite");
@@ -126,7 +128,7 @@ hq_status check_workspace(const void* ws, size_t bytes, size_t need) {
     return HQ_OK;
 }
 
-// Keys and values are read through tensor maps: positive strides below 2^40 bytes.
+// Queries, keys and values are read through tensor maps: positive strides below 2^40 bytes.
 hq_status check_map(long long stride, long long count, const char* what) {
     if (count > 1 && (stride <= 0 || stride >= (1LL << 39)))
         return fail(HQ_ERR_UNSUPPORTED_SHAPE, "%s stride %lld", what, stride);
@@ -155,9 +157,9 @@ HQ_API hq_status hq_attn_prompt(const hq_attn_shape* shape, const hq_rows* q, co
         (st = check_rows(out, "out")) != HQ_OK)
         return st;
     if (!cu_seqlens) return fail(HQ_ERR_INVALID_ARG, "null cu_seqlens");
-    for (const hq_rows* r : {k, v})
+    for (const hq_rows* r : {q, k, v})
         if ((st = check_map(r->stride_token, shape->n_tokens, "token")) != HQ_OK ||
-            (st = check_map(r->stride_head, shape->n_kv_heads, "head")) != HQ_OK)
+            (st = check_map(r->stride_head, r == q ? shape->n_heads : shape->n_kv_heads, "head")) != HQ_OK)
             return st;
     if ((st = check_workspace(workspace, ws_bytes, hq_attn_prompt_workspace_size(shape))) != HQ_OK) return st;
     int dev = 0;
@@ -195,6 +197,9 @@ HQ_API hq_status hq_attn_paged(const hq_attn_shape* shape, const hq_rows* q, con
     if (prefix_len > 0 && !prefix_table) return fail(HQ_ERR_INVALID_ARG, "null prefix_table");
     if (!cu_q && shape->n_tokens < shape->n_seqs)
         return fail(HQ_ERR_INVALID_ARG, "%d sequences of one row in %d rows", shape->n_seqs, shape->n_tokens);
+    if ((st = check_map(q->stride_token, shape->n_tokens, "token")) != HQ_OK ||
+        (st = check_map(q->stride_head, shape->n_heads, "head")) != HQ_OK)
+        return st;
     for (const hq_pages* r : {&cache->k, &cache->v})
         if ((st = check_map(r->stride_token, cache->page_size, "token")) != HQ_OK ||
             (st = check_map(r->stride_head, shape->n_kv_heads, "head")) != HQ_OK ||

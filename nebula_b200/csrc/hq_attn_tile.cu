@@ -4,8 +4,9 @@
 // The rows of a key/value head are its sequence's tokens times the G query heads
 // that share it, row r being head r % G of token r / G: a tile's rows read the
 // same keys, so one pass over K and V serves all of them, and few rows of the
-// causal triangle's edge are wasted.  One CTA takes 256 rows as two tiles of 128
-// and walks the keys 128 at a time:
+// causal triangle's edge are wasted.  A tile of 128 rows holds as many tokens as fit
+// with all their G heads, so that it is one box of a tensor map (G = 5 leaves 3 rows
+// idle); one CTA takes two tiles and walks the keys 128 at a time:
 //   S = Q K^T        tcgen05.mma, both operands in shared memory, S (fp32) in
 //                    tensor memory
 //   P = 2^(c S - m)  one thread a row: running maximum m, running sum l (fp32);
@@ -23,15 +24,15 @@
 // Where there are more blocks than SMs it asks the launch hardware for the next
 // (cluster launch control), so that CTAs share them as they get done; else every CTA
 // has its own, and blocks that the lengths leave without rows cost nothing.
-//   warp 0        the blocks, and their loads: one TMA box per 64 dims and up to 128
-//                 keys of a page (page numbers from the table), K and V tiles
+//   warp 0        the blocks, and their loads: Q, and one TMA box per 64 dims and up to
+//                 128 keys of a page (page numbers from the table), K and V tiles
 //                 alternate in a ring
 //   warp 1        issues the MMAs; owns the tensor memory
 //   warps 2, 3    V tiles that some row does not see in full: rows behind the last
 //                 key are zeroed (0 x NaN would reach the sum), and values that
 //                 are not finite are taken out and noted, to be put back into the
 //                 rows that see them
-//   warps 4-7, 8-11  Q, softmax and output of tile 0, tile 1: thread = row = lane
+//   warps 4-7, 8-11  softmax and output of tile 0, tile 1: thread = row = lane
 //                 of tensor memory
 // Bound: the tensor cores and the exponentials (16 a clock and SM) alike take
 // 1024 cycles for a tile's 128 rows x 128 keys x 128 dims.
@@ -68,9 +69,8 @@ struct TileLayout {
 };
 
 struct alignas(64) TileParams {
+    CUtensorMap q_map;         // {dim, head, token}: a box is the rows of a tile
     CUtensorMap k_map, v_map;  // {dim, token, head, page}
-    const void* q;
-    long long q_st, q_sh;
     void* o;
     long long o_st, o_sh;
     float* lse;
@@ -81,6 +81,7 @@ struct alignas(64) TileParams {
     long long table_stride;
     const int* kv_lens;
     int T, B, Hq, Hk, G, D;
+    int tile_tokens;  // tokens of a tile: 128 / G
     int causal;
     float scale_log2;
     int page_size, box_rows, num_pages, max_pages;  // page_size 0: packed rows
@@ -96,14 +97,14 @@ struct alignas(64) TileParams {
 struct Item {
     int first, n, len;       // the sequence: first row (token), tokens, keys
     const int* table;        // its pages
-    int row0, hk, split;
+    int token0, hk, split;   // first token of the block
     int ni[2];               // key tiles of each row tile
     int k_first, m_first;    // first key; first tile in which a row does not see every key
     int stop;                // no more blocks
 };
 
 struct TileShared {
-    uint64_t full[8], empty[8], q_full[2], s_full[2], p_full[2][2], o_full[2], v_req, v_clean;
+    uint64_t full[8], empty[8], q_full[2], q_read[2], s_full[2], p_full[2][2], o_full[2], v_req, v_clean;
     uint64_t item_full[2], item_empty[2], next;
     uint4 next_block;
     Item item[2];
@@ -217,7 +218,7 @@ __device__ __forceinline__ int find_block(const TileParams& p, int want, int& bl
         bool ok = seq_rows(p.cu_q, s, p.T, first, n);
         if (ok && p.page_size) ok = len_ok(p.kv_lens[s], p.max_pages, p.page_size);
         if (!ok) bad_index(p.err);
-        return ok && n * p.G > p.skip_rows ? (int)(((unsigned)(n * p.G) + 2 * kRows - 1) / (2 * kRows)) : 0;
+        return ok && n * p.G > p.skip_rows ? (int)((unsigned)(n + 2 * p.tile_tokens - 1) / (unsigned)(2 * p.tile_tokens)) : 0;
     };
     const int mine = blocks_of(lane);  // the first 32 sequences'
     // blocks with a place below b
@@ -273,16 +274,16 @@ __device__ __forceinline__ bool make_item(const TileParams& p, int index, Item& 
         it.len = p.page_size ? p.kv_lens[seq] : it.n;
         it.table = p.table + seq * p.table_stride;
     }
-    const int R = it.n * p.G, causal = p.causal && !p.prefix_len;  // fits: n_tokens * n_heads does
-    it.row0 = block * 2 * kRows;
-    auto seen = [&](int r) { return keys_seen(it.len, it.n, min(r, R - 1) / p.G, causal); };
-    const int end1 = (seen(it.row0 + 2 * kRows - 1) + kKeys - 1) / kKeys;
-    const int end0 = (seen(it.row0 + kRows - 1) + kKeys - 1) / kKeys;
+    const int causal = p.causal && !p.prefix_len, tile = p.tile_tokens;
+    it.token0 = block * 2 * tile;
+    auto seen = [&](int token) { return keys_seen(it.len, it.n, min(token, it.n - 1), causal); };
+    const int end1 = (seen(it.token0 + 2 * tile - 1) + kKeys - 1) / kKeys;
+    const int end0 = (seen(it.token0 + tile - 1) + kKeys - 1) / kKeys;
     const int a = end1 * split / p.splits, b = end1 * (split + 1) / p.splits;  // end1 <= 2^24, splits <= 32
     it.ni[0] = max(0, min(b, end0) - a);
-    it.ni[1] = it.row0 + kRows < R ? b - a : 0;
+    it.ni[1] = it.token0 + tile < it.n ? b - a : 0;
     it.k_first = a * kKeys;
-    it.m_first = max(0, seen(it.row0) / kKeys - a);
+    it.m_first = max(0, seen(it.token0) / kKeys - a);
     it.stop = 0;
     return true;
 }
@@ -382,7 +383,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
                 mbar_init(&sh.empty[i], 1);
             }
             for (int t = 0; t < 2; ++t) {
-                mbar_init(&sh.q_full[t], 128);
+                mbar_init(&sh.q_full[t], 1);
+                mbar_init(&sh.q_read[t], 1);
                 mbar_init(&sh.s_full[t], 1);
                 mbar_init(&sh.p_full[t][0], 128);
                 mbar_init(&sh.p_full[t][1], 128);
@@ -404,6 +406,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
         if (lane < 2) sh.any_bad[lane] = 0;
         if (lane == 2) sh.gave_up = 0;
     }
+    // rows of a tile behind its last token's
+    for (int i = p.tile_tokens * p.G * 8 + (int)threadIdx.x; i < kRows * 8; i += kThreads)
+#pragma unroll
+        for (int b = 0; b < 2 * L::kBlk; ++b) sts128(smem_u32(qs) + b * L::kBlkBytes + i * 16, make_uint4(0u, 0u, 0u, 0u));
+    fence_async_smem();
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -421,6 +428,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
         regs_down<kRegsLoad>();
         const int boxes = kKeys / p.box_rows;
         int index = (int)blockIdx.x, use = 0;
+        uint32_t loads[2] = {0, 0};
         bool any = true;
         for (int k = 0, asked = 0;; ++asked) {
             if (p.ask && lane == 0) next_block_request(&sh.next_block, &sh.next);
@@ -445,6 +453,19 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
                 const int nt = max(it.ni[0], it.ni[1]);
 #pragma unroll 1
                 for (int i = 0; i < 2 * nt; ++i, ++use) {  // K, V of tile 0, of tile 1, ...
+                    if (i == 1) {  // Q, once the block before has read its own; its first K may come before
+#pragma unroll
+                        for (int t = 0; t < 2; ++t) {
+                            if (it.ni[t] <= 0) continue;
+                            if (loads[t] > 0) wait(&sh.q_read[t], loads[t] - 1);
+                            ++loads[t];
+                            if (lane == 0) mbar_arrive_expect_tx(&sh.q_full[t], (uint32_t)(L::kBlk * p.tile_tokens * p.G * 128));
+                            __syncwarp();
+                            if (lane < L::kBlk)
+                                tma_load_3d(qs + t * L::kTile + lane * L::kBlkBytes, &p.q_map, lane * 64, it.hk * p.G,
+                                            it.first + it.token0 + t * p.tile_tokens, &sh.q_full[t]);
+                        }
+                    }
                     const int k0 = it.k_first + (i >> 1) * kKeys, slot = use % S;
                     const int live = min(boxes, (it.len - k0 + p.box_rows - 1) / p.box_rows);
                     wait(&sh.empty[slot], ((uint32_t)(use / S) & 1u) ^ 1u);
@@ -491,6 +512,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
         // Every stage filled here has been consumed (its commits have landed) before exit.
 #pragma unroll 1
         for (int j = max(0, use - S); j < use; ++j) mbar_wait(&sh.empty[j % S], (uint32_t)(j / S) & 1u, p.err);
+        for (int t = 0; t < 2; ++t)
+            if (loads[t] > 0) mbar_wait(&sh.q_read[t], (loads[t] - 1) & 1u, p.err);
     } else if (warp == 1) {
         // ----------------------------------------------------------- MMAs
         // The whole warp walks the loops, on values that the compiler can see to be
@@ -552,6 +575,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
                                 mma_ss(sp, qd + off, kd + off, kIdescS, j != 0);
                             }
                             umma_commit(&sh.s_full[t]);
+                            if (i + 2 == my) umma_commit(&sh.q_read[t]);
                         }
                         __syncwarp();
                     }
@@ -573,12 +597,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
         // phase or the one before it, and stays until v_clean.
         regs_down<kRegsLoad>();
         uint32_t use = 0, asked = 0;
+        constexpr int C = DP / 8, RS = 64 / C;  // 16-byte chunks of a row, rows of a step
+        const int x = threadIdx.x - 64, c = x % C;
         for (int k = 0; item_wait(k); ++k) {
             const Item it = sh.item[k & 1];
             const int nt = max(it.ni[0], it.ni[1]);
-            const int causal = p.causal && !p.prefix_len, R = it.n * p.G;
-            const int lim_min = keys_seen(it.len, it.n, it.row0 / p.G, causal);
-            const int lim_max = keys_seen(it.len, it.n, (min(it.row0 + 2 * kRows, R) - 1) / p.G, causal);
+            const int causal = p.causal && !p.prefix_len;
+            const int lim_min = keys_seen(it.len, it.n, it.token0, causal);
+            const int lim_max = keys_seen(it.len, it.n, min(it.token0 + 2 * p.tile_tokens, it.n) - 1, causal);
             const int base = it.k_first + it.m_first * kKeys;
 #pragma unroll 1
             for (int i = it.m_first; i < nt; ++i) {
@@ -590,8 +616,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
                 const int k0 = it.k_first + i * kKeys;
                 // keys [lo, hi) are seen by some rows only, those behind by none
                 const int hi = min(kKeys, lim_max - k0), lo = min(hi, max(0, lim_min - k0));
-                constexpr int C = DP / 8, RS = 64 / C;  // 16-byte chunks of a row, rows of a step
-                const int x = threadIdx.x - 64, c = x % C;
                 // chunk c of row r of a block lies at chunk c ^ (r & 7)
                 const uint32_t col = vt + (c >> 3) * L::kBlkBytes;
                 auto at = [&](int r) { return col + r * 128 + (((c & 7) ^ (r & 7)) << 4); };
@@ -622,70 +646,26 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
             if (lane == 0) mbar_arrive(&sh.item_empty[k & 1]);
         }
     } else {
-        // ------------------------------------------ Q, softmax and output
+        // --------------------------------------------- softmax and output
         regs_up<kRegsSoftmax>();
         const int t = (warp - 4) >> 2, i0 = (threadIdx.x - 128) & 127;
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
         const uint32_t ts = tmem + lanes + 128u * t, to = tmem + lanes + kColO + (uint32_t)DP * t;
         const int causal = p.causal && !p.prefix_len;
-        uint32_t steps = 0;  // key tiles of this row tile so far
-        // Takes item k: this thread's row, and requests its warp's rows of Q (the MMAs of
-        // the item before have read theirs).  16 lanes (DP 128) a row, so that a request
-        // takes whole lines; rows behind the last and dims behind D are zeros.
-        int next_token = 0, next_head = 0, next_lim = 0;
-        bool next_live = false;
-        auto take = [&](int k) {
-            if (!item_wait(k)) return false;
-            const Item& it = sh.item[k & 1];  // stays until this warp has arrived on item_empty
-            const int R = it.n * p.G, r = it.row0 + t * kRows + i0;
-            next_live = r < R;
-            const int tok = min(r, R - 1) / p.G;  // rows behind the last see what it sees
-            next_lim = keys_seen(it.len, it.n, tok, causal);
-            next_token = it.first + tok;
-            next_head = it.hk * p.G + (next_live ? r - tok * p.G : 0);
-            if (it.ni[t] > 0) {
-                constexpr int C = DP / 8, RS = 32 / C;
-                const long long mine = next_live ? next_token * p.q_st + next_head * p.q_sh : -1;
-                const int c = lane % C, w0 = i0 & ~31;
-                const uint32_t dst = smem_u32(qs) + t * L::kTile + (c >> 3) * L::kBlkBytes;
-#pragma unroll 4
-                for (int i = 0; i < 32 / RS; ++i) {
-                    const int row = i * RS + lane / C;
-                    const long long off = __shfl_sync(~0u, mine, row);
-                    const bool have = off >= 0 && c * 8 < p.D;
-                    cp_async16_zfill(dst + (w0 + row) * 128 + (((c & 7) ^ (row & 7)) << 4),
-                                     static_cast<const T16*>(p.q) + (have ? off + c * 8 : 0), have);
-                }
-            }
-            return true;
-        };
-        // Hands the Q that take() requested to the MMAs.
-        auto hand_q = [&](int k) {
-            if (sh.item[k & 1].ni[t] <= 0) return;
-            asm volatile("cp.async.wait_all;" ::: "memory");
-            fence_async_smem();
-            mbar_arrive(&sh.q_full[t]);
-        };
-        bool more = take(0);
-        if (more) hand_q(0);
-        for (int k = 0; more; ++k) {
+        const int tok = i0 / p.G, head0 = i0 - tok * p.G;  // this row's place in a tile
+        uint32_t steps = 0;                                // key tiles of this row tile so far
+        for (int k = 0; item_wait(k); ++k) {
             float m = -INFINITY, l = 0.f;
-            const Item& it = sh.item[k & 1];
+            const Item& it = sh.item[k & 1];  // stays until this warp has arrived on item_empty
             const int my = it.ni[t], k_first = it.k_first, m_first = it.m_first;
-            const int token = next_token, head = next_head, lim = next_lim;
-            const bool live = next_live;
-            bool took = false;
+            // rows behind the last see what it sees
+            const int place = min(it.token0 + t * p.tile_tokens + tok, it.n - 1);
+            const int lim = keys_seen(it.len, it.n, place, causal);
 #pragma unroll 1
             for (int i = 0; i < my; ++i) {
                 wait(&sh.s_full[t], steps + i);
                 __syncwarp();
                 tc_fence_after();
-                if (i == my - 1 && __all_sync(~0u, mbar_test(&sh.item_full[(k + 1) & 1], (uint32_t)((k + 1) >> 1) & 1u))) {
-                    // the last S is there, so Q has been read: the next one can be on its way.
-                    // (Not waited for: the next block may be published only after this one.)
-                    more = take(k + 1);
-                    took = true;
-                }
                 const int cut = i >= m_first ? lim - (k_first + i * kKeys) : kKeys;  // columns from here on are not seen
                 float s[128];
                 tmem_ld128_now(ts, s);
@@ -757,11 +737,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
                 l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
             }
             steps += my;
+            const int token = it.first + place, head = it.hk * p.G + head0;
+            const bool live = tok < p.tile_tokens && it.token0 + t * p.tile_tokens + tok < it.n;
             const size_t hrow = (size_t)token * p.Hq + head;
             const size_t prow = (size_t)it.split * p.T * p.Hq + hrow;
             const int bad_lim = lim - (k_first + m_first * kKeys);
-            if (!took) more = take(k + 1);
-            if (more) hand_q(k + 1);
             if (my > 0) {
                 wait(&sh.o_full[t], steps - 1);
                 __syncwarp();
@@ -778,46 +758,53 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
             const uint32_t stage = smem_u32(smem + L::kOut) + (warp - 4) * 4096;
             uint8_t* const to_out = part ? reinterpret_cast<uint8_t*>(p.part_o) : static_cast<uint8_t*>(p.o);
             const long long mine = !live ? -1 : part ? (long long)prow * p.D * 4 : 2 * (token * p.o_st + head * p.o_sh);
-            const int per = part ? 4 : 8;  // values of 16 bytes
+            const uint32_t own = stage + lane * 128;  // chunk c of row r lies at chunk c ^ (r & 7)
+            // The staged 128 bytes of every row, the dims from `dim` on, `per` in 16 bytes.
+            auto flush = [&](int dim, int per) {
+                __syncwarp();
+                dim += per * (lane & 7);
+                uint4 v[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int r = 4 * i + (lane >> 3);
+                    v[i] = lds128(stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const long long off = __shfl_sync(~0u, mine, 4 * i + (lane >> 3));
+                    if (off >= 0 && dim < p.D) *reinterpret_cast<uint4*>(to_out + off + dim * (16 / per)) = v[i];
+                }
+                __syncwarp();
+            };
 #pragma unroll 1
-            for (int c = 0; c < DP / 32; ++c) {
+            for (int c = 0; c < DP; c += 32) {
                 float o[32];
-                if (my > 0) tmem_ld32_now(to + 32u * c, o);
+                if (my > 0) tmem_ld32_now(to + c, o);
 #pragma unroll
                 for (int e = 0; e < 32; ++e) o[e] = my > 0 && l != 0.f ? o[e] * inv : inv;
                 if (any_bad) {
 #pragma unroll
                     for (int e = 0; e < 32; ++e) {
-                        if ((int)sh.bad[k & 1][1][32 * c + e] < bad_lim) o[e] += INFINITY;
-                        if ((int)sh.bad[k & 1][2][32 * c + e] < bad_lim) o[e] -= INFINITY;
-                        if ((int)sh.bad[k & 1][0][32 * c + e] < bad_lim) o[e] = NAN;
+                        if ((int)sh.bad[k & 1][1][c + e] < bad_lim) o[e] += INFINITY;
+                        if ((int)sh.bad[k & 1][2][c + e] < bad_lim) o[e] -= INFINITY;
+                        if ((int)sh.bad[k & 1][0][c + e] < bad_lim) o[e] = NAN;
                     }
                 }
-                const uint32_t row = stage + lane * 128;  // chunk c of row r lies at chunk c ^ (r & 7)
                 if (part) {
 #pragma unroll
                     for (int e = 0; e < 32; e += 4)
-                        sts128(row + ((e / 4 ^ (lane & 7)) << 4),
+                        sts128(own + ((e / 4 ^ (lane & 7)) << 4),
                                make_uint4(__float_as_uint(o[e]), __float_as_uint(o[e + 1]), __float_as_uint(o[e + 2]),
                                           __float_as_uint(o[e + 3])));
                 } else {
 #pragma unroll
                     for (int e = 0; e < 32; e += 8)
-                        sts128(row + (((4 * (c & 1) + e / 8) ^ (lane & 7)) << 4),
+                        sts128(own + (((c & 32 ? 4 : 0) + e / 8 ^ (lane & 7)) << 4),
                                make_uint4(pack2<kBF16>(o[e], o[e + 1]), pack2<kBF16>(o[e + 2], o[e + 3]),
                                           pack2<kBF16>(o[e + 4], o[e + 5]), pack2<kBF16>(o[e + 6], o[e + 7])));
-                    if (!(c & 1)) continue;
                 }
-                __syncwarp();
-                const int ch = lane & 7, dim = (part ? 32 * c : 32 * (c - 1)) + per * ch;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int r = 4 * i + (lane >> 3);
-                    const long long off = __shfl_sync(~0u, mine, r);
-                    if (off >= 0 && dim < p.D)
-                        *reinterpret_cast<uint4*>(to_out + off + dim * (16 / per)) = lds128(stage + r * 128 + ((ch ^ (r & 7)) << 4));
-                }
-                __syncwarp();
+                if (part) flush(c, 4);
+                else if (c & 32) flush(c - 32, 8);
             }
             if (live) {
                 const float l2 = l == 0.f ? -INFINITY : m - kShift + log2f(l);
@@ -908,10 +895,18 @@ cudaError_t launch_tile_any(const AttnArgs& a, const TileParams& p) {
     return a.dtype == DType::BF16 ? launch_tile<true, 128>(p, a.dev, a.sm_count, a.stream) : launch_tile<false, 128>(p, a.dev, a.sm_count, a.stream);
 }
 
-// Key splits of `blocks` x Hk CTAs over `keys` keys: enough to fill the SMs once,
+cudaError_t q_map(const AttnArgs& a, CUtensorMap* m) {
+    const uint64_t any = 16;  // a dimension of one element takes any legal stride
+    const uint64_t dims[3] = {(uint64_t)a.D, (uint64_t)a.Hq, (uint64_t)a.T};
+    const uint64_t strides[2] = {a.Hq > 1 ? 2 * (uint64_t)a.q_sh : any, a.T > 1 ? 2 * (uint64_t)a.q_st : any};
+    const uint32_t box[3] = {64, (uint32_t)a.G, (uint32_t)(kRows / a.G)};
+    return make_tmap_16bit(m, a.q, 3, dims, strides, box);
+}
+
+// Key splits of `row_blocks` x Hk CTAs over `keys` keys: enough to fill the SMs once,
 // at least two key tiles each.
-int key_splits(long long rows, int Hk, int keys, int sms) {
-    const long long items = (long long)std::max(1, ceil_div(rows, 2 * kRows)) * Hk;
+int key_splits(int row_blocks, int Hk, int keys, int sms) {
+    const long long items = (long long)row_blocks * Hk;
     const int by_keys = ceil_div(keys, kKeys) / 2;
     return (int)std::max(1LL, std::min({(long long)sms / items, (long long)by_keys, 32LL}));
 }
@@ -946,14 +941,16 @@ cudaError_t kv_maps_128(const AttnArgs& a, int box_rows, CUtensorMap* k_map, CUt
     return e != cudaSuccess ? e : one(v_map, a.v, a.v_st, a.v_sh, a.v_sp);
 }
 
+// Blocks of two tiles of n tokens.
+static int blocks_of(int n, int G) { return ceil_div(n, 2 * (kRows / G)); }
+
 AttnPlan attn_plan(int T, int B, int max_q, int Hq, int Hk, int D, bool paged, int max_kv, int prefix_len, int sms) {
     AttnPlan pl{};
-    const int G = Hq / Hk;
-    const long long rows = (long long)T * G;
+    const int G = Hq / Hk, row_blocks = blocks_of(T, G);
     pl.tile = !paged || (long long)max_q * G > kDecodeRows;
     pl.decode = paged && G <= kDecodeRows && (!pl.tile || B > 1);
-    pl.prefix = prefix_len > 0 ? key_splits(rows, Hk, prefix_len, sms) : 0;
-    pl.own = pl.tile ? key_splits(rows, Hk, max_kv, sms) : 0;
+    pl.prefix = prefix_len > 0 ? key_splits(row_blocks, Hk, prefix_len, sms) : 0;
+    pl.own = pl.tile ? key_splits(row_blocks, Hk, max_kv, sms) : 0;
     pl.planes = pl.prefix;
     if (pl.tile && pl.own + pl.prefix > 1) pl.planes += pl.own;
     if (pl.decode) {
@@ -980,9 +977,6 @@ cudaError_t launch_attn(const AttnArgs& a) {
     TileParams p;
     memset(&p, 0, sizeof p);
     if (pl.tile || pl.prefix) {
-        p.q = a.q;
-        p.q_st = a.q_st;
-        p.q_sh = a.q_sh;
         p.o = a.o;
         p.o_st = a.o_st;
         p.o_sh = a.o_sh;
@@ -994,6 +988,7 @@ cudaError_t launch_attn(const AttnArgs& a) {
         p.Hq = a.Hq;
         p.Hk = a.Hk;
         p.G = a.G;
+        p.tile_tokens = kRows / a.G;
         p.D = a.D;
         p.causal = a.causal;
         p.scale_log2 = a.scale * 1.44269504088896340736f;
@@ -1002,9 +997,9 @@ cudaError_t launch_attn(const AttnArgs& a) {
         p.num_pages = a.num_pages;
         p.max_pages = a.max_pages;
         p.err = a.err;
-        if ((e = kv_maps(a, p.box_rows, &p.k_map, &p.v_map)) != cudaSuccess) return e;
+        if ((e = kv_maps(a, p.box_rows, &p.k_map, &p.v_map)) != cudaSuccess || (e = q_map(a, &p.q_map)) != cudaSuccess) return e;
     }
-    const int row_blocks = ceil_div((long long)a.T * a.G, 2 * kRows);
+    const int row_blocks = blocks_of(a.T, a.G);
     if (pl.prefix) {
         TileParams x = p;
         x.prefix_len = a.prefix_len;
