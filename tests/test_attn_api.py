@@ -77,12 +77,16 @@ def test_refusals_of_shapes_and_rows(call):
     I, U, M = _lib.HQ_ERR_INVALID_ARG, _lib.HQ_ERR_UNSUPPORTED_SHAPE, _lib.HQ_ERR_MISALIGNED
     for kw, status in ((dict(dtype=_lib.HQ_F32), I), (dict(dtype=9), I), (dict(n_tokens=-1), I), (dict(n_seqs=-1), I),
                        (dict(max_q_len=-1), I), (dict(n_kv_heads=0), I), (dict(n_heads=0), U), (dict(n_heads=5), U),
+                       (dict(n_heads=129, n_kv_heads=1), U),
                        (dict(head_dim=0), U), (dict(head_dim=12), U), (dict(head_dim=136), U), (dict(scale=0.0), I),
                        (dict(scale=-1.0), I), (dict(scale=float("nan")), I), (dict(scale=float("inf")), I),
                        (dict(n_tokens=1 << 30), U)):
         assert call(shape(**kw)) == status, kw
     for bad, status in ((rows(p=0), I), (rows(p=P + 8), M), (rows(st=100), M), (rows(sh=-64), M)):
         assert call(q=bad) == status and call(out=bad) == status
+    # q is read through a tensor map: no broadcast dimension, unless it has one element
+    U = _lib.HQ_ERR_UNSUPPORTED_SHAPE
+    assert call(q=rows(st=0)) == U and call(q=rows(sh=0)) == U and call(q=rows(st=1 << 40)) == U
     assert call(shape(n_tokens=0)) == _lib.HQ_OK and call(shape(n_seqs=0)) == _lib.HQ_OK  # nothing to do
     assert _lib.lib().hq_last_error_string()
 
@@ -90,6 +94,8 @@ def test_refusals_of_shapes_and_rows(call):
 def test_refusals_of_prompts():
     I, M = _lib.HQ_ERR_INVALID_ARG, _lib.HQ_ERR_MISALIGNED
     assert prompt(cu=None) == I
+    for bad in (rows(st=0), rows(sh=0), rows(st=1 << 40)):
+        assert prompt(k=bad) == prompt(v=bad) == _lib.HQ_ERR_UNSUPPORTED_SHAPE
     for bad, status in ((rows(p=0), I), (rows(p=P + 8), M), (rows(st=100), M)):
         assert prompt(k=bad) == status and prompt(v=bad) == status
 
@@ -106,6 +112,8 @@ def test_refusals_of_caches():
                       (view(stride=-1), I), (view(table=None), I), (view(lens=None), I), (view(num=1 << 28), U),
                       (view(pages=1 << 28), U)):
         assert paged(c=c) == status and append(c) == status
+    for c in (view(sp=0), view(st=0), view(sh=0)):
+        assert paged(c=c) == U
     assert paged(max_kv=-1) == I and paged(pl=-1) == I and paged(pl=5) == I
     assert paged(cu=None, sh=shape(n_seqs=5)) == I and append(cu=None, sh=shape(n_seqs=5)) == I
     assert append(k=rows(p=P + 4)) == M and append(k=rows(p=0)) == I and append(sh=shape(head_dim=4)) == U

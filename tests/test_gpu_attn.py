@@ -48,6 +48,15 @@ PROMPTS = [
     (8, 8, 120, BF16, [640], False),
     (32, 4, 128, F16, [1100], True),
     (5, 1, 128, BF16, [2500, 1, 37], True),
+    # more blocks than SMs, of very different lengths
+    (16, 16, 64, F16, [700, 90, 1, 512, 333, 0, 256, 601, 44, 129, 700, 511], True),
+    (40, 8, 128, BF16, [600, 128, 601, 37, 400], True),
+    (20, 20, 128, F16, [1024, 300], False),
+    # as many query heads a key/value head as a tile has rows, and numbers that leave rows of it idle
+    (128, 1, 64, BF16, [5, 40], True),
+    (100, 1, 128, F16, [3, 130], True),
+    (86, 2, 8, F16, [70], True),
+    (21, 3, 64, BF16, [19, 150], False),
 ]
 
 
@@ -211,6 +220,27 @@ PAGED = [
     (8, 1, 64, BF16, [80, 9], [70, 9], 16, 200, "nhd"),
     (40, 8, 128, F16, [12] * 60, [1] * 60, 16, 515, "nhd"),
     (24, 2, 80, F16, [40, 41], [1, 30], 16, 333, "kv"),
+    # many short streams: groups of 4, 2 and 1 warps an item, in one round and in several
+    (40, 8, 128, BF16, [1 + 7 * i % 60 for i in range(25)], [1] * 25, 16, 0, "nhd"),
+    (16, 8, 64, F16, [1 + 5 * i % 40 for i in range(64)], [1] * 64, 16, 0, "hnd"),
+    (10, 10, 128, F16, [i % 33 for i in range(130)], [1] * 130, 16, 0, "nhd"),
+    (8, 8, 64, BF16, [1 + i % 47 for i in range(333)], [1] * 333, 16, 0, "nhd"),
+    (8, 8, 64, BF16, [1 + i % 47 for i in range(333)], [1] * 333, 16, 100, "nhd"),
+    # lines of units that CTAs share: one long stream, several, more sequences than threads, empty ones between
+    (2, 2, 128, F16, [20000], [1], 64, 0, "nhd"),
+    (10, 2, 64, BF16, [0, 9000, 1, 0, 12000, 17, 0], [1] * 7, 128, 0, "hnd"),
+    (3, 1, 64, F16, [(37 * i) % 2000 for i in range(300)], [1] * 300, 16, 0, "nhd"),
+    (3, 1, 64, F16, [(37 * i) % 2000 for i in range(300)], [1] * 300, 16, 77, "nhd"),
+    (10, 2, 128, BF16, [20000, 3, 15000], [1] * 3, 64, 500, "nhd"),
+    (30, 2, 128, BF16, [20000, 3, 15000], [1] * 3, 64, 0, "nhd"),
+    (4, 2, 64, F16, [20000, 3, 15000], [4, 2, 3], 64, 129, "nhd"),
+    # chunks beside streams that CTAs share
+    (10, 2, 128, F16, [3000, 9000, 40, 13500], [1, 1, 1, 100], 16, 0, "nhd"),
+    (24, 2, 64, BF16, [3000, 9000, 40, 13500], [1, 100, 1, 1], 16, 300, "hnd"),
+    (64, 1, 64, F16, [300, 900], [1, 2], 16, 40, "nhd"),
+    (128, 1, 128, BF16, [300, 900], [1, 2], 16, 0, "nhd"),
+    # a prefix under more rows than the SMs take at once
+    (16, 16, 64, F16, [600, 601, 40], [600, 300, 1], 32, 200, "nhd"),
 ]
 
 
@@ -381,6 +411,87 @@ def test_bad_numbers_are_reported_and_touch_nothing():
         c["cu"].copy_(good[2])
         check(run_paged(c)[:n3], o, m, F16)
         hq.check_device_error()
+
+
+def test_captured_prompts_follow_their_offsets():
+    """A captured call replayed with other prompts in the same rows."""
+    T, Hq, Hk, D = 900, 10, 2, 128
+    q, k, v = qkv_rows(T, Hq, Hk, D, BF16, gen(30))
+    cu = torch.tensor([0, 1, 2, 3], dtype=torch.int32, device="cuda")
+    out = torch.zeros((T, Hq, D), dtype=BF16, device="cuda")
+    at.attn_prompt(q, k, v, cu, T, out=out)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        at.attn_prompt(q, k, v, cu, T, out=out)
+    for new in ([0, 900, 900, 900], [0, 300, 301, 800], [0, 0, 0, 0], [0, 17, 400, 900]):
+        cu.copy_(torch.tensor(new, dtype=torch.int32))
+        q.normal_()
+        out.fill_(7.0)
+        graph.replay()
+        o, _, m = prompt_ref(q, k, v, new, D ** -0.5)
+        check(out[: new[-1]], o, m, BF16)
+        assert bool((out[new[-1]:] == 7).all())
+
+
+def test_calls_on_two_streams_at_once():
+    """Eager calls without a workspace of the caller's, on two streams: each has its own."""
+    cs = [paged_case(40, 8, 128, F16, [2000 + i, 1500, 700], [1, 1, 70], 16, 300, seed=40 + i) for i in range(2)]
+    q, k, v = qkv_rows(1100, 32, 4, 128, BF16, gen(42))
+    cu = torch.tensor([0, 1100], dtype=torch.int32, device="cuda")
+    want = [run_paged(c) for c in cs] + [at.attn_prompt(q, k, v, cu, 1100)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = []
+    for _ in range(8):
+        got += [run_paged(c, stream=s) for c, s in zip(cs, streams)]
+        got.append(at.attn_prompt(q, k, v, cu, 1100, stream=streams[2]))
+    torch.cuda.synchronize()
+    for i, g in enumerate(got):
+        n = cs[i % 3]["cu_host"][-1] if i % 3 < 2 else 1100
+        assert torch.equal(g[:n], want[i % 3][:n])
+
+
+def test_workspaces():
+    """What the size call asks for suffices; less, none and a misaligned one are refused."""
+    c = paged_case(10, 2, 128, F16, [3000, 9000], [1, 30], 16, 300, seed=50)
+    T, n = c["q"].shape[0], c["cu_host"][-1]
+    shape = at._SHAPE(T, 2, 30, 10, 2, 128, _lib.HQ_F16, 1.0)
+    need = _lib.lib().hq_attn_paged_workspace_size(shape, 9000, 300)
+    assert need > 0
+    want = run_paged(c, max_kv_len=9000)
+    ws = torch.full((need + 16,), 0xFF, dtype=torch.uint8, device="cuda")  # its first contents do not matter
+    assert torch.equal(run_paged(c, max_kv_len=9000, workspace=ws[:need])[:n], want[:n])
+    for bad, name in ((ws[: need - 1], "WORKSPACE_TOO_SMALL"), (ws[8:], "MISALIGNED"), (ws[:0], "INVALID_ARG|TOO_SMALL")):
+        with pytest.raises(_lib.HQError, match=name):
+            run_paged(c, max_kv_len=9000, workspace=bad)
+    with pytest.raises(_lib.HQError, match="on device"):
+        run_paged(c, max_kv_len=9000, workspace=torch.empty(need, dtype=torch.uint8))
+
+
+def test_more_rows_than_announced():
+    """A sequence of more rows than max_q_len is left out and reported where the launch has no kernel for it; the
+    others are right."""
+    c = paged_case(10, 2, 128, F16, [40, 100, 50], [1, 3, 1], 16, 0, seed=51)
+    o, _, m = paged_ref(c)
+    c["max_q"] = 1
+    got = run_paged(c, out=torch.full_like(c["q"], 7.0))
+    with pytest.raises(_lib.HQError, match="HQ_ERR_BAD_INDEX"):
+        hq.check_device_error()
+    assert bool((got[1:4] == 7).all())
+    check(got[:1], o[:1], m[:1], F16), check(got[4:5], o[4:5], m[4:5], F16)
+
+
+def test_bad_offsets_of_prompts_are_reported():
+    q, k, v = qkv_rows(300, 10, 2, 128, F16, gen(52))
+    o, _, m = prompt_ref(q, k, v, [0, 100], 128 ** -0.5)
+    for bad in ([0, 100, 301], [0, 100, 50], [0, 100, -4], [0, 100, 2 ** 31 - 1]):
+        out = torch.full_like(q, 7.0)
+        at.attn_prompt(q, k, v, torch.tensor(bad, dtype=torch.int32, device="cuda"), 300, out=out)
+        with pytest.raises(_lib.HQError, match="HQ_ERR_BAD_INDEX"):
+            hq.check_device_error()
+        check(out[:100], o, m, F16)
+        assert bool((out[100:] == 7).all())
 
 
 def test_cache_offsets_past_32_bits():

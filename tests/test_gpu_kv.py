@@ -19,6 +19,10 @@ F16, BF16 = torch.float16, torch.bfloat16
     (2, 96, F16, 32, [500, 33, 64], [1, 33, 40]),
     (16, 64, BF16, 64, [1000] * 9, [1000] * 9),
     (8, 128, F16, 16, list(range(1, 301)), [1] * 300),
+    (40, 128, BF16, 256, [70, 300], [70, 5]),
+    (5, 8, F16, 16, [40, 3], [9, 3]),
+    (3, 40, BF16, 16, [100], [37]),
+    (7, 120, F16, 32, [0, 65], [0, 65]),
 ])
 def test_append(Hk, D, dt, page, lens, rows, layout):
     g = torch.Generator(device="cuda").manual_seed(1)
@@ -90,6 +94,25 @@ def test_copy_pages_of_interleaved_and_head_first_pools():
     at.kv_copy_pages([both[:, 0].transpose(1, 2)], [3], [5])
     at.kv_copy_pages([both[:, 1].transpose(1, 2)], [3, 3], [5, 2])
     assert torch.equal(both, want)
+
+
+def test_on_another_stream():
+    """Append, copy and attention on a stream that is not the current one, one behind the other."""
+    g = torch.Generator(device="cuda").manual_seed(7)
+    k, v = (torch.zeros((64, 16, 2, 64), device="cuda", dtype=F16) for _ in range(2))
+    nk, nv, q = (torch.randn((500, h, 64), generator=g, device="cuda", dtype=F16) for h in (2, 2, 10))
+    table = torch.arange(32, dtype=torch.int32, device="cuda")[None]
+    lens = torch.tensor([500], dtype=torch.int32, device="cuda")
+    cu = torch.tensor([0, 500], dtype=torch.int32, device="cuda")
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    at.kv_append(nk, nv, k, v, table, lens, cu, stream=s)
+    at.kv_copy_pages([k, v], range(32), range(32, 64), stream=s)
+    got = at.attn_paged(q, k, v, table + 32, lens, cu, 500, stream=s)
+    s.synchronize()
+    o, _, mag = attend(q, nk, nv, torch.arange(1, 501), 64 ** -0.5)
+    check(got, o, mag, F16)
+    assert torch.equal(k[32:], k[:32]) and torch.equal(v[32:], v[:32])
 
 
 def test_copy_pages_in_a_captured_call():
