@@ -71,6 +71,10 @@ __device__ __forceinline__ void wait_bar(uint64_t* bar, uint32_t parity, int* ga
     }
 }
 
+__device__ __forceinline__ void tmap_prefetch(const void* map) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
+}
+
 // A box of the tensor map into shared memory; its bytes count on `bar`.
 __device__ __forceinline__ void tma_load_3d(void* dst, const void* map, int c0, int c1, int c2, uint64_t* bar) {
     asm volatile(

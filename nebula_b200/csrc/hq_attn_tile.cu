@@ -376,7 +376,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     pdl_launch_dependents();
-    if (warp == 1) {
+    if (warp == 0) {
+        if (lane < 3) tmap_prefetch(lane == 0 ? &p.q_map : lane == 1 ? &p.k_map : &p.v_map);
+    } else if (warp == 1) {
         if (lane == 0) {
             for (int i = 0; i < S; ++i) {
                 mbar_init(&sh.full[i], 1);
@@ -406,15 +408,20 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
         if (lane < 2) sh.any_bad[lane] = 0;
         if (lane == 2) sh.gave_up = 0;
     }
-    // rows of a tile behind its last token's
-    for (int i = p.tile_tokens * p.G * 8 + (int)threadIdx.x; i < kRows * 8; i += kThreads)
+    auto ready = [&] {
+        fence_async_smem();
+        tc_fence_before();
+        __syncthreads();
+        tc_fence_after();
+    };
+    if (warp != 0) {  // warp 0 works its first block out before it comes to this barrier
+        // rows of a tile behind its last token's
+        for (int i = p.tile_tokens * p.G * 8 + (int)threadIdx.x - 32; i < kRows * 8; i += kThreads - 32)
 #pragma unroll
-        for (int b = 0; b < 2 * L::kBlk; ++b) sts128(smem_u32(qs) + b * L::kBlkBytes + i * 16, make_uint4(0u, 0u, 0u, 0u));
-    fence_async_smem();
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    const uint32_t tmem = sh.tmem;
+            for (int b = 0; b < 2 * L::kBlk; ++b) sts128(smem_u32(qs) + b * L::kBlkBytes + i * 16, make_uint4(0u, 0u, 0u, 0u));
+        ready();
+    }
+    const uint32_t tmem = warp != 0 ? sh.tmem : 0u;
     auto wait = [&](uint64_t* bar, uint32_t parity) { wait_bar(bar, parity & 1u, &sh.gave_up, p.err); };
     auto gave_up = [&] { return *reinterpret_cast<volatile int*>(&sh.gave_up) != 0; };
     // Item k of this CTA is in slot k & 1; false: there is none.
@@ -431,11 +438,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
         uint32_t loads[2] = {0, 0};
         bool any = true;
         for (int k = 0, asked = 0;; ++asked) {
-            if (p.ask && lane == 0) next_block_request(&sh.next_block, &sh.next);
-            __syncwarp();
             Item it;
             const bool found = any && make_item(p, index, it);
             any = found;  // the numbers behind one without rows have none either
+            if (asked == 0) ready();
+            if (p.ask && lane == 0) next_block_request(&sh.next_block, &sh.next);
+            __syncwarp();
             if (found) {
                 if (k >= 2) wait(&sh.item_empty[k & 1], (uint32_t)((k - 2) >> 1));
                 __syncwarp();
@@ -764,17 +772,17 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
                 __syncwarp();
                 dim += per * (lane & 7);
                 uint4 v[8];
+                long long off[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const int r = 4 * i + (lane >> 3);
                     v[i] = lds128(stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
-                }
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const long long off = __shfl_sync(~0u, mine, 4 * i + (lane >> 3));
-                    if (off >= 0 && dim < p.D) *reinterpret_cast<uint4*>(to_out + off + dim * (16 / per)) = v[i];
+                    off[i] = __shfl_sync(~0u, mine, r);
                 }
                 __syncwarp();
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (off[i] >= 0 && dim < p.D) *reinterpret_cast<uint4*>(to_out + off[i] + dim * (16 / per)) = v[i];
             };
 #pragma unroll 1
             for (int c = 0; c < DP; c += 32) {
@@ -843,14 +851,13 @@ struct MergeParams {
 template <bool kBF16>
 __global__ void __launch_bounds__(256) attn_merge_kernel(const MergeParams p) {
     const int lane = threadIdx.x & 31;
-    const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const size_t rows = (size_t)p.T * p.Hq;
-    pdl_wait();
-    if (row >= (long long)rows) return;
-    const int t = (int)(row / p.Hq), h = (int)(row % p.Hq);
-    // the row's sequence; rows of none, and those of the decode kernel, have no partials here
+    const unsigned row = blockIdx.x * 8 + (threadIdx.x >> 5);
+    const size_t rows = (size_t)p.T * p.Hq;  // below 2^31
+    const int t = (int)(row / (unsigned)p.Hq), h = (int)(row - (unsigned)t * p.Hq);
+    // the row's sequence (while the kernels before this one run: they write none of what
+    // this reads); rows of none, and those of the decode kernel, have no partials here
     int seen = -1;
-    for (int s0 = 0; s0 < p.B && seen < 0; s0 += 32) {
+    for (int s0 = 0; s0 < p.B && seen < 0 && row < rows; s0 += 32) {
         const int s = s0 + lane;
         int first = 0, n = 0, k = -1;
         if (s < p.B && seq_rows(p.cu_q, s, p.T, first, n) && t >= first && t < first + n &&
@@ -861,6 +868,7 @@ __global__ void __launch_bounds__(256) attn_merge_kernel(const MergeParams p) {
         const unsigned hit = __ballot_sync(~0u, k >= 0);
         if (hit) seen = __shfl_sync(~0u, k, __ffs(hit) - 1);
     }
+    pdl_wait();
     if (seen < 0) return;
     Row x{};
     x.top = -INFINITY;
