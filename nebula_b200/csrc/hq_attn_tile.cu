@@ -85,9 +85,11 @@ struct alignas(64) TileParams {
     int causal;
     float scale_log2;
     int page_size, box_rows, num_pages, max_pages;  // page_size 0: packed rows
+    int page_shift, box_shift;                      // their base-2 logarithms
     int prefix_len;                                 // > 0: all T rows over the pages table[0..]
     int blocks, splits;  // the grid: row blocks x Hk x splits
     int ask;        // blocks are shared out by cluster launch control
+    int ctas;       // else: at most
     int overlap;    // launched while the kernel before it runs
     int skip_rows;  // sequences of at most this many rows (tokens x G) are not this kernel's
     unsigned* err;
@@ -459,6 +461,15 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
                 __syncwarp();
                 ++k;
                 const int nt = max(it.ni[0], it.ni[1]);
+                // Lane b looks up the page of a tile's box b, a tile ahead; one lane requests all
+                // boxes.  (With a box a lane a tile over pages of 16 took 2000 cycles: a
+                // request's operands come from uniform registers, so it is lane after lane.)
+                const int box = lane;
+                auto live_at = [&](int k0) { return min(boxes, (it.len - k0 + p.box_rows - 1) >> p.box_shift); };
+                auto page_at = [&](int k0) {
+                    return p.page_size && box < live_at(k0) ? __ldg(it.table + ((k0 + (box << p.box_shift)) >> p.page_shift)) : 0;
+                };
+                int page = 0, next_page = nt > 0 ? page_at(it.k_first) : 0;
 #pragma unroll 1
                 for (int i = 0; i < 2 * nt; ++i, ++use) {  // K, V of tile 0, of tile 1, ...
                     if (i == 1) {  // Q, once the block before has read its own; its first K may come before
@@ -475,25 +486,30 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
                         }
                     }
                     const int k0 = it.k_first + (i >> 1) * kKeys, slot = use % S;
-                    const int live = min(boxes, (it.len - k0 + p.box_rows - 1) / p.box_rows);
+                    const int live = live_at(k0);
+                    if (!(i & 1)) {
+                        page = next_page;
+                        if (p.page_size && box < live && !page_ok(page, p.num_pages)) {
+                            bad_index(p.err);
+                            page = p.num_pages;  // out of range: the box reads zeros
+                        }
+                        if (i + 2 < 2 * nt) next_page = page_at(k0 + kKeys);
+                    }
                     wait(&sh.empty[slot], ((uint32_t)(use / S) & 1u) ^ 1u);
                     uint8_t* dst = ring + slot * L::kTile;
                     if (lane == 0) mbar_arrive_expect_tx(&sh.full[slot], (uint32_t)(live * L::kBlk * p.box_rows * 128));
                     __syncwarp();
-                    if (lane < live * L::kBlk) {
-                        const int box = lane / L::kBlk, blk = lane % L::kBlk;
-                        const int key = k0 + box * p.box_rows;
-                        int token = it.first + key, page = 0;
-                        if (p.page_size) {
-                            token = key & (p.page_size - 1);
-                            page = it.table[key / p.page_size];
-                            if (!page_ok(page, p.num_pages)) {
-                                bad_index(p.err);
-                                page = p.num_pages;  // out of range: the box reads zeros
-                            }
+#pragma unroll 1
+                    for (int b = 0; b < live; ++b) {
+                        const int at = b << p.box_shift, pg = __shfl_sync(~0u, page, b);
+                        const int token = p.page_size ? (k0 + at) & (p.page_size - 1) : it.first + k0 + at;
+                        if (elect_one()) {
+#pragma unroll
+                            for (int blk = 0; blk < L::kBlk; ++blk)
+                                tma_load_4d(dst + blk * L::kBlkBytes + at * 128, i & 1 ? &p.v_map : &p.k_map, blk * 64, token,
+                                            it.hk, pg, &sh.full[slot]);
                         }
-                        tma_load_4d(dst + blk * L::kBlkBytes + box * p.box_rows * 128, i & 1 ? &p.v_map : &p.k_map, blk * 64,
-                                    token, it.hk, page, &sh.full[slot]);
+                        __syncwarp();
                     }
                 }
             }
@@ -885,7 +901,7 @@ __global__ void __launch_bounds__(256) attn_merge_kernel(const MergeParams p) {
 int ceil_div(long long a, int b) { return (int)((a + b - 1) / b); }
 
 template <bool kBF16, int DP>
-cudaError_t launch_tile(const TileParams& p, int dev, int sms, cudaStream_t s) {
+cudaError_t launch_tile(const TileParams& p, int dev, cudaStream_t s) {
     constexpr int kSmem = TileLayout<DP>::kShared + (int)sizeof(TileShared);
     static_assert(kSmem <= 227 * 1024, "shared memory of an SM");
     auto fn = attn_tile_kernel<kBF16, DP>;
@@ -893,14 +909,14 @@ cudaError_t launch_tile(const TileParams& p, int dev, int sms, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     const long long all = (long long)p.blocks * p.Hk * p.splits;
     if (all > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
-    const long long grid = p.ask ? all : std::min<long long>(all, sms);
+    const long long grid = p.ask ? all : std::min<long long>(all, p.ctas);
     return launch_overlapped(fn, (unsigned)grid, kThreads, kSmem, s, p.overlap, p);
 }
 
 cudaError_t launch_tile_any(const AttnArgs& a, const TileParams& p) {
     if (a.D <= 64)
-        return a.dtype == DType::BF16 ? launch_tile<true, 64>(p, a.dev, a.sm_count, a.stream) : launch_tile<false, 64>(p, a.dev, a.sm_count, a.stream);
-    return a.dtype == DType::BF16 ? launch_tile<true, 128>(p, a.dev, a.sm_count, a.stream) : launch_tile<false, 128>(p, a.dev, a.sm_count, a.stream);
+        return a.dtype == DType::BF16 ? launch_tile<true, 64>(p, a.dev, a.stream) : launch_tile<false, 64>(p, a.dev, a.stream);
+    return a.dtype == DType::BF16 ? launch_tile<true, 128>(p, a.dev, a.stream) : launch_tile<false, 128>(p, a.dev, a.stream);
 }
 
 cudaError_t q_map(const AttnArgs& a, CUtensorMap* m) {
@@ -958,7 +974,12 @@ AttnPlan attn_plan(int T, int B, int max_q, int Hq, int Hk, int D, bool paged, i
     pl.tile = !paged || (long long)max_q * G > kDecodeRows;
     pl.decode = paged && G <= kDecodeRows && (!pl.tile || B > 1);
     pl.prefix = prefix_len > 0 ? key_splits(row_blocks, Hk, prefix_len, sms) : 0;
-    pl.own = pl.tile ? key_splits(row_blocks, Hk, max_kv, sms) : 0;
+    // Beside the decode kernel the tiles leave it its share of the SMs (a block counted as
+    // three sequences), so that the two run at the same time.  16 streams and a chunk of 64
+    // rows over 1500 keys: 36.8 us with all SMs for the tiles first (9 splits), 32.2 with 2
+    // splits on 32 SMs, 36.6 with 1 on 16.
+    pl.tile_sms = pl.decode ? std::max(1, (int)(3LL * row_blocks * sms / (3LL * row_blocks + B))) : sms;
+    pl.own = pl.tile ? key_splits(row_blocks, Hk, max_kv, pl.tile_sms) : 0;
     pl.planes = pl.prefix;
     if (pl.tile && pl.own + pl.prefix > 1) pl.planes += pl.own;
     if (pl.decode) {
@@ -1002,6 +1023,8 @@ cudaError_t launch_attn(const AttnArgs& a) {
         p.scale_log2 = a.scale * 1.44269504088896340736f;
         p.page_size = a.page_size;
         p.box_rows = a.page_size ? std::min(a.page_size, kKeys) : kKeys;
+        while ((1 << p.page_shift) < a.page_size) ++p.page_shift;
+        while ((1 << p.box_shift) < p.box_rows) ++p.box_shift;
         p.num_pages = a.num_pages;
         p.max_pages = a.max_pages;
         p.err = a.err;
@@ -1017,6 +1040,7 @@ cudaError_t launch_attn(const AttnArgs& a) {
         x.part_l = plane_l;
         x.blocks = row_blocks;
         x.ask = (long long)row_blocks * a.Hk * x.splits > a.sm_count;
+        x.ctas = a.sm_count;
         if ((e = launch_tile_any(a, x)) != cudaSuccess) return e;
     }
     if (pl.tile) {
@@ -1030,7 +1054,9 @@ cudaError_t launch_attn(const AttnArgs& a) {
         p.part_l = part ? plane_l + pl.prefix * rows : nullptr;
         // every sequence may end inside a block
         p.blocks = (int)std::min((long long)row_blocks + a.B, 0x7fffffffLL);
-        p.ask = (long long)row_blocks * a.Hk * p.splits > a.sm_count;
+        const long long ctas = (long long)row_blocks * a.Hk * p.splits;
+        p.ask = ctas > a.sm_count;
+        p.ctas = (int)std::min<long long>(a.sm_count, std::max<long long>(pl.tile_sms, ctas));
         if ((e = launch_tile_any(a, p)) != cudaSuccess) return e;
     }
     if (pl.decode) {
