@@ -339,11 +339,21 @@ HQ_API hq_status hq_allreduce_sum(void* const* peer_bufs, unsigned* const* peer_
  * a row does not see do not reach it, whatever they hold (Inf and NaN included).
  *
  * Strides count elements; the innermost dimension (head_dim) is contiguous;
- * strides are multiples of 8 and pointers 16-byte aligned.  head_dim is a
- * multiple of 8 up to 128, dtype HQ_F16 or HQ_BF16 for q, k, v and out alike.
+ * strides are multiples of 8 and pointers 16-byte aligned; those of q, k, v and
+ * the pages are positive and below 2^39 where their dimension has more than one
+ * element.  head_dim is a multiple of 8 up to 128, n_heads a multiple of
+ * n_kv_heads and at most 128 times that, dtype HQ_F16 or HQ_BF16 for q, k, v and
+ * out alike.
  * Lengths, row offsets and page tables are int32 arrays on the device, read
  * when the kernels run, so that a captured call follows them on every replay.
- * Rows of q and out outside every sequence are neither read nor written.
+ * Rows of out and lse outside every sequence keep what they hold.  What q, k and
+ * v hold in such rows, or in a page's slots behind a sequence's last key, does not
+ * matter.  out overlaps none of the inputs.
+ * A length, row offset or page number out of range is reported by
+ * hq_check_device_error: rows of a sequence whose length or offsets are wrong are
+ * left as they are, those of one with a wrong page number are undefined, and
+ * all other sequences' rows are right.  A sequence of more than max_q_len rows
+ * counts as one with wrong offsets, or is computed all the same.
  */
 
 /* [tokens][heads][head_dim] rows, e.g. a third of the QKV layer's output. */
@@ -476,9 +486,8 @@ HQ_API void hq_set_launch_overlap(int enable);
  * bounded time and record a code here instead of hanging.  Synchronises the
  * current device, returns HQ_ERR_TIMEOUT (and clears the word) if any kernel
  * recorded a timeout since the last call, HQ_ERR_BAD_INDEX if an attention or
- * cache kernel met a length, row or page number out of range (it skips what
- * that number names, and never reads or writes outside the caller's buffers),
- * else HQ_OK.
+ * cache kernel met a length, row or page number out of range (no such number
+ * makes it read or write outside the caller's buffers), else HQ_OK.
  */
 HQ_API hq_status hq_check_device_error(void);
 

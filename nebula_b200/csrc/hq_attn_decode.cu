@@ -742,23 +742,30 @@ DecodePlan decode_plan(int B, int Hk, int max_q, int max_kv, int sms) {
     pl.cluster = 1;
     pl.group = kWarps;
     // A cluster per item while they fill no more than the SMs and no CTA has more than
-    // 8 units (1024 keys, 0.5 MB): beyond, a share of every SM is faster in spite of
-    // the join's launch.
+    // 16 units (2048 keys, 1 MB): beyond, a share of every SM is faster in spite of the
+    // join's launch.  One stream over 8 key/value heads of 128, in clusters / as whole
+    // items / in shares: 777 keys 8.9 / 12.0 / 10.6 us, 2000 keys 10.0 / 20.0 / 11.5, 16000
+    // keys 24.1 / 128 / 24.6, 24000 keys 31.9 / 184 / 30.4.
     int cs = 1;
     while (cs < 8 && items * cs * 2 <= sms && cs < tiles) cs *= 2;
-    if (cs > 1 && tiles <= 8 * cs) {
+    if (cs > 1 && tiles <= 16 * cs) {
         pl.mode = kCluster;
         pl.cluster = cs;
         pl.ctas = (int)items * cs;
         return pl;
     }
-    // Whole items where no group has more than 24 units of work, with so many warps an
-    // item that one round takes all items if it can.  (Groups of fewer than 8 warps
-    // have no room for values that only some of a sequence's rows see: one row each.)
+    // Whole items, with so many warps each that one round takes all items if it can (64
+    // streams of 100 keys: 11.3 us with 2 warps an item, 19.7 with 8), while no group has
+    // more units than the shares' own costs and the join's launch are worth; smaller
+    // groups, several a CTA, even out among themselves.  Streams of a tenth to all of the
+    // longest, whole items / shares: 16 up to 3500 keys 36.9 / 41.5 us, up to 6000 keys 55.9 /
+    // 51.7; 64 up to 1000 keys 39.4 / 56.7, up to 2000 keys 69.1 / 74.9.  (Groups of fewer than
+    // 8 warps have no room for values that only some of a sequence's rows see: one row
+    // each.)
     int W = kWarps;
     while (W > 1 && max_q == 1 && items * W > (long long)sms * kWarps) W /= 2;
     const long long slots = (long long)sms * (kWarps / W), rounds = (items + slots - 1) / slots;
-    if (rounds * std::max(1, (max_kv + kSlice * W - 1) / (kSlice * W)) <= 24) {
+    if (rounds * std::max(1, (max_kv + kSlice * W - 1) / (kSlice * W)) <= (W == kWarps ? 40 : 64)) {
         pl.mode = kWhole;
         pl.group = W;
         pl.ctas = (int)std::min<long long>(sms, (items + kWarps / W - 1) / (kWarps / W));

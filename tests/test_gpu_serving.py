@@ -94,3 +94,20 @@ def test_batches_through_layers_and_cache(dtype, Hq, Hk, D, page, prefix_len):
     assert cache.pool.free_pages == num
     hq.check_device_error()
     b.close()
+
+
+def test_a_step_without_rows():
+    """A request with no prompt is a chunk of no rows: nothing runs, and its decode steps follow."""
+    cache = KVCache(1, 4, 16, 2, 64, dtype=torch.float16)
+    b = SplitFuseBatcher(cache=cache)
+    b.submit_request(0, 1)
+    for rows in (0, 1):
+        batch = b.assemble_step_batch()
+        step = b.plan_attention(batch)
+        q, k = torch.randn((rows, 4, 64), device="cuda").half(), torch.randn((rows, 2, 64), device="cuda").half()
+        got = b.attend(step, 0, q, k, k)
+        assert got.shape == q.shape and torch.equal(got, k.repeat_interleave(2, 1))  # one key: its value
+        b.update_step_completion(batch)
+    assert not b.has_active_work() and cache.pool.free_pages == 4
+    hq.check_device_error()
+    b.close()
