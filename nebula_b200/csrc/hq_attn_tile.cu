@@ -438,11 +438,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
         const int boxes = kKeys / p.box_rows;
         int index = (int)blockIdx.x, use = 0;
         uint32_t loads[2] = {0, 0};
-        bool any = true;
+        int none = INT_MAX;  // blocks from this number on have no rows
         for (int k = 0, asked = 0;; ++asked) {
             Item it;
-            const bool found = any && make_item(p, index, it);
-            any = found;  // the numbers behind one without rows have none either
+            const bool found = index < none && make_item(p, index, it);
+            if (!found) none = min(none, index);
             if (asked == 0) ready();
             if (p.ask && lane == 0) next_block_request(&sh.next_block, &sh.next);
             __syncwarp();
@@ -519,7 +519,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
                 index = gave_up() ? -1 : next_block_answer(&sh.next_block);
             } else {
                 const bool last = index >= p.blocks * p.Hk * p.splits - (int)gridDim.x;
-                index = last || !any || gave_up() ? -1 : index + (int)gridDim.x;
+                index = last || !found || gave_up() ? -1 : index + (int)gridDim.x;
             }
             if (index < 0) {
                 if (k >= 2) wait(&sh.item_empty[k & 1], (uint32_t)((k - 2) >> 1));

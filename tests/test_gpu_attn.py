@@ -413,6 +413,43 @@ def test_bad_numbers_are_reported_and_touch_nothing():
         hq.check_device_error()
 
 
+@pytest.mark.parametrize("causal", [True, False])
+def test_a_long_prompt(causal):
+    """40000 tokens; rows at the begin, in the middle and at the end."""
+    T, D = 40000, 64
+    q, k, v = qkv_rows(T, 2, 1, D, BF16, gen(31))
+    got = at.attn_prompt(q, k, v, torch.tensor([0, T], dtype=torch.int32, device="cuda"), T, causal=causal)
+    for a in (0, 19990, T - 64):
+        seen = torch.arange(a + 1, a + 65) if causal else torch.full((64,), T)
+        o, _, m = attend(q[a: a + 64], k, v, seen, D ** -0.5)
+        check(got[a: a + 64], o, m, BF16)
+
+
+def test_a_bound_of_the_prompts_that_is_wrong():
+    """max_seqlen sizes the launch only."""
+    q, k, v = qkv_rows(700, 10, 2, 128, F16, gen(32))
+    cu = torch.tensor([0, 600, 700], dtype=torch.int32, device="cuda")
+    o, _, m = prompt_ref(q, k, v, [0, 600, 700], 128 ** -0.5)
+    for bound in (0, 1, 600, 10 ** 6):
+        check(at.attn_prompt(q, k, v, cu, bound), o, m, F16)
+
+
+def test_row_offsets_past_32_bits():
+    """q, k, v and out as columns of rows 2^20 elements apart."""
+    T, Hq, Hk, D = 2300, 4, 2, 64
+    wide = torch.zeros((T, 1 << 20), dtype=F16, device="cuda")  # 2.4e9 elements
+    base = torch.randn((T, 16, D), generator=gen(33), device="cuda", dtype=F16)
+    part = wide[:, : 16 * D].view(T, 16, D)
+    part.copy_(base)
+    q, k, v, out = part[:, :4], part[:, 4:6], part[:, 6:8], part[:, 8:12]
+    cu = torch.tensor([0, 5, T], dtype=torch.int32, device="cuda")
+    at.attn_prompt(q, k, v, cu, T, out=out)
+    seen = torch.arange(T - 5 - 100 + 1, T - 5 + 1)
+    o, _, m = attend(q[T - 100:], k[5:], v[5:], seen, D ** -0.5)
+    check(out[T - 100:], o, m, F16)
+    assert torch.equal(part[:, :8], base[:, :8]) and torch.equal(part[:, 12:], base[:, 12:])
+
+
 def test_captured_prompts_follow_their_offsets():
     """A captured call replayed with other prompts in the same rows."""
     T, Hq, Hk, D = 900, 10, 2, 128
