@@ -18,6 +18,7 @@ from __future__ import annotations
 
 import ctypes
 import struct
+from array import array
 
 import numpy as np
 import torch
@@ -224,10 +225,10 @@ def _moves(src, dst) -> bytes:
     n = len(src)
     if len(dst) != n:
         _bad(f"{n} source pages and {len(dst)} destinations")
-    both = np.empty((n, 2), np.int32)
-    both[:, 0] = src
-    both[:, 1] = dst
-    return both.tobytes()  # (its .ctypes.data costs as much as all of this)
+    both = array("i", bytes(8 * n))  # half of what numpy takes for lists, few moves or many
+    both[0::2] = array("i", src)
+    both[1::2] = array("i", dst)
+    return both.tobytes()
 
 
 def _page_bytes(shape, stride, size: int) -> int:
@@ -256,17 +257,17 @@ def kv_copy_pages(pools, src, dst, *, stream=None) -> None:
     if ctx is not None:
         with ctx:
             return kv_copy_pages(pools, src, dst)
-    bases, geometry = [], None
+    bases, geometry, last = [], None, None
     for t in pools:
-        shape, stride, size = t.shape, t.stride(), t.element_size()
+        like = shape, stride, size = t.shape, t.stride(), t.element_size()
         if t.get_device() != dev or len(shape) not in (4, 5):
             _bad(f"pools must be on {first.device}, of 4 or 5 dimensions: got {list(shape)} on {t.device}")
         at = len(shape) - 4
-        g = (shape[at], stride[at] * size, _page_bytes(shape[at + 1:], stride[at + 1:], size))
-        if geometry is None:
-            geometry = g
-        elif geometry != g:
-            _bad("pools of different geometry")
+        if like != last:
+            g = (shape[at], stride[at] * size, _page_bytes(shape[at + 1:], stride[at + 1:], size))
+            if geometry not in (None, g):
+                _bad("pools of different geometry")
+            geometry, last = g, like
         p = t.data_ptr()
         if at:
             step = stride[0] * size

@@ -79,7 +79,7 @@ struct AttnPlan {
     bool decode, tile;
     int prefix;          // key splits of the shared prefix (0: none)
     int own;             // key splits of the tile kernel
-    int tile_sms;        // SMs that it takes
+    int tile_blocks, tile_sms;  // its row blocks, as far as the sizes tell, and SMs
     DecodePlan dec;
     int dec_rows;
     bool join;           // partials of the decode kernel are joined by a kernel

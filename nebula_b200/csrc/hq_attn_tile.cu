@@ -975,17 +975,25 @@ AttnPlan attn_plan(int T, int B, int max_q, int Hq, int Hk, int D, bool paged, i
     pl.tile = !paged || (long long)max_q * G > kDecodeRows;
     pl.decode = paged && G <= kDecodeRows && (!pl.tile || B > 1);
     pl.prefix = prefix_len > 0 ? key_splits(row_blocks, Hk, prefix_len, sms) : 0;
+    if (pl.decode) pl.dec_rows = !pl.tile ? max_q * G : G <= 8 ? 8 : kDecodeRows;
     // Beside the decode kernel the tiles leave it its share of the SMs (a block counted as
     // three sequences), so that the two run at the same time.  16 streams and a chunk of 64
     // rows over 1500 keys: 36.8 us with all SMs for the tiles first (9 splits), 32.2 with 2
-    // splits on 32 SMs, 36.6 with 1 on 16.
-    pl.tile_sms = pl.decode ? std::max(1, (int)(3LL * row_blocks * sms / (3LL * row_blocks + B))) : sms;
-    pl.own = pl.tile ? key_splits(row_blocks, Hk, max_kv, pl.tile_sms) : 0;
+    // splits on 32 SMs, 36.6 with 1 on 16.  Of the sequences at least `big` are the tiles',
+    // by their rows.
+    pl.tile_blocks = row_blocks;
+    pl.tile_sms = sms;
+    if (pl.tile && pl.decode) {
+        const long long few = (long long)B * (pl.dec_rows / G);
+        const int big = (int)std::min<long long>(B, T > few ? ceil_div(T - few, max_q) : 0);
+        pl.tile_blocks = std::max(row_blocks, big * blocks_of(std::min(max_q, T), G));
+        pl.tile_sms = (int)std::max(1LL, 3LL * pl.tile_blocks * sms / (3LL * pl.tile_blocks + B - big));
+    }
+    pl.own = pl.tile ? key_splits(pl.tile_blocks, Hk, max_kv, pl.tile_sms) : 0;
     pl.planes = pl.prefix;
     if (pl.tile && pl.own + pl.prefix > 1) pl.planes += pl.own;
     if (pl.decode) {
         pl.dec = decode_plan(B, Hk, max_q, max_kv, sms);
-        pl.dec_rows = !pl.tile ? max_q * G : G <= 8 ? 8 : kDecodeRows;
         pl.join = pl.dec.mode == kFlat;
         if (pl.join) pl.slots = (size_t)pl.dec.ctas * 2 * kDecodeRows;
         if (pl.join && pl.prefix) ++pl.planes;
@@ -1055,7 +1063,7 @@ cudaError_t launch_attn(const AttnArgs& a) {
         p.part_l = part ? plane_l + pl.prefix * rows : nullptr;
         // every sequence may end inside a block
         p.blocks = (int)std::min((long long)row_blocks + a.B, 0x7fffffffLL);
-        const long long ctas = (long long)row_blocks * a.Hk * p.splits;
+        const long long ctas = (long long)pl.tile_blocks * a.Hk * p.splits;
         p.ask = ctas > a.sm_count;  // 12 prompts of 172 to 1500 tokens: 46.3 us, 53.0 without
         p.ctas = (int)std::min<long long>(a.sm_count, std::max<long long>(pl.tile_sms, ctas));
         if ((e = launch_tile_any(a, p)) != cudaSuccess) return e;

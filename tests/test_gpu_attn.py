@@ -239,6 +239,9 @@ PAGED = [
     (24, 2, 64, BF16, [3000, 9000, 40, 13500], [1, 100, 1, 1], 16, 300, "hnd"),
     (64, 1, 64, F16, [300, 900], [1, 2], 16, 40, "nhd"),
     (128, 1, 128, BF16, [300, 900], [1, 2], 16, 0, "nhd"),
+    # a few rows each of many sequences
+    (10, 2, 128, F16, [20 + 9 * i for i in range(100)], [4 - i % 4 for i in range(100)], 16, 0, "nhd"),
+    (5, 1, 64, BF16, [20 + 9 * i for i in range(100)], [4] * 100, 32, 50, "nhd"),
     # a prefix under more rows than the SMs take at once
     (16, 16, 64, F16, [600, 601, 40], [600, 300, 1], 32, 200, "nhd"),
 ]
