@@ -225,9 +225,14 @@ def _moves(src, dst) -> bytes:
     n = len(src)
     if len(dst) != n:
         _bad(f"{n} source pages and {len(dst)} destinations")
-    both = array("i", bytes(8 * n))  # half of what numpy takes for lists, few moves or many
-    both[0::2] = array("i", src)
-    both[1::2] = array("i", dst)
+    if isinstance(src, np.ndarray):
+        both = np.empty((n, 2), np.int32)
+        both[:, 0] = src
+        both[:, 1] = dst
+    else:  # lists: half of what numpy takes, few moves or many
+        both = array("i", bytes(8 * n))
+        both[0::2] = array("i", src)
+        both[1::2] = array("i", dst)
     return both.tobytes()
 
 

@@ -163,6 +163,9 @@ def test_python_refusals():
                 (pages[..., ::2], pages[..., ::2], table, lens)):
         with pytest.raises(E):
             at._view(*bad, F16, -1, 64)
+    for kind in (list, np.array, tuple, lambda x: torch.tensor(x)):
+        assert at._moves(kind([3, 4]), kind([7, 1])) == np.array([3, 7, 4, 1], np.int32).tobytes()
+    assert at._moves([], []) == b""
     with pytest.raises(E, match="one block"):
         at._page_bytes((16, 2, 64), (256, 64, 1), 2)
     assert at._page_bytes((16, 2, 64), (64, 1024, 1), 2) == 4096
