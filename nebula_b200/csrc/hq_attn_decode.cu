@@ -516,6 +516,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_decode_kernel(const __grid_c
         // Rows 8 pass .. 8 pass + 7 of the group's warps are joined, one warp a row, four
         // dims a lane; in a cluster then the CTAs' joined rows.
         const int levels = p.mode == kCluster ? 2 : 1;
+        int taken_out = 0;  // this item's any_bad
 #pragma unroll 1
         for (int pass = 0; pass < (R > 8 ? 2 : 1) + levels - 1; ++pass) {
             const bool across = p.mode == kCluster && pass == (R > 8 ? 2 : 1);  // the CTAs of a cluster
@@ -611,10 +612,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_decode_kernel(const __grid_c
                     if (lane == 0) (whole ? p.own_l[row] : p.slot_l[slot]) = l2;
                 }
             }
+            // All warps have set it before the first barrier of this item's, and the next item's
+            // first cannot set it before all are past the last one: read between the two, it is
+            // the same in all threads.
+            taken_out = sh.any_bad;
             if (across) cluster_sync();  // the others' rows have been read
             else group_sync();
         }
-        if (p.mode != kCluster && sh.any_bad) {  // W = 8: the same in all threads since the barriers above
+        if (p.mode != kCluster && taken_out) {  // W = 8: groups of fewer warps take nothing out
             __syncthreads();
             if (tid < 2 * DP) (&sh.bad[0][0])[tid] = 0;
             if (tid == 0) sh.any_bad = 0;
