@@ -17,6 +17,7 @@ Row offsets, lengths and page tables are int32 device tensors, read when the ker
 from __future__ import annotations
 
 import ctypes
+import operator
 import struct
 from array import array
 
@@ -220,6 +221,27 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: 
                              _rows(v, "v", dtype, dev, shape), view, _index(cu_q, "cu_q", B + 1, dev), _raw_stream(dev)))
 
 
+def _int32(x, name: str) -> np.ndarray:
+    """x as int32, without a number changed on the way."""
+    a = np.asarray(x)
+    if a.dtype == np.int32:
+        return a
+    if a.size and (a.dtype.kind not in "iub" or int(a.min()) < -2 ** 31 or int(a.max()) >= 2 ** 31):
+        _bad(f"{name} must be integers that int32 holds, got {a.dtype} {a.reshape(-1)[:8].tolist()}")
+    return a.astype(np.int32)
+
+
+def _int(x, name: str) -> int:
+    """x as an int of C's (ctypes takes the lower 32 bits of any)."""
+    try:
+        n = operator.index(x)
+    except TypeError:
+        n = None
+    if n is None or not -2 ** 31 <= n < 2 ** 31:
+        _bad(f"no {name} {x!r}")
+    return n
+
+
 def _moves(src, dst) -> bytes:
     """hq_page_move[n]."""
     n = len(src)
@@ -227,12 +249,12 @@ def _moves(src, dst) -> bytes:
         _bad(f"{n} source pages and {len(dst)} destinations")
     if isinstance(src, np.ndarray):
         both = np.empty((n, 2), np.int32)
-        both[:, 0] = src
-        both[:, 1] = dst
+        both[:, 0] = _int32(src, "source pages")
+        both[:, 1] = _int32(dst, "destination pages")
     else:  # lists: half of what numpy takes, few moves or many
         both = array("i", bytes(8 * n))
         both[0::2] = array("i", src)
-        both[1::2] = array("i", dst)
+        both[1::2] = array("i", dst if not isinstance(dst, np.ndarray) else _int32(dst, "destination pages"))
     return both.tobytes()
 
 
@@ -287,6 +309,8 @@ class PagePool:
     """Pages of a cache by sequence: reference counts and page lists on the host (hq_kv_pool_*)."""
 
     def __init__(self, num_pages: int, page_size: int):
+        self._h = None
+        num_pages, page_size = _int(num_pages, "number of pages"), _int(page_size, "page size")
         self._h = lib().hq_kv_pool_create(num_pages, page_size)
         if not self._h:
             _bad(f"no pool of {num_pages} pages of {page_size} (a power of two from 16 to 256)")
@@ -315,7 +339,7 @@ class PagePool:
 
     def fork(self, seq: int) -> int:
         """A sequence with the same keys; pages are shared until one of the two is extended."""
-        s = int(lib().hq_kv_pool_fork(self._h, seq))
+        s = int(lib().hq_kv_pool_fork(self._h, _int(seq, "sequence")))
         if s < 0:
             _bad(f"no sequence {seq}")
         return s
@@ -323,7 +347,7 @@ class PagePool:
     def extend(self, seqs, counts) -> list[tuple[int, int]]:
         """Room for counts[i] more keys of seqs[i] (integers, or lists of them), for all or for none; returns the page
         copies, (source, destination), to make first."""
-        seqs, counts = np.atleast_1d(np.asarray(seqs, np.int32)), np.atleast_1d(np.asarray(counts, np.int32))
+        seqs, counts = np.atleast_1d(_int32(seqs, "sequences")), np.atleast_1d(_int32(counts, "counts"))
         if seqs.ndim != 1 or seqs.shape != counts.shape:
             _bad(f"{seqs.size} sequences and {counts.size} counts")
         moves, n = np.empty((max(1, seqs.size), 2), np.int32), ctypes.c_int(0)
@@ -334,17 +358,18 @@ class PagePool:
         return [tuple(m) for m in moves[: n.value].tolist()]
 
     def free(self, seq: int) -> None:
-        status = lib().hq_kv_pool_free(self._h, seq)
+        status = lib().hq_kv_pool_free(self._h, _int(seq, "sequence"))
         if status != _lib.HQ_OK:
             raise HQError(status, f"no sequence {seq}")
 
     def seq_len(self, seq: int) -> int:
-        n = int(lib().hq_kv_pool_seq_len(self._h, seq))
+        n = int(lib().hq_kv_pool_seq_len(self._h, _int(seq, "sequence")))
         if n < 0:
             _bad(f"no sequence {seq}")
         return n
 
     def seq_pages(self, seq: int) -> np.ndarray:
+        seq = _int(seq, "sequence")
         n = int(lib().hq_kv_pool_seq_pages(self._h, seq, None, 0))
         if n < 0:
             _bad(f"no sequence {seq}")
@@ -354,7 +379,7 @@ class PagePool:
 
     def tables(self, seqs) -> tuple[np.ndarray, np.ndarray]:
         """(page table [n, pages], lengths [n]) of the sequences, int32 on the host."""
-        seqs = np.asarray(seqs, np.int32).reshape(-1)
+        seqs = _int32(seqs, "sequences").reshape(-1)
         L, lens = lib(), np.empty(seqs.size, np.int32)
         pages = int(L.hq_kv_pool_tables(self._h, seqs.ctypes.data, seqs.size, None, 0, lens.ctypes.data))
         if pages < 0:
