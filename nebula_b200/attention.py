@@ -222,13 +222,13 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: 
 
 
 def _int32(x, name: str) -> np.ndarray:
-    """x as int32, without a number changed on the way."""
+    """x as int32 one behind the other, without a number changed on the way."""
     a = np.asarray(x)
     if a.dtype == np.int32:
-        return a
+        return np.ascontiguousarray(a)
     if a.size and (a.dtype.kind not in "iub" or int(a.min()) < -2 ** 31 or int(a.max()) >= 2 ** 31):
         _bad(f"{name} must be integers that int32 holds, got {a.dtype} {a.reshape(-1)[:8].tolist()}")
-    return a.astype(np.int32)
+    return a.astype(np.int32, order="C")
 
 
 def _int(x, name: str) -> int:

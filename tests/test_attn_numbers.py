@@ -71,3 +71,21 @@ def test_sizes_of_a_pool():
     for size in ((2 ** 32 + 4, 16), (4, 2 ** 32 + 16), (4.0, 16), (4, 16.0)):
         with pytest.raises(_lib.HQError, match="HQ_ERR_INVALID_ARG"):
             at.PagePool(*size)
+
+
+@pytest.mark.parametrize("dt", [np.int32, np.int64])
+def test_sequences_and_counts_in_strided_arrays(dt):
+    """Every second element, in either order: the numbers that the array shows, not those that lie beside them."""
+    pool = at.PagePool(20, 16)
+    seqs = np.array([pool.new_seq() for _ in range(6)], dt)
+    counts = np.array([1, 20, 3, 40, 5, 60], dt)
+    pool.extend(seqs[::2], counts[::2])
+    pool.extend(seqs[::-2], counts[::-2])
+    assert [pool.seq_len(int(s)) for s in seqs] == counts.tolist()
+    table, lens = pool.tables(seqs[::-1])
+    assert lens.tolist() == counts[::-1].tolist()
+    assert [row[0] for row in table] == [pool.seq_pages(int(s))[0] for s in seqs[::-1]]
+    both = np.stack([seqs, counts], 1)  # columns
+    pool.extend(both[:, 0], both[:, 1])
+    assert pool.tables(both[:, 0])[1].tolist() == (2 * counts).tolist()
+    pool.close()
