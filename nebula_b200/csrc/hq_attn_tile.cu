@@ -971,6 +971,7 @@ static int blocks_of(int n, int G) { return ceil_div(n, 2 * (kRows / G)); }
 
 AttnPlan attn_plan(int T, int B, int max_q, int Hq, int Hk, int D, bool paged, int max_kv, int prefix_len, int sms) {
     AttnPlan pl{};
+    max_q = std::max(1, max_q);  // a bound of 0 may be wrong, too: rows of one each still have their kernel
     const int G = Hq / Hk, row_blocks = blocks_of(T, G);
     pl.tile = !paged || (long long)max_q * G > kDecodeRows;
     pl.decode = paged && G <= kDecodeRows && (!pl.tile || B > 1);
