@@ -742,7 +742,8 @@ cudaError_t launch_any(const AttnArgs& a, const DecodeParams& p, int ctas) {
 
 DecodePlan decode_plan(int B, int Hk, int max_q, int max_kv, int sms) {
     const long long items = (long long)B * Hk;
-    const int tiles = std::max(1, (max_kv + kUnit - 1) / kUnit);
+    const int last = std::max(1, max_kv) - 1;  // the last key; max_kv may be the largest int
+    const int tiles = 1 + last / kUnit;
     DecodePlan pl{};
     pl.cluster = 1;
     pl.group = kWarps;
@@ -770,7 +771,7 @@ DecodePlan decode_plan(int B, int Hk, int max_q, int max_kv, int sms) {
     int W = kWarps;
     while (W > 1 && max_q == 1 && items * W > (long long)sms * kWarps) W /= 2;
     const long long slots = (long long)sms * (kWarps / W), rounds = (items + slots - 1) / slots;
-    if (rounds * std::max(1, (max_kv + kSlice * W - 1) / (kSlice * W)) <= (W == kWarps ? 40 : 64)) {
+    if (rounds * (1 + last / (kSlice * W)) <= (W == kWarps ? 40 : 64)) {
         pl.mode = kWhole;
         pl.group = W;
         pl.ctas = (int)std::min<long long>(sms, (items + kWarps / W - 1) / (kWarps / W));
