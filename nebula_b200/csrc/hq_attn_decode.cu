@@ -103,7 +103,7 @@ __device__ __forceinline__ Seq seq_of(const int* cu_q, const int* kv_lens, int T
         bad_index(err);
         return q;
     }
-    q.tiles = max(1, (int)((unsigned)(q.len + unit - 1) / (unsigned)unit));
+    q.tiles = max(1, (int)(((unsigned)q.len + (unsigned)unit - 1u) / (unsigned)unit));
     return q;
 }
 
@@ -598,7 +598,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_decode_kernel(const __grid_c
                 if (out && p.prefix_splits)
                     join_parts(x, p.prefix_splits, p.pre_o, p.pre_l, p.D, d, [&](int i) { return i * rows + row; });
                 // no key: zeros; scores that are all -inf: NaN, or left to the join
-                const float l2 = finish_row(x, out && see + p.prefix_len > 0);
+                const float l2 = finish_row(x, out && sees_any(see, p.prefix_len));
                 if (out) {
                     if (d < p.D)
                         *reinterpret_cast<uint2*>(static_cast<T16*>(p.o) + (size_t)(at.seq.first + tok) * p.o_st +
@@ -692,7 +692,7 @@ __global__ void __launch_bounds__(kThreads) attn_join_kernel(const JoinParams p)
                 return k ? i * rows + row : whole ? row : (size_t)(2 * (c0 + i) + (i == 0 && mid ? 1 : 0)) * kMaxRows + r;
             });
         }
-        const float l2 = finish_row(x, p.prefix_len + keys_seen(me.len, me.n, tok, 1) > 0);
+        const float l2 = finish_row(x, sees_any(keys_seen(me.len, me.n, tok, 1), p.prefix_len));
         if (d < p.D)
             *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.o) + (size_t)(me.first + tok) * p.o_st + (size_t)hd * p.o_sh +
                                       d) = make_uint2(pack2<kBF16>(x.acc[0], x.acc[1]), pack2<kBF16>(x.acc[2], x.acc[3]));

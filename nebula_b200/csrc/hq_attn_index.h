@@ -38,4 +38,10 @@ HQ_HD int keys_seen(int len, int n, int i, int causal) {
     return x < 0 ? 0 : x;
 }
 
+// Tiles of `unit` keys that hold `keys` of them, which may be the largest int.
+HQ_HD int key_tiles(int keys, int unit) { return keys / unit + (keys % unit != 0); }
+
+// A row that sees `own` keys of its sequence and all `prefix` before them sees one.
+HQ_HD bool sees_any(int own, int prefix) { return own > 0 || prefix > 0; }
+
 }  // namespace hq

@@ -279,8 +279,7 @@ __device__ __forceinline__ bool make_item(const TileParams& p, int index, Item& 
     const int causal = p.causal && !p.prefix_len, tile = p.tile_tokens;
     it.token0 = block * 2 * tile;
     auto seen = [&](int token) { return keys_seen(it.len, it.n, min(token, it.n - 1), causal); };
-    const int end1 = (seen(it.token0 + 2 * tile - 1) + kKeys - 1) / kKeys;
-    const int end0 = (seen(it.token0 + tile - 1) + kKeys - 1) / kKeys;
+    const int end1 = key_tiles(seen(it.token0 + 2 * tile - 1), kKeys), end0 = key_tiles(seen(it.token0 + tile - 1), kKeys);
     const int a = end1 * split / p.splits, b = end1 * (split + 1) / p.splits;  // end1 <= 2^24, splits <= 32
     it.ni[0] = max(0, min(b, end0) - a);
     it.ni[1] = it.token0 + tile < it.n ? b - a : 0;
@@ -465,7 +464,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tile_kernel(const __grid_con
                 // boxes.  (With a box a lane a tile over pages of 16 took 2000 cycles: a
                 // request's operands come from uniform registers, so it is lane after lane.)
                 const int box = lane;
-                auto live_at = [&](int k0) { return min(boxes, (it.len - k0 + p.box_rows - 1) >> p.box_shift); };
+                auto live_at = [&](int k0) { return min(boxes, ((it.len - k0 - 1) >> p.box_shift) + 1); };
                 auto page_at = [&](int k0) {
                     return p.page_size && box < live_at(k0) ? __ldg(it.table + ((k0 + (box << p.box_shift)) >> p.page_shift)) : 0;
                 };
@@ -890,7 +889,7 @@ __global__ void __launch_bounds__(256) attn_merge_kernel(const MergeParams p) {
     x.top = -INFINITY;
     const int d = 4 * lane;
     join_parts(x, p.splits, p.part_o, p.part_l, p.D, d, [&](int s) { return s * rows + row; });
-    const float l2 = finish_row(x, seen + p.prefix_len > 0);
+    const float l2 = finish_row(x, sees_any(seen, p.prefix_len));
     if (d < p.D) {
         uint16_t* dst = static_cast<uint16_t*>(p.o) + (size_t)t * p.o_st + (size_t)h * p.o_sh + d;
         *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<kBF16>(x.acc[0], x.acc[1]), pack2<kBF16>(x.acc[2], x.acc[3]));
