@@ -110,9 +110,14 @@ class SplitFuseBatcher:
         writes to them, and prompt_tokens counts the tokens after them."""
         if parent is not None and parent not in self._seqs:
             raise ValueError(f"request {parent} holds no keys")
-        request = int(lib().hq_batcher_submit(self._h, prompt_tokens, max_decode_tokens))
-        if parent is not None:
-            seq = self.cache.fork(self._seqs[parent][0])
+        seq = self.cache.fork(self._seqs[parent][0]) if parent is not None else None
+        try:
+            request = int(lib().hq_batcher_submit(self._h, prompt_tokens, max_decode_tokens))
+        except ctypes.ArgumentError:
+            if seq is not None:
+                self.cache.free(seq)
+            raise
+        if seq is not None:
             self._seqs[request] = seq, self.cache.pool.seq_len(seq)
         return request
 
