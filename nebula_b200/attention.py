@@ -398,13 +398,15 @@ class PagePool:
 
 
 class KVCache:
-    """A paged cache of all layers: k and v [layers, num_pages, page_size, kv_heads, head_dim], and its pool."""
+    """A paged cache of all layers: k and v [layers, num_pages, page_size, kv_heads, head_dim], and its pool.  The page
+    copies of an extend or compact that raised are made by the next one, before its own."""
 
     def __init__(self, layers: int, num_pages: int, page_size: int, kv_heads: int, head_dim: int, dtype=torch.bfloat16,
                  device="cuda"):
         self.pool = PagePool(num_pages, page_size)
         self.k = torch.zeros((layers, num_pages, page_size, kv_heads, head_dim), dtype=dtype, device=device)
         self.v = torch.zeros_like(self.k)
+        self._owed = []  # lists of copies that the pool counts on, in their order
 
     def new_seq(self) -> int:
         return self.pool.new_seq()
@@ -418,13 +420,19 @@ class KVCache:
     def extend(self, seqs, counts, stream=None) -> None:
         """Room for counts[i] more keys of seqs[i], for all or for none; pages that forks still share are copied, all
         layers in one call."""
-        self._copy(self.pool.extend(seqs, counts), stream)
+        self._move(self.pool.extend(seqs, counts), stream)
 
     def compact(self, stream=None) -> int:
         """Moves the pages in use to the front; returns how many moved."""
         moves = self.pool.compact()
-        self._copy(moves, stream)
+        self._move(moves, stream)
         return len(moves)
+
+    def _move(self, moves, stream):
+        self._owed.append(moves)
+        while self._owed:
+            self._copy(self._owed[0], stream)
+            del self._owed[0]
 
     def _copy(self, moves, stream):
         if moves:

@@ -34,3 +34,57 @@ def test_a_request_that_is_refused_forks_nothing():
         b.submit_request(3.5, 4, parent)
     assert b.num_active_requests() == 1 and cache.new_seq() == 1  # the number after the parent's: no fork has it
     b.close()
+
+
+class FailingCache(HostCache):
+    """Its next `failures` copies of pages raise."""
+    failures = 0
+
+    def _copy(self, moves, stream):
+        if moves and self.failures:
+            self.failures -= 1
+            raise RuntimeError("no copy")
+        super()._copy(moves, stream)
+
+
+def marked(cache, n):
+    """A sequence of n keys with the marks 1 .. n."""
+    s = cache.new_seq()
+    cache.extend([s], [n])
+    for j, (page, slot) in enumerate((p, i) for p in cache.pool.seq_pages(s) for i in range(cache.pool.page_size)):
+        if j < n:
+            cache.k[0, int(page), slot, 0, 0] = j + 1.0
+    return s
+
+
+@pytest.mark.parametrize("again", ["same", "nothing", "other", "compact"])
+def test_copies_that_fail_are_made_by_the_next_call(again):
+    """The pool has moved on by then: the copy is owed, not lost."""
+    cache = FailingCache(9, 16)
+    a = marked(cache, 21)
+    b, other = cache.fork(a), marked(cache, 3)
+    cache.failures = 1
+    with pytest.raises(RuntimeError, match="no copy"):
+        cache.extend([b], [2])
+    assert cache.pool.seq_len(b) == 23 and cache.pool.seq_pages(a)[1] != cache.pool.seq_pages(b)[1]
+    if again == "compact":
+        cache.free(other)
+        cache.compact()
+    else:
+        cache.extend(*{"same": ([b], [0]), "nothing": ([], []), "other": ([other], [1])}[again])
+    for s in (a, b):
+        assert keys(cache, cache.pool.seq_pages(s), 21) == [j + 1.0 for j in range(21)]
+
+
+def test_a_compaction_that_fails_is_made_up_for():
+    cache = FailingCache(9, 16)
+    a, b = marked(cache, 40), marked(cache, 21)
+    c = cache.fork(b)
+    cache.free(a)
+    cache.failures = 3
+    for call in (cache.compact, lambda: cache.extend([c], [1]), cache.compact):  # owed in turn: moved, copied, moved
+        with pytest.raises(RuntimeError, match="no copy"):
+            call()
+    cache.extend([], [])
+    for s in (b, c):
+        assert keys(cache, cache.pool.seq_pages(s), 21) == [j + 1.0 for j in range(21)]
