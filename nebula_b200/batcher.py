@@ -7,7 +7,7 @@ from __future__ import annotations
 import ctypes
 from dataclasses import dataclass
 
-from ._lib import check, lib
+from ._lib import HQError, check, lib
 
 QUEUED, RUNNING_PREFILL, RUNNING_DECODE, COMPLETED = range(4)
 
@@ -93,6 +93,11 @@ class SplitFuseBatcher:
         if self._h:
             lib().hq_batcher_destroy(self._h)
             self._h = None
+            for request in list(self._seqs):
+                try:
+                    self._release(request)
+                except HQError:  # the cache is closed
+                    pass
 
     def __del__(self):
         try:

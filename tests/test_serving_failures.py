@@ -88,3 +88,21 @@ def test_a_compaction_that_fails_is_made_up_for():
     cache.extend([], [])
     for s in (b, c):
         assert keys(cache, cache.pool.seq_pages(s), 21) == [j + 1.0 for j in range(21)]
+
+
+def test_a_closed_batcher_gives_its_pages_back():
+    cache = HostCache(8, 16)
+    b = SplitFuseBatcher(cache=cache)
+    parent = b.submit_request(20, 4)
+    b.plan_attention(b.assemble_step_batch())
+    b.submit_request(3, 4, parent)
+    assert cache.pool.free_pages == 6
+    b.close()
+    assert cache.pool.free_pages == 8 and not b._seqs
+    b.close()
+    cache.pool.close()  # before its batcher: nothing to give back to
+    b = SplitFuseBatcher(cache=HostCache(8, 16))
+    b.submit_request(20, 4)
+    b.plan_attention(b.assemble_step_batch())
+    b.cache.pool.close()
+    b.close()
