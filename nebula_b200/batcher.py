@@ -178,8 +178,8 @@ class SplitFuseBatcher:
         """One layer's attention of a planned step: k and v [rows, Hkv, D] go into the layer's pages, then q
         [rows, Hq, D] attends to its sequences' keys.  Returns [rows, Hq, D]."""
         from . import attention
-        if q.shape[0] != step.rows:
-            raise ValueError(f"{q.shape[0]} rows for a step of {step.rows}")
+        if q.shape[0] != step.rows or min(k.shape[0], v.shape[0]) < step.rows:
+            raise ValueError(f"{q.shape[0]} rows for a step of {step.rows}, with {k.shape[0]} keys and {v.shape[0]} values")
         kp, vp = self.cache.k[layer], self.cache.v[layer]
         attention.kv_append(k, v, kp, vp, step.page_table, step.kv_lens, step.cu_q, stream=stream)
         return attention.attn_paged(q, kp, vp, step.page_table, step.kv_lens, step.cu_q, step.max_q_len,

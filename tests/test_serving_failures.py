@@ -106,3 +106,14 @@ def test_a_closed_batcher_gives_its_pages_back():
     b.plan_attention(b.assemble_step_batch())
     b.cache.pool.close()
     b.close()
+
+
+@pytest.mark.parametrize("q,k,v", [(3, 4, 4), (4, 3, 4), (4, 3, 3), (4, 4, 3), (4, 0, 0)])
+def test_attend_takes_the_rows_of_its_step(q, k, v):
+    """With too few keys the last sequences would attend to what their pages held before."""
+    b = SplitFuseBatcher(cache=HostCache(3, 16))
+    b.submit_request(4, 4)
+    step = b.plan_attention(b.assemble_step_batch())
+    with pytest.raises(ValueError, match="rows for a step of 4"):
+        b.attend(step, 0, *[torch.zeros((n, 1, 8), dtype=torch.float16) for n in (q, k, v)])
+    b.close()
