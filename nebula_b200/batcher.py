@@ -69,6 +69,8 @@ class AttentionStep:
     max_kv_len: int
     prefix_table: object
     prefix_len: int
+    stream: object = None     # the one that the plan was given
+    planned_on: object = None  # that one, or the one that was current
 
 
 class SplitFuseBatcher:
@@ -78,7 +80,8 @@ class SplitFuseBatcher:
     With a ``cache`` (attention.KVCache) the batcher keeps the requests' keys and values there: plan_attention makes
     room for a batch's rows, attend runs a layer's attention, update_step_completion frees what completed requests
     held.  ``prefix``: a sequence of the cache whose keys every request sees before its own.  All device work belongs
-    on one stream, and the cache is compacted between steps only."""
+    on one stream, the current one or the one that plan_attention is given, and the cache is compacted between steps
+    only."""
 
     def __init__(self, max_prefill_chunk_tokens=64, max_decode_streams=16, max_batch_tokens=512, *, cache=None,
                  prefix=None):
@@ -148,9 +151,11 @@ class SplitFuseBatcher:
             if c.request_id in self._seqs and self.request_state(c.request_id)["status"] == COMPLETED:
                 self._release(c.request_id)
 
-    def plan_attention(self, batch: FusedBatch) -> AttentionStep:
+    def plan_attention(self, batch: FusedBatch, stream=None) -> AttentionStep:
         """Room in the cache for the batch's rows, for all or (HQ_ERR_OUT_OF_PAGES) for none, and their places.  To be
-        called before the batch's attend; again for the same batch it gives the same."""
+        called before the batch's attend; again for the same batch it gives the same.  The copies of pages that forks
+        share run on ``stream``, which is attend's then, too."""
+        import contextlib
         import numpy as np
         import torch
         cache = self.cache
@@ -162,22 +167,34 @@ class SplitFuseBatcher:
                 self._seqs[c.request_id] = cache.new_seq(), 0
         seqs = [self._seqs[c.request_id][0] for c in chunks]
         ends = [self._seqs[c.request_id][1] + c.start_token + c.num_tokens for c in chunks]
-        cache.extend(seqs, [max(0, e - cache.pool.seq_len(s)) for s, e in zip(seqs, ends)])
+        cache.extend(seqs, [max(0, e - cache.pool.seq_len(s)) for s, e in zip(seqs, ends)], stream)
         table, _ = cache.pool.tables(seqs)
         prefix = cache.pool.seq_pages(self.prefix) if self.prefix is not None else np.empty(0, np.int32)
         n = len(seqs)
         counts = [c.num_tokens for c in chunks]
         host = np.concatenate([table.reshape(-1), prefix, np.array(ends, np.int32),
                                np.cumsum([0] + counts, dtype=np.int32)])
-        dev = torch.from_numpy(host).to(cache.k.device)  # one copy for all four
+        on = stream
+        if on is None and cache.k.is_cuda:
+            on = torch.cuda.current_stream(cache.k.device)
+        with torch.cuda.stream(stream) if stream is not None and cache.k.is_cuda else contextlib.nullcontext():
+            dev = torch.from_numpy(host).to(cache.k.device)  # one copy for all four
         pages, pre, lens, cu = dev.split([table.size, prefix.size, n, n + 1])
         return AttentionStep(sum(counts), cu, pages.view(table.shape), lens, max(counts, default=0), max(ends, default=0), pre,
-                             cache.pool.seq_len(self.prefix) if self.prefix is not None else 0)
+                             cache.pool.seq_len(self.prefix) if self.prefix is not None else 0, stream, on)
 
     def attend(self, step: AttentionStep, layer: int, q, k, v, *, scale=None, out=None, workspace=None, stream=None):
         """One layer's attention of a planned step: k and v [rows, Hkv, D] go into the layer's pages, then q
-        [rows, Hq, D] attends to its sequences' keys.  Returns [rows, Hq, D]."""
+        [rows, Hq, D] attends to its sequences' keys.  Returns [rows, Hq, D].  On the stream that the plan was given,
+        else on the current one; ``stream`` may name the plan's own, no other."""
+        import torch
+
         from . import attention
+        if stream is None:
+            stream = step.stream
+        elif step.planned_on is not None and stream.cuda_stream != step.planned_on.cuda_stream and \
+                not (q.is_cuda and torch.cuda.is_current_stream_capturing()):  # a captured call runs where it is replayed
+            raise ValueError("attend on another stream than plan_attention's, whose page copies it would not wait for")
         if q.shape[0] != step.rows or min(k.shape[0], v.shape[0]) < step.rows:
             raise ValueError(f"{q.shape[0]} rows for a step of {step.rows}, with {k.shape[0]} keys and {v.shape[0]} values")
         kp, vp = self.cache.k[layer], self.cache.v[layer]

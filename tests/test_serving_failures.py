@@ -117,3 +117,35 @@ def test_attend_takes_the_rows_of_its_step(q, k, v):
     with pytest.raises(ValueError, match="rows for a step of 4"):
         b.attend(step, 0, *[torch.zeros((n, 1, 8), dtype=torch.float16) for n in (q, k, v)])
     b.close()
+
+
+class Stream:
+    def __init__(self, handle):
+        self.cuda_stream = handle
+
+
+def test_a_steps_copies_and_attention_are_of_one_stream():
+    """The copy of a page that a fork shares is made on the plan's stream, and attend refuses another."""
+    class Cache(HostCache):
+        def _copy(self, moves, stream):
+            if moves:
+                self.on = stream
+            super()._copy(moves, stream)
+
+    cache = Cache(8, 16)
+    b = SplitFuseBatcher(cache=cache)
+    parent = b.submit_request(20, 4)
+    batch = b.assemble_step_batch()
+    b.plan_attention(batch)
+    b.update_step_completion(batch)
+    b.submit_request(3, 4, parent)
+    mine, same, other = Stream(7), Stream(7), Stream(8)
+    step = b.plan_attention(b.assemble_step_batch(), stream=mine)
+    assert cache.on is mine and step.stream is mine
+    rows = [torch.zeros((step.rows, 1, 8), dtype=torch.float16)] * 3
+    with pytest.raises(ValueError, match="another stream"):
+        b.attend(step, 0, *rows, stream=other)
+    for ok in (None, mine, same):
+        with pytest.raises(_lib.HQError, match="CUDA device"):  # the host's cache comes no further
+            b.attend(step, 0, *rows, stream=ok)
+    b.close()
