@@ -574,6 +574,10 @@ HQ_API uint32_t hq_batcher_submit(hq_batcher* b, uint32_t prompt_tokens, uint32_
 HQ_API int hq_batcher_assemble(hq_batcher* b, hq_batch_chunk* chunks, int max_chunks, hq_batch_info* info);
 /* update_step_completion. */
 HQ_API hq_status hq_batcher_complete(hq_batcher* b, const hq_batch_chunk* chunks, int n);
+/* Gives an active request up: it leaves the queue or the decode streams as
+ * HQ_REQ_COMPLETED, and its chunk of a batch assembled before does nothing at
+ * hq_batcher_complete.  HQ_ERR_INVALID_ARG: no such request, or not active. */
+HQ_API hq_status hq_batcher_cancel(hq_batcher* b, uint32_t request_id);
 HQ_API int hq_batcher_has_work(const hq_batcher* b);
 HQ_API size_t hq_batcher_active_requests(const hq_batcher* b);
 HQ_API hq_status hq_batcher_request_state(const hq_batcher* b, uint32_t request_id, hq_request_state* out);

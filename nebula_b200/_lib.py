@@ -70,6 +70,7 @@ SIGNATURES = {
     "hq_batcher_submit": (_u32, [_vp, _u32, _u32]),
     "hq_batcher_assemble": (_i, [_vp, _vp, _i, _vp]),
     "hq_batcher_complete": (_i, [_vp, _vp, _i]),
+    "hq_batcher_cancel": (_i, [_vp, _u32]),
     "hq_batcher_has_work": (_i, [_vp]),
     "hq_batcher_active_requests": (_sz, [_vp]),
     "hq_batcher_request_state": (_i, [_vp, _u32, _vp]),

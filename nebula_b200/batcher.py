@@ -7,7 +7,7 @@ from __future__ import annotations
 import ctypes
 from dataclasses import dataclass
 
-from ._lib import HQError, check, lib
+from ._lib import HQ_ERR_INVALID_ARG, HQ_OK, HQError, check, lib
 
 QUEUED, RUNNING_PREFILL, RUNNING_DECODE, COMPLETED = range(4)
 
@@ -75,7 +75,7 @@ class AttentionStep:
 
 class SplitFuseBatcher:
     """SplitFuseBatcher's scheduling surface: submit_request, assemble_step_batch, update_step_completion,
-    has_active_work, num_active_requests, reset; plus execute_step over real quantized layers.
+    has_active_work, num_active_requests, reset, and cancel_request; plus execute_step over real quantized layers.
 
     With a ``cache`` (attention.KVCache) the batcher keeps the requests' keys and values there: plan_attention makes
     room for a batch's rows, attend runs a layer's attention, update_step_completion frees what completed requests
@@ -129,6 +129,15 @@ class SplitFuseBatcher:
             self._seqs[request] = seq, self.cache.pool.seq_len(seq)
         return request
 
+    def cancel_request(self, request: int):
+        """Gives an active request up, between two steps or where a step finds no pages: what it holds in the cache is
+        freed, and batches are to be assembled anew."""
+        status = lib().hq_batcher_cancel(self._h, request) if 0 < request < 2 ** 32 else HQ_ERR_INVALID_ARG
+        if status != HQ_OK:
+            raise HQError(status, f"no active request {request}")
+        if request in self._seqs:
+            self._release(request)
+
     def _release(self, request: int):
         self.cache.free(self._seqs.pop(request)[0])
 
@@ -164,6 +173,8 @@ class SplitFuseBatcher:
         chunks = [c for c in batch.chunks if c.num_tokens]
         for c in chunks:
             if c.request_id not in self._seqs:
+                if self.request_state(c.request_id)["status"] == COMPLETED:
+                    raise ValueError(f"request {c.request_id} is not active")
                 self._seqs[c.request_id] = cache.new_seq(), 0
         seqs = [self._seqs[c.request_id][0] for c in chunks]
         ends = [self._seqs[c.request_id][1] + c.start_token + c.num_tokens for c in chunks]

@@ -28,6 +28,7 @@ namespace {
 struct Request {
     uint32_t id = 0, prompt = 0, prefilled = 0, generated = 0, max_decode = 0;
     int status = HQ_REQ_QUEUED;
+    bool cancelled = false;
 };
 
 }  // namespace
@@ -112,6 +113,7 @@ HQ_API hq_status hq_batcher_complete(hq_batcher* b, const hq_batch_chunk* chunks
     for (int i = 0; i < n; ++i) {
         const hq_batch_chunk& c = chunks[i];
         Request& r = b->requests[c.request_id - 1];
+        if (r.cancelled) continue;  // since the batch was assembled
         if (c.is_prefill) {
             r.prefilled += c.num_tokens;
             if (r.prefilled >= r.prompt) {
@@ -127,6 +129,17 @@ HQ_API hq_status hq_batcher_complete(hq_batcher* b, const hq_batch_chunk* chunks
     b->decode.erase(std::remove_if(b->decode.begin(), b->decode.end(),
                                    [b](uint32_t id) { return b->requests[id - 1].status == HQ_REQ_COMPLETED; }),
                     b->decode.end());
+    return HQ_OK;
+}
+
+HQ_API hq_status hq_batcher_cancel(hq_batcher* b, uint32_t request_id) {
+    if (!b || request_id == 0 || request_id > b->requests.size()) return HQ_ERR_INVALID_ARG;
+    Request& r = b->requests[request_id - 1];
+    if (r.status == HQ_REQ_COMPLETED) return HQ_ERR_INVALID_ARG;
+    r.status = HQ_REQ_COMPLETED;
+    r.cancelled = true;
+    b->prefill_queue.erase(std::remove(b->prefill_queue.begin(), b->prefill_queue.end(), request_id), b->prefill_queue.end());
+    b->decode.erase(std::remove(b->decode.begin(), b->decode.end(), request_id), b->decode.end());
     return HQ_OK;
 }
 

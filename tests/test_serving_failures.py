@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from nebula_b200 import _lib
-from nebula_b200.batcher import SplitFuseBatcher
+from nebula_b200.batcher import COMPLETED, SplitFuseBatcher
 from test_serving import HostCache, keys, write
 
 
@@ -148,4 +148,72 @@ def test_a_steps_copies_and_attention_are_of_one_stream():
     for ok in (None, mine, same):
         with pytest.raises(_lib.HQError, match="CUDA device"):  # the host's cache comes no further
             b.attend(step, 0, *rows, stream=ok)
+    b.close()
+
+
+def test_a_request_given_up_makes_room_for_the_others():
+    """A step without pages: one request leaves, its pages with it, and the step goes on."""
+    cache = HostCache(3, 16)
+    b = SplitFuseBatcher(16, 16, 64, cache=cache)
+    a, c = b.submit_request(30, 4), b.submit_request(16, 9)
+    for _ in range(3):
+        batch = b.assemble_step_batch()
+        b.plan_attention(batch)
+        b.update_step_completion(batch)
+    old = b.assemble_step_batch()
+    with pytest.raises(_lib.HQError, match="HQ_ERR_OUT_OF_PAGES"):
+        b.plan_attention(old)
+    b.cancel_request(a)
+    assert cache.pool.free_pages == 2 and b.num_active_requests() == 1
+    assert b.request_state(a)["status"] == COMPLETED and b.request_state(a)["decode_tokens_generated"] == 1
+    with pytest.raises(ValueError, match=f"request {a} is not active"):
+        b.plan_attention(old)  # a batch from before
+    with pytest.raises(_lib.HQError, match="HQ_ERR_INVALID_ARG"):
+        b.cancel_request(a)
+    batch = b.assemble_step_batch()
+    assert [x.request_id for x in batch.chunks] == [c]
+    while b.has_active_work():
+        batch = b.assemble_step_batch()
+        b.plan_attention(batch)
+        b.update_step_completion(batch)
+    assert cache.pool.free_pages == 3
+    b.close()
+
+
+def test_requests_given_up_at_any_stage():
+    """Queued, in prefill, decoding; children keep the shared keys; a batch assembled before completes the others only."""
+    cache = HostCache(20, 16)
+    b = SplitFuseBatcher(16, 16, 64, cache=cache)
+    first, second, third = b.submit_request(40, 9), b.submit_request(5, 9), b.submit_request(5, 2)
+    for bad in (0, 4, 99, -1, 2 ** 32 + 1):
+        with pytest.raises(_lib.HQError, match="HQ_ERR_INVALID_ARG"):
+            b.cancel_request(bad)
+    batch = b.assemble_step_batch()
+    write(cache, b.plan_attention(batch), range(1, 17))
+    child = b.submit_request(1, 1, first)
+    b.cancel_request(second)  # queued
+    b.cancel_request(first)   # in prefill, in a batch
+    b.update_step_completion(batch)
+    assert b.request_state(first)["prefill_completed_tokens"] == 0 and b.num_active_requests() == 2
+    batch = b.assemble_step_batch()
+    assert [x.request_id for x in batch.chunks] == [third]
+    b.plan_attention(batch)
+    b.update_step_completion(batch)
+    batch = b.assemble_step_batch()
+    assert [(x.request_id, x.is_prefill) for x in batch.chunks] == [(third, False), (child, True)]
+    step = b.plan_attention(batch)
+    assert keys(cache, step.page_table[1], 16) == [float(i) for i in range(1, 17)]
+    b.cancel_request(third)   # decoding, in a batch
+    b.update_step_completion(batch)
+    batch = b.assemble_step_batch()
+    assert [x.request_id for x in batch.chunks] == [child]
+    b.plan_attention(batch)
+    b.update_step_completion(batch)
+    assert not b.has_active_work() and cache.pool.free_pages == 20
+    b.reset()
+    plain = SplitFuseBatcher()  # without a cache
+    n = plain.submit_request(4, 4)
+    plain.cancel_request(n)
+    assert not plain.has_active_work()
+    plain.close()
     b.close()
