@@ -221,11 +221,19 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: 
                              _rows(v, "v", dtype, dev, shape), view, _index(cu_q, "cu_q", B + 1, dev), _raw_stream(dev)))
 
 
+_I32 = np.dtype(np.int32)
+
+
 def _int32(x, name: str) -> np.ndarray:
     """x as int32 one behind the other, without a number changed on the way."""
-    a = np.asarray(x)
-    if a.dtype == np.int32:
-        return np.ascontiguousarray(a)
+    if type(x) is list:  # a tenth of the time that numpy takes to look at one
+        try:
+            return np.asarray(array("i", x))
+        except (TypeError, OverflowError):
+            pass  # said below
+    a = x if type(x) is np.ndarray else np.asarray(x)
+    if a.dtype is _I32:
+        return a if a.flags.c_contiguous else a.copy()
     if a.size and (a.dtype.kind not in "iub" or int(a.min()) < -2 ** 31 or int(a.max()) >= 2 ** 31):
         _bad(f"{name} must be integers that int32 holds, got {a.dtype} {a.reshape(-1)[:8].tolist()}")
     return a.astype(np.int32, order="C")
