@@ -256,9 +256,9 @@ def _moves(src, dst) -> bytes:
     if len(dst) != n:
         _bad(f"{n} source pages and {len(dst)} destinations")
     if isinstance(src, np.ndarray):
-        both = np.empty((n, 2), np.int32)
-        both[:, 0] = _int32(src, "source pages")
-        both[:, 1] = _int32(dst, "destination pages")
+        both = np.empty((n, 2), _I32)
+        both[:, 0] = src if src.dtype is _I32 else _int32(src, "source pages")
+        both[:, 1] = dst if type(dst) is np.ndarray and dst.dtype is _I32 else _int32(dst, "destination pages")
     else:  # lists: half of what numpy takes, few moves or many
         both = array("i", bytes(8 * n))
         both[0::2] = array("i", src)
