@@ -354,6 +354,8 @@ HQ_API hq_status hq_allreduce_sum(void* const* peer_bufs, unsigned* const* peer_
  * left as they are, those of one with a wrong page number are undefined, and
  * all other sequences' rows are right.  A sequence of more than max_q_len rows
  * counts as one with wrong offsets, or is computed all the same.
+ * Every block of rows searches for its sequence among all: the time of a call
+ * over thousands of prompts grows with the square of their number.
  */
 
 /* [tokens][heads][head_dim] rows, e.g. a third of the QKV layer's output. */
@@ -410,8 +412,9 @@ HQ_API hq_status hq_attn_prompt(const hq_attn_shape* shape, const hq_rows* q, co
  * in the pages prefix_table[0 .. ceil(prefix_len / page_size) - 1] of the same
  * cache; they stand before the sequences' own keys and are read once for all
  * rows.  kv_lens and page_table count and hold the own keys only.
- * max_kv_len: a bound of kv_lens that sizes the launch (results do not depend
- * on it).  Workspace: hq_attn_paged_workspace_size bytes, 16-byte aligned, no
+ * max_kv_len: a bound of kv_lens that the split of the work is chosen by.  With
+ * another one, too small or too large, sums are taken in another order: results
+ * are the same within rounding.  Workspace: hq_attn_paged_workspace_size bytes, 16-byte aligned, no
  * initial value needed; calls that may run at the same time need different ones.
  */
 HQ_API size_t hq_attn_paged_workspace_size(const hq_attn_shape* shape, int max_kv_len, int prefix_len);

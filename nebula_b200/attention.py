@@ -177,7 +177,8 @@ def attn_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pa
     """Attention of a step's rows over a paged cache: q [T, Hq, D]; sequence s has the rows cu_q[s] .. cu_q[s+1]-1
     (cu_q None: row s alone), at most max_q_len, and kv_lens[s] keys, its rows' own last (kv_append writes them
     first).  Row i of n sees keys 0 .. kv_lens[s] - n + i, after the prefix_len keys of the pages prefix_table that
-    every sequence shares.  max_kv_len: a bound of kv_lens that sizes the launch."""
+    every sequence shares.  max_kv_len: a bound of kv_lens by which the work is split (another one: the same results
+    within rounding)."""
     dtype, dt, dev = _kind(q, "q")
     ctx = _elsewhere(dev, stream)
     if ctx is not None:

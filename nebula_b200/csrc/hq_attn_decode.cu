@@ -479,6 +479,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_decode_kernel(const __grid_c
                     w[e] = ex2(fmaf(s[nt][e], p.scale_log2, sub));
                     l[nt][e & 1] += w[e];
                 }
+                // rounded to V's type for the MMA, as in the tile kernel; l has them in fp32
                 pf[nt][0] = transpose8x8(pack2<kBF16>(w[0], w[1]));
                 pf[nt][1] = transpose8x8(pack2<kBF16>(w[2], w[3]));
             }

@@ -82,6 +82,10 @@ struct CopyParams {
     size_t stride, bytes;
 };
 
+// One block a page and array, one 16-byte load in flight a thread. 801 pages of 64 KB in
+// 16 layers' keys and values: 557 us, 6.0 TB/s. A large page alone is bound by its
+// block's round trips: one of 256 KB in 4 layers 14.8 us, eight 16.7 us (2.0 TB/s), 64 of
+// them 57.8 us (4.6 TB/s); one of 32 KB 5.1 us.
 __global__ void __launch_bounds__(256) kv_copy_pages_kernel(const __grid_constant__ CopyParams p) {
     const PageMove mv = p.moves[blockIdx.x];
     uint8_t* base = static_cast<uint8_t*>(p.bases[blockIdx.y]);
